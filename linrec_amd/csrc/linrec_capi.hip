@@ -25,6 +25,7 @@
 #include "sweep_kernel.hpp"
 #include "team_kernel.hpp"
 #include "tile_kernel.hpp"
+#include "workspace.hpp"
 
 // Scratch of linrec_fwd_noalloc, the entry point for callers that cannot allocate: every GPU the library
 // runs on holds one copy of this array, at its own address, until the process ends.  In host code the
@@ -1567,30 +1568,9 @@ int make_plan(const Problem& q, const linrec_tuning_t* tune, linrec_plan_t* out)
   return LINREC_OK;
 }
 
-// Workspace = header | completion counters | descriptors.  The counter tree of T tiles needs
-// sum_l ceil(T / 32^l) < T/31 + 8 words; T/16 + 64 words are reserved.
-struct WorkspaceLayout {
-  size_t counters_offset, desc_offset;
-  int64_t tiles;  // descriptors (and tiles of one launch) the workspace has room for
-};
-
-size_t counter_bytes_for(int64_t tiles) { return ((size_t(tiles) / 16 + 64) * 4 + 15) & ~size_t(15); }
-
-// (All of this in the lower half of the buffer; the upper half is scratch without a life beyond
-// one call: the maps of the segmented column launches.  A map must never land where a later launch
-// reads descriptors, whose validity is a bit pattern.)
-WorkspaceLayout workspace_layout(size_t whole_bytes) {
-  const size_t bytes = whole_bytes / 2;
-  WorkspaceLayout lay{sizeof(linrec::CarryHeader), 0, 0};
-  const size_t fixed = sizeof(linrec::CarryHeader) + 64 * 4 + 16;
-  if (bytes <= fixed) return lay;
-  // 16 bytes of descriptors and a quarter byte of counters per tile
-  int64_t tiles = int64_t((bytes - fixed) * 4 / 65);
-  while (tiles > 0 && sizeof(linrec::CarryHeader) + counter_bytes_for(tiles) + size_t(tiles) * 16 > bytes) --tiles;
-  lay.tiles = tiles;
-  lay.desc_offset = sizeof(linrec::CarryHeader) + counter_bytes_for(tiles);
-  return lay;
-}
+using linrec::WorkspaceLayout;
+using linrec::counter_bytes_for;
+using linrec::workspace_layout;
 
 // Polls of one look-back window before a tile gives up (about a second of waiting by default).  One value
 // for the process: a wait that runs out costs time, never the result, so no caller depends on another's choice.

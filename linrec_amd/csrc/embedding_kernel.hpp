@@ -1,0 +1,332 @@
+// Token embedding, y[n] = scale W[token[n]], and its gradient, d_W[v] = scale * sum of d_y[n] over the n with token[n] == v.
+//
+// Forward: a wave copies 64 slots of channels of a few rows.  Bound by memory; a row that is looked up again comes from a cache.
+//
+// Backward, without atomics on values: the positions are sorted by token (stably, so that each list of positions ascends), then
+// every row of the table is written once, by the wave that finds its list in the sorted tokens.
+//   sort   up to SORT_SMALL tokens in one launch: the place of a position is the number of smaller (token, position) pairs, all
+//          pairs compared; more are sorted by digits of at most DIGIT_BITS bits from the lowest on, two launches each (counts
+//          of blocks; places).  Places are counted, never drawn, so the order is the same in every run.
+//   sums   a list may be as long as all positions.  Aligned runs of 64 sorted positions with one token are summed first, a wave
+//          each, then aligned runs of 64 of those; a row adds up what is left before, the two kinds of runs, and what is left
+//          after, at most 63 of each kind and end.  The grouping depends on the tokens alone.
+// Bound by memory: d_y is read once, the table's gradient written once.
+#pragma once
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+#include "../../include/linrec_layers.h"
+#include "collook_kernel.hpp"  // Held, ld_any, st_any, widen
+
+namespace linrec {
+
+__device__ __forceinline__ int64_t token_at(const linrec_embedding_t& p, int64_t n) {
+  return p.token_bytes == 8 ? static_cast<const int64_t*>(p.token)[n] : int64_t(static_cast<const int32_t*>(p.token)[n]);
+}
+// What a position is sorted by: its token, behind all of them if it has no part in the gradient.
+__device__ __forceinline__ int sort_key(const linrec_embedding_t& p, int64_t n) {
+  const int64_t v = token_at(p, n);
+  return v >= 0 && v < p.vocab && v != p.padding ? int(v) : int(p.vocab);
+}
+
+// The channels of a lane of column wave `cw`: the last lanes start early where the channels end and compute, and store, what
+// the lane before them does (the same bits).
+template <int VEC>
+__device__ __forceinline__ int64_t wave_channel(int64_t cw, int lane, int64_t channels) {
+  const int64_t c = (cw * 64 + lane) * VEC, last = channels - VEC;
+  return c < last ? c : last;
+}
+
+// ---- forward ----------------------------------------------------------------------------------
+template <typename T, int VEC, int ROWS>
+__global__ __launch_bounds__(256) void embedding_fwd_kernel(linrec_embedding_t p, int64_t column_waves) {
+  const int lane = threadIdx.x & 63;
+  const int64_t unit = int64_t(blockIdx.x) * 4 + (threadIdx.x >> 6);
+  const int64_t row_set = unit / column_waves, cw = unit - row_set * column_waves;
+  const int64_t c = wave_channel<VEC>(cw, lane, p.channels), n0 = row_set * ROWS;
+  Held<T, VEC> h[ROWS];
+  bool there[ROWS];
+#pragma unroll
+  for (int i = 0; i < ROWS; ++i) {
+    const int64_t v = n0 + i < p.tokens ? token_at(p, n0 + i) : -1;
+    there[i] = v >= 0 && v < p.vocab;
+    h[i] = held_zero<T, VEC>();
+    if (there[i]) h[i] = ld_any<VEC, false>(static_cast<const T*>(p.weight) + v * p.channels + c);
+  }
+#pragma unroll
+  for (int i = 0; i < ROWS; ++i) {
+    if (n0 + i < p.tokens) {
+      Lanes<VEC> v = widen(h[i]);
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) v.v[e] = there[i] ? v.v[e] * p.scale : 0.0f;
+      st_any<VEC>(static_cast<T*>(p.y) + (n0 + i) * p.channels + c, v);
+    }
+  }
+}
+
+// ---- sort -------------------------------------------------------------------------------------
+struct Sorted {
+  int* key;
+  int* pos;
+};
+
+constexpr int SORT_SMALL = 8192;
+constexpr int SMALL_TAKE = 32;  // positions a workgroup places
+
+// All pairs: 1024 lanes compare SMALL_TAKE positions with a 32nd of all keys each.
+__global__ __launch_bounds__(1024) void sort_small_kernel(linrec_embedding_t p, Sorted out) {
+  __shared__ alignas(16) int keys[SORT_SMALL];
+  __shared__ int counts[32][SMALL_TAKE + 1];
+  const int n = int(p.tokens), tid = int(threadIdx.x);
+  const int padded = (n + 127) & ~127;
+  for (int i = tid; i < padded; i += 1024) keys[i] = i < n ? sort_key(p, i) : 2147483647;
+  __syncthreads();
+  const int mine = int(blockIdx.x) * SMALL_TAKE + (tid & 31), slice = tid >> 5, per_slice = padded / 32;
+  const int key = mine < n ? keys[mine] : 2147483647;
+  int count = 0;
+  const int first = slice * per_slice;
+  for (int j = first; j < first + per_slice; j += 4) {
+    const int4 k = *reinterpret_cast<const int4*>(&keys[j]);
+    count += (k.x < key || (k.x == key && j < mine)) + (k.y < key || (k.y == key && j + 1 < mine)) +
+             (k.z < key || (k.z == key && j + 2 < mine)) + (k.w < key || (k.w == key && j + 3 < mine));
+  }
+  counts[slice][tid & 31] = count;
+  __syncthreads();
+  if (tid < SMALL_TAKE && mine < n) {
+    int place = 0;
+    for (int s = 0; s < 32; ++s) place += counts[s][tid];
+    out.key[place] = key;
+    out.pos[place] = mine;
+  }
+}
+
+constexpr int DIGIT_BITS = 9, DIGITS = 1 << DIGIT_BITS;
+constexpr int SORT_LANES = 1024, SORT_WAVES = SORT_LANES / 64, SORT_ROUNDS = 2, SORT_BLOCK = SORT_LANES * SORT_ROUNDS;
+
+__device__ __forceinline__ int key_of(const linrec_embedding_t& p, const int* keys, int64_t i) { return keys ? keys[i] : sort_key(p, i); }
+
+__global__ __launch_bounds__(SORT_LANES) void digit_counts_kernel(linrec_embedding_t p, const int* keys, int shift, int* counts) {
+  __shared__ int bins[DIGITS];
+  const int tid = int(threadIdx.x);
+  if (tid < DIGITS) bins[tid] = 0;
+  __syncthreads();
+#pragma unroll
+  for (int r = 0; r < SORT_ROUNDS; ++r) {
+    const int64_t i = int64_t(blockIdx.x) * SORT_BLOCK + r * SORT_LANES + tid;
+    if (i < p.tokens) atomicAdd(&bins[(key_of(p, keys, i) >> shift) & (DIGITS - 1)], 1);
+  }
+  __syncthreads();
+  if (tid < DIGITS) counts[int64_t(blockIdx.x) * DIGITS + tid] = bins[tid];
+}
+
+// A position goes behind all of smaller digits, those of its digit in blocks before, in waves before and before it in its wave.
+__global__ __launch_bounds__(SORT_LANES) void digit_places_kernel(linrec_embedding_t p, const int* keys, const int* positions, int shift,
+                                                                  const int* counts, int blocks, Sorted out) {
+  __shared__ int base[DIGITS];
+  __shared__ int wave_sums[DIGITS / 64];
+  __shared__ int bins[SORT_WAVES][DIGITS];
+  const int tid = int(threadIdx.x), lane = tid & 63, wave = tid >> 6;
+  for (int i = tid; i < SORT_WAVES * DIGITS; i += SORT_LANES) (&bins[0][0])[i] = 0;
+  int all = 0, before = 0;
+  if (tid < DIGITS) {
+#pragma unroll 8
+    for (int b = 0; b < blocks; ++b) {
+      const int c = counts[int64_t(b) * DIGITS + tid];
+      all += c;
+      before += b < int(blockIdx.x) ? c : 0;
+    }
+  }
+  int scan = all;  // over the digits: within waves, then over the waves' sums
+#pragma unroll
+  for (int s = 1; s < 64; s <<= 1) {
+    const int up = __shfl_up(scan, s);
+    if (lane >= s) scan += up;
+  }
+  if (wave < DIGITS / 64 && lane == 63) wave_sums[wave] = scan;
+  __syncthreads();
+  if (tid < DIGITS) {
+    int lower = 0;
+    for (int w = 0; w < wave; ++w) lower += wave_sums[w];
+    base[tid] = lower + scan - all + before;
+  }
+  // a wave takes 64 * SORT_ROUNDS adjacent positions, in order
+  const int64_t first = int64_t(blockIdx.x) * SORT_BLOCK + wave * (64 * SORT_ROUNDS) + lane;
+  int key[SORT_ROUNDS], pos[SORT_ROUNDS], rank[SORT_ROUNDS];
+#pragma unroll
+  for (int r = 0; r < SORT_ROUNDS; ++r) {
+    const int64_t i = first + r * 64;
+    const bool there = i < p.tokens;
+    key[r] = there ? key_of(p, keys, i) : 0;
+    pos[r] = there ? (positions ? positions[i] : int(i)) : 0;
+    const int digit = (key[r] >> shift) & (DIGITS - 1);
+    uint64_t same = __ballot(there);
+#pragma unroll
+    for (int b = 0; b < DIGIT_BITS; ++b) {
+      const uint64_t ones = __ballot(digit >> b & 1);
+      same &= (digit >> b & 1) ? ones : ~ones;
+    }
+    const int ahead = __popcll(same & ((1ull << lane) - 1ull));
+    int so_far = 0;
+    if (there && ahead == 0) so_far = atomicAdd(&bins[wave][digit], __popcll(same));
+    // (the first lane of each digit has asked; the others read what it got)
+    so_far = __shfl(so_far, there ? __builtin_ctzll(same) : 0);
+    rank[r] = so_far + ahead;
+  }
+  __syncthreads();
+  if (tid < DIGITS) {
+    int sum = base[tid];
+#pragma unroll
+    for (int w = 0; w < SORT_WAVES; ++w) {
+      const int c = bins[w][tid];
+      bins[w][tid] = sum;
+      sum += c;
+    }
+  }
+  __syncthreads();
+#pragma unroll
+  for (int r = 0; r < SORT_ROUNDS; ++r) {
+    if (first + r * 64 < p.tokens) {
+      const int place = bins[wave][(key[r] >> shift) & (DIGITS - 1)] + rank[r];
+      out.key[place] = key[r];
+      out.pos[place] = pos[r];
+    }
+  }
+}
+
+// ---- sums -------------------------------------------------------------------------------------
+constexpr int RUN = 64, RUN2 = RUN * RUN;
+
+template <int VEC>
+__device__ __forceinline__ void add_to(Lanes<VEC>& s, const Lanes<VEC>& v) {
+#pragma unroll
+  for (int e = 0; e < VEC; ++e) s.v[e] += v.v[e];
+}
+// Adds `count` rows, row(i) their first value for this lane, in order.
+template <int VEC, typename Row>
+__device__ __forceinline__ void add_rows(Lanes<VEC>& sum, int count, Row&& row) {
+  int i = 0;
+  for (; i + 8 <= count; i += 8) {
+    decltype(ld_any<VEC, false>(row(0))) h[8];
+#pragma unroll
+    for (int q = 0; q < 8; ++q) h[q] = ld_any<VEC, false>(row(i + q));
+#pragma unroll
+    for (int q = 0; q < 8; ++q) add_to(sum, widen(h[q]));
+  }
+  for (; i < count; ++i) add_to(sum, widen(ld_any<VEC, false>(row(i))));
+}
+template <int VEC>
+__device__ __forceinline__ Lanes<VEC> zeros() {
+  Lanes<VEC> r;
+#pragma unroll
+  for (int e = 0; e < VEC; ++e) r.v[e] = 0.0f;
+  return r;
+}
+
+// Runs of 64 positions of one token (SECOND: of 64 such sums): a wave each, for 64 slots of channels.
+template <typename T, int VEC, bool SECOND>
+__global__ __launch_bounds__(256) void run_sums_kernel(linrec_embedding_t p, Sorted sorted, const float* in, float* out, int64_t runs,
+                                                       int64_t column_waves) {
+  const int lane = threadIdx.x & 63;
+  const int64_t unit = int64_t(blockIdx.x) * 4 + (threadIdx.x >> 6);
+  const int64_t run = unit / column_waves, cw = unit - run * column_waves;
+  if (run >= runs) return;
+  constexpr int LENGTH = SECOND ? RUN2 : RUN;
+  const int key = sorted.key[run * LENGTH];
+  if (key != sorted.key[run * LENGTH + LENGTH - 1] || key >= int(p.vocab)) return;
+  const int64_t c = wave_channel<VEC>(cw, lane, p.channels);
+  Lanes<VEC> sum = zeros<VEC>();
+  if constexpr (SECOND) {
+    add_rows<VEC>(sum, RUN, [&](int i) { return in + (run * RUN + i) * p.channels + c; });
+  } else {
+    const int pos = sorted.pos[run * RUN + lane];
+    const T* dy = static_cast<const T*>(p.d_y) + c;
+    add_rows<VEC>(sum, RUN, [&](int i) { return dy + int64_t(__builtin_amdgcn_readlane(pos, i)) * p.d_y_stride; });
+  }
+  float* to = out + run * p.channels + c;
+#pragma unroll
+  for (int e = 0; e < VEC; ++e) to[e] = sum.v[e];
+}
+
+// Number of sorted keys below `key`: every lane asks for one of 64 evenly spaced ones at a time.
+__device__ __forceinline__ int keys_below(const int* keys, int n, int key, int lane) {
+  int lo = 0, len = n;  // the answer lies in [lo, lo + len]
+  while (len > 0) {
+    const int step = (len + 63) >> 6, i = lane * step;
+    const uint64_t below = __ballot(i < len && keys[lo + (i < len ? i : 0)] < key);
+    const int hits = __popcll(below);
+    if (hits == 0) return lo;
+    // the keys at 0, step, .. (hits - 1) * step are below, the next one asked for is not
+    const int skip = (hits - 1) * step + 1, rest = len - skip;
+    lo += skip;
+    len = rest < step - 1 ? rest : step - 1;
+  }
+  return lo;
+}
+
+// A wave writes `rows` adjacent rows of the table's gradient, 64 slots of channels of each.
+template <typename T, int VEC>
+__global__ __launch_bounds__(256) void table_rows_kernel(linrec_embedding_t p, Sorted sorted, const float* runs, const float* runs2, int rows,
+                                                         int64_t column_waves) {
+  const int lane = threadIdx.x & 63;
+  const int64_t unit = int64_t(blockIdx.x) * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int64_t row_set = unit / column_waves, cw = unit - row_set * column_waves;
+  const int64_t v0 = row_set * rows;
+  if (v0 >= p.vocab) return;
+  const int64_t v1 = v0 + rows < p.vocab ? v0 + rows : p.vocab;
+  const int64_t c = wave_channel<VEC>(cw, lane, p.channels);
+  const T* dy = static_cast<const T*>(p.d_y) + c;
+  T* out = static_cast<T*>(p.d_weight) + c;
+  const int n = int(p.tokens);
+  int at = __builtin_amdgcn_readfirstlane(keys_below(sorted.key, n, int(v0), lane));
+  // a window of 64 aligned sorted positions
+  int base = at & ~(RUN - 1), key = 2147483647, pos = 0;
+  auto look = [&]() __attribute__((always_inline)) {
+    const bool there = base + lane < n;
+    key = there ? sorted.key[base + lane] : 2147483647;
+    pos = there ? sorted.pos[base + lane] : 0;
+  };
+  look();
+  for (int64_t v = v0; v < v1; ++v) {
+    Lanes<VEC> sum = zeros<VEC>();
+    for (;;) {
+      const uint64_t ours = __ballot(key == int(v)) >> (at - base);
+      const int count = ours == ~0ull ? 64 : __builtin_ctzll(~ours);
+      if (count == 64) {  // a whole run, perhaps many
+        int whole = 0, length = RUN;
+        const float* from = runs;
+        if ((base & (RUN2 - 1)) == 0) {
+          const int64_t i = int64_t(base) + int64_t(lane) * RUN2 + RUN2 - 1;
+          const uint64_t m = __ballot(i < n && sorted.key[i < n ? i : 0] == int(v));
+          whole = m == ~0ull ? 64 : __builtin_ctzll(~m);
+          if (whole > 0) {
+            length = RUN2;
+            from = runs2;
+          }
+        }
+        if (whole == 0) {
+          const int64_t i = int64_t(base) + int64_t(lane) * RUN + RUN - 1;
+          const int until = RUN - (base / RUN & (RUN - 1));  // runs up to the next run of runs
+          const uint64_t m = __ballot(lane < until && i < n && sorted.key[i < n ? i : 0] == int(v));
+          whole = m == ~0ull ? 64 : __builtin_ctzll(~m);
+        }
+        const float* first = from + int64_t(base / length) * p.channels + c;
+        add_rows<VEC>(sum, whole, [&](int i) { return first + int64_t(i) * p.channels; });
+        at = base += whole * length;
+        look();
+        continue;
+      }
+      add_rows<VEC>(sum, count, [&](int i) {
+        return dy + int64_t(__builtin_amdgcn_readlane(pos, at - base + i)) * p.d_y_stride;
+      });
+      at += count;
+      if (at - base < 64) break;  // a position of another token comes next (or none: their keys are the largest)
+      base += RUN;
+      look();
+    }
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) sum.v[e] *= p.scale;
+    st_any<VEC>(out + v * p.channels, sum);
+  }
+}
+
+}  // namespace linrec

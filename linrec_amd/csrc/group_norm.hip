@@ -1,134 +1,179 @@
-// Group norm with an activation, channels last: a workgroup per (batch, group).
-#include "layer_common.hpp"
+// Launches of group norm with an activation (group_norm_kernel.hpp).
+#include "group_norm_kernel.hpp"
 
 namespace linrec {
 namespace {
 
-__device__ __forceinline__ float act_value(int act, float z) {
-  switch (act) {
-    case LINREC_ACT_RELU: return z < 0.0f ? 0.0f : z;  // (NaN stays)
-    case LINREC_ACT_SILU: return z / (1.0f + expf(-z));
-    case LINREC_ACT_GELU: return 0.5f * z * erfcf(-z * 0.70710678118654752f);
-  }
-  return z;
+// d_bias and d_weight from rows of (sums of e, sums of e xh).
+__global__ __launch_bounds__(64 * SUM_WAVES) void param_sum_kernel(const float* in, int64_t rows, int64_t columns, int64_t per_chunk, float* out) {
+  column_sum_block(in, rows, columns, per_chunk, [&](int64_t c, float s) { out[blockIdx.y * columns + c] = s; });
 }
-__device__ __forceinline__ float act_slope(int act, float z) {
-  switch (act) {
-    case LINREC_ACT_RELU: return z > 0.0f ? 1.0f : 0.0f;
-    case LINREC_ACT_SILU: {
-      const float s = 1.0f / (1.0f + expf(-z));
-      return s * (1.0f + z * (1.0f - s));
+__global__ __launch_bounds__(64 * SUM_WAVES) void param_gradient_kernel(const float* in, int64_t rows, int64_t channels, int dtype, void* d_weight,
+                                                                        void* d_bias) {
+  column_sum_block(in, rows, 2 * channels, rows, [&](int64_t c, float s) {
+    void* to = c < channels ? d_bias : d_weight;
+    if (c >= channels) c -= channels;
+    if (dtype == LINREC_DTYPE_F32) static_cast<float*>(to)[c] = s;
+    else if (dtype == LINREC_DTYPE_F16) static_cast<_Float16*>(to)[c] = _Float16(s);
+    else static_cast<__bf16*>(to)[c] = __bf16(s);
+  });
+}
+
+enum class Shape { tokens, held, chunks };
+struct NormPlan {
+  Shape shape;
+  int vec;
+  int lanes;           // of a workgroup
+  int64_t grid;
+  int64_t param_rows;  // rows of partial sums of d_weight and d_bias
+  int64_t pieces;      // floats of partial statistics
+  TokenArgs tokens;
+  int items_per_lane;  // tokens: slots of a lane
+  BlockArgs block;
+};
+
+int pow2_at_least(int64_t n) {
+  int p = 1;
+  while (p < n) p <<= 1;
+  return p;
+}
+
+NormPlan make_norm_plan(int dtype, int64_t batch, int64_t positions, int64_t channels, int64_t groups, bool bwd) {
+  NormPlan pl{};
+  const int64_t width = channels / groups;
+  const int size = dtype == LINREC_DTYPE_F32 ? 4 : 2;
+  pl.vec = 16 / size;
+  while (width % pl.vec) pl.vec >>= 1;
+  const int64_t columns = width / pl.vec;  // of a group
+
+  if (positions == 1 && width <= 1024) {
+    pl.shape = Shape::tokens;
+    TokenArgs& t = pl.tokens;
+    t.team = columns < 64 ? pow2_at_least(columns) : 64;
+    pl.items_per_lane = columns <= 64 ? 1 : 16 / pl.vec;
+    const int64_t waves = cdiv(groups, 64 / t.team);  // of a row
+    t.column_waves = waves < TOKEN_WAVES ? pow2_at_least(waves) : TOKEN_WAVES;
+    t.column_blocks = int(cdiv(waves, t.column_waves));
+    const int64_t slots = TOKEN_WAVES / t.column_waves;
+    // enough workgroups for the chip; in the backward each leaves a row of sums behind
+    const int64_t most = bwd ? 512 : 1024;
+    int64_t row_blocks = cdiv(batch, slots);
+    const int64_t cap = most / t.column_blocks > 1 ? most / t.column_blocks : 1;
+    if (row_blocks > cap) row_blocks = cap;
+    t.row_blocks = int(row_blocks < 1 ? 1 : row_blocks);
+    pl.lanes = 64 * TOKEN_WAVES;
+    pl.grid = int64_t(t.row_blocks) * t.column_blocks;
+    pl.param_rows = t.row_blocks;
+    return pl;
+  }
+
+  BlockArgs& a = pl.block;
+  a.whole = int(columns);
+  const int bytes = pl.vec * size;
+  const int keep = 32 / (bytes >= 4 ? bytes / 4 : 1);
+  auto rows_of = [&](int lanes, int64_t wide) { return wide > 0 && wide <= lanes ? lanes / wide : int64_t(0); };
+  // held: positions * columns of a group in registers
+  for (int lanes : {256, 1024}) {
+    if (!rows_of(lanes, columns) || cdiv(positions, rows_of(lanes, columns)) > keep) continue;
+    if (lanes == 256 && columns * positions > 4 * 256 && batch * groups < 1024) continue;  // few groups: more lanes to each
+    int64_t g = 1, items = 1;
+    auto fits = [&](int64_t gg, int64_t it) {
+      const int64_t R = rows_of(lanes, gg * columns * it);
+      return R > 0 && cdiv(positions, R) <= keep / 2 + 1 && cdiv(groups, gg) * cdiv(batch, it) >= 1024;
+    };
+    while (2 * g <= groups && fits(2 * g, 1)) g *= 2;
+    if (g * 2 > groups && fits(groups, 1)) g = groups;
+    if (g == groups)
+      while (2 * items <= batch && fits(g, 2 * items)) items *= 2;
+    pl.shape = Shape::held;
+    pl.lanes = lanes;
+    a.per_group = int(columns); a.groups = int(g); a.items = int(items); a.parts = 1; a.chunks = 1;
+    a.blocks = int(cdiv(groups, g));
+    a.columns = int(items * g * columns);
+    a.R = int(rows_of(lanes, a.columns));
+    a.rows = int(positions);
+    pl.param_rows = cdiv(batch, items);
+    pl.grid = pl.param_rows * a.blocks;
+    return pl;
+  }
+
+  pl.shape = Shape::chunks;
+  pl.lanes = 256;
+  a.parts = int(cdiv(columns, 256));
+  a.per_group = int(cdiv(columns, a.parts));
+  a.parts = int(cdiv(columns, a.per_group));  // (none of them empty)
+  a.groups = a.parts > 1 ? 1 : int(256 / columns < groups ? 256 / columns : groups);
+  a.items = 1;
+  a.blocks = int(cdiv(groups, a.groups) * a.parts);
+  a.columns = a.groups * a.per_group;
+  a.R = 256 / a.columns;
+  const int64_t side = batch * a.blocks;
+  int64_t chunks = cdiv(2048, side), most = cdiv(positions, int64_t(a.R) * 8);
+  if (chunks > most) chunks = most;
+  if (chunks > 256) chunks = 256;
+  if (chunks < 1) chunks = 1;
+  a.rows = int(cdiv(cdiv(positions, chunks), a.R) * a.R);
+  a.chunks = int(cdiv(positions, a.rows));
+  pl.grid = side * a.chunks;
+  pl.param_rows = batch * a.chunks;
+  pl.pieces = 2 * batch * a.chunks * a.parts * groups;
+  return pl;
+}
+
+int64_t partial_floats(const NormPlan& pl, int64_t channels, bool bwd) {
+  if (!bwd) return pl.pieces;
+  const int64_t chunks = column_sum_chunks(pl.param_rows);
+  return pl.pieces + 2 * channels * (pl.param_rows + (chunks > 1 ? chunks : 0));
+}
+
+template <typename T, int VEC, bool BWD>
+int launch_tokens(const linrec_group_norm_t& p, const NormPlan& pl) {
+  TokenArgs a = pl.tokens;
+  a.p = p;
+  if (BWD) a.p.partial = p.partial + pl.pieces;
+  return pl.items_per_lane == 1 ? launch_kernel(norm_tokens_kernel<T, VEC, 1, BWD>, pl.grid, 1, pl.lanes, p.stream, a)
+                                : launch_kernel(norm_tokens_kernel<T, VEC, 16 / VEC, BWD>, pl.grid, 1, pl.lanes, p.stream, a);
+}
+
+template <typename T, int VEC>
+int launch_norm(const linrec_group_norm_t& p, const NormPlan& pl, bool bwd) {
+  if (pl.shape == Shape::tokens) return bwd ? launch_tokens<T, VEC, true>(p, pl) : launch_tokens<T, VEC, false>(p, pl);
+  BlockArgs a = pl.block;
+  a.p = p;
+  float* sums = p.partial + pl.pieces;
+  if (!bwd) {
+    if (pl.shape == Shape::held)
+      return pl.lanes == 256 ? launch_kernel(norm_fwd_kernel<T, VEC, 256, NORM_HELD>, pl.grid, 1, 256, p.stream, a)
+                             : launch_kernel(norm_fwd_kernel<T, VEC, 1024, NORM_HELD>, pl.grid, 1, 1024, p.stream, a);
+    if (const int rc = launch_kernel(norm_fwd_kernel<T, VEC, 256, NORM_STATS>, pl.grid, 1, 256, p.stream, a)) return rc;
+    return launch_kernel(norm_fwd_kernel<T, VEC, 256, NORM_APPLY>, pl.grid, 1, 256, p.stream, a);
+  }
+  if (pl.shape == Shape::held)
+    return pl.lanes == 256 ? launch_kernel(norm_bwd_kernel<T, VEC, 256, NORM_HELD>, pl.grid, 1, 256, p.stream, a, sums)
+                           : launch_kernel(norm_bwd_kernel<T, VEC, 1024, NORM_HELD>, pl.grid, 1, 1024, p.stream, a, sums);
+  if (const int rc = launch_kernel(norm_bwd_kernel<T, VEC, 256, NORM_STATS>, pl.grid, 1, 256, p.stream, a, sums)) return rc;
+  return launch_kernel(norm_bwd_kernel<T, VEC, 256, NORM_APPLY>, pl.grid, 1, 256, p.stream, a, sums);
+}
+
+int launch_norm(const linrec_group_norm_t& p, const NormPlan& pl, bool bwd) {
+  return with_dtype(p.dtype, [&](auto t) {
+    using T = decltype(t);
+    switch (pl.vec) {
+      case 1: return launch_norm<T, 1>(p, pl, bwd);
+      case 2: return launch_norm<T, 2>(p, pl, bwd);
+      case 4: return launch_norm<T, 4>(p, pl, bwd);
     }
-    case LINREC_ACT_GELU: return 0.5f * erfcf(-z * 0.70710678118654752f) + z * expf(-0.5f * z * z) * 0.39894228040143268f;
-  }
-  return 1.0f;
-}
-__device__ __forceinline__ float param(const void* p, int dtype, int64_t c, float none) {
-  if (!p) return none;
-  switch (dtype) {
-    case LINREC_DTYPE_F16: return float(static_cast<const _Float16*>(p)[c]);
-    case LINREC_DTYPE_BF16: return float(static_cast<const __bf16*>(p)[c]);
-  }
-  return static_cast<const float*>(p)[c];
-}
-__device__ __forceinline__ void set_param(void* p, int dtype, int64_t c, float v) {
-  switch (dtype) {
-    case LINREC_DTYPE_F16: static_cast<_Float16*>(p)[c] = _Float16(v); return;
-    case LINREC_DTYPE_BF16: static_cast<__bf16*>(p)[c] = __bf16(v); return;
-  }
-  static_cast<float*>(p)[c] = v;
-}
-// Sum over the 256 lanes of a workgroup, the same in all of them.
-__device__ float block_sum(float v) {
-  __shared__ float sh[256];
-  __syncthreads();
-  sh[threadIdx.x] = v;
-  __syncthreads();
-  for (int o = 128; o; o >>= 1) {
-    if (int(threadIdx.x) < o) sh[threadIdx.x] += sh[threadIdx.x + o];
-    __syncthreads();
-  }
-  return sh[0];
-}
-
-template <typename T>
-__global__ void norm_fwd_kernel(linrec_group_norm_t p) {
-  const int64_t n = blockIdx.x / p.groups, g = blockIdx.x % p.groups, cg = p.channels / p.groups, count = cg * p.positions;
-  const T* x = static_cast<const T*>(p.x) + n * p.x_stride[0];
-  float s = 0.0f;
-  for (int64_t i = threadIdx.x; i < count; i += 256) s += float(x[(i / cg) * p.x_stride[1] + g * cg + i % cg]);
-  const float mean = block_sum(s) / float(count);
-  s = 0.0f;
-  for (int64_t i = threadIdx.x; i < count; i += 256) {
-    const float d = float(x[(i / cg) * p.x_stride[1] + g * cg + i % cg]) - mean;
-    s += d * d;
-  }
-  const float rstd = rsqrtf(block_sum(s) / float(count) + p.eps);
-  for (int64_t i = threadIdx.x; i < count; i += 256) {
-    const int64_t c = g * cg + i % cg;
-    const float z = (float(x[(i / cg) * p.x_stride[1] + c]) - mean) * rstd * param(p.weight, p.weight_dtype, c, 1.0f) +
-                    param(p.bias, p.weight_dtype, c, 0.0f);
-    static_cast<T*>(p.y)[(n * p.positions + i / cg) * p.channels + c] = T(act_value(p.act, z));
-  }
-  if (threadIdx.x == 0) {
-    p.mean[n * p.groups + g] = mean;
-    p.rstd[n * p.groups + g] = rstd;
-  }
-}
-
-template <typename T>
-__global__ void norm_bwd_kernel(linrec_group_norm_t p) {
-  const int64_t n = blockIdx.x / p.groups, g = blockIdx.x % p.groups, cg = p.channels / p.groups, count = cg * p.positions;
-  const T* x = static_cast<const T*>(p.x) + n * p.x_stride[0];
-  const T* dy = static_cast<const T*>(p.d_y) + n * p.d_y_stride[0];
-  const float mean = p.mean[n * p.groups + g], rstd = p.rstd[n * p.groups + g];
-  float s1 = 0.0f, s2 = 0.0f;
-  auto at = [&](int64_t i, float& xh, float& ew) {
-    const int64_t c = g * cg + i % cg;
-    const float w = param(p.weight, p.weight_dtype, c, 1.0f);
-    xh = (float(x[(i / cg) * p.x_stride[1] + c]) - mean) * rstd;
-    ew = float(dy[(i / cg) * p.d_y_stride[1] + c]) * act_slope(p.act, xh * w + param(p.bias, p.weight_dtype, c, 0.0f)) * w;
-  };
-  for (int64_t i = threadIdx.x; i < count; i += 256) {
-    float xh, ew;
-    at(i, xh, ew);
-    s1 += ew;
-    s2 += ew * xh;
-  }
-  s1 = block_sum(s1) / float(count);
-  s2 = block_sum(s2) / float(count);
-  for (int64_t i = threadIdx.x; i < count; i += 256) {
-    float xh, ew;
-    at(i, xh, ew);
-    static_cast<T*>(p.d_x)[(n * p.positions + i / cg) * p.channels + g * cg + i % cg] = T(rstd * (ew - s1 - xh * s2));
-  }
-}
-
-template <typename T>
-__global__ void norm_params_kernel(linrec_group_norm_t p) {
-  const int64_t c = blockIdx.x, cg = p.channels / p.groups, g = c / cg;
-  const float w = param(p.weight, p.weight_dtype, c, 1.0f), b = param(p.bias, p.weight_dtype, c, 0.0f);
-  float s1 = 0.0f, s2 = 0.0f;
-  for (int64_t i = threadIdx.x; i < p.batch * p.positions; i += 256) {
-    const int64_t n = i / p.positions, q = i % p.positions;
-    const float xh = (float(static_cast<const T*>(p.x)[n * p.x_stride[0] + q * p.x_stride[1] + c]) - p.mean[n * p.groups + g]) *
-                     p.rstd[n * p.groups + g];
-    const float e = float(static_cast<const T*>(p.d_y)[n * p.d_y_stride[0] + q * p.d_y_stride[1] + c]) * act_slope(p.act, xh * w + b);
-    s1 += e;
-    s2 += e * xh;
-  }
-  s1 = block_sum(s1);
-  s2 = block_sum(s2);
-  if (threadIdx.x == 0) {
-    set_param(p.d_bias, p.weight_dtype, c, s1);
-    set_param(p.d_weight, p.weight_dtype, c, s2);
-  }
+    if constexpr (sizeof(T) == 2) return launch_norm<T, 8>(p, pl, bwd);
+    return int(LINREC_E_UNSUPPORTED);
+  });
 }
 
 int check_norm(const linrec_group_norm_t* p) {
   if (!p || p->batch < 0 || p->positions < 0 || p->channels < 0 || p->groups < 1 || p->channels % p->groups) return LINREC_E_INVALID;
   if (p->act < LINREC_ACT_NONE || p->act > LINREC_ACT_GELU || !p->weight != !p->bias) return LINREC_E_INVALID;
-  if (p->dtype < LINREC_DTYPE_F32 || p->dtype > LINREC_DTYPE_BF16 || p->weight_dtype < LINREC_DTYPE_F32 || p->weight_dtype > LINREC_DTYPE_BF16) return LINREC_E_UNSUPPORTED;
+  if (p->dtype < LINREC_DTYPE_F32 || p->dtype > LINREC_DTYPE_BF16 || p->weight_dtype < LINREC_DTYPE_F32 || p->weight_dtype > LINREC_DTYPE_BF16)
+    return LINREC_E_UNSUPPORTED;
+  if (p->batch > 2147483647LL || p->positions > 2147483647LL - 65536 || p->channels > 2147483647LL - 65536) return LINREC_E_TOO_LARGE;
   if (p->batch > 0 && p->positions > 0 && p->channels > 0 && (!p->x || !p->mean || !p->rstd)) return LINREC_E_INVALID;
   return LINREC_OK;
 }
@@ -140,25 +185,43 @@ using namespace linrec;
 
 extern "C" {
 
-int64_t linrec_group_norm_partial_floats(int, int64_t, int64_t, int64_t, int64_t, int) { return 0; }
+int64_t linrec_group_norm_partial_floats(int dtype, int64_t batch, int64_t positions, int64_t channels, int64_t groups, int is_bwd) {
+  if (batch <= 0 || positions <= 0 || channels <= 0 || groups <= 0 || channels % groups) return is_bwd ? 2 * (channels > 0 ? channels : 0) : 0;
+  return partial_floats(make_norm_plan(dtype, batch, positions, channels, groups, is_bwd != 0), channels, is_bwd != 0);
+}
 
 int linrec_group_norm_fwd(const linrec_group_norm_t* p) {
   if (const int rc = check_norm(p)) return rc;
   if (p->batch == 0 || p->positions == 0 || p->channels == 0) return LINREC_OK;
-  if (!p->y) return LINREC_E_INVALID;
-  return with_dtype(p->dtype, [&](auto t) { return launch_kernel(norm_fwd_kernel<decltype(t)>, p->batch * p->groups, 1, 256, p->stream, *p); });
+  const NormPlan pl = make_norm_plan(p->dtype, p->batch, p->positions, p->channels, p->groups, false);
+  if (!p->y || (partial_floats(pl, p->channels, false) && !p->partial)) return LINREC_E_INVALID;
+  return launch_norm(*p, pl, false);
 }
 
 int linrec_group_norm_bwd(const linrec_group_norm_t* p) {
   if (const int rc = check_norm(p)) return rc;
   if (p->channels == 0) return LINREC_OK;
   if (p->weight && (!p->d_weight || !p->d_bias)) return LINREC_E_INVALID;
-  if (p->batch > 0 && p->positions > 0 && (!p->d_y || !p->d_x)) return LINREC_E_INVALID;
-  return with_dtype(p->dtype, [&](auto t) {
-    if (p->positions > 0 && p->channels > 0)
-      if (const int rc = launch_kernel(norm_bwd_kernel<decltype(t)>, p->batch * p->groups, 1, 256, p->stream, *p)) return rc;
-    return p->weight ? launch_kernel(norm_params_kernel<decltype(t)>, p->channels, 1, 256, p->stream, *p) : LINREC_OK;
-  });
+  int64_t rows = 0;
+  const float* sums = p->partial;
+  if (p->batch > 0 && p->positions > 0) {
+    if (!p->d_y || !p->d_x || !p->partial) return LINREC_E_INVALID;
+    const NormPlan pl = make_norm_plan(p->dtype, p->batch, p->positions, p->channels, p->groups, true);
+    if (const int rc = launch_norm(*p, pl, true)) return rc;
+    rows = pl.param_rows;
+    sums += pl.pieces;
+  }
+  if (!p->weight) return LINREC_OK;
+  const int64_t chunks = column_sum_chunks(rows), columns = 2 * p->channels;
+  if (chunks > 1) {
+    float* out = const_cast<float*>(sums) + rows * columns;
+    if (const int rc = launch_kernel(param_sum_kernel, cdiv(columns, 64), chunks, 64 * SUM_WAVES, p->stream, sums, rows, columns, SUM_ROWS, out))
+      return rc;
+    sums = out;
+    rows = chunks;
+  }
+  return launch_kernel(param_gradient_kernel, cdiv(columns, 64), 1, 64 * SUM_WAVES, p->stream, sums, rows, p->channels, p->weight_dtype,
+                       p->d_weight, p->d_bias);
 }
 
 }  // extern "C"

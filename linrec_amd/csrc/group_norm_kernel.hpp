@@ -1,0 +1,676 @@
+// Group norm with an activation, channels last, forward and backward.
+//
+//   xh = (x - mean) rstd,  z = xh w + b,  y = act(z)
+//   e = d_y act'(z),  d_x = rstd (e w - s1 - xh s2),  s1 = sum e w / M,  s2 = sum e w xh / M  over the M values of a group,
+//   d_b = sum e,  d_w = sum e xh  over all rows
+//
+// What bounds it: memory.  Three shapes, by how much one group is:
+//   tokens  one position: a team of 1 .. 64 adjacent lanes holds a group in registers; waves keep their channels and walk down
+//           the rows, so weights are read once and the sums of d_w and d_b stay in registers.
+//   held    a workgroup holds all positions of one or more groups (and batch items) in registers: every value is read once.
+//   chunks  larger groups: partial statistics of chunks of positions, and a second launch that puts them together and reads
+//           the values again.
+//
+// Statistics: tokens and held take the mean first and the squares of the differences then.  Chunks cannot; a lane sums
+// differences to its own first value, d and d^2 over n <= a few hundred values, so what cancels in M2 = sum d^2 - (sum d)^2 / n is
+// at most n times M2 itself (the first value is one of those it is spread by), whatever the mean; lanes and chunks are then
+// merged as (count, mean, M2) (T. F. Chan, G. H. Golub, R. J. LeVeque, "Updating formulae and a pairwise algorithm for computing
+// sample variances", 1979).  All sums are trees whose shape depends on the sizes alone: the same bits in every run.
+#pragma once
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+#include "../../include/linrec_layers.h"
+#include "collook_kernel.hpp"  // Held, ld_any, st_any, widen
+#include "column_sum.hpp"
+
+namespace linrec {
+
+// ---- activation -------------------------------------------------------------------------------
+// erfc(|v|) / exp(-v^2) as a polynomial in t = 1 / (1 + p |v|): M. Abramowitz, I. A. Stegun, "Handbook of Mathematical
+// Functions", 7.1.26, at most 1.5e-7 off in erf.
+__device__ __forceinline__ float erfc_scaled(float abs_v) {
+  const float t = __builtin_amdgcn_rcpf(fmaf(0.3275911f, abs_v, 1.0f));
+  return t * fmaf(t, fmaf(t, fmaf(t, fmaf(t, 1.061405429f, -1.453152027f), 1.421413741f), -0.284496736f), 0.254829592f);
+}
+__device__ __forceinline__ float norm_exp(float v) { return __builtin_amdgcn_exp2f(1.4426950408889634f * v); }
+
+template <int N>
+__device__ __forceinline__ void activate(int act, float (&z)[N]) {
+  switch (act) {  // (the same for all lanes)
+    case LINREC_ACT_RELU:
+#pragma unroll
+      for (int i = 0; i < N; ++i) z[i] = z[i] < 0.0f ? 0.0f : z[i];  // (NaN stays)
+      break;
+    case LINREC_ACT_SILU:
+#pragma unroll
+      for (int i = 0; i < N; ++i) z[i] *= __builtin_amdgcn_rcpf(1.0f + norm_exp(-z[i]));
+      break;
+    case LINREC_ACT_GELU:
+#pragma unroll
+      for (int i = 0; i < N; ++i) {
+        const float half = 0.5f * erfc_scaled(0.70710678118654752f * fabsf(z[i])) * norm_exp(-0.5f * z[i] * z[i]);
+        z[i] *= z[i] > 0.0f ? 1.0f - half : half;
+      }
+      break;
+    default: break;
+  }
+}
+// e[i] *= act'(z[i])
+template <int N>
+__device__ __forceinline__ void activate_slope(int act, const float (&z)[N], float (&e)[N]) {
+  switch (act) {
+    case LINREC_ACT_RELU:
+#pragma unroll
+      for (int i = 0; i < N; ++i) e[i] = z[i] > 0.0f ? e[i] : 0.0f * z[i] * e[i];
+      break;
+    case LINREC_ACT_SILU:
+#pragma unroll
+      for (int i = 0; i < N; ++i) {
+        const float s = __builtin_amdgcn_rcpf(1.0f + norm_exp(-z[i]));
+        e[i] *= s * fmaf(z[i], 1.0f - s, 1.0f);
+      }
+      break;
+    case LINREC_ACT_GELU:
+#pragma unroll
+      for (int i = 0; i < N; ++i) {
+        const float g = norm_exp(-0.5f * z[i] * z[i]);
+        const float half = 0.5f * erfc_scaled(0.70710678118654752f * fabsf(z[i])) * g;
+        e[i] *= fmaf(z[i], 0.39894228040143268f * g, z[i] > 0.0f ? 1.0f - half : half);
+      }
+      break;
+    default: break;
+  }
+}
+
+template <int VEC>
+__device__ __forceinline__ void load_params(const void* p, int dtype, int64_t c, float none, float (&out)[VEC]) {
+#pragma unroll
+  for (int e = 0; e < VEC; ++e)
+    out[e] = !p                              ? none
+             : dtype == LINREC_DTYPE_F32     ? static_cast<const float*>(p)[c + e]
+             : dtype == LINREC_DTYPE_F16     ? float(static_cast<const _Float16*>(p)[c + e])
+                                             : float(static_cast<const __bf16*>(p)[c + e]);
+}
+
+// ---- sums over the lanes of a team ------------------------------------------------------------
+template <int CTRL>
+__device__ __forceinline__ float dpp_add(float v) {
+  return v + __builtin_bit_cast(float, __builtin_amdgcn_mov_dpp(__builtin_bit_cast(int, v), CTRL, 0xf, 0xf, true));
+}
+// Sum over teams of `lanes` (a power of two) adjacent lanes, in all of them.
+__device__ __forceinline__ float team_sum(float v, int lanes) {
+  if (lanes > 1) v = dpp_add<0xb1>(v);   // quad_perm 1 0 3 2
+  if (lanes > 2) v = dpp_add<0x4e>(v);   // quad_perm 2 3 0 1
+  if (lanes > 4) v = dpp_add<0x141>(v);  // row_half_mirror: the other quad of eight
+  if (lanes > 8) v = dpp_add<0x140>(v);  // row_mirror: the other eight of a row
+  if (lanes > 16) {
+    const unsigned u = __builtin_bit_cast(unsigned, v);
+    const auto r = __builtin_amdgcn_permlane16_swap(u, u, false, false);
+    v = __builtin_bit_cast(float, unsigned(r[0])) + __builtin_bit_cast(float, unsigned(r[1]));
+  }
+  if (lanes > 32) {
+    const unsigned u = __builtin_bit_cast(unsigned, v);
+    const auto r = __builtin_amdgcn_permlane32_swap(u, u, false, false);
+    v = __builtin_bit_cast(float, unsigned(r[0])) + __builtin_bit_cast(float, unsigned(r[1]));
+  }
+  return v;
+}
+
+// ---- tokens: one position ---------------------------------------------------------------------
+constexpr int TOKEN_WAVES = 8;
+struct TokenArgs {
+  linrec_group_norm_t p;
+  int team;          // lanes of a group
+  int column_waves;  // waves of a workgroup side by side over the channels (a power of two), the others take other rows
+  int column_blocks;
+  int row_blocks;
+};
+
+template <typename T, int VEC, int ITEMS, bool BWD>
+__global__ __launch_bounds__(64 * TOKEN_WAVES) void norm_tokens_kernel(TokenArgs args) {
+  constexpr int N = VEC * ITEMS;
+  const linrec_group_norm_t& p = args.p;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int block = int(blockIdx.x % unsigned(args.column_blocks)), row_block = int(blockIdx.x / unsigned(args.column_blocks));
+  const int cw = wave & (args.column_waves - 1), row_slot = wave / args.column_waves, row_slots = TOKEN_WAVES / args.column_waves;
+  const int width = int(p.channels / p.groups);
+  const int64_t g = (int64_t(block) * args.column_waves + cw) * (64 / args.team) + lane / args.team;
+  const int in_team = lane & (args.team - 1);
+  const bool there = g < p.groups;
+  const int64_t c0 = (there ? g : 0) * width;
+  bool has[ITEMS];
+  int64_t c[ITEMS];
+  float w[N], b[N];
+#pragma unroll
+  for (int i = 0; i < ITEMS; ++i) {
+    const int o = (i * args.team + in_team) * VEC;  // (VEC divides the width: a slot lies in the group or not)
+    has[i] = there && o < width;
+    c[i] = c0 + (has[i] ? o : 0);
+    float wi[VEC], bi[VEC];
+    load_params<VEC>(p.weight, p.weight_dtype, c[i], 1.0f, wi);
+    load_params<VEC>(p.bias, p.weight_dtype, c[i], 0.0f, bi);
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) {
+      w[i * VEC + e] = wi[e];
+      b[i * VEC + e] = bi[e];
+    }
+  }
+  const int64_t step = int64_t(args.row_blocks) * row_slots;
+  const float inv_count = 1.0f / float(width);
+  const T* x = static_cast<const T*>(p.x);
+  const T* dy = static_cast<const T*>(p.d_y);
+  float dw[BWD ? N : 1], db[BWD ? N : 1];
+#pragma unroll
+  for (int i = 0; i < (BWD ? N : 1); ++i) dw[i] = db[i] = 0.0f;
+
+  Held<T, VEC> hx[ITEMS], hd[BWD ? ITEMS : 1];
+  float mean = 0.0f, rstd = 0.0f;
+  auto load = [&](int64_t n) __attribute__((always_inline)) {
+#pragma unroll
+    for (int i = 0; i < ITEMS; ++i) {
+      hx[i] = ld_any<VEC, true>(x + n * p.x_stride[0] + c[i]);
+      if constexpr (BWD) hd[i] = ld_any<VEC, true>(dy + n * p.d_y_stride[0] + c[i]);
+    }
+    if constexpr (BWD) {
+      mean = p.mean[n * p.groups + (there ? g : 0)];
+      rstd = p.rstd[n * p.groups + (there ? g : 0)];
+    }
+  };
+  int64_t n = int64_t(row_block) * row_slots + row_slot;
+  if (n < p.batch) load(n);
+  for (; n < p.batch; n += step) {
+    float v[N], d[BWD ? N : 1];
+    float m = mean, r = rstd;
+#pragma unroll
+    for (int i = 0; i < ITEMS; ++i) {
+      const Lanes<VEC> t = widen(hx[i]);
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) v[i * VEC + e] = t.v[e];
+      if constexpr (BWD) {
+        const Lanes<VEC> u = widen(hd[i]);
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) d[i * VEC + e] = u.v[e];
+      }
+    }
+    if (n + step < p.batch) load(n + step);  // (under way while this row is worked on)
+    if constexpr (!BWD) {
+      float s = 0.0f;
+#pragma unroll
+      for (int i = 0; i < N; ++i) s += has[i / VEC] ? v[i] : 0.0f;
+      m = team_sum(s, args.team) * inv_count;
+      s = 0.0f;
+#pragma unroll
+      for (int i = 0; i < N; ++i) {
+        v[i] -= m;
+        s = fmaf(has[i / VEC] ? v[i] : 0.0f, v[i], s);
+      }
+      r = __builtin_amdgcn_rsqf(fmaf(team_sum(s, args.team), inv_count, p.eps));
+      if (there && in_team == 0) {
+        p.mean[n * p.groups + g] = m;
+        p.rstd[n * p.groups + g] = r;
+      }
+#pragma unroll
+      for (int i = 0; i < N; ++i) v[i] = fmaf(v[i] * r, w[i], b[i]);
+      activate<N>(p.act, v);
+    } else {
+      float z[N], s1 = 0.0f, s2 = 0.0f;
+#pragma unroll
+      for (int i = 0; i < N; ++i) {
+        v[i] = (v[i] - m) * r;
+        z[i] = fmaf(v[i], w[i], b[i]);
+      }
+      activate_slope<N>(p.act, z, d);
+#pragma unroll
+      for (int i = 0; i < N; ++i) {
+        if (!has[i / VEC]) d[i] = v[i] = 0.0f;
+        dw[i] = fmaf(d[i], v[i], dw[i]);
+        db[i] += d[i];
+        d[i] *= w[i];
+        s1 += d[i];
+        s2 = fmaf(d[i], v[i], s2);
+      }
+      s1 = team_sum(s1, args.team) * inv_count;
+      s2 = team_sum(s2, args.team) * inv_count;
+#pragma unroll
+      for (int i = 0; i < N; ++i) v[i] = r * (d[i] - fmaf(v[i], s2, s1));
+    }
+    T* out = static_cast<T*>(BWD ? p.d_x : p.y) + n * p.channels;
+#pragma unroll
+    for (int i = 0; i < ITEMS; ++i) {
+      Lanes<VEC> t;
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) t.v[e] = v[i * VEC + e];
+      if (has[i]) st_any<VEC>(out + c[i], t);
+    }
+  }
+  if constexpr (BWD) {
+    if (!p.weight) return;
+    // the waves that had the same channels
+    __shared__ float sh[TOKEN_WAVES][64];
+    float* row = p.partial + int64_t(row_block) * 2 * p.channels;
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+#pragma unroll
+      for (int which = 0; which < 2; ++which) {
+        __syncthreads();
+        sh[wave][lane] = which ? dw[i] : db[i];
+        __syncthreads();
+        if (row_slot == 0 && has[i / VEC]) {
+          float s = sh[cw][lane];
+          for (int q = 1; q < row_slots; ++q) s += sh[q * args.column_waves + cw][lane];
+          row[which * p.channels + c[i / VEC] + i % VEC] = s;
+        }
+      }
+    }
+  }
+}
+
+// ---- held and chunks: the lanes of a workgroup over (row, batch item, column) --------------------
+// A column is a slot of VEC channels; a group is `per_group` columns.  A workgroup has `groups` whole groups of `items` batch
+// items side by side (or one of `parts` parts of one group's columns) and R rows of positions at a time.
+struct BlockArgs {
+  linrec_group_norm_t p;
+  int per_group;   // columns of a group (of a part of it)
+  int groups;      // of a workgroup
+  int items;       // batch items of a workgroup
+  int parts;       // workgroups that share a group's columns
+  int blocks;      // workgroups over the channels
+  int chunks;      // workgroups over the positions
+  int rows;        // positions of a chunk
+  int columns;     // items * groups * per_group: lanes of a row
+  int R;           // rows at a time
+  int whole;       // columns of a whole group
+};
+
+struct BlockLane {
+  int vc, r, q, g;  // column and row; column in its group; group of the workgroup (over all its items)
+  int64_t n, group, channel, first, end;  // batch item, group, first channel; positions of the chunk
+  bool there;
+};
+template <int VEC>
+__device__ __forceinline__ BlockLane block_lane(const BlockArgs& a) {
+  BlockLane l;
+  const int tid = int(threadIdx.x);
+  unsigned id = blockIdx.x;
+  const int chunk = int(id % unsigned(a.chunks));
+  id /= unsigned(a.chunks);
+  const int block = int(id % unsigned(a.blocks));
+  const int64_t item_block = id / unsigned(a.blocks);
+  l.r = tid / a.columns;
+  l.vc = tid - l.r * a.columns;
+  l.g = l.vc / a.per_group;
+  l.q = l.vc - l.g * a.per_group;
+  const int item = l.g / a.groups, g = l.g - item * a.groups;
+  const int part = block % a.parts;
+  l.n = item_block * a.items + item;
+  l.group = int64_t(block / a.parts) * a.groups + g;
+  const int column = part * a.per_group + l.q;
+  l.channel = (l.group * a.whole + column) * VEC;
+  l.there = l.r < a.R && l.n < a.p.batch && l.group < a.p.groups && column < a.whole;
+  l.first = int64_t(chunk) * a.rows + l.r;
+  l.end = int64_t(chunk + 1) * a.rows;
+  if (l.end > a.p.positions) l.end = a.p.positions;
+  return l;
+}
+
+// Tree over the rows: v of row 0 becomes the sum of its column.  sh: N * blockDim floats.
+template <int N>
+__device__ __forceinline__ void sum_rows(float (&v)[N], float* sh, const BlockArgs& a, const BlockLane& l) {
+  const int lanes = int(blockDim.x), tid = int(threadIdx.x);
+  if (a.R == 1) return;
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < N; ++i) sh[i * lanes + tid] = v[i];
+  int s = 1;
+  while (s < a.R) s <<= 1;
+  for (s >>= 1; s > 0; s >>= 1) {
+    __syncthreads();
+    if (l.r < s && l.r + s < a.R) {
+#pragma unroll
+      for (int i = 0; i < N; ++i) {
+        v[i] += sh[i * lanes + tid + s * a.columns];
+        sh[i * lanes + tid] = v[i];
+      }
+    }
+  }
+}
+// Tree over the columns of a group among the lanes of row 0; every lane gets its group's sum.
+template <int N>
+__device__ __forceinline__ void sum_group(float (&v)[N], float* sh, const BlockArgs& a, const BlockLane& l) {
+  const int lanes = int(blockDim.x), tid = int(threadIdx.x);
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < N; ++i) sh[i * lanes + tid] = v[i];
+  for (int s = 1; s < a.per_group; s <<= 1) {
+    __syncthreads();
+    if (l.r == 0 && (l.q & (2 * s - 1)) == 0 && l.q + s < a.per_group) {
+#pragma unroll
+      for (int i = 0; i < N; ++i) {
+        v[i] += sh[i * lanes + tid + s];
+        sh[i * lanes + tid] = v[i];
+      }
+    }
+  }
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < N; ++i) v[i] = sh[i * lanes + l.g * a.per_group];
+}
+
+struct Moments {
+  float count, mean, m2;
+};
+__device__ __forceinline__ Moments merge(Moments a, Moments b) {
+  if (b.count == 0.0f) return a;
+  if (a.count == 0.0f) return b;
+  const float n = a.count + b.count, f = b.count / n, d = b.mean - a.mean;
+  return {n, fmaf(d, f, a.mean), fmaf(d * d, a.count * f, a.m2 + b.m2)};
+}
+// The moments of all lanes of a group, in all of them.  sh: 3 * blockDim floats.
+__device__ __forceinline__ Moments merge_group(Moments v, float* sh, const BlockArgs& a, const BlockLane& l) {
+  const int lanes = int(blockDim.x), tid = int(threadIdx.x);
+  auto put = [&](const Moments& m) {
+    sh[tid] = m.count;
+    sh[lanes + tid] = m.mean;
+    sh[2 * lanes + tid] = m.m2;
+  };
+  auto get = [&](int i) { return Moments{sh[i], sh[lanes + i], sh[2 * lanes + i]}; };
+  __syncthreads();
+  put(v);
+  int s = 1;
+  while (s < a.R) s <<= 1;
+  for (s >>= 1; s > 0; s >>= 1) {
+    __syncthreads();
+    if (l.r < s && l.r + s < a.R) put(v = merge(v, get(tid + s * a.columns)));
+  }
+  for (s = 1; s < a.per_group; s <<= 1) {
+    __syncthreads();
+    if (l.r == 0 && (l.q & (2 * s - 1)) == 0 && l.q + s < a.per_group) put(v = merge(v, get(tid + s)));
+  }
+  __syncthreads();
+  return get(l.g * a.per_group);
+}
+
+// Where a workgroup's part of a group's statistics lies, and the values of one.
+__device__ __forceinline__ int64_t piece_index(const BlockArgs& a, int64_t n, int64_t group, int64_t piece) {
+  return ((n * a.chunks * a.parts + piece) * a.p.groups + group) * 2;
+}
+
+constexpr int NORM_HELD = 0, NORM_STATS = 1, NORM_APPLY = 2;
+template <int VEC, typename T>
+constexpr int held_rows() {  // of a lane: 32 registers' worth of one tensor
+  return 32 / (VEC * int(sizeof(T)) >= 4 ? VEC * int(sizeof(T)) / 4 : 1);
+}
+
+template <typename T, int VEC, int LANES, int PHASE>
+__global__ __launch_bounds__(LANES) void norm_fwd_kernel(BlockArgs args) {
+  constexpr int KEEP = held_rows<VEC, T>();
+  __shared__ float sh[(PHASE == NORM_HELD ? 1 : 3) * LANES];
+  const linrec_group_norm_t& p = args.p;
+  const BlockLane l = block_lane<VEC>(args);
+  const T* x = static_cast<const T*>(p.x) + l.n * p.x_stride[0] + l.channel;
+  T* y = static_cast<T*>(p.y) + l.n * p.positions * p.channels + l.channel;
+  float w[VEC], b[VEC];
+  if (PHASE != NORM_STATS && l.there) {
+    load_params<VEC>(p.weight, p.weight_dtype, l.channel, 1.0f, w);
+    load_params<VEC>(p.bias, p.weight_dtype, l.channel, 0.0f, b);
+  }
+  float mean, rstd;
+  auto apply = [&](const Held<T, VEC>& h, int64_t pos) __attribute__((always_inline)) {
+    Lanes<VEC> v = widen(h);
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) v.v[e] = fmaf((v.v[e] - mean) * rstd, w[e], b[e]);
+    activate<VEC>(p.act, v.v);
+    st_any<VEC>(y + pos * p.channels, v);
+  };
+  const bool writes = l.there && l.r == 0 && l.q == 0 && (PHASE != NORM_APPLY || (l.first == 0 && l.channel == l.group * args.whole * VEC));
+
+  if constexpr (PHASE == NORM_HELD) {
+    Held<T, VEC> held[KEEP];
+    float s[1] = {0.0f};
+#pragma unroll
+    for (int i = 0; i < KEEP; ++i) {
+      const int64_t pos = l.first + i * args.R;
+      if (l.there && pos < l.end) held[i] = ld_any<VEC, true>(x + pos * p.x_stride[1]);
+    }
+#pragma unroll
+    for (int i = 0; i < KEEP; ++i)
+      if (l.there && l.first + i * args.R < l.end) {
+        const Lanes<VEC> v = widen(held[i]);
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) s[0] += v.v[e];
+      }
+    const float inv_count = 1.0f / (float(p.positions) * float(args.whole * VEC));
+    sum_rows<1>(s, sh, args, l);
+    sum_group<1>(s, sh, args, l);
+    mean = s[0] * inv_count;
+    s[0] = 0.0f;
+#pragma unroll
+    for (int i = 0; i < KEEP; ++i)
+      if (l.there && l.first + i * args.R < l.end) {
+        const Lanes<VEC> v = widen(held[i]);
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) {
+          const float d = v.v[e] - mean;
+          s[0] = fmaf(d, d, s[0]);
+        }
+      }
+    sum_rows<1>(s, sh, args, l);
+    sum_group<1>(s, sh, args, l);
+    rstd = __builtin_amdgcn_rsqf(fmaf(s[0], inv_count, p.eps));
+#pragma unroll
+    for (int i = 0; i < KEEP; ++i)
+      if (l.there && l.first + i * args.R < l.end) apply(held[i], l.first + i * args.R);
+  } else if constexpr (PHASE == NORM_STATS) {
+    Moments m{0.0f, 0.0f, 0.0f};
+    if (l.there && l.first < l.end) {
+      const float shift = float(x[l.first * p.x_stride[1]]);
+      float s = 0.0f, s2 = 0.0f, count = 0.0f;
+      for (int64_t pos = l.first; pos < l.end; pos += 4 * args.R) {
+        Held<T, VEC> h[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          if (pos + i * args.R < l.end) h[i] = ld_any<VEC, false>(x + (pos + i * args.R) * p.x_stride[1]);
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          if (pos + i * args.R < l.end) {
+            const Lanes<VEC> v = widen(h[i]);
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) {
+              const float d = v.v[e] - shift;
+              s += d;
+              s2 = fmaf(d, d, s2);
+            }
+            count += float(VEC);
+          }
+      }
+      const float off = s / count;
+      m = {count, shift + off, fmaxf(fmaf(-off, s, s2), s2 != s2 ? s2 : 0.0f)};
+    }
+    m = merge_group(m, sh, args, l);
+    if (writes) {
+      const int64_t piece = int64_t(blockIdx.x % unsigned(args.chunks)) * args.parts + (blockIdx.x / unsigned(args.chunks)) % unsigned(args.blocks) % unsigned(args.parts);
+      float* out = p.partial + piece_index(args, l.n, l.group, piece);
+      out[0] = m.mean;
+      out[1] = m.m2;
+    }
+    return;
+  } else {
+    // the lanes of a group share its pieces out
+    Moments m{0.0f, 0.0f, 0.0f};
+    const int pieces = args.chunks * args.parts;
+    if (l.there) {
+      for (int i = l.r * args.per_group + l.q; i < pieces; i += args.R * args.per_group) {
+        const int chunk = i / args.parts, part = i - chunk * args.parts;
+        const int64_t first = int64_t(chunk) * args.rows, rows = first + args.rows < p.positions ? args.rows : p.positions - first;
+        const int columns = (part + 1) * args.per_group < args.whole ? args.per_group : args.whole - part * args.per_group;
+        const float* in = p.partial + piece_index(args, l.n, l.group, i);
+        m = merge(m, {float(rows) * float(columns * VEC), in[0], in[1]});
+      }
+    }
+    m = merge_group(m, sh, args, l);
+    mean = m.mean;
+    rstd = __builtin_amdgcn_rsqf(m.m2 / m.count + p.eps);
+    if (l.there)
+      for (int64_t pos = l.first; pos < l.end; pos += 4 * args.R) {
+        Held<T, VEC> h[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          if (pos + i * args.R < l.end) h[i] = ld_any<VEC, false>(x + (pos + i * args.R) * p.x_stride[1]);
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          if (pos + i * args.R < l.end) apply(h[i], pos + i * args.R);
+      }
+  }
+  if (writes) {
+    p.mean[l.n * p.groups + l.group] = mean;
+    p.rstd[l.n * p.groups + l.group] = rstd;
+  }
+}
+
+// PARTIAL layout of the backward: the pieces' sums (chunks only), then a row of 2 * channels sums for every (item block, chunk).
+template <typename T, int VEC, int LANES, int PHASE>
+__global__ __launch_bounds__(LANES) void norm_bwd_kernel(BlockArgs args, float* param_sums) {
+  constexpr int KEEP = held_rows<VEC, T>();
+  __shared__ float sh[(PHASE == NORM_APPLY ? 2 : 2 * VEC) * LANES];
+  const linrec_group_norm_t& p = args.p;
+  const BlockLane l = block_lane<VEC>(args);
+  const T* x = static_cast<const T*>(p.x) + l.n * p.x_stride[0] + l.channel;
+  const T* dy = static_cast<const T*>(p.d_y) + l.n * p.d_y_stride[0] + l.channel;
+  T* dx = static_cast<T*>(p.d_x) + l.n * p.positions * p.channels + l.channel;
+  float w[VEC], b[VEC];
+  float mean = 0.0f, rstd = 0.0f;
+  if (l.there) {
+    load_params<VEC>(p.weight, p.weight_dtype, l.channel, 1.0f, w);
+    load_params<VEC>(p.bias, p.weight_dtype, l.channel, 0.0f, b);
+    mean = p.mean[l.n * p.groups + l.group];
+    rstd = p.rstd[l.n * p.groups + l.group];
+  }
+  // xh and e of one slot
+  auto expand = [&](const Held<T, VEC>& hx, const Held<T, VEC>& hd, float (&xh)[VEC], float (&e)[VEC]) __attribute__((always_inline)) {
+    const Lanes<VEC> vx = widen(hx), vd = widen(hd);
+    float z[VEC];
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) {
+      xh[i] = (vx.v[i] - mean) * rstd;
+      z[i] = fmaf(xh[i], w[i], b[i]);
+      e[i] = vd.v[i];
+    }
+    activate_slope<VEC>(p.act, z, e);
+  };
+  float sums[2 * VEC], s[2] = {0.0f, 0.0f};
+#pragma unroll
+  for (int i = 0; i < 2 * VEC; ++i) sums[i] = 0.0f;
+  auto add = [&](const Held<T, VEC>& hx, const Held<T, VEC>& hd) __attribute__((always_inline)) {
+    float xh[VEC], e[VEC];
+    expand(hx, hd, xh, e);
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) {
+      sums[i] += e[i];
+      sums[VEC + i] = fmaf(e[i], xh[i], sums[VEC + i]);
+    }
+  };
+  auto apply = [&](const Held<T, VEC>& hx, const Held<T, VEC>& hd, int64_t pos) __attribute__((always_inline)) {
+    float xh[VEC], e[VEC];
+    expand(hx, hd, xh, e);
+    Lanes<VEC> out;
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) out.v[i] = rstd * (fmaf(e[i], w[i], -s[0]) - xh[i] * s[1]);
+    st_any<VEC>(dx + pos * p.channels, out);
+  };
+  // the columns' sums, from there those of d_weight and d_bias and the group's
+  auto finish_sums = [&]() __attribute__((always_inline)) {
+    sum_rows<2 * VEC>(sums, sh, args, l);
+    if (l.there && l.r == 0) {
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) {
+        s[0] = fmaf(sums[i], w[i], s[0]);
+        s[1] = fmaf(sums[VEC + i], w[i], s[1]);
+      }
+    }
+    if (p.weight) {
+      __syncthreads();
+      if (l.r == 0) {
+#pragma unroll
+        for (int i = 0; i < 2 * VEC; ++i) sh[i * LANES + l.vc] = l.there ? sums[i] : 0.0f;
+      }
+      __syncthreads();
+      const int width = args.groups * args.per_group;
+      if (l.there && l.r == 0 && l.vc < width) {  // (the lanes of the first batch item)
+#pragma unroll
+        for (int i = 0; i < 2 * VEC; ++i) {
+          float t = sh[i * LANES + l.vc];
+          for (int q = 1; q < args.items; ++q) t += sh[i * LANES + q * width + l.vc];
+          const unsigned id = blockIdx.x;
+          const int64_t row = int64_t(id / unsigned(args.chunks) / unsigned(args.blocks)) * args.chunks + id % unsigned(args.chunks);
+          param_sums[(row * 2 + i / VEC) * p.channels + l.channel + i % VEC] = t;
+        }
+      }
+    }
+    sum_group<2>(s, sh, args, l);
+  };
+  const float inv_count = 1.0f / (float(p.positions) * float(args.whole * VEC));
+
+  if constexpr (PHASE == NORM_HELD) {
+    Held<T, VEC> hx[KEEP], hd[KEEP];
+#pragma unroll
+    for (int i = 0; i < KEEP; ++i) {
+      const int64_t pos = l.first + i * args.R;
+      if (l.there && pos < l.end) {
+        hx[i] = ld_any<VEC, true>(x + pos * p.x_stride[1]);
+        hd[i] = ld_any<VEC, true>(dy + pos * p.d_y_stride[1]);
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < KEEP; ++i)
+      if (l.there && l.first + i * args.R < l.end) add(hx[i], hd[i]);
+    finish_sums();
+    s[0] *= inv_count;
+    s[1] *= inv_count;
+#pragma unroll
+    for (int i = 0; i < KEEP; ++i)
+      if (l.there && l.first + i * args.R < l.end) apply(hx[i], hd[i], l.first + i * args.R);
+  } else {
+    auto walk = [&](auto&& f) __attribute__((always_inline)) {
+      if (!l.there) return;
+      for (int64_t pos = l.first; pos < l.end; pos += 2 * args.R) {
+        Held<T, VEC> hx[2], hd[2];
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+          if (pos + i * args.R < l.end) {
+            hx[i] = ld_any<VEC, false>(x + (pos + i * args.R) * p.x_stride[1]);
+            hd[i] = ld_any<VEC, false>(dy + (pos + i * args.R) * p.d_y_stride[1]);
+          }
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+          if (pos + i * args.R < l.end) f(hx[i], hd[i], pos + i * args.R);
+      }
+    };
+    if constexpr (PHASE == NORM_STATS) {
+      walk([&](const Held<T, VEC>& hx, const Held<T, VEC>& hd, int64_t) { add(hx, hd); });
+      finish_sums();
+      if (l.there && l.r == 0 && l.q == 0) {
+        const int64_t piece = int64_t(blockIdx.x % unsigned(args.chunks)) * args.parts + (blockIdx.x / unsigned(args.chunks)) % unsigned(args.blocks) % unsigned(args.parts);
+        float* out = p.partial + piece_index(args, l.n, l.group, piece);
+        out[0] = s[0];
+        out[1] = s[1];
+      }
+    } else {
+      const int pieces = args.chunks * args.parts;
+      if (l.there) {
+        for (int i = l.r * args.per_group + l.q; i < pieces; i += args.R * args.per_group) {
+          const float* in = p.partial + piece_index(args, l.n, l.group, i);
+          s[0] += in[0];
+          s[1] += in[1];
+        }
+      }
+      sum_rows<2>(s, sh, args, l);
+      sum_group<2>(s, sh, args, l);
+      s[0] *= inv_count;
+      s[1] *= inv_count;
+      walk([&](const Held<T, VEC>& hx, const Held<T, VEC>& hd, int64_t pos) { apply(hx, hd, pos); });
+    }
+  }
+}
+
+}  // namespace linrec

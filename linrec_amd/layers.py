@@ -14,17 +14,24 @@ from . import _layers
 __all__ = ["gated_linrec", "gated_linrec_step", "group_norm_act", "embedding"]
 
 Tensor = torch.Tensor
-_PLAIN = (torch.Tensor, torch.nn.Parameter)
+_PLAIN = (torch.Tensor, torch.nn.Parameter)  # (subclasses, fake ones among them, take the registered operators)
 
 
 def _traced(*tensors):
     """The call has to go through the registered operator: compilation, tracing, a tensor subclass or a function transform."""
-    return (torch.compiler.is_compiling() or any(t is not None and type(t) not in _PLAIN for t in tensors)
-            or torch._C._are_functorch_transforms_active() or torch._C._get_tracing_state() is not None)
+    for t in tensors:
+        if t is not None and type(t) not in _PLAIN:
+            return True
+    return (torch.compiler.is_compiling() or torch._C._are_functorch_transforms_active()
+            or torch._C._get_tracing_state() is not None)
 
 
 def _recorded(*tensors):
-    return (torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)) or forward_ad._current_level >= 0
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t is not None and t.requires_grad:
+                return True
+    return forward_ad._current_level >= 0
 
 
 # ---- gated linear recurrence -------------------------------------------------------------------
@@ -139,38 +146,37 @@ def gated_linrec_step(x: Tensor, gate_a: Tensor, gate_x: Tensor, rate: Tensor, s
 # ---- group norm with an activation -------------------------------------------------------------
 @torch.library.custom_op("linrec_amd::group_norm_act_fwd", mutates_args=(), device_types="cuda")
 def group_norm_act_fwd(x: Tensor, groups: int, weight: Optional[Tensor], bias: Optional[Tensor], eps: float,
-                       act: str) -> Tuple[Tensor, Tensor, Tensor]:
+                       act: str) -> Tuple[Tensor, Tensor]:
     return _layers.norm_fwd(x, groups, weight, bias, eps, act)
 
 
 @torch.library.custom_op("linrec_amd::group_norm_act_bwd", mutates_args=(), device_types="cuda")
-def group_norm_act_bwd(d_y: Tensor, x: Tensor, groups: int, weight: Optional[Tensor], bias: Optional[Tensor], mean: Tensor,
-                       rstd: Tensor, eps: float, act: str) -> Tuple[Tensor, Tensor, Tensor]:
-    d_x, d_weight, d_bias = _layers.norm_bwd(d_y, x, groups, weight, bias, mean, rstd, eps, act)
-    return (d_x, mean.new_empty(0), mean.new_empty(0)) if weight is None else (d_x, d_weight, d_bias)
+def group_norm_act_bwd(d_y: Tensor, x: Tensor, groups: int, weight: Optional[Tensor], bias: Optional[Tensor], stats: Tensor,
+                       eps: float, act: str) -> Tuple[Tensor, Tensor, Tensor]:
+    d_x, d_weight, d_bias = _layers.norm_bwd(d_y, x, groups, weight, bias, stats, eps, act)
+    return (d_x, stats.new_empty(0), stats.new_empty(0)) if weight is None else (d_x, d_weight, d_bias)
 
 
 @group_norm_act_fwd.register_fake
 def _(x, groups, weight, bias, eps, act):
     torch._check(x.dim() >= 2 and x.size(-1) % groups == 0, lambda: "group_norm_act: channels cannot be cut into groups")
-    stats = [x.new_empty((x.size(0), groups), dtype=torch.float32) for _ in range(2)]
-    return (x.new_empty(x.size()), *stats)
+    return x.new_empty(x.size()), x.new_empty((2, x.size(0), groups), dtype=torch.float32)
 
 
 @group_norm_act_bwd.register_fake
-def _(d_y, x, groups, weight, bias, mean, rstd, eps, act):
-    params = [mean.new_empty(0) if weight is None else weight.new_empty(weight.size()) for _ in range(2)]
+def _(d_y, x, groups, weight, bias, stats, eps, act):
+    params = [stats.new_empty(0) if weight is None else weight.new_empty(weight.size()) for _ in range(2)]
     return (x.new_empty(x.size()), *params)
 
 
 def _norm_setup(ctx, inputs, output):
     x, ctx.groups, weight, bias, ctx.eps, ctx.act = inputs
-    ctx.save_for_backward(x, weight, bias, output[1], output[2])
+    ctx.save_for_backward(x, weight, bias, output[1])
 
 
-def _norm_backward(ctx, d_y, _, __):
-    x, weight, bias, mean, rstd = ctx.saved_tensors
-    d_x, d_weight, d_bias = group_norm_act_bwd(d_y, x, ctx.groups, weight, bias, mean, rstd, ctx.eps, ctx.act)
+def _norm_backward(ctx, d_y, _):
+    x, weight, bias, stats = ctx.saved_tensors
+    d_x, d_weight, d_bias = group_norm_act_bwd(d_y, x, ctx.groups, weight, bias, stats, ctx.eps, ctx.act)
     if weight is None:
         d_weight = d_bias = None
     return d_x, None, d_weight, d_bias, None, None
@@ -182,16 +188,16 @@ torch.library.register_autograd("linrec_amd::group_norm_act_fwd", _norm_backward
 class _NormFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, groups, weight, bias, eps, act):
-        y, mean, rstd = _layers.norm_fwd(x, groups, weight, bias, eps, act)
-        ctx.save_for_backward(x, weight, bias, mean, rstd)
+        y, stats = _layers.norm_fwd(x, groups, weight, bias, eps, act)
+        ctx.save_for_backward(x, weight, bias, stats)
         ctx.groups, ctx.eps, ctx.act = groups, eps, act
         return y
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, d_y):
-        x, weight, bias, mean, rstd = ctx.saved_tensors
-        d_x, d_weight, d_bias = _layers.norm_bwd(d_y, x, ctx.groups, weight, bias, mean, rstd, ctx.eps, ctx.act)
+        x, weight, bias, stats = ctx.saved_tensors
+        d_x, d_weight, d_bias = _layers.norm_bwd(d_y, x, ctx.groups, weight, bias, stats, ctx.eps, ctx.act)
         return d_x, None, d_weight, d_bias, None, None
 
 

@@ -64,8 +64,8 @@ typedef struct linrec_gated {
   void* stream;
 } linrec_gated_t;
 
-int64_t linrec_gated_saved_floats(int64_t batch, int64_t time, int64_t channels);
-int64_t linrec_gated_partial_floats(int64_t batch, int64_t time, int64_t channels);
+int64_t linrec_gated_saved_floats(int dtype, int64_t batch, int64_t time, int64_t channels);
+int64_t linrec_gated_partial_floats(int dtype, int64_t batch, int64_t time, int64_t channels);
 size_t linrec_gated_workspace_bytes(int dtype, int64_t batch, int64_t time, int64_t channels, int is_bwd);
 int linrec_gated_fwd(const linrec_gated_t* args);
 int linrec_gated_bwd(const linrec_gated_t* args);

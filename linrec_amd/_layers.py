@@ -52,8 +52,8 @@ class Embedding(ctypes.Structure):
 
 
 EXPORTS = {
-    "linrec_gated_saved_floats": (_i64, [_i64] * 3),
-    "linrec_gated_partial_floats": (_i64, [_i64] * 3),
+    "linrec_gated_saved_floats": (_i64, [ctypes.c_int] + [_i64] * 3),
+    "linrec_gated_partial_floats": (_i64, [ctypes.c_int] + [_i64] * 3),
     "linrec_gated_workspace_bytes": (ctypes.c_size_t, [ctypes.c_int, _i64, _i64, _i64, ctypes.c_int]),
     "linrec_gated_fwd": (ctypes.c_int, [ctypes.POINTER(Gated)]),
     "linrec_gated_bwd": (ctypes.c_int, [ctypes.POINTER(Gated)]),
@@ -216,8 +216,8 @@ def _with_adjacent_channels(*tensors):
     return [t if _adjacent_channels(t) else t.contiguous() for t in tensors]
 
 
-def gated_saved_numel(batch, time, channels):
-    return _lib.linrec_gated_saved_floats(batch, time, channels)
+def gated_saved_numel(dtype, batch, time, channels):
+    return _lib.linrec_gated_saved_floats(DTYPES[dtype], batch, time, channels)
 
 
 def gated_fwd(x, gate_a, gate_x, rate, h0, cu_seqlens, reverse, scale, save):
@@ -229,7 +229,7 @@ def gated_fwd(x, gate_a, gate_x, rate, h0, cu_seqlens, reverse, scale, save):
         a = _gated_args(x, gate_a, gate_x, rate, h0, cu_seqlens, reverse, scale)
         e = _remember(key, _Entry() if a is None else _Entry(
             a, _lib.linrec_gated_workspace_bytes(a.dtype, a.batch, a.time, a.channels, 0),
-            ((a.sequences, a.channels), gated_saved_numel(a.batch, a.time, a.channels))))
+            ((a.sequences, a.channels), gated_saved_numel(x.dtype, a.batch, a.time, a.channels))))
     a = e.args
     if a is None:
         return gated_fwd(*_with_adjacent_channels(x, gate_a, gate_x), *_dense(rate, h0, cu_seqlens), reverse, scale, save)
@@ -261,7 +261,7 @@ def gated_bwd(d_h, d_state, x, gate_a, gate_x, rate, h0, cu_seqlens, saved, reve
         else:
             a.d_h_stride = _time_strides(d_h)
             e = _Entry(a, _lib.linrec_gated_workspace_bytes(a.dtype, a.batch, a.time, a.channels, 1),
-                       (_lib.linrec_gated_partial_floats(a.batch, a.time, a.channels),))
+                       (_lib.linrec_gated_partial_floats(a.dtype, a.batch, a.time, a.channels),))
         _remember(key, e)
     a = e.args
     if a is None:

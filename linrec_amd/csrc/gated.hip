@@ -81,18 +81,23 @@ int check_gated(const linrec_gated_t* p) {
 
 // Channels of a lane: 4 bytes' worth, one where there are no two.
 int lane_width(int dtype, int64_t channels) { return dtype == LINREC_DTYPE_F32 || channels < 2 ? 1 : 2; }
-constexpr int kFwdRun = 16, kBwdRun = 8, kWaves = 8;
 
+constexpr int kFwdRun = 16, kFwdWaves = 4, kBwdRun = 8;
+template <typename T>
+constexpr int kBwdWaves = sizeof(T) == 4 ? 8 : 4;
 struct Geometry {
   int64_t segments, channel_blocks, grid, tiles;
+  int save;
 };
 Geometry geometry(int dtype, int64_t batch, int64_t time, int64_t channels, bool bwd) {
   Geometry g;
   const int64_t rows = 64 * lane_width(dtype, channels);
-  g.segments = cdiv(time, kWaves * (bwd ? kBwdRun : kFwdRun));
   g.channel_blocks = cdiv(channels, rows);
-  g.grid = g.segments * g.channel_blocks * batch;
-  g.tiles = g.grid * rows;
+  const int64_t blocks = g.channel_blocks * batch;
+  g.save = kBwdRun * (dtype == LINREC_DTYPE_F32 ? kBwdWaves<float> : kBwdWaves<__bf16>);
+  g.segments = cdiv(time, bwd ? g.save : kFwdWaves * kFwdRun);
+  g.grid = g.segments * blocks;
+  g.tiles = (g.segments + cdiv(g.segments, GROUP)) * blocks * rows;  // places of words
   return g;
 }
 
@@ -101,6 +106,7 @@ int fill_args(const linrec_gated_t* p, const Geometry& g, GatedArgs* a) {
   a->chain = TileArgs{};
   a->segments = int(g.segments);
   a->channel_blocks = int(g.channel_blocks);
+  a->save = g.save;
   if (g.grid > 2147483647LL) return LINREC_E_TOO_LARGE;
   if (g.segments <= 1) return LINREC_OK;
   if (!p->workspace || (reinterpret_cast<uintptr_t>(p->workspace) & 15u)) return LINREC_E_WORKSPACE;
@@ -115,21 +121,20 @@ int fill_args(const linrec_gated_t* p, const Geometry& g, GatedArgs* a) {
   return LINREC_OK;
 }
 
-template <typename T, int VEC>
+template <typename T, int VEC, bool PACKED>
 int launch_pass(const GatedArgs& a, const Geometry& g, bool bwd) {
-  const bool packed = a.p.cu_seqlens != nullptr;
-  auto kernel = bwd ? (packed ? gated_bwd_kernel<T, VEC, kBwdRun, kWaves, true> : gated_bwd_kernel<T, VEC, kBwdRun, kWaves, false>)
-                    : (packed ? gated_fwd_kernel<T, VEC, kFwdRun, kWaves, true> : gated_fwd_kernel<T, VEC, kFwdRun, kWaves, false>);
-  return launch_kernel(kernel, g.grid, 1, 64 * kWaves, a.p.stream, a);
+  return bwd ? launch_kernel(gated_bwd_kernel<T, VEC, kBwdRun, kBwdWaves<T>, PACKED>, g.grid, 1, 64 * kBwdWaves<T>, a.p.stream, a)
+             : launch_kernel(gated_fwd_kernel<T, VEC, kFwdRun, kFwdWaves, PACKED>, g.grid, 1, 64 * kFwdWaves, a.p.stream, a);
 }
 
 int launch_pass(const GatedArgs& a, const Geometry& g, bool bwd) {
   return with_dtype(a.p.dtype, [&](auto t) {
     using T = decltype(t);
+    const bool packed = a.p.cu_seqlens != nullptr;
     if constexpr (sizeof(T) == 2) {
-      if (lane_width(a.p.dtype, a.p.channels) == 2) return launch_pass<T, 2>(a, g, bwd);
+      if (lane_width(a.p.dtype, a.p.channels) == 2) return packed ? launch_pass<T, 2, true>(a, g, bwd) : launch_pass<T, 2, false>(a, g, bwd);
     }
-    return launch_pass<T, 1>(a, g, bwd);
+    return packed ? launch_pass<T, 1, true>(a, g, bwd) : launch_pass<T, 1, false>(a, g, bwd);
   });
 }
 
@@ -140,11 +145,15 @@ using namespace linrec;
 
 extern "C" {
 
-int64_t linrec_gated_saved_floats(int64_t batch, int64_t time, int64_t channels) { return batch * cdiv(time, GATED_SAVE) * channels; }
+int64_t linrec_gated_saved_floats(int dtype, int64_t batch, int64_t time, int64_t channels) {
+  if (batch <= 0 || time <= 0 || channels <= 0) return 0;
+  return batch * geometry(dtype, batch, time, channels, true).segments * channels;
+}
 
 // a row for every backward segment, and the sums of their chunks
-int64_t linrec_gated_partial_floats(int64_t batch, int64_t time, int64_t channels) {
-  const int64_t rows = batch * cdiv(time, GATED_SAVE), chunks = column_sum_chunks(rows);
+int64_t linrec_gated_partial_floats(int dtype, int64_t batch, int64_t time, int64_t channels) {
+  if (batch <= 0 || time <= 0 || channels <= 0) return 0;
+  const int64_t rows = batch * geometry(dtype, batch, time, channels, true).segments, chunks = column_sum_chunks(rows);
   return (rows + (chunks > 1 ? chunks : 0)) * channels;
 }
 

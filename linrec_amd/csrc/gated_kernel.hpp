@@ -34,13 +34,13 @@
 
 namespace linrec {
 
-constexpr int GATED_SAVE = 64;  // positions from one saved value to the next, and of a backward segment
 
 struct GatedArgs {
   linrec_gated_t p;
   TileArgs chain;
   int segments;         // of the scan axis
   int channel_blocks;
+  int save;             // positions from one saved value to the next: those of a backward segment
 };
 
 // ---- arithmetic -------------------------------------------------------------------------------
@@ -57,26 +57,22 @@ __device__ __forceinline__ float fast_softplus(float v) {
   const float l = d == 0.0f ? e : LN2 * __builtin_amdgcn_logf(w) * e * __builtin_amdgcn_rcpf(d);
   return (v > 0.0f ? v : 0.0f) + (v != v ? v : l);
 }
-// 1 - exp(u) for u <= 0: the difference cancels where u is small, the series of seven terms is off by 5e-8 of the result at 1/4.
-__device__ __forceinline__ float one_minus_exp(float u, float exp_u) {
-  const float s = fmaf(u, fmaf(u, fmaf(u, fmaf(u, fmaf(u, 1.0f / 720.0f, 1.0f / 120.0f), 1.0f / 24.0f), 1.0f / 6.0f), 0.5f), 1.0f);
-  return u > -0.25f ? -u * s : 1.0f - exp_u;
-}
-
 struct Gate {
-  float sa, sx;   // sigmoids
-  float log2_a;   // log a in base 2
+  float sa, sx;  // sigmoids
   float a;
-  float m2;       // 1 - a^2
+  float m2;      // 1 - a^2
 };
-// decay2: the decay rate in base 2
+// decay2: the decay rate in base 2.  1 - a^2 = 1 - exp(u), u = 2 log a: the difference cancels where u is small, and six terms of
+// the series are off by 4e-8 of the result at u = -1/8 (in l = log2 a: the coefficients are (2 ln 2)^n / n!).
 __device__ __forceinline__ Gate gate_of(float ga, float gx, float decay2) {
+  constexpr float C1 = 2.0f * LN2, C2 = C1 * C1 / 2.0f, C3 = C2 * C1 / 3.0f, C4 = C3 * C1 / 4.0f, C5 = C4 * C1 / 5.0f, C6 = C5 * C1 / 6.0f;
   Gate g;
   g.sa = fast_sigmoid(ga);
   g.sx = fast_sigmoid(gx);
-  g.log2_a = -decay2 * g.sa;
-  g.a = __builtin_amdgcn_exp2f(g.log2_a);
-  g.m2 = one_minus_exp(2.0f * LN2 * g.log2_a, g.a * g.a);
+  const float l = -decay2 * g.sa;
+  g.a = __builtin_amdgcn_exp2f(l);
+  const float series = -l * fmaf(l, fmaf(l, fmaf(l, fmaf(l, fmaf(l, C6, C5), C4), C3), C2), C1);
+  g.m2 = l > -0.125f / C1 ? series : fmaf(-g.a, g.a, 1.0f);
   return g;
 }
 __device__ __forceinline__ float taken_in(const Gate& g, float x) { return __builtin_amdgcn_sqrtf(g.m2) * g.sx * x; }
@@ -139,6 +135,13 @@ __device__ __forceinline__ void mark_segment(SegmentMarks<SEG>& m, const linrec_
     }
   }
 }
+template <int SEG>
+__device__ __forceinline__ bool any_mark(const SegmentMarks<SEG>& m) {  // (the same for all lanes)
+  unsigned bits = 0;
+#pragma unroll
+  for (int i = 0; i < (SEG + 31) / 32; ++i) bits |= m.starts[i] | m.ends[i];
+  return __builtin_amdgcn_readfirstlane(int(bits)) != 0;
+}
 template <int U>
 __device__ __forceinline__ unsigned run_bits(const unsigned* mask, int run) {  // of positions run * U .. run * U + U - 1
   static_assert(32 % U == 0, "a run lies in one word");
@@ -177,14 +180,19 @@ __device__ __forceinline__ Channels<VEC> lane_channels(int block, int lane, int 
   ch.whole = c0 + 64 * VEC <= channels;
   return ch;
 }
-template <int VEC, typename T>
+// WHOLE: every lane of the block stores all its channels.
+template <bool WHOLE, int VEC, typename T>
 __device__ __forceinline__ void store_channels(T* p, const Lanes<VEC>& v, const Channels<VEC>& ch) {
-  if (ch.whole) {
+  if constexpr (WHOLE) {
     st_any<VEC>(p, v);
   } else {
+    if (ch.own == 0) {
+      st_any<VEC>(p, v);
+    } else {
 #pragma unroll
-    for (int e = 0; e < VEC; ++e)
-      if (e >= ch.own) p[e] = T(v.v[e]);
+      for (int e = 1; e < VEC; ++e)
+        if (e >= ch.own) p[e] = T(v.v[e]);
+    }
   }
 }
 template <int VEC>
@@ -207,115 +215,208 @@ __device__ __forceinline__ P* plus_bytes(P* p, uint32_t bytes) {
 }
 
 // ---- the chain of segments --------------------------------------------------------------------
-// One wave, a channel to a lane: publishes the map (ta, tb) of segment k (in scan order), waits for what enters it and
-// publishes what leaves it.  `cut`: a sequence starts inside, so tb leaves whatever enters.  `walk` computes what enters from
-// the channel's own data.  mine: this segment's first word of the lane; a segment's words lie `per_segment` from the next one's,
-// first words before second words, RPB each.
-template <int RPB, typename W>
-__device__ __forceinline__ float enter_segment(const TileArgs& ch, uint64_t* mine, long long per_segment, int k, int segments,
-                                               uint32_t seq, int lane, float first, float ta, float tb, bool cut, W&& walk) {
-  constexpr int LOOK = 4;
-  const uint32_t want = (seq << 2) | STATUS_AGGREGATE, done = (seq << 2) | STATUS_INCLUSIVE;
-  const bool last = k + 1 >= segments;
-  if (!last) {
-    if (cut) {
-      st_desc(mine + RPB, pack_desc(done, tb));
-    } else if (k > 0) {
-      st_desc(mine, pack_desc(want, ta));
-      st_desc(mine + RPB, pack_desc(want, tb));
-    }
-  }
-  float entering = first;
-  if (k > 0) {
-    bool found = false;
-    for (int polls = 0; polls < ch.spin_limit; ++polls) {
-      uint64_t w0[LOOK], w1[LOOK];
-#pragma unroll
-      for (int q = 0; q < LOOK; ++q) {
-        const uint64_t* d = mine - (q < k ? q + 1 : k) * per_segment;  // (beyond segment 0: asked for again, not used)
-        w0[q] = ld_desc(d);
-        w1[q] = ld_desc(d + RPB);
-      }
-      int from = -1;
-      bool blocked = false;
-#pragma unroll
-      for (int q = 0; q < LOOK; ++q) {
-        const uint32_t f1 = uint32_t(w1[q] >> 32);
-        if (from < 0 && !blocked) {
-          if (__ballot(f1 != done) == 0) from = q;
-          else blocked = __ballot(f1 != done && !(f1 == want && uint32_t(w0[q] >> 32) == want)) != 0;
-        }
-      }
-      if (from >= 0) {
-#pragma unroll
-        for (int q = LOOK - 1; q >= 0; --q) {
-          const float a = __builtin_bit_cast(float, uint32_t(w0[q])), b = __builtin_bit_cast(float, uint32_t(w1[q]));
-          if (q == from) entering = b;
-          else if (q < from) entering = uint32_t(w1[q] >> 32) == done ? b : fmaf(a, entering, b);
-        }
-        found = true;
-        break;
-      }
-      __builtin_amdgcn_s_sleep(1);
-    }
-    if (__builtin_expect(!found, 0)) {
-      if (lane == 0) __hip_atomic_fetch_add(&ch.ws->gave_up, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-      entering = walk();
-    }
-  }
-  if (!last && !cut) st_desc(mine + RPB, pack_desc(done, fmaf(ta, entering, tb)));
-  return entering;
+// What enters a segment is a chain of multiply-adds over the maps of the segments before, and every link costs a store and a load
+// through memory, about 1.5 us, however many lanes do it side by side.  So the chain goes over groups of GROUP segments: a
+// segment publishes its map; the last one of a group composes the group's maps and publishes that; and what enters a segment is
+// what enters its group, which the chain of groups says, taken through the maps of the segments before it in the group.
+// LOOK groups are looked at at a time, so the value advances by LOOK * GROUP segments a link.  Which groups had published what
+// does not matter to the result: the value that leaves a group is the same multiply-add whoever makes it.
+//
+// Words of a place (a segment's, a group's): first the factors of the block's channels, then the addends, RPB each, with the
+// launch's number; an addend marked `done` leaves the place whatever enters it (a sequence starts inside, or what entered is in it).
+constexpr int LOOK = 4;   // groups looked at at a time
+constexpr int GROUP = 8;  // segments of a group
+struct Chain {
+  uint64_t* segment_words;  // of segment 0, this lane's
+  uint64_t* group_words;    // of group 0
+  long long per_place;      // from one place's words to the next one's
+  int k, segments;
+  uint32_t seq;
+  __device__ __forceinline__ uint32_t map() const { return (seq << 2) | STATUS_AGGREGATE; }
+  __device__ __forceinline__ uint32_t done() const { return (seq << 2) | STATUS_INCLUSIVE; }
+};
+struct Words {
+  uint64_t a, b;
+};
+template <int RPB>
+__device__ __forceinline__ Words load_words(const uint64_t* d) {
+  return {ld_desc(d), ld_desc(d + RPB)};
 }
+template <int RPB>
+__device__ __forceinline__ void publish(const Chain& c, uint64_t* d, float a, float b, bool constant) {
+  if (!constant) st_desc(d, pack_desc(c.map(), a));
+  st_desc(d + RPB, pack_desc(constant ? c.done() : c.map(), b));
+}
+__device__ __forceinline__ float word_value(uint64_t w) { return __builtin_bit_cast(float, uint32_t(w)); }
+__device__ __forceinline__ bool is_done(const Chain& c, const Words& w) { return uint32_t(w.b >> 32) == c.done(); }
+__device__ __forceinline__ bool is_there(const Chain& c, const Words& w) {
+  return is_done(c, w) || (uint32_t(w.b >> 32) == c.map() && uint32_t(w.a >> 32) == c.map());
+}
+__device__ __forceinline__ float through(const Chain& c, const Words& w, float v) {
+  return is_done(c, w) ? word_value(w.b) : fmaf(word_value(w.a), v, word_value(w.b));
+}
+
+// One wave, a channel to a lane: publishes the segment's map (ta, tb; cut: a sequence starts inside) and returns what enters it.
+// `walk` computes that from the channel's own data.
+template <int RPB, typename W>
+__device__ __forceinline__ float enter_segment(const TileArgs& args, const Chain& c, int lane, float first, float ta, float tb, bool cut, W&& walk) {
+  const int in_group = c.k % GROUP, g = c.k / GROUP;
+  const bool last = c.k + 1 >= c.segments, closes = !last && in_group == GROUP - 1;
+  uint64_t* mine = c.segment_words + c.k * c.per_place;
+  uint64_t* of_group = c.group_words + g * c.per_place;
+  if (!last && !closes) publish<RPB>(c, mine, ta, tb, cut);
+  // The map of the segments before this one in its group; a constant one needs nothing of what enters the group.  (Asking for
+  // what enters the group in the same round trip takes registers that the data needs: 8 x 4096 x 2048 bf16 164 / 281 us against
+  // 127 / 220.)
+  float ga = 1.0f, gb = 0.0f;
+  bool constant = false, there = in_group == 0;
+  for (int polls = 0; !there && polls < args.spin_limit; ++polls) {
+    if (polls > 0) __builtin_amdgcn_s_sleep(1);
+    Words w[GROUP - 1];  // the farthest first
+#pragma unroll
+    for (int q = 0; q < GROUP - 1; ++q)
+      if (q < in_group) w[q] = load_words<RPB>(mine - (in_group - q) * c.per_place);
+    there = true;
+#pragma unroll
+    for (int q = 0; q < GROUP - 1; ++q)
+      if (q < in_group && __ballot(!is_there(c, w[q])) != 0) there = false;
+    if (there) {
+#pragma unroll
+      for (int q = 0; q < GROUP - 1; ++q)
+        if (q < in_group) {
+          const bool cuts = __ballot(!is_done(c, w[q])) == 0;
+          gb = through(c, w[q], gb);
+          ga = cuts ? 1.0f : never_zero(ga * word_value(w[q].a));
+          constant = constant || cuts;
+        }
+    }
+  }
+  // that of the whole group, by its last segment (the first group never shows a map: who looks beyond it sees it again, and must
+  // not take it twice)
+  const float whole_a = never_zero(ga * ta), whole_b = cut ? tb : fmaf(ta, gb, tb);
+  const bool whole_constant = constant || cut;
+  if (there && closes && (g > 0 || whole_constant)) publish<RPB>(c, of_group, whole_a, whole_b, whole_constant);
+  float v = first;  // what enters the group
+  bool known = there && (g == 0 || constant);
+  for (int polls = 0; there && !known && polls < args.spin_limit; ++polls) {
+    if (polls > 0) __builtin_amdgcn_s_sleep(1);
+    Words x[LOOK];
+#pragma unroll
+    for (int q = 0; q < LOOK; ++q) x[q] = load_words<RPB>(of_group - (q < g ? q + 1 : g) * c.per_place);  // (beyond group 0: not used)
+    int from = -1;
+    bool blocked = false;
+#pragma unroll
+    for (int q = 0; q < LOOK; ++q) {
+      if (from < 0 && !blocked) {
+        if (__ballot(!is_done(c, x[q])) == 0) from = q;
+        else blocked = __ballot(!is_there(c, x[q])) != 0;
+      }
+    }
+    if (from >= 0) {
+#pragma unroll
+      for (int q = LOOK - 1; q >= 0; --q) {
+        if (q == from) v = word_value(x[q].b);
+        else if (q < from) v = through(c, x[q], v);
+      }
+      known = true;
+    }
+  }
+  if (known) {
+    if (closes && !whole_constant) st_desc(of_group + RPB, pack_desc(c.done(), fmaf(whole_a, v, whole_b)));
+    v = constant ? gb : in_group == 0 ? v : fmaf(ga, v, gb);
+  }
+  if (__builtin_expect(!known, 0)) {
+    if (lane == 0) __hip_atomic_fetch_add(&args.ws->gave_up, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    v = walk();
+    // (whoever looks for what leaves the group waits for it: it leaves through this segment)
+    if (closes && !cut) st_desc(of_group + RPB, pack_desc(c.done(), fmaf(ta, v, tb)));
+    else if (closes) st_desc(of_group + RPB, pack_desc(c.done(), tb));
+  }
+  return v;
+}
+
+// ---- positions of a wave ----------------------------------------------------------------------
+// A tensor's positions from the first of a run on, in scan order: a scalar address that goes on by a scalar step, the lane's
+// part 32 bits beside it.  (Read as a scalar at each access, or the lane's part is
+// added first and every access carries a 64-bit vector address.)
+template <typename P>
+struct Walk {
+  P* at;
+  int64_t step;  // elements
+  __device__ __forceinline__ Walk(P* tensor, int64_t stride, int n0, int time, bool reverse)
+      : at(tensor + int64_t(reverse ? time - 1 - n0 : n0) * stride), step(reverse ? -stride : stride) {}
+  static __device__ __forceinline__ P* scalar(P* p) {  // (the same for all lanes, which the compiler need not know)
+    const uint64_t v = reinterpret_cast<uint64_t>(p);
+    return reinterpret_cast<P*>(uint64_t(uint32_t(__builtin_amdgcn_readfirstlane(int(v)))) |
+                                (uint64_t(uint32_t(__builtin_amdgcn_readfirstlane(int(v >> 32)))) << 32));
+  }
+  __device__ __forceinline__ P* lane(uint32_t bytes) const { return plus_bytes(scalar(at), bytes); }
+  __device__ __forceinline__ void next() { at += step; }
+  __device__ __forceinline__ void back() { at -= step; }
+};
 
 // ---- forward ----------------------------------------------------------------------------------
 template <typename T, int VEC, int U, int NW, bool PACKED>
-__global__ __launch_bounds__(64 * NW) void gated_fwd_kernel(GatedArgs args) {
+__global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(4))) void gated_fwd_kernel(GatedArgs args) {
   constexpr int RPB = 64 * VEC, SEG = NW * U;
-  static_assert(VEC <= NW && GATED_SAVE % U == 0, "a wave per channel of a lane looks back; values are saved where runs start");
+  static_assert(VEC <= NW, "a wave per channel of a lane looks back");
   __shared__ float sh_a[NW][RPB];
-  __shared__ float sh_b[NW][RPB];
-  __shared__ float sh_in[RPB];
+  __shared__ float sh_b[NW][RPB];  // the waves' maps, then what enters the waves
   __shared__ float sh_decay[RPB];
   __shared__ SegmentMarks<PACKED ? SEG : 1> marks;
   const linrec_gated_t& p = args.p;
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const unsigned blocks = unsigned(args.channel_blocks) * unsigned(p.batch);
-  const int k = int(blockIdx.x / blocks);
+  const int k = __builtin_amdgcn_readfirstlane(int(blockIdx.x / blocks));
   const unsigned block = blockIdx.x - unsigned(k) * blocks;
-  const int batch = int(block / unsigned(args.channel_blocks));
+  const int batch = __builtin_amdgcn_readfirstlane(int(block / unsigned(args.channel_blocks)));
   const int channels = int(p.channels), time = int(p.time);
   const Channels<VEC> ch = lane_channels<VEC>(int(block) - batch * args.channel_blocks, lane, channels);
   const uint32_t seq = args.segments > 1 ? load_seq_through_caches(args.chain.ws) : 0u;
+  const bool reverse = p.reverse != 0;
 
   const uint32_t lane_bytes = ch.rel * uint32_t(sizeof(T));
   const T* x = static_cast<const T*>(p.x) + batch * p.x_stride[0] + ch.base;
   const T* ga = static_cast<const T*>(p.gate_a) + batch * p.gate_a_stride[0] + ch.base;
   const T* gx = static_cast<const T*>(p.gate_x) + batch * p.gate_x_stride[0] + ch.base;
-  T* h = static_cast<T*>(p.h) + (int64_t)batch * time * channels + ch.base;
   const int n0 = k * SEG + wave * U;
-  auto position = [&](int n) __attribute__((always_inline)) { return int64_t(p.reverse ? time - 1 - n : n); };
+  const bool full = time - k * SEG >= SEG;
 
-  auto segment = [&](auto full_tag) __attribute__((always_inline)) {
-    constexpr bool FULL = decltype(full_tag)::value;
-    Held<T, VEC> hx[U], ha[U], hg[U];
+  bool plain = full;
+  if constexpr (PACKED) {
+    mark_segment<SEG, 64 * NW>(marks, p, k * SEG);
+    __syncthreads();
+    plain = plain && !any_mark(marks);
+  }
+
+  // PLAIN: every position of the segment exists and no sequence starts or ends in it.
+  auto segment = [&](auto plain_tag, auto whole_tag) __attribute__((always_inline)) {
+    constexpr bool PLAIN = decltype(plain_tag)::value, WHOLE = decltype(whole_tag)::value, CUTS = PACKED && !PLAIN;
+  Held<T, VEC> hx[U], ha[U], hg[U];
+  {
+    Walk<const T> wx(x, p.x_stride[1], n0, time, reverse), wa(ga, p.gate_a_stride[1], n0, time, reverse),
+        wg(gx, p.gate_x_stride[1], n0, time, reverse);
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      if (FULL || n0 + u < time) {
-        const int64_t l = position(n0 + u);
-        hx[u] = ld_any<VEC, true>(plus_bytes(x + l * p.x_stride[1], lane_bytes));
-        ha[u] = ld_any<VEC, true>(plus_bytes(ga + l * p.gate_a_stride[1], lane_bytes));
-        hg[u] = ld_any<VEC, true>(plus_bytes(gx + l * p.gate_x_stride[1], lane_bytes));
+      if (PLAIN || n0 + u < time) {
+        hx[u] = ld_any<VEC, true>(wx.lane(lane_bytes));
+        ha[u] = ld_any<VEC, true>(wa.lane(lane_bytes));
+        hg[u] = ld_any<VEC, true>(wg.lane(lane_bytes));
       }
+      wx.next();
+      wa.next();
+      wg.next();
     }
-    if (wave < VEC) {  // a channel to a lane
-      const float rate = p.rate[ch.base + int(ch.rel) + wave];
-      sh_decay[wave * 64 + lane] = LOG2E * p.scale * fast_softplus(rate);
-    }
+  }
+  if (wave < VEC) {  // a channel to a lane
+    const float rate = p.rate[ch.base + int(ch.rel) + wave];
+    sh_decay[wave * 64 + lane] = LOG2E * p.scale * fast_softplus(rate);
+  }
+  __syncthreads();
+
     unsigned starts = 0, ends = 0;
-    if constexpr (PACKED) mark_segment<SEG, 64 * NW>(marks, p, k * SEG);
-    __syncthreads();
-    if constexpr (PACKED) {
+    if constexpr (CUTS) {
       starts = run_bits<U>(marks.starts, wave);
       ends = run_bits<U>(marks.ends, wave);
     }
@@ -334,9 +435,9 @@ __global__ __launch_bounds__(64 * NW) void gated_fwd_kernel(GatedArgs args) {
     }
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      if (FULL || n0 + u < time) {
+      if (PLAIN || n0 + u < time) {
         const Lanes<VEC> vx = widen(hx[u]), va = widen(ha[u]), vg = widen(hg[u]);
-        if constexpr (PACKED) {
+        if constexpr (CUTS) {
           if (starts >> u & 1u) mb = initial(u);
         }
 #pragma unroll
@@ -355,81 +456,86 @@ __global__ __launch_bounds__(64 * NW) void gated_fwd_kernel(GatedArgs args) {
       sh_b[wave][e * 64 + lane] = mb.v[e];
     }
     __syncthreads();
-    if (wave < VEC) {
-      const int i = wave * 64 + lane;
-      const int c = ch.base + int(ch.rel) + wave;
-      float ta = sh_a[0][i], tb = sh_b[0][i];
-      bool cut = PACKED && run_bits<U>(marks.starts, 0) != 0;
+    if (wave < VEC) {  // a channel to a lane
+      const int e = wave, i = e * 64 + lane;
+      const int c = ch.base + int(ch.rel) + e;
+      bool any = false;
+      float ta = 1.0f, tb = 0.0f;
+      {
 #pragma unroll
-      for (int w = 1; w < NW; ++w) {
-        if (PACKED && run_bits<U>(marks.starts, w) != 0) {
-          tb = sh_b[w][i];
-          cut = true;
-        } else {
-          tb = fmaf(sh_a[w][i], tb, sh_b[w][i]);
-          ta = never_zero(ta * sh_a[w][i]);
+        for (int w = 0; w < NW; ++w) {
+          const float wa = sh_a[w][i], wb = sh_b[w][i];
+          if (CUTS && run_bits<U>(marks.starts, w) != 0) {
+            tb = wb;
+            any = true;
+          } else {
+            tb = fmaf(wa, tb, wb);
+            ta = never_zero(ta * wa);
+          }
         }
       }
-      const float first = !PACKED && p.h0 ? p.h0[int64_t(batch) * channels + c] : 0.0f;
       const long long per_segment = 2ll * blocks * RPB;
-      uint64_t* mine = args.chain.desc + k * per_segment + 2ll * block * RPB + i;
-      sh_in[i] = enter_segment<RPB>(args.chain, mine, per_segment, k, args.segments, seq, lane, first, ta, tb, cut, [&] {
+      uint64_t* words = args.chain.desc + 2ll * block * RPB + i;
+      const Chain chain{words, words + args.segments * per_segment, per_segment, k, args.segments, seq};
+      const float first = !PACKED && p.h0 ? p.h0[int64_t(batch) * channels + c] : 0.0f;
+      auto walk = [&] {
         int from = 0;
-        float v = first;
+        float w = first;
         if constexpr (PACKED) {
           const int64_t j = bounds_up_to(p, k * SEG - 1) - 1;
           if (j >= 0) {
             from = scan_bound(p, j);
-            if (p.h0 && j < p.sequences) v = p.h0[scan_sequence(p, j) * channels + c];
+            if (p.h0 && j < p.sequences) w = p.h0[scan_sequence(p, j) * channels + c];
           }
         }
         const float d2 = sh_decay[i];
         for (int n = from; n < k * SEG; ++n) {
-          const int64_t l = position(n), o = int64_t(ch.rel) + wave;
+          const int64_t l = reverse ? time - 1 - n : n, o = int64_t(ch.rel) + e;
           const Gate g = gate_of(float(ga[l * p.gate_a_stride[1] + o]), float(gx[l * p.gate_x_stride[1] + o]), d2);
-          v = fmaf(g.a, v, taken_in(g, float(x[l * p.x_stride[1] + o])));
+          w = fmaf(g.a, w, taken_in(g, float(x[l * p.x_stride[1] + o])));
         }
-        return v;
-      });
+        return w;
+      };
+      float v = enter_segment<RPB>(args.chain, chain, lane, first, ta, tb, any, walk);
+      {
+#pragma unroll
+        for (int w = 0; w < NW; ++w) {
+          const float wa = sh_a[w][i], wb = sh_b[w][i];
+          sh_b[w][i] = v;
+          v = CUTS && run_bits<U>(marks.starts, w) != 0 ? wb : fmaf(wa, v, wb);
+        }
+      }
     }
     __syncthreads();
     Lanes<VEC> val;
 #pragma unroll
-    for (int e = 0; e < VEC; ++e) val.v[e] = sh_in[e * 64 + lane];
-    for (int w = 0; w < wave; ++w) {
-      const bool cut = PACKED && run_bits<U>(marks.starts, w) != 0;
-#pragma unroll
-      for (int e = 0; e < VEC; ++e) {
-        const float wa = sh_a[w][e * 64 + lane], wb = sh_b[w][e * 64 + lane];
-        val.v[e] = cut ? wb : fmaf(wa, val.v[e], wb);
-      }
+    for (int e = 0; e < VEC; ++e) val.v[e] = sh_b[wave][e * 64 + lane];
+    if (p.saved && (n0 & (args.save - 1)) == 0 && n0 < time) {
+      const int saves = (time + args.save - 1) / args.save;
+      store_floats(p.saved + (int64_t(batch) * saves + n0 / args.save) * channels + ch.base + ch.rel, val, ch);
     }
-    if (p.saved && n0 % GATED_SAVE == 0 && n0 < time) {
-      const int saves = (time + GATED_SAVE - 1) / GATED_SAVE;
-      store_floats(p.saved + (int64_t(batch) * saves + n0 / GATED_SAVE) * channels + ch.base + ch.rel, val, ch);
-    }
+    Walk<T> wh(static_cast<T*>(p.h) + (int64_t)batch * time * channels + ch.base, channels, n0, time, reverse);
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      if (FULL || n0 + u < time) {
-        if constexpr (PACKED) {
+      if (PLAIN || n0 + u < time) {
+        if constexpr (CUTS) {
           if (starts >> u & 1u) val = initial(u);
         }
 #pragma unroll
         for (int e = 0; e < VEC; ++e) val.v[e] = fmaf(a[u].v[e], val.v[e], b[u].v[e]);
-        store_channels(plus_bytes(h + position(n0 + u) * channels, lane_bytes), val, ch);
-        if (p.state) {
-          if constexpr (PACKED) {
-            if (ends >> u & 1u)
-              store_floats(p.state + int64_t(__builtin_amdgcn_readfirstlane(marks.end[wave * U + u])) * channels + ch.base + ch.rel, val, ch);
-          } else if (n0 + u == time - 1) {
-            store_floats(p.state + int64_t(batch) * channels + ch.base + ch.rel, val, ch);
-          }
-        }
+        T* to = wh.lane(lane_bytes);
+        wh.next();
+        store_channels<WHOLE>(to, val, ch);
+        if (CUTS && p.state && (ends >> u & 1u))
+          store_floats(p.state + int64_t(__builtin_amdgcn_readfirstlane(marks.end[wave * U + u])) * channels + ch.base + ch.rel, val, ch);
+        if (!PACKED && (!PLAIN || u == U - 1) && n0 + u == time - 1 && p.state)
+          store_floats(p.state + int64_t(batch) * channels + ch.base + ch.rel, val, ch);
       }
     }
   };
-  if ((k + 1) * int64_t(SEG) <= time) segment(std::true_type{});
-  else segment(std::false_type{});
+  if (plain && ch.whole) segment(std::true_type{}, std::true_type{});
+  else if (plain) segment(std::true_type{}, std::false_type{});
+  else segment(std::false_type{}, std::false_type{});
 
   if (PACKED && k == 0 && p.state)
     for_empty_sequences<NW>(p, wave, lane, [&](int64_t n) {
@@ -446,61 +552,71 @@ __global__ __launch_bounds__(64 * NW) void gated_fwd_kernel(GatedArgs args) {
 
 // ---- backward ---------------------------------------------------------------------------------
 template <typename T, int VEC, int U, int NW, bool PACKED>
-__global__ __launch_bounds__(64 * NW) void gated_bwd_kernel(GatedArgs args) {
+__global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(4))) void gated_bwd_kernel(GatedArgs args) {
   constexpr int RPB = 64 * VEC, SEG = NW * U;
-  static_assert(VEC <= NW && SEG == GATED_SAVE, "a segment starts where a value was saved");
+  static_assert(2 * VEC <= NW, "a wave per channel of a lane and direction");
   __shared__ float sh_a[NW][RPB];
-  __shared__ float sh_b[NW][RPB];
-  __shared__ float sh_g[NW][RPB];
-  __shared__ float sh_in[RPB];
+  __shared__ float sh_b[NW][RPB];  // forward maps, then what enters the waves forward
+  __shared__ float sh_g[NW][RPB];  // the same backward
+  __shared__ Lanes<VEC> sigmoids[SEG][2][64];
   __shared__ float sh_decay[RPB];
   __shared__ SegmentMarks<PACKED ? SEG : 1> marks;
   const linrec_gated_t& p = args.p;
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const unsigned blocks = unsigned(args.channel_blocks) * unsigned(p.batch);
-  const int kk = int(blockIdx.x / blocks);  // segments from the far end
+  const int kk = __builtin_amdgcn_readfirstlane(int(blockIdx.x / blocks));  // segments from the far end
   const int k = args.segments - 1 - kk;
   const unsigned block = blockIdx.x - unsigned(kk) * blocks;
-  const int batch = int(block / unsigned(args.channel_blocks));
+  const int batch = __builtin_amdgcn_readfirstlane(int(block / unsigned(args.channel_blocks)));
   const int channels = int(p.channels), time = int(p.time);
   const Channels<VEC> ch = lane_channels<VEC>(int(block) - batch * args.channel_blocks, lane, channels);
   const uint32_t seq = args.segments > 1 ? load_seq_through_caches(args.chain.ws) : 0u;
+  const bool reverse = p.reverse != 0;
 
   const uint32_t lane_bytes = ch.rel * uint32_t(sizeof(T));
   const T* x = static_cast<const T*>(p.x) + batch * p.x_stride[0] + ch.base;
   const T* ga = static_cast<const T*>(p.gate_a) + batch * p.gate_a_stride[0] + ch.base;
   const T* gx = static_cast<const T*>(p.gate_x) + batch * p.gate_x_stride[0] + ch.base;
   const T* dh = static_cast<const T*>(p.d_h) + batch * p.d_h_stride[0] + ch.base;
-  const int64_t dense = (int64_t)batch * time * channels + ch.base;
-  T* dx = static_cast<T*>(p.d_x) + dense;
-  T* dga = static_cast<T*>(p.d_gate_a) + dense;
-  T* dgx = static_cast<T*>(p.d_gate_x) + dense;
   const int n0 = k * SEG + wave * U;
-  auto position = [&](int n) __attribute__((always_inline)) { return int64_t(p.reverse ? time - 1 - n : n); };
+  const bool full = time - k * SEG >= SEG;
 
-  auto segment = [&](auto full_tag) __attribute__((always_inline)) {
-    constexpr bool FULL = decltype(full_tag)::value;
-    Held<T, VEC> hx[U], ha[U], hg[U], hd[U];
+  bool plain = full;
+  if constexpr (PACKED) {
+    mark_segment<SEG, 64 * NW>(marks, p, k * SEG);
+    __syncthreads();
+    plain = plain && !any_mark(marks);
+  }
+
+  auto segment = [&](auto plain_tag, auto whole_tag) __attribute__((always_inline)) {
+    constexpr bool PLAIN = decltype(plain_tag)::value, WHOLE = decltype(whole_tag)::value, CUTS = PACKED && !PLAIN;
+  Held<T, VEC> hx[U], ha[U], hg[U], hd[U];
+  {
+    Walk<const T> wx(x, p.x_stride[1], n0, time, reverse), wa(ga, p.gate_a_stride[1], n0, time, reverse),
+        wg(gx, p.gate_x_stride[1], n0, time, reverse), wd(dh, p.d_h_stride[1], n0, time, reverse);
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      if (FULL || n0 + u < time) {
-        const int64_t l = position(n0 + u);
-        hx[u] = ld_any<VEC, true>(plus_bytes(x + l * p.x_stride[1], lane_bytes));
-        ha[u] = ld_any<VEC, true>(plus_bytes(ga + l * p.gate_a_stride[1], lane_bytes));
-        hg[u] = ld_any<VEC, true>(plus_bytes(gx + l * p.gate_x_stride[1], lane_bytes));
-        hd[u] = ld_any<VEC, true>(plus_bytes(dh + l * p.d_h_stride[1], lane_bytes));
+      if (PLAIN || n0 + u < time) {
+        hx[u] = ld_any<VEC, true>(wx.lane(lane_bytes));
+        ha[u] = ld_any<VEC, true>(wa.lane(lane_bytes));
+        hg[u] = ld_any<VEC, true>(wg.lane(lane_bytes));
+        hd[u] = ld_any<VEC, true>(wd.lane(lane_bytes));
       }
+      wx.next();
+      wa.next();
+      wg.next();
+      wd.next();
     }
-    Lanes<VEC> val = load_floats<VEC>(p.saved + (int64_t(batch) * args.segments + k) * channels + ch.base + ch.rel);
-    if (wave < VEC) {
-      const float rate = p.rate[ch.base + int(ch.rel) + wave];
-      sh_decay[wave * 64 + lane] = LOG2E * p.scale * fast_softplus(rate);
-    }
+  }
+  if (wave < VEC) {
+    const float rate = p.rate[ch.base + int(ch.rel) + wave];
+    sh_decay[wave * 64 + lane] = LOG2E * p.scale * fast_softplus(rate);
+  }
+  __syncthreads();
+
     unsigned starts = 0, ends = 0;
-    if constexpr (PACKED) mark_segment<SEG, 64 * NW>(marks, p, k * SEG);
-    __syncthreads();
-    if constexpr (PACKED) {
+    if constexpr (CUTS) {
       starts = run_bits<U>(marks.starts, wave);
       ends = run_bits<U>(marks.ends, wave);
     }
@@ -510,7 +626,8 @@ __global__ __launch_bounds__(64 * NW) void gated_bwd_kernel(GatedArgs args) {
       else for (int e = 0; e < VEC; ++e) r.v[e] = 0.0f;
       return r;
     };
-    Lanes<VEC> decay, ma, mb, mg, a[U], b[U];
+    // a and m of every position stay in registers until its gradients are made, its sigmoids in LDS
+    Lanes<VEC> decay, ma, mb, mg, a[U], b[U], m[U];
 #pragma unroll
     for (int e = 0; e < VEC; ++e) {
       decay.v[e] = sh_decay[e * 64 + lane];
@@ -519,26 +636,32 @@ __global__ __launch_bounds__(64 * NW) void gated_bwd_kernel(GatedArgs args) {
     }
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      if (FULL || n0 + u < time) {
+      if (PLAIN || n0 + u < time) {
         const Lanes<VEC> vx = widen(hx[u]), va = widen(ha[u]), vg = widen(hg[u]);
-        if constexpr (PACKED) {
+        if constexpr (CUTS) {
           if (starts >> u & 1u) mb = rows_of(p.h0, marks.start, u);
         }
+        Lanes<VEC> sa, sx;
 #pragma unroll
         for (int e = 0; e < VEC; ++e) {
           const Gate g = gate_of(va.v[e], vg.v[e], decay.v[e]);
           a[u].v[e] = g.a;
-          b[u].v[e] = taken_in(g, vx.v[e]);
+          sa.v[e] = g.sa;
+          sx.v[e] = g.sx;
+          m[u].v[e] = __builtin_amdgcn_sqrtf(g.m2);
+          b[u].v[e] = m[u].v[e] * g.sx * vx.v[e];
           mb.v[e] = fmaf(g.a, mb.v[e], b[u].v[e]);
           ma.v[e] *= g.a;
         }
+        sigmoids[wave * U + u][0][lane] = sa;
+        sigmoids[wave * U + u][1][lane] = sx;
       }
     }
 #pragma unroll
     for (int u = U - 1; u >= 0; --u) {
-      if (FULL || n0 + u < time) {
+      if (PLAIN || n0 + u < time) {
         const Lanes<VEC> vd = widen(hd[u]);
-        if constexpr (PACKED) {
+        if constexpr (CUTS) {
           if (ends >> u & 1u) mg = rows_of(p.d_state, marks.end, u);
         }
 #pragma unroll
@@ -552,72 +675,81 @@ __global__ __launch_bounds__(64 * NW) void gated_bwd_kernel(GatedArgs args) {
       sh_g[wave][e * 64 + lane] = mg.v[e];
     }
     __syncthreads();
-    if (wave < VEC) {
-      const int i = wave * 64 + lane;
-      const int c = ch.base + int(ch.rel) + wave;
-      float ta = sh_a[NW - 1][i], tg = sh_g[NW - 1][i];
-      bool cut = PACKED && run_bits<U>(marks.ends, NW - 1) != 0;
+    if (wave >= VEC && wave < 2 * VEC) {  // forward, from the saved value
+      const int e = wave - VEC, i = e * 64 + lane;
+      float v = p.saved[(int64_t(batch) * args.segments + k) * channels + ch.base + int(ch.rel) + e];
 #pragma unroll
-      for (int w = NW - 2; w >= 0; --w) {
-        if (PACKED && run_bits<U>(marks.ends, w) != 0) {
-          tg = sh_g[w][i];
-          cut = true;
-        } else {
-          tg = fmaf(sh_a[w][i], tg, sh_g[w][i]);
-          ta = never_zero(ta * sh_a[w][i]);
+      for (int w = 0; w < NW; ++w) {
+        const float wa = sh_a[w][i], wb = sh_b[w][i];
+        sh_b[w][i] = v;
+        v = CUTS && run_bits<U>(marks.starts, w) != 0 ? wb : fmaf(wa, v, wb);
+      }
+    }
+    if (wave < VEC) {
+      const int e = wave, i = e * 64 + lane;
+      const int c = ch.base + int(ch.rel) + e;
+      bool any = false;
+      float ta = 1.0f, tg = 0.0f;
+      {
+#pragma unroll
+        for (int w = NW - 1; w >= 0; --w) {
+          const float wa = sh_a[w][i], wg = sh_g[w][i];
+          if (CUTS && run_bits<U>(marks.ends, w) != 0) {
+            tg = wg;
+            any = true;
+          } else {
+            tg = fmaf(wa, tg, wg);
+            ta = never_zero(ta * wa);
+          }
         }
       }
-      const float first = !PACKED && p.d_state ? p.d_state[int64_t(batch) * channels + c] : 0.0f;
       const long long per_segment = 2ll * blocks * RPB;
-      uint64_t* mine = args.chain.desc + kk * per_segment + 2ll * block * RPB + i;
-      sh_in[i] = enter_segment<RPB>(args.chain, mine, per_segment, kk, args.segments, seq, lane, first, ta, tg, cut, [&] {
+      uint64_t* words = args.chain.desc + 2ll * block * RPB + i;
+      const Chain chain{words, words + args.segments * per_segment, per_segment, kk, args.segments, seq};
+      const float first = !PACKED && p.d_state ? p.d_state[int64_t(batch) * channels + c] : 0.0f;
+      auto walk = [&] {
         int from = time;
-        float v = first;
+        float w = first;
         if constexpr (PACKED) {
           const int64_t j = bounds_up_to(p, (k + 1) * SEG) - 1;  // the sequence of the position after this segment
           if (j >= 0 && j < p.sequences) {
             from = scan_bound(p, j + 1);
-            // (a sequence that starts right there ends its own walk at its start: nothing of it enters this segment)
-            if (p.d_state) v = p.d_state[scan_sequence(p, j) * channels + c];
+            // (where that sequence starts right there, nothing of it enters: the segment's last position is an end)
+            if (p.d_state) w = p.d_state[scan_sequence(p, j) * channels + c];
           }
         }
         const float d2 = sh_decay[i];
         for (int n = from - 1; n >= (k + 1) * SEG; --n) {
-          const int64_t l = position(n), o = int64_t(ch.rel) + wave;
+          const int64_t l = reverse ? time - 1 - n : n, o = int64_t(ch.rel) + e;
           const float an = __builtin_amdgcn_exp2f(-d2 * fast_sigmoid(float(ga[l * p.gate_a_stride[1] + o])));
-          v = an * (v + float(dh[l * p.d_h_stride[1] + o]));
+          w = an * (w + float(dh[l * p.d_h_stride[1] + o]));
         }
-        return v;
-      });
+        return w;
+      };
+      float v = enter_segment<RPB>(args.chain, chain, lane, first, ta, tg, any, walk);
+      {
+#pragma unroll
+        for (int w = NW - 1; w >= 0; --w) {
+          const float wa = sh_a[w][i], wg = sh_g[w][i];
+          sh_g[w][i] = v;
+          v = CUTS && run_bits<U>(marks.ends, w) != 0 ? wg : fmaf(wa, v, wg);
+        }
+      }
     }
     __syncthreads();
-    for (int w = 0; w < wave; ++w) {
-      const bool cut = PACKED && run_bits<U>(marks.starts, w) != 0;
-#pragma unroll
-      for (int e = 0; e < VEC; ++e) {
-        const float wa = sh_a[w][e * 64 + lane], wb = sh_b[w][e * 64 + lane];
-        val.v[e] = cut ? wb : fmaf(wa, val.v[e], wb);
-      }
-    }
-    Lanes<VEC> back, sum;
+    Lanes<VEC> val, back, sum, neg_decay;
 #pragma unroll
     for (int e = 0; e < VEC; ++e) {
-      back.v[e] = sh_in[e * 64 + lane];
+      neg_decay.v[e] = -LN2 * decay.v[e];
+      val.v[e] = sh_b[wave][e * 64 + lane];
+      back.v[e] = sh_g[wave][e * 64 + lane];
       sum.v[e] = 0.0f;
     }
-    for (int w = NW - 1; w > wave; --w) {
-      const bool cut = PACKED && run_bits<U>(marks.ends, w) != 0;
-#pragma unroll
-      for (int e = 0; e < VEC; ++e) {
-        const float wa = sh_a[w][e * 64 + lane], wg = sh_g[w][e * 64 + lane];
-        back.v[e] = cut ? wg : fmaf(wa, back.v[e], wg);
-      }
-    }
-    // the values before each position, in the place of what the position takes in
+    // the value before each position, in the place of what the position takes in
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      if (FULL || n0 + u < time) {
-        if constexpr (PACKED) {
+      if (PLAIN || n0 + u < time) {
+        if constexpr (CUTS) {
           if (starts >> u & 1u) val = rows_of(p.h0, marks.start, u);
         }
 #pragma unroll
@@ -628,58 +760,62 @@ __global__ __launch_bounds__(64 * NW) void gated_bwd_kernel(GatedArgs args) {
         }
       }
     }
+    const int64_t dense = (int64_t)batch * time * channels + ch.base;
+    Walk<T> ox(static_cast<T*>(p.d_x) + dense, channels, n0 + U - 1, time, reverse),
+        oa(static_cast<T*>(p.d_gate_a) + dense, channels, n0 + U - 1, time, reverse),
+        og(static_cast<T*>(p.d_gate_x) + dense, channels, n0 + U - 1, time, reverse);
 #pragma unroll
     for (int u = U - 1; u >= 0; --u) {
-      if (FULL || n0 + u < time) {
-        const Lanes<VEC> vx = widen(held_again(hx[u])), va = widen(held_again(ha[u])), vg = widen(held_again(hg[u])),
-                         vd = widen(held_again(hd[u]));
-        Lanes<VEC> ox, oa, og;
-        if constexpr (PACKED) {
+      if (PLAIN || n0 + u < time) {
+        const Lanes<VEC> vx = widen(held_again(hx[u])), vd = widen(held_again(hd[u]));
+        const Lanes<VEC> sa = sigmoids[wave * U + u][0][lane], sx = sigmoids[wave * U + u][1][lane];
+        Lanes<VEC> rx, ra, rg;
+        if constexpr (CUTS) {
           if (ends >> u & 1u) back = rows_of(p.d_state, marks.end, u);
         }
 #pragma unroll
         for (int e = 0; e < VEC; ++e) {
-          const Gate g = gate_of(va.v[e], vg.v[e], decay.v[e]);
-          const float grad = vd.v[e] + back.v[e];
-          const float log_a = LN2 * g.log2_a;
-          const float inv_m = g.m2 > 0.0f ? __builtin_amdgcn_rsqf(g.m2) : 0.0f;
-          const float gmx = grad * (g.m2 * inv_m) * g.sx;
-          const float sx_x = g.sx * vx.v[e];
-          const float q = grad * log_a * g.a * fmaf(-sx_x * g.a, inv_m, b[u].v[e]);
-          ox.v[e] = gmx;
-          og.v[e] = gmx * vx.v[e] * (1.0f - g.sx);
-          oa.v[e] = q * (1.0f - g.sa);
+          const float av = a[u].v[e], mv = m[u].v[e], sxv = sx.v[e], sav = sa.v[e];
+          const float grad = vd.v[e] + back.v[e], back_on = av * grad;
+          const float inv_m = __builtin_amdgcn_rcpf(fmaxf(mv, 1e-19f));  // (m is 0 only with log a, which makes the product 0)
+          const float sxx = sxv * vx.v[e];
+          rx.v[e] = grad * mv * sxv;
+          rg.v[e] = grad * mv * fmaf(-sxx, sxv, sxx);
+          // P = g log a a (h' - a sx x / m)
+          const float q = back_on * (neg_decay.v[e] * sav) * fmaf(-sxx * av, inv_m, b[u].v[e]);
+          ra.v[e] = fmaf(-q, sav, q);
           sum.v[e] += q;
-          back.v[e] = g.a * grad;
+          back.v[e] = back_on;
         }
-        const int64_t o = position(n0 + u) * channels;
-        store_channels(plus_bytes(dx + o, lane_bytes), ox, ch);
-        store_channels(plus_bytes(dga + o, lane_bytes), oa, ch);
-        store_channels(plus_bytes(dgx + o, lane_bytes), og, ch);
-        if (p.d_h0) {
-          if constexpr (PACKED) {
-            if (starts >> u & 1u)
-              store_floats(p.d_h0 + int64_t(__builtin_amdgcn_readfirstlane(marks.start[wave * U + u])) * channels + ch.base + ch.rel, back, ch);
-          } else if (n0 + u == 0) {
-            store_floats(p.d_h0 + int64_t(batch) * channels + ch.base + ch.rel, back, ch);
-          }
-        }
+        T* to_x = ox.lane(lane_bytes);
+        T* to_a = oa.lane(lane_bytes);
+        T* to_g = og.lane(lane_bytes);
+        store_channels<WHOLE>(to_x, rx, ch);
+        store_channels<WHOLE>(to_a, ra, ch);
+        store_channels<WHOLE>(to_g, rg, ch);
+        if (CUTS && p.d_h0 && (starts >> u & 1u))
+          store_floats(p.d_h0 + int64_t(__builtin_amdgcn_readfirstlane(marks.start[wave * U + u])) * channels + ch.base + ch.rel, back, ch);
+        if (!PACKED && u == 0 && n0 == 0 && p.d_h0) store_floats(p.d_h0 + int64_t(batch) * channels + ch.base + ch.rel, back, ch);
       }
+      ox.back();
+      oa.back();
+      og.back();
     }
     __syncthreads();
 #pragma unroll
-    for (int e = 0; e < VEC; ++e) sh_b[wave][e * 64 + lane] = sum.v[e];
+    for (int e = 0; e < VEC; ++e) sh_a[wave][e * 64 + lane] = sum.v[e];
     __syncthreads();
     if (wave < VEC) {
       const int i = wave * 64 + lane;
-      float s = sh_b[0][i];
+      float s = sh_a[0][i];
 #pragma unroll
-      for (int w = 1; w < NW; ++w) s += sh_b[w][i];
+      for (int w = 1; w < NW; ++w) s += sh_a[w][i];
       if (wave >= ch.own) p.partial[(int64_t(batch) * args.segments + k) * channels + ch.base + int(ch.rel) + wave] = s;
     }
   };
-  if ((k + 1) * int64_t(SEG) <= time) segment(std::true_type{});
-  else segment(std::false_type{});
+  if (plain && ch.whole) segment(std::true_type{}, std::true_type{});
+  else if (plain) segment(std::true_type{}, std::false_type{});
+  else segment(std::false_type{}, std::false_type{});
 
   if (PACKED && kk == 0 && p.d_h0)
     for_empty_sequences<NW>(p, wave, lane, [&](int64_t n) {

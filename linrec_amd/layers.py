@@ -54,7 +54,7 @@ def _(x, gate_a, gate_x, rate, h0, cu_seqlens, reverse, scale):
     batch, time, channels, sequences = _layers.gated_shape(x, cu_seqlens)
     torch._check(gate_a.size() == x.size() and gate_x.size() == x.size(), lambda: "gated_linrec: x, gate_a and gate_x differ in size")
     return (x.new_empty(x.size()), x.new_empty((sequences, channels), dtype=torch.float32),
-            x.new_empty(_layers.gated_saved_numel(batch, time, channels), dtype=torch.float32))
+            x.new_empty(_layers.gated_saved_numel(x.dtype, batch, time, channels), dtype=torch.float32))
 
 
 @gated_linrec_bwd.register_fake

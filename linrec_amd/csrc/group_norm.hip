@@ -19,6 +19,9 @@ __global__ __launch_bounds__(64 * SUM_WAVES) void param_gradient_kernel(const fl
   });
 }
 
+#ifndef HELD_LINE
+#define HELD_LINE 64
+#endif
 enum class Shape { tokens, held, chunks };
 struct NormPlan {
   Shape shape;
@@ -69,32 +72,39 @@ NormPlan make_norm_plan(int dtype, int64_t batch, int64_t positions, int64_t cha
 
   BlockArgs& a = pl.block;
   a.whole = int(columns);
+  // held: whole groups in registers, side by side where one is narrower than a line
   const int bytes = pl.vec * size;
-  const int keep = 32 / (bytes >= 4 ? bytes / 4 : 1);
-  auto rows_of = [&](int lanes, int64_t wide) { return wide > 0 && wide <= lanes ? lanes / wide : int64_t(0); };
-  // held: positions * columns of a group in registers
-  for (int lanes : {256, 1024}) {
-    if (!rows_of(lanes, columns) || cdiv(positions, rows_of(lanes, columns)) > keep) continue;
-    if (lanes == 256 && columns * positions > 4 * 256 && batch * groups < 1024) continue;  // few groups: more lanes to each
-    int64_t g = 1, items = 1;
-    auto fits = [&](int64_t gg, int64_t it) {
-      const int64_t R = rows_of(lanes, gg * columns * it);
-      return R > 0 && cdiv(positions, R) <= keep / 2 + 1 && cdiv(groups, gg) * cdiv(batch, it) >= 1024;
-    };
-    while (2 * g <= groups && fits(2 * g, 1)) g *= 2;
-    if (g * 2 > groups && fits(groups, 1)) g = groups;
-    if (g == groups)
-      while (2 * items <= batch && fits(g, 2 * items)) items *= 2;
-    pl.shape = Shape::held;
-    pl.lanes = lanes;
-    a.per_group = int(columns); a.groups = int(g); a.items = int(items); a.parts = 1; a.chunks = 1;
-    a.blocks = int(cdiv(groups, g));
-    a.columns = int(items * g * columns);
-    a.R = int(rows_of(lanes, a.columns));
-    a.rows = int(positions);
-    pl.param_rows = cdiv(batch, items);
-    pl.grid = pl.param_rows * a.blocks;
-    return pl;
+  const int keep = (bwd && size == 2 ? 24 : 32) / (bytes >= 4 ? bytes / 4 : 1);
+  auto rows_of = [](int lanes, int64_t wide) { return wide <= lanes ? lanes / wide : int64_t(0); };
+  auto rounds = [&](int lanes, int64_t wide) { return rows_of(lanes, wide) ? cdiv(positions, rows_of(lanes, wide)) : int64_t(1) << 40; };
+  for (const int line : {128, HELD_LINE}) {
+    int64_t g = cdiv(line, columns * bytes);
+    if (g > groups) g = groups;
+    for (const int lanes : {256, 1024}) {
+      if (rounds(lanes, g * columns) > keep) continue;
+      // few workgroups: more lanes to each
+      if (lanes == 256 && cdiv(groups, g) * batch <= 256 && rounds(lanes, g * columns) > 2) continue;
+      int64_t items = 1;
+      // lanes that have nothing to do take more groups, or more batch items; so do short walks while the chip stays full
+      auto grows = [&](int64_t gg, int64_t it) {
+        const int64_t n = rounds(lanes, gg * columns * it);
+        return n == 1 || (n <= keep / 2 && cdiv(groups, gg) * cdiv(batch, it) >= 1024);
+      };
+      while (2 * g <= groups && grows(2 * g, 1)) g *= 2;
+      if (g < groups && 2 * g > groups && grows(groups, 1)) g = groups;
+      if (g == groups)
+        while (2 * items <= batch && grows(g, 2 * items)) items *= 2;
+      pl.shape = Shape::held;
+      pl.lanes = lanes;
+      a.per_group = int(columns); a.groups = int(g); a.items = int(items); a.parts = 1; a.chunks = 1;
+      a.blocks = int(cdiv(groups, g));
+      a.columns = int(items * g * columns);
+      a.R = int(rows_of(lanes, a.columns));
+      a.rows = int(positions);
+      pl.param_rows = cdiv(batch, items);
+      pl.grid = pl.param_rows * a.blocks;
+      return pl;
+    }
   }
 
   pl.shape = Shape::chunks;

@@ -288,11 +288,17 @@ struct BlockLane {
   int64_t n, group, channel, first, end;  // batch item, group, first channel; positions of the chunk
   bool there;
 };
+// Workgroups are dealt to the eight XCDs in turn; numbered so that neighbours run on one of them, groups narrower than a
+// 128-byte line share its lines in one L2.
+__device__ __forceinline__ unsigned block_number() {
+  const unsigned xcd = blockIdx.x & 7u, whole = gridDim.x >> 3, rest = gridDim.x & 7u;
+  return xcd * whole + (xcd < rest ? xcd : rest) + (blockIdx.x >> 3);
+}
 template <int VEC>
 __device__ __forceinline__ BlockLane block_lane(const BlockArgs& a) {
   BlockLane l;
   const int tid = int(threadIdx.x);
-  unsigned id = blockIdx.x;
+  unsigned id = block_number();
   const int chunk = int(id % unsigned(a.chunks));
   id /= unsigned(a.chunks);
   const int block = int(id % unsigned(a.blocks));
@@ -314,11 +320,54 @@ __device__ __forceinline__ BlockLane block_lane(const BlockArgs& a) {
   return l;
 }
 
-// Tree over the rows: v of row 0 becomes the sum of its column.  sh: N * blockDim floats.
+// Columns that are a power of two up to a wave: sums go over the lanes of a wave first.
+__device__ __forceinline__ bool columns_in_wave(const BlockArgs& a) { return (a.columns & (a.columns - 1)) == 0 && a.columns <= 64; }
+// Sum over the lanes of a wave that are a multiple of `columns` apart (a power of two), in all of them.
+__device__ __forceinline__ float same_column_sum(float v, int columns) {
+  if (columns < 2) v = dpp_add<0x121>(v);   // row_ror:1
+  if (columns < 4) v = dpp_add<0x122>(v);   // row_ror:2
+  if (columns < 8) v = dpp_add<0x124>(v);   // row_ror:4
+  if (columns < 16) v = dpp_add<0x128>(v);  // row_ror:8
+  if (columns < 32) {
+    const unsigned u = __builtin_bit_cast(unsigned, v);
+    const auto r = __builtin_amdgcn_permlane16_swap(u, u, false, false);
+    v = __builtin_bit_cast(float, unsigned(r[0])) + __builtin_bit_cast(float, unsigned(r[1]));
+  }
+  if (columns < 64) {
+    const unsigned u = __builtin_bit_cast(unsigned, v);
+    const auto r = __builtin_amdgcn_permlane32_swap(u, u, false, false);
+    v = __builtin_bit_cast(float, unsigned(r[0])) + __builtin_bit_cast(float, unsigned(r[1]));
+  }
+  return v;
+}
+// Sums over the rows: v of row 0 (of all rows if columns_in_wave) becomes the sum of its column.  sh: N * blockDim floats.
 template <int N>
 __device__ __forceinline__ void sum_rows(float (&v)[N], float* sh, const BlockArgs& a, const BlockLane& l) {
   const int lanes = int(blockDim.x), tid = int(threadIdx.x);
   if (a.R == 1) return;
+  if (columns_in_wave(a)) {
+    const int lane = tid & 63, wave = tid >> 6, waves = lanes >> 6, total = a.columns * N;
+#pragma unroll
+    for (int i = 0; i < N; ++i) v[i] = same_column_sum(v[i], a.columns);
+    __syncthreads();
+    if (lane < a.columns) {
+#pragma unroll
+      for (int i = 0; i < N; ++i) sh[wave * total + i * a.columns + lane] = v[i];
+    }
+    for (int j = tid; j - tid < total; j += lanes) {
+      __syncthreads();
+      float t = 0.0f;
+      if (j < total) {
+        t = sh[j];
+        for (int w = 1; w < waves; ++w) t += sh[w * total + j];
+      }
+      if (j < total) sh[j] = t;  // (no other lane reads it)
+    }
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < N; ++i) v[i] = sh[i * a.columns + l.vc];
+    return;
+  }
   __syncthreads();
 #pragma unroll
   for (int i = 0; i < N; ++i) sh[i * lanes + tid] = v[i];
@@ -335,10 +384,15 @@ __device__ __forceinline__ void sum_rows(float (&v)[N], float* sh, const BlockAr
     }
   }
 }
-// Tree over the columns of a group among the lanes of row 0; every lane gets its group's sum.
+// Sums over the columns of a group among the lanes of row 0; every lane gets its group's sum.
 template <int N>
 __device__ __forceinline__ void sum_group(float (&v)[N], float* sh, const BlockArgs& a, const BlockLane& l) {
   const int lanes = int(blockDim.x), tid = int(threadIdx.x);
+  if (columns_in_wave(a) && (a.per_group & (a.per_group - 1)) == 0) {  // (every row has the columns' sums)
+#pragma unroll
+    for (int i = 0; i < N; ++i) v[i] = team_sum(v[i], a.per_group);
+    return;
+  }
   __syncthreads();
 #pragma unroll
   for (int i = 0; i < N; ++i) sh[i * lanes + tid] = v[i];
@@ -355,6 +409,49 @@ __device__ __forceinline__ void sum_group(float (&v)[N], float* sh, const BlockA
   __syncthreads();
 #pragma unroll
   for (int i = 0; i < N; ++i) v[i] = sh[i * lanes + l.g * a.per_group];
+}
+
+// Sums over all rows and columns of a group, in all its lanes.  sh: N * blockDim floats.
+template <int N>
+__device__ __forceinline__ void sum_all(float (&v)[N], float* sh, const BlockArgs& a, const BlockLane& l) {
+  const int tid = int(threadIdx.x), lane = tid & 63, wave = tid >> 6, waves = int(blockDim.x) >> 6;
+  if (columns_in_wave(a)) {  // (so is the width of a group a power of two)
+    // every wave has all groups
+    const int groups = a.columns / a.per_group, total = groups * N;
+#pragma unroll
+    for (int i = 0; i < N; ++i) v[i] = team_sum(same_column_sum(v[i], a.columns), a.per_group);
+    __syncthreads();
+    if (lane < a.columns && l.q == 0) {
+#pragma unroll
+      for (int i = 0; i < N; ++i) sh[wave * total + i * groups + l.g] = v[i];
+    }
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      v[i] = 0.0f;
+      for (int w = 0; w < waves; ++w) v[i] += sh[w * total + i * groups + l.g];
+    }
+  } else if ((a.per_group & 63) == 0) {
+    // a wave has one group
+    const int per_row = a.columns >> 6, per_group = a.per_group >> 6, first = l.g * per_group;
+#pragma unroll
+    for (int i = 0; i < N; ++i) v[i] = team_sum(v[i], 64);
+    __syncthreads();
+    if (lane == 0) {
+#pragma unroll
+      for (int i = 0; i < N; ++i) sh[i * waves + wave] = v[i];
+    }
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      v[i] = 0.0f;
+      for (int r = 0; r < a.R; ++r)
+        for (int w = 0; w < per_group; ++w) v[i] += sh[i * waves + r * per_row + first + w];
+    }
+  } else {
+    sum_rows<N>(v, sh, a, l);
+    sum_group<N>(v, sh, a, l);
+  }
 }
 
 struct Moments {
@@ -391,20 +488,24 @@ __device__ __forceinline__ Moments merge_group(Moments v, float* sh, const Block
   return get(l.g * a.per_group);
 }
 
-// Where a workgroup's part of a group's statistics lies, and the values of one.
+// The number of this workgroup's part of its groups' statistics, and where it lies.
+__device__ __forceinline__ int64_t piece_of(const BlockArgs& a) {
+  const unsigned id = block_number(), chunk = id % unsigned(a.chunks), block = id / unsigned(a.chunks) % unsigned(a.blocks);
+  return int64_t(chunk) * a.parts + block % unsigned(a.parts);
+}
 __device__ __forceinline__ int64_t piece_index(const BlockArgs& a, int64_t n, int64_t group, int64_t piece) {
   return ((n * a.chunks * a.parts + piece) * a.p.groups + group) * 2;
 }
 
 constexpr int NORM_HELD = 0, NORM_STATS = 1, NORM_APPLY = 2;
 template <int VEC, typename T>
-constexpr int held_rows() {  // of a lane: 32 registers' worth of one tensor
-  return 32 / (VEC * int(sizeof(T)) >= 4 ? VEC * int(sizeof(T)) / 4 : 1);
+constexpr int held_rows(bool two) {  // of a lane: 32 registers' worth, 24 of each of two 16-bit tensors (what they widen to needs more)
+  return (two && sizeof(T) == 2 ? 24 : 32) / (VEC * int(sizeof(T)) >= 4 ? VEC * int(sizeof(T)) / 4 : 1);
 }
 
 template <typename T, int VEC, int LANES, int PHASE>
 __global__ __launch_bounds__(LANES) void norm_fwd_kernel(BlockArgs args) {
-  constexpr int KEEP = held_rows<VEC, T>();
+  constexpr int KEEP = held_rows<VEC, T>(false);
   __shared__ float sh[(PHASE == NORM_HELD ? 1 : 3) * LANES];
   const linrec_group_norm_t& p = args.p;
   const BlockLane l = block_lane<VEC>(args);
@@ -441,26 +542,24 @@ __global__ __launch_bounds__(LANES) void norm_fwd_kernel(BlockArgs args) {
         for (int e = 0; e < VEC; ++e) s[0] += v.v[e];
       }
     const float inv_count = 1.0f / (float(p.positions) * float(args.whole * VEC));
-    sum_rows<1>(s, sh, args, l);
-    sum_group<1>(s, sh, args, l);
+    sum_all<1>(s, sh, args, l);
     mean = s[0] * inv_count;
     s[0] = 0.0f;
 #pragma unroll
     for (int i = 0; i < KEEP; ++i)
       if (l.there && l.first + i * args.R < l.end) {
-        const Lanes<VEC> v = widen(held[i]);
+        const Lanes<VEC> v = widen(held_again(held[i]));
 #pragma unroll
         for (int e = 0; e < VEC; ++e) {
           const float d = v.v[e] - mean;
           s[0] = fmaf(d, d, s[0]);
         }
       }
-    sum_rows<1>(s, sh, args, l);
-    sum_group<1>(s, sh, args, l);
+    sum_all<1>(s, sh, args, l);
     rstd = __builtin_amdgcn_rsqf(fmaf(s[0], inv_count, p.eps));
 #pragma unroll
     for (int i = 0; i < KEEP; ++i)
-      if (l.there && l.first + i * args.R < l.end) apply(held[i], l.first + i * args.R);
+      if (l.there && l.first + i * args.R < l.end) apply(held_again(held[i]), l.first + i * args.R);
   } else if constexpr (PHASE == NORM_STATS) {
     Moments m{0.0f, 0.0f, 0.0f};
     if (l.there && l.first < l.end) {
@@ -489,7 +588,7 @@ __global__ __launch_bounds__(LANES) void norm_fwd_kernel(BlockArgs args) {
     }
     m = merge_group(m, sh, args, l);
     if (writes) {
-      const int64_t piece = int64_t(blockIdx.x % unsigned(args.chunks)) * args.parts + (blockIdx.x / unsigned(args.chunks)) % unsigned(args.blocks) % unsigned(args.parts);
+      const int64_t piece = piece_of(args);
       float* out = p.partial + piece_index(args, l.n, l.group, piece);
       out[0] = m.mean;
       out[1] = m.m2;
@@ -531,7 +630,7 @@ __global__ __launch_bounds__(LANES) void norm_fwd_kernel(BlockArgs args) {
 // PARTIAL layout of the backward: the pieces' sums (chunks only), then a row of 2 * channels sums for every (item block, chunk).
 template <typename T, int VEC, int LANES, int PHASE>
 __global__ __launch_bounds__(LANES) void norm_bwd_kernel(BlockArgs args, float* param_sums) {
-  constexpr int KEEP = held_rows<VEC, T>();
+  constexpr int KEEP = held_rows<VEC, T>(true);
   __shared__ float sh[(PHASE == NORM_APPLY ? 2 : 2 * VEC) * LANES];
   const linrec_group_norm_t& p = args.p;
   const BlockLane l = block_lane<VEC>(args);
@@ -581,7 +680,7 @@ __global__ __launch_bounds__(LANES) void norm_bwd_kernel(BlockArgs args, float* 
   // the columns' sums, from there those of d_weight and d_bias and the group's
   auto finish_sums = [&]() __attribute__((always_inline)) {
     sum_rows<2 * VEC>(sums, sh, args, l);
-    if (l.there && l.r == 0) {
+    if (l.there && (l.r == 0 || columns_in_wave(args))) {
 #pragma unroll
       for (int i = 0; i < VEC; ++i) {
         s[0] = fmaf(sums[i], w[i], s[0]);
@@ -601,13 +700,14 @@ __global__ __launch_bounds__(LANES) void norm_bwd_kernel(BlockArgs args, float* 
         for (int i = 0; i < 2 * VEC; ++i) {
           float t = sh[i * LANES + l.vc];
           for (int q = 1; q < args.items; ++q) t += sh[i * LANES + q * width + l.vc];
-          const unsigned id = blockIdx.x;
+          const unsigned id = block_number();
           const int64_t row = int64_t(id / unsigned(args.chunks) / unsigned(args.blocks)) * args.chunks + id % unsigned(args.chunks);
           param_sums[(row * 2 + i / VEC) * p.channels + l.channel + i % VEC] = t;
         }
       }
     }
-    sum_group<2>(s, sh, args, l);
+    if (!columns_in_wave(args) && (args.per_group & 63) == 0) sum_all<2>(s, sh, args, l);  // (nothing in the rows but the first)
+    else sum_group<2>(s, sh, args, l);
   };
   const float inv_count = 1.0f / (float(p.positions) * float(args.whole * VEC));
 
@@ -629,7 +729,7 @@ __global__ __launch_bounds__(LANES) void norm_bwd_kernel(BlockArgs args, float* 
     s[1] *= inv_count;
 #pragma unroll
     for (int i = 0; i < KEEP; ++i)
-      if (l.there && l.first + i * args.R < l.end) apply(hx[i], hd[i], l.first + i * args.R);
+      if (l.there && l.first + i * args.R < l.end) apply(held_again(hx[i]), held_again(hd[i]), l.first + i * args.R);
   } else {
     auto walk = [&](auto&& f) __attribute__((always_inline)) {
       if (!l.there) return;
@@ -650,7 +750,7 @@ __global__ __launch_bounds__(LANES) void norm_bwd_kernel(BlockArgs args, float* 
       walk([&](const Held<T, VEC>& hx, const Held<T, VEC>& hd, int64_t) { add(hx, hd); });
       finish_sums();
       if (l.there && l.r == 0 && l.q == 0) {
-        const int64_t piece = int64_t(blockIdx.x % unsigned(args.chunks)) * args.parts + (blockIdx.x / unsigned(args.chunks)) % unsigned(args.blocks) % unsigned(args.parts);
+        const int64_t piece = piece_of(args);
         float* out = p.partial + piece_index(args, l.n, l.group, piece);
         out[0] = s[0];
         out[1] = s[1];
@@ -664,8 +764,7 @@ __global__ __launch_bounds__(LANES) void norm_bwd_kernel(BlockArgs args, float* 
           s[1] += in[1];
         }
       }
-      sum_rows<2>(s, sh, args, l);
-      sum_group<2>(s, sh, args, l);
+      sum_all<2>(s, sh, args, l);
       s[0] *= inv_count;
       s[1] *= inv_count;
       walk([&](const Held<T, VEC>& hx, const Held<T, VEC>& hd, int64_t pos) { apply(hx, hd, pos); });

@@ -19,9 +19,6 @@ __global__ __launch_bounds__(64 * SUM_WAVES) void param_gradient_kernel(const fl
   });
 }
 
-#ifndef HELD_LINE
-#define HELD_LINE 64
-#endif
 enum class Shape { tokens, held, chunks };
 struct NormPlan {
   Shape shape;
@@ -49,21 +46,29 @@ NormPlan make_norm_plan(int dtype, int64_t batch, int64_t positions, int64_t cha
   while (width % pl.vec) pl.vec >>= 1;
   const int64_t columns = width / pl.vec;  // of a group
 
-  if (positions == 1 && width <= 1024) {
+  // 16 channels to a lane, at most eight waves to a group
+  if (positions == 1 && width <= 16 * 64 * TOKEN_WAVES) {
     pl.shape = Shape::tokens;
     TokenArgs& t = pl.tokens;
-    t.team = columns < 64 ? pow2_at_least(columns) : 64;
-    pl.items_per_lane = columns <= 64 ? 1 : 16 / pl.vec;
-    const int64_t waves = cdiv(groups, 64 / t.team);  // of a row
+    // one slot to a lane while eight waves hold a group so: the registers of more cost rows under way
+    const int64_t slots_of_lane = columns <= 64 * TOKEN_WAVES ? 1 : 16 / pl.vec;
+    pl.items_per_lane = int(slots_of_lane);
+    t.team = pow2_at_least(cdiv(columns, slots_of_lane));
+    const int64_t waves = t.team < 64 ? cdiv(groups, 64 / t.team) : groups * (t.team / 64);  // of a row
     t.column_waves = waves < TOKEN_WAVES ? pow2_at_least(waves) : TOKEN_WAVES;
     t.column_blocks = int(cdiv(waves, t.column_waves));
     const int64_t slots = TOKEN_WAVES / t.column_waves;
-    // enough workgroups for the chip; in the backward each leaves a row of sums behind
-    const int64_t most = bwd ? 512 : 1024;
+    // enough workgroups for the chip; in the backward each leaves a row of sums behind, 8 bytes a channel, so a wave walks eight
+    // rows first (2048 x 4096 in bf16: 32 us with a row of sums to every four)
     int64_t row_blocks = cdiv(batch, slots);
+    int64_t most = 1024;
+    if (bwd) {
+      most = cdiv(batch, slots * 8);
+      most = most < 128 ? 128 : most > 512 ? 512 : most;
+    }
     const int64_t cap = most / t.column_blocks > 1 ? most / t.column_blocks : 1;
     if (row_blocks > cap) row_blocks = cap;
-    t.row_blocks = int(row_blocks < 1 ? 1 : row_blocks);
+    t.row_blocks = int(row_blocks);
     pl.lanes = 64 * TOKEN_WAVES;
     pl.grid = int64_t(t.row_blocks) * t.column_blocks;
     pl.param_rows = t.row_blocks;
@@ -77,9 +82,10 @@ NormPlan make_norm_plan(int dtype, int64_t batch, int64_t positions, int64_t cha
   const int keep = (bwd && size == 2 ? 24 : 32) / (bytes >= 4 ? bytes / 4 : 1);
   auto rows_of = [](int lanes, int64_t wide) { return wide <= lanes ? lanes / wide : int64_t(0); };
   auto rounds = [&](int lanes, int64_t wide) { return rows_of(lanes, wide) ? cdiv(positions, rows_of(lanes, wide)) : int64_t(1) << 40; };
-  for (const int line : {128, HELD_LINE}) {
+  for (const int line : {128, 64}) {
     int64_t g = cdiv(line, columns * bytes);
     if (g > groups) g = groups;
+    while (g > 1 && cdiv(groups, g) * batch < 256) g = g / 2;  // (so few that the chip idles: latency, not lines)
     for (const int lanes : {256, 1024}) {
       if (rounds(lanes, g * columns) > keep) continue;
       // few workgroups: more lanes to each
@@ -88,7 +94,7 @@ NormPlan make_norm_plan(int dtype, int64_t batch, int64_t positions, int64_t cha
       // lanes that have nothing to do take more groups, or more batch items; so do short walks while the chip stays full
       auto grows = [&](int64_t gg, int64_t it) {
         const int64_t n = rounds(lanes, gg * columns * it);
-        return n == 1 || (n <= keep / 2 && cdiv(groups, gg) * cdiv(batch, it) >= 1024);
+        return n == 1 || (n <= (bwd ? keep : keep / 2) && cdiv(groups, gg) * cdiv(batch, it) >= (bwd ? 512 : 1024));
       };
       while (2 * g <= groups && grows(2 * g, 1)) g *= 2;
       if (g < groups && 2 * g > groups && grows(groups, 1)) g = groups;

@@ -83,14 +83,24 @@ __device__ __forceinline__ void activate_slope(int act, const float (&z)[N], flo
   }
 }
 
+template <int VEC, typename T>
+__device__ __forceinline__ void widen_params(const void* p, int64_t c, float (&out)[VEC]) {
+  const Lanes<VEC> v = widen(ld_any<VEC, false>(static_cast<const T*>(p) + c));
+#pragma unroll
+  for (int e = 0; e < VEC; ++e) out[e] = v.v[e];
+}
 template <int VEC>
 __device__ __forceinline__ void load_params(const void* p, int dtype, int64_t c, float none, float (&out)[VEC]) {
+  if (!p) {
 #pragma unroll
-  for (int e = 0; e < VEC; ++e)
-    out[e] = !p                              ? none
-             : dtype == LINREC_DTYPE_F32     ? static_cast<const float*>(p)[c + e]
-             : dtype == LINREC_DTYPE_F16     ? float(static_cast<const _Float16*>(p)[c + e])
-                                             : float(static_cast<const __bf16*>(p)[c + e]);
+    for (int e = 0; e < VEC; ++e) out[e] = none;
+  } else if (dtype == LINREC_DTYPE_F32) {
+    widen_params<VEC, float>(p, c, out);
+  } else if (dtype == LINREC_DTYPE_F16) {
+    widen_params<VEC, _Float16>(p, c, out);
+  } else {
+    widen_params<VEC, __bf16>(p, c, out);
+  }
 }
 
 // ---- sums over the lanes of a team ------------------------------------------------------------
@@ -121,52 +131,64 @@ __device__ __forceinline__ float team_sum(float v, int lanes) {
 constexpr int TOKEN_WAVES = 8;
 struct TokenArgs {
   linrec_group_norm_t p;
-  int team;          // lanes of a group
+  int team;          // lanes of a group: a power of two up to 64, or whole waves side by side
   int column_waves;  // waves of a workgroup side by side over the channels (a power of two), the others take other rows
   int column_blocks;
   int row_blocks;
 };
 
+// Sums over a team; one of several waves goes through LDS (`turn` alternates, so that one barrier a sum is enough).
+template <int N>
+__device__ __forceinline__ void team_sums(float (&v)[N], int team, float (*sh)[TOKEN_WAVES][N], int& turn, int wave) {
+#pragma unroll
+  for (int i = 0; i < N; ++i) v[i] = team_sum(v[i], team);
+  if (team > 64) {
+    float(*mine)[N] = sh[turn];
+    turn ^= 1;
+    if ((threadIdx.x & 63) == 0) {
+#pragma unroll
+      for (int i = 0; i < N; ++i) mine[wave][i] = v[i];
+    }
+    __syncthreads();
+    const int waves = team >> 6, first = wave & ~(waves - 1);
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      v[i] = 0.0f;
+      for (int w = 0; w < waves; ++w) v[i] += mine[first + w][i];
+    }
+  }
+}
+
 template <typename T, int VEC, int ITEMS, bool BWD>
 __global__ __launch_bounds__(64 * TOKEN_WAVES) void norm_tokens_kernel(TokenArgs args) {
   constexpr int N = VEC * ITEMS;
+  __shared__ float sh_team[2][TOKEN_WAVES][BWD ? 2 : 1];
   const linrec_group_norm_t& p = args.p;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int block = int(blockIdx.x % unsigned(args.column_blocks)), row_block = int(blockIdx.x / unsigned(args.column_blocks));
   const int cw = wave & (args.column_waves - 1), row_slot = wave / args.column_waves, row_slots = TOKEN_WAVES / args.column_waves;
   const int width = int(p.channels / p.groups);
-  const int64_t g = (int64_t(block) * args.column_waves + cw) * (64 / args.team) + lane / args.team;
-  const int in_team = lane & (args.team - 1);
+  const int64_t column = (int64_t(block) * args.column_waves + cw) * 64 + lane;  // lane of the row
+  const int64_t g = column / args.team;
+  const int in_team = int(column - g * args.team);
   const bool there = g < p.groups;
   const int64_t c0 = (there ? g : 0) * width;
   bool has[ITEMS];
   int64_t c[ITEMS];
-  float w[N], b[N];
 #pragma unroll
   for (int i = 0; i < ITEMS; ++i) {
     const int o = (i * args.team + in_team) * VEC;  // (VEC divides the width: a slot lies in the group or not)
     has[i] = there && o < width;
     c[i] = c0 + (has[i] ? o : 0);
-    float wi[VEC], bi[VEC];
-    load_params<VEC>(p.weight, p.weight_dtype, c[i], 1.0f, wi);
-    load_params<VEC>(p.bias, p.weight_dtype, c[i], 0.0f, bi);
-#pragma unroll
-    for (int e = 0; e < VEC; ++e) {
-      w[i * VEC + e] = wi[e];
-      b[i * VEC + e] = bi[e];
-    }
   }
   const int64_t step = int64_t(args.row_blocks) * row_slots;
   const float inv_count = 1.0f / float(width);
   const T* x = static_cast<const T*>(p.x);
   const T* dy = static_cast<const T*>(p.d_y);
-  float dw[BWD ? N : 1], db[BWD ? N : 1];
-#pragma unroll
-  for (int i = 0; i < (BWD ? N : 1); ++i) dw[i] = db[i] = 0.0f;
-
   Held<T, VEC> hx[ITEMS], hd[BWD ? ITEMS : 1];
   float mean = 0.0f, rstd = 0.0f;
   auto load = [&](int64_t n) __attribute__((always_inline)) {
+    if (n >= p.batch) n = p.batch - 1;  // (read and not used)
 #pragma unroll
     for (int i = 0; i < ITEMS; ++i) {
       hx[i] = ld_any<VEC, true>(x + n * p.x_stride[0] + c[i]);
@@ -177,9 +199,28 @@ __global__ __launch_bounds__(64 * TOKEN_WAVES) void norm_tokens_kernel(TokenArgs
       rstd = p.rstd[n * p.groups + (there ? g : 0)];
     }
   };
-  int64_t n = int64_t(row_block) * row_slots + row_slot;
-  if (n < p.batch) load(n);
-  for (; n < p.batch; n += step) {
+  int64_t base = int64_t(row_block) * row_slots;  // the same for all waves: they meet at barriers
+  load(base + row_slot);
+  float w[N], b[N];
+#pragma unroll
+  for (int i = 0; i < ITEMS; ++i) {
+    float wi[VEC], bi[VEC];
+    load_params<VEC>(p.weight, p.weight_dtype, c[i], 1.0f, wi);
+    load_params<VEC>(p.bias, p.weight_dtype, c[i], 0.0f, bi);
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) {
+      w[i * VEC + e] = wi[e];
+      b[i * VEC + e] = bi[e];
+    }
+  }
+  float dw[BWD ? N : 1], db[BWD ? N : 1];
+#pragma unroll
+  for (int i = 0; i < (BWD ? N : 1); ++i) dw[i] = db[i] = 0.0f;
+
+  int turn = 0;
+  for (; base < p.batch; base += step) {
+    const int64_t n = base + row_slot;
+    const bool row = n < p.batch;
     float v[N], d[BWD ? N : 1];
     float m = mean, r = rstd;
 #pragma unroll
@@ -193,20 +234,22 @@ __global__ __launch_bounds__(64 * TOKEN_WAVES) void norm_tokens_kernel(TokenArgs
         for (int e = 0; e < VEC; ++e) d[i * VEC + e] = u.v[e];
       }
     }
-    if (n + step < p.batch) load(n + step);  // (under way while this row is worked on)
+    load(n + step);  // (under way while this row is worked on; two rows ahead gained nothing)
     if constexpr (!BWD) {
-      float s = 0.0f;
+      float s[1] = {0.0f};
 #pragma unroll
-      for (int i = 0; i < N; ++i) s += has[i / VEC] ? v[i] : 0.0f;
-      m = team_sum(s, args.team) * inv_count;
-      s = 0.0f;
+      for (int i = 0; i < N; ++i) s[0] += has[i / VEC] ? v[i] : 0.0f;
+      team_sums<1>(s, args.team, sh_team, turn, wave);
+      m = s[0] * inv_count;
+      s[0] = 0.0f;
 #pragma unroll
       for (int i = 0; i < N; ++i) {
         v[i] -= m;
-        s = fmaf(has[i / VEC] ? v[i] : 0.0f, v[i], s);
+        s[0] = fmaf(has[i / VEC] ? v[i] : 0.0f, v[i], s[0]);
       }
-      r = __builtin_amdgcn_rsqf(fmaf(team_sum(s, args.team), inv_count, p.eps));
-      if (there && in_team == 0) {
+      team_sums<1>(s, args.team, sh_team, turn, wave);
+      r = __builtin_amdgcn_rsqf(fmaf(s[0], inv_count, p.eps));
+      if (row && there && in_team == 0) {
         p.mean[n * p.groups + g] = m;
         p.rstd[n * p.groups + g] = r;
       }
@@ -214,7 +257,7 @@ __global__ __launch_bounds__(64 * TOKEN_WAVES) void norm_tokens_kernel(TokenArgs
       for (int i = 0; i < N; ++i) v[i] = fmaf(v[i] * r, w[i], b[i]);
       activate<N>(p.act, v);
     } else {
-      float z[N], s1 = 0.0f, s2 = 0.0f;
+      float z[N], s[2] = {0.0f, 0.0f};
 #pragma unroll
       for (int i = 0; i < N; ++i) {
         v[i] = (v[i] - m) * r;
@@ -223,15 +266,15 @@ __global__ __launch_bounds__(64 * TOKEN_WAVES) void norm_tokens_kernel(TokenArgs
       activate_slope<N>(p.act, z, d);
 #pragma unroll
       for (int i = 0; i < N; ++i) {
-        if (!has[i / VEC]) d[i] = v[i] = 0.0f;
+        if (!(has[i / VEC] && row)) d[i] = v[i] = 0.0f;
         dw[i] = fmaf(d[i], v[i], dw[i]);
         db[i] += d[i];
         d[i] *= w[i];
-        s1 += d[i];
-        s2 = fmaf(d[i], v[i], s2);
+        s[0] += d[i];
+        s[1] = fmaf(d[i], v[i], s[1]);
       }
-      s1 = team_sum(s1, args.team) * inv_count;
-      s2 = team_sum(s2, args.team) * inv_count;
+      team_sums<2>(s, args.team, sh_team, turn, wave);
+      const float s1 = s[0] * inv_count, s2 = s[1] * inv_count;
 #pragma unroll
       for (int i = 0; i < N; ++i) v[i] = r * (d[i] - fmaf(v[i], s2, s1));
     }
@@ -241,14 +284,14 @@ __global__ __launch_bounds__(64 * TOKEN_WAVES) void norm_tokens_kernel(TokenArgs
       Lanes<VEC> t;
 #pragma unroll
       for (int e = 0; e < VEC; ++e) t.v[e] = v[i * VEC + e];
-      if (has[i]) st_any<VEC>(out + c[i], t);
+      if (has[i] && row) st_any<VEC>(out + c[i], t);
     }
   }
   if constexpr (BWD) {
     if (!p.weight) return;
     // the waves that had the same channels
     __shared__ float sh[TOKEN_WAVES][64];
-    float* row = p.partial + int64_t(row_block) * 2 * p.channels;
+    float* to = p.partial + int64_t(row_block) * 2 * p.channels;
 #pragma unroll
     for (int i = 0; i < N; ++i) {
 #pragma unroll
@@ -259,7 +302,7 @@ __global__ __launch_bounds__(64 * TOKEN_WAVES) void norm_tokens_kernel(TokenArgs
         if (row_slot == 0 && has[i / VEC]) {
           float s = sh[cw][lane];
           for (int q = 1; q < row_slots; ++q) s += sh[q * args.column_waves + cw][lane];
-          row[which * p.channels + c[i / VEC] + i % VEC] = s;
+          to[which * p.channels + c[i / VEC] + i % VEC] = s;
         }
       }
     }
@@ -512,10 +555,12 @@ __global__ __launch_bounds__(LANES) void norm_fwd_kernel(BlockArgs args) {
   const T* x = static_cast<const T*>(p.x) + l.n * p.x_stride[0] + l.channel;
   T* y = static_cast<T*>(p.y) + l.n * p.positions * p.channels + l.channel;
   float w[VEC], b[VEC];
-  if (PHASE != NORM_STATS && l.there) {
-    load_params<VEC>(p.weight, p.weight_dtype, l.channel, 1.0f, w);
-    load_params<VEC>(p.bias, p.weight_dtype, l.channel, 0.0f, b);
-  }
+  auto params = [&]() __attribute__((always_inline)) {
+    if (l.there) {
+      load_params<VEC>(p.weight, p.weight_dtype, l.channel, 1.0f, w);
+      load_params<VEC>(p.bias, p.weight_dtype, l.channel, 0.0f, b);
+    }
+  };
   float mean, rstd;
   auto apply = [&](const Held<T, VEC>& h, int64_t pos) __attribute__((always_inline)) {
     Lanes<VEC> v = widen(h);
@@ -534,6 +579,7 @@ __global__ __launch_bounds__(LANES) void norm_fwd_kernel(BlockArgs args) {
       const int64_t pos = l.first + i * args.R;
       if (l.there && pos < l.end) held[i] = ld_any<VEC, true>(x + pos * p.x_stride[1]);
     }
+    params();
 #pragma unroll
     for (int i = 0; i < KEEP; ++i)
       if (l.there && l.first + i * args.R < l.end) {
@@ -595,6 +641,7 @@ __global__ __launch_bounds__(LANES) void norm_fwd_kernel(BlockArgs args) {
     }
     return;
   } else {
+    params();
     // the lanes of a group share its pieces out
     Moments m{0.0f, 0.0f, 0.0f};
     const int pieces = args.chunks * args.parts;

@@ -99,25 +99,42 @@ int linrec_embedding_bwd(const linrec_embedding_t* p) {
     int* key = reinterpret_cast<int*>(scratch + s.sorted[i]);
     return Sorted{key, key + p->tokens};
   };
+  // the gradient is cleared in equal shares by the sort's launches
+  const int64_t bytes = p->vocab * p->channels * (p->dtype == LINREC_DTYPE_F32 ? 4 : 2), slots = bytes / 16;
+  const int passes = int(cdiv(bit_length(p->vocab), DIGIT_BITS));  // (the key of what takes no part is `vocab`)
+  const int shares = p->tokens <= SORT_SMALL ? 1 : 2 * passes;
+  int share = 0;
+  auto next_share = [&](int64_t* blocks) {
+    Clear c{slots * share / shares, slots * (share + 1) / shares, 0};
+    if (++share == shares) c.tail = int(bytes % 16 / 2);
+    const int64_t n = cdiv(c.end - c.first, 4096);
+    *blocks = n < 1 ? 1 : n > 256 ? 256 : n;
+    return c;
+  };
   Sorted sorted = lists(0);
-  if (p->tokens == 0) {
-  } else if (p->tokens <= SORT_SMALL) {
-    if (const int rc = launch_kernel(sort_small_kernel, cdiv(p->tokens, SMALL_TAKE), 1, 1024, p->stream, *p, sorted)) return rc;
+  int64_t clearing;
+  if (p->tokens <= SORT_SMALL) {
+    const int64_t blocks = cdiv(p->tokens, SMALL_TAKE);
+    const Clear c = next_share(&clearing);
+    if (const int rc = launch_kernel(sort_small_kernel, blocks + clearing, 1, 1024, p->stream, *p, sorted, int(blocks), c)) return rc;
   } else {
     int* counts = reinterpret_cast<int*>(scratch + s.counts);
-    const int passes = int(cdiv(bit_length(p->vocab), DIGIT_BITS));  // (the key of what takes no part is `vocab`)
     const int* keys = nullptr;
     const int* positions = nullptr;
     for (int i = 0; i < passes; ++i) {
       sorted = lists(i & 1);
-      if (const int rc = launch_kernel(digit_counts_kernel, s.blocks, 1, SORT_LANES, p->stream, *p, keys, i * DIGIT_BITS, counts)) return rc;
-      if (const int rc = launch_kernel(digit_places_kernel, s.blocks, 1, SORT_LANES, p->stream, *p, keys, positions, i * DIGIT_BITS, counts,
-                                       int(s.blocks), sorted))
+      Clear c = next_share(&clearing);
+      if (const int rc = launch_kernel(digit_counts_kernel, s.blocks + clearing, 1, SORT_LANES, p->stream, *p, keys, i * DIGIT_BITS, counts, int(s.blocks), c))
+        return rc;
+      c = next_share(&clearing);
+      if (const int rc = launch_kernel(digit_places_kernel, s.blocks + clearing, 1, SORT_LANES, p->stream, *p, keys, positions, i * DIGIT_BITS, counts,
+                                       int(s.blocks), sorted, c))
         return rc;
       keys = sorted.key;
       positions = sorted.pos;
     }
   }
+  if (p->tokens == 0) return LINREC_OK;
   return with_slot(p->dtype, p->channels, [&](auto t, auto vec) {
     using T = decltype(t);
     constexpr int VEC = decltype(vec)::value;
@@ -130,10 +147,7 @@ int linrec_embedding_bwd(const linrec_embedding_t* p) {
     if (const int rc = launch_kernel(run_sums_kernel<T, VEC, true>, cdiv(s.n_runs2 * column_waves, 4), 1, 256, p->stream, *p, sorted, runs, runs2,
                                      s.n_runs2, column_waves))
       return rc;
-    int64_t rows = p->vocab * column_waves / 16384;  // enough waves for the chip first
-    rows = rows < 1 ? 1 : rows > 8 ? 8 : rows;
-    return launch_kernel(table_rows_kernel<T, VEC>, cdiv(cdiv(p->vocab, rows) * column_waves, 4), 1, 256, p->stream, *p, sorted, runs, runs2, int(rows),
-                         column_waves);
+    return launch_kernel(list_sums_kernel<T, VEC>, cdiv(cdiv(p->tokens, OWN) * column_waves, 4), 1, 256, p->stream, *p, sorted, runs, runs2, column_waves);
   });
 }
 

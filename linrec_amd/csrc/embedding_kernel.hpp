@@ -2,15 +2,19 @@
 //
 // Forward: a wave copies 64 slots of channels of a few rows.  Bound by memory; a row that is looked up again comes from a cache.
 //
-// Backward, without atomics on values: the positions are sorted by token (stably, so that each list of positions ascends), then
-// every row of the table is written once, by the wave that finds its list in the sorted tokens.
+// Backward, without atomics on values: the positions are sorted by token (stably, so that each list of positions ascends), the
+// gradient is cleared meanwhile, and every list is summed by the wave that finds its start in the sorted tokens.
 //   sort   up to SORT_SMALL tokens in one launch: the place of a position is the number of smaller (token, position) pairs, all
 //          pairs compared; more are sorted by digits of at most DIGIT_BITS bits from the lowest on, two launches each (counts
 //          of blocks; places).  Places are counted, never drawn, so the order is the same in every run.
-//   sums   a list may be as long as all positions.  Aligned runs of 64 sorted positions with one token are summed first, a wave
-//          each, then aligned runs of 64 of those; a row adds up what is left before, the two kinds of runs, and what is left
-//          after, at most 63 of each kind and end.  The grouping depends on the tokens alone.
-// Bound by memory: d_y is read once, the table's gradient written once.
+//   clear  a few workgroups sort; the others of the same launches write zeros, whole lines front to back, a share in each launch.
+//          (Rows of zeros written one by one where a row has no list: 128000 x 333 fp32 58 us for that launch alone.)
+//   sums   a list may be as long as all positions, and a wave takes a microsecond for every eight rows it adds up.  Aligned runs of
+//          16 sorted positions with one token are summed first, a wave each, then aligned runs of 16 of those; a long list adds
+//          up what is left before, the two kinds of runs, and what is left after, at most 15 of the smaller kinds at each end.
+//          The grouping depends on the tokens alone.  (Runs of 64 and of 64 times 64: 36 us for the sums of 32768 words where
+//          these take 28.)
+// Bound by memory: d_y is read once, the table's gradient written once, rows that have a list twice.
 #pragma once
 #include <hip/hip_runtime.h>
 #include <stdint.h>
@@ -64,6 +68,19 @@ __global__ __launch_bounds__(256) void embedding_fwd_kernel(linrec_embedding_t p
   }
 }
 
+// ---- clear ------------------------------------------------------------------------------------
+// The share of a launch: `first` .. `end` of the gradient's 16-byte slots, and what is left of a slot at its end.
+struct Clear {
+  int64_t first, end;
+  int tail;  // 2-byte words behind the last slot
+};
+__device__ __forceinline__ void clear_share(const linrec_embedding_t& p, const Clear& c, int64_t block, int64_t blocks) {
+  typedef unsigned Slot __attribute__((ext_vector_type(4), aligned(2)));  // (any alignment that a tensor has)
+  Slot* to = static_cast<Slot*>(p.d_weight);
+  for (int64_t i = c.first + block * blockDim.x + threadIdx.x; i < c.end; i += blocks * blockDim.x) __builtin_nontemporal_store(Slot{0u, 0u, 0u, 0u}, to + i);
+  if (block == 0 && int(threadIdx.x) < c.tail) reinterpret_cast<unsigned short*>(to + c.end)[threadIdx.x] = 0;
+}
+
 // ---- sort -------------------------------------------------------------------------------------
 struct Sorted {
   int* key;
@@ -74,7 +91,8 @@ constexpr int SORT_SMALL = 8192;
 constexpr int SMALL_TAKE = 32;  // positions a workgroup places
 
 // All pairs: 1024 lanes compare SMALL_TAKE positions with a 32nd of all keys each.
-__global__ __launch_bounds__(1024) void sort_small_kernel(linrec_embedding_t p, Sorted out) {
+__global__ __launch_bounds__(1024) void sort_small_kernel(linrec_embedding_t p, Sorted out, int blocks, Clear clear) {
+  if (int(blockIdx.x) >= blocks) return clear_share(p, clear, blockIdx.x - blocks, gridDim.x - blocks);
   __shared__ alignas(16) int keys[SORT_SMALL];
   __shared__ int counts[32][SMALL_TAKE + 1];
   const int n = int(p.tokens), tid = int(threadIdx.x);
@@ -105,7 +123,9 @@ constexpr int SORT_LANES = 1024, SORT_WAVES = SORT_LANES / 64, SORT_ROUNDS = 2, 
 
 __device__ __forceinline__ int key_of(const linrec_embedding_t& p, const int* keys, int64_t i) { return keys ? keys[i] : sort_key(p, i); }
 
-__global__ __launch_bounds__(SORT_LANES) void digit_counts_kernel(linrec_embedding_t p, const int* keys, int shift, int* counts) {
+__global__ __launch_bounds__(SORT_LANES) void digit_counts_kernel(linrec_embedding_t p, const int* keys, int shift, int* counts, int blocks,
+                                                                  Clear clear) {
+  if (int(blockIdx.x) >= blocks) return clear_share(p, clear, blockIdx.x - blocks, gridDim.x - blocks);
   __shared__ int bins[DIGITS];
   const int tid = int(threadIdx.x);
   if (tid < DIGITS) bins[tid] = 0;
@@ -121,11 +141,22 @@ __global__ __launch_bounds__(SORT_LANES) void digit_counts_kernel(linrec_embeddi
 
 // A position goes behind all of smaller digits, those of its digit in blocks before, in waves before and before it in its wave.
 __global__ __launch_bounds__(SORT_LANES) void digit_places_kernel(linrec_embedding_t p, const int* keys, const int* positions, int shift,
-                                                                  const int* counts, int blocks, Sorted out) {
+                                                                  const int* counts, int blocks, Sorted out, Clear clear) {
+  if (int(blockIdx.x) >= blocks) return clear_share(p, clear, blockIdx.x - blocks, gridDim.x - blocks);
   __shared__ int base[DIGITS];
   __shared__ int wave_sums[DIGITS / 64];
   __shared__ int bins[SORT_WAVES][DIGITS];
   const int tid = int(threadIdx.x), lane = tid & 63, wave = tid >> 6;
+  // a wave takes 64 * SORT_ROUNDS adjacent positions, in order
+  const int64_t first = int64_t(blockIdx.x) * SORT_BLOCK + wave * (64 * SORT_ROUNDS) + lane;
+  int key[SORT_ROUNDS], pos[SORT_ROUNDS], rank[SORT_ROUNDS];
+#pragma unroll
+  for (int r = 0; r < SORT_ROUNDS; ++r) {
+    const int64_t i = first + r * 64;
+    const bool there = i < p.tokens;
+    key[r] = there ? key_of(p, keys, i) : 0;
+    pos[r] = there ? (positions ? positions[i] : int(i)) : 0;
+  }
   for (int i = tid; i < SORT_WAVES * DIGITS; i += SORT_LANES) (&bins[0][0])[i] = 0;
   int all = 0, before = 0;
   if (tid < DIGITS) {
@@ -149,15 +180,9 @@ __global__ __launch_bounds__(SORT_LANES) void digit_places_kernel(linrec_embeddi
     for (int w = 0; w < wave; ++w) lower += wave_sums[w];
     base[tid] = lower + scan - all + before;
   }
-  // a wave takes 64 * SORT_ROUNDS adjacent positions, in order
-  const int64_t first = int64_t(blockIdx.x) * SORT_BLOCK + wave * (64 * SORT_ROUNDS) + lane;
-  int key[SORT_ROUNDS], pos[SORT_ROUNDS], rank[SORT_ROUNDS];
 #pragma unroll
   for (int r = 0; r < SORT_ROUNDS; ++r) {
-    const int64_t i = first + r * 64;
-    const bool there = i < p.tokens;
-    key[r] = there ? key_of(p, keys, i) : 0;
-    pos[r] = there ? (positions ? positions[i] : int(i)) : 0;
+    const bool there = first + r * 64 < p.tokens;
     const int digit = (key[r] >> shift) & (DIGITS - 1);
     uint64_t same = __ballot(there);
 #pragma unroll
@@ -194,7 +219,7 @@ __global__ __launch_bounds__(SORT_LANES) void digit_places_kernel(linrec_embeddi
 }
 
 // ---- sums -------------------------------------------------------------------------------------
-constexpr int RUN = 64, RUN2 = RUN * RUN;
+constexpr int RUN = 16, RUN2 = RUN * RUN;
 
 template <int VEC>
 __device__ __forceinline__ void add_to(Lanes<VEC>& s, const Lanes<VEC>& v) {
@@ -202,15 +227,15 @@ __device__ __forceinline__ void add_to(Lanes<VEC>& s, const Lanes<VEC>& v) {
   for (int e = 0; e < VEC; ++e) s.v[e] += v.v[e];
 }
 // Adds `count` rows, row(i) their first value for this lane, in order.
-template <int VEC, typename Row>
+template <int VEC, int AT_ONCE = 8, typename Row>
 __device__ __forceinline__ void add_rows(Lanes<VEC>& sum, int count, Row&& row) {
   int i = 0;
-  for (; i + 8 <= count; i += 8) {
-    decltype(ld_any<VEC, false>(row(0))) h[8];
+  for (; i + AT_ONCE <= count; i += AT_ONCE) {
+    decltype(ld_any<VEC, false>(row(0))) h[AT_ONCE];
 #pragma unroll
-    for (int q = 0; q < 8; ++q) h[q] = ld_any<VEC, false>(row(i + q));
+    for (int q = 0; q < AT_ONCE; ++q) h[q] = ld_any<VEC, false>(row(i + q));
 #pragma unroll
-    for (int q = 0; q < 8; ++q) add_to(sum, widen(h[q]));
+    for (int q = 0; q < AT_ONCE; ++q) add_to(sum, widen(h[q]));
   }
   for (; i < count; ++i) add_to(sum, widen(ld_any<VEC, false>(row(i))));
 }
@@ -222,7 +247,7 @@ __device__ __forceinline__ Lanes<VEC> zeros() {
   return r;
 }
 
-// Runs of 64 positions of one token (SECOND: of 64 such sums): a wave each, for 64 slots of channels.
+// Runs of 16 positions of one token (SECOND: of 16 such sums): a wave each, for 64 slots of channels.
 template <typename T, int VEC, bool SECOND>
 __global__ __launch_bounds__(256) void run_sums_kernel(linrec_embedding_t p, Sorted sorted, const float* in, float* out, int64_t runs,
                                                        int64_t column_waves) {
@@ -236,97 +261,114 @@ __global__ __launch_bounds__(256) void run_sums_kernel(linrec_embedding_t p, Sor
   const int64_t c = wave_channel<VEC>(cw, lane, p.channels);
   Lanes<VEC> sum = zeros<VEC>();
   if constexpr (SECOND) {
-    add_rows<VEC>(sum, RUN, [&](int i) { return in + (run * RUN + i) * p.channels + c; });
+    add_rows<VEC, 16>(sum, RUN, [&](int i) { return in + (run * RUN + i) * p.channels + c; });
   } else {
-    const int pos = sorted.pos[run * RUN + lane];
+    const int pos = sorted.pos[run * RUN + (lane & (RUN - 1))];
     const T* dy = static_cast<const T*>(p.d_y) + c;
-    add_rows<VEC>(sum, RUN, [&](int i) { return dy + int64_t(__builtin_amdgcn_readlane(pos, i)) * p.d_y_stride; });
+    add_rows<VEC, 16>(sum, RUN, [&](int i) { return dy + int64_t(__builtin_amdgcn_readlane(pos, i)) * p.d_y_stride; });
   }
   float* to = out + run * p.channels + c;
 #pragma unroll
   for (int e = 0; e < VEC; ++e) to[e] = sum.v[e];
 }
 
-// Number of sorted keys below `key`: every lane asks for one of 64 evenly spaced ones at a time.
-__device__ __forceinline__ int keys_below(const int* keys, int n, int key, int lane) {
-  int lo = 0, len = n;  // the answer lies in [lo, lo + len]
-  while (len > 0) {
-    const int step = (len + 63) >> 6, i = lane * step;
-    const uint64_t below = __ballot(i < len && keys[lo + (i < len ? i : 0)] < key);
-    const int hits = __popcll(below);
-    if (hits == 0) return lo;
-    // the keys at 0, step, .. (hits - 1) * step are below, the next one asked for is not
-    const int skip = (hits - 1) * step + 1, rest = len - skip;
-    lo += skip;
-    len = rest < step - 1 ? rest : step - 1;
-  }
-  return lo;
+// Number of runs of `length` sorted positions from `at` on, at most `most` (up to 64), that hold token v alone (the first position
+// does).
+__device__ __forceinline__ int whole_runs(const int* keys, int n, int at, int length, int most, int v, int lane) {
+  const int64_t i = int64_t(at) + int64_t(lane + 1) * length - 1;
+  const uint64_t others = ~__ballot(lane < most && i < n && keys[i < n ? i : 0] == v);
+  return others ? __builtin_ctzll(others) : 64;
 }
 
-// A wave writes `rows` adjacent rows of the table's gradient, 64 slots of channels of each.
+// A wave sums the lists that start among OWN adjacent sorted positions, for 64 slots of channels, and writes their rows.
+constexpr int OWN = 8;
 template <typename T, int VEC>
-__global__ __launch_bounds__(256) void table_rows_kernel(linrec_embedding_t p, Sorted sorted, const float* runs, const float* runs2, int rows,
-                                                         int64_t column_waves) {
+__global__ __launch_bounds__(256) void list_sums_kernel(linrec_embedding_t p, Sorted sorted, const float* runs, const float* runs2,
+                                                        int64_t column_waves) {
   const int lane = threadIdx.x & 63;
   const int64_t unit = int64_t(blockIdx.x) * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int64_t row_set = unit / column_waves, cw = unit - row_set * column_waves;
-  const int64_t v0 = row_set * rows;
-  if (v0 >= p.vocab) return;
-  const int64_t v1 = v0 + rows < p.vocab ? v0 + rows : p.vocab;
+  const int64_t set = unit / column_waves, cw = unit - set * column_waves;
+  const int n = int(p.tokens), vocab = int(p.vocab);
+  if (set * OWN >= n) return;
+  const int first = int(set) * OWN;
   const int64_t c = wave_channel<VEC>(cw, lane, p.channels);
   const T* dy = static_cast<const T*>(p.d_y) + c;
   T* out = static_cast<T*>(p.d_weight) + c;
-  const int n = int(p.tokens);
-  int at = __builtin_amdgcn_readfirstlane(keys_below(sorted.key, n, int(v0), lane));
-  // a window of 64 aligned sorted positions
-  int base = at & ~(RUN - 1), key = 2147483647, pos = 0;
+  // 64 sorted positions; what lies behind them all, or has no part in the gradient, has keys of `vocab` and up
+  int base = first, key = 2147483647, pos = 0;
   auto look = [&]() __attribute__((always_inline)) {
     const bool there = base + lane < n;
     key = there ? sorted.key[base + lane] : 2147483647;
     pos = there ? sorted.pos[base + lane] : 0;
   };
   look();
-  for (int64_t v = v0; v < v1; ++v) {
-    Lanes<VEC> sum = zeros<VEC>();
-    for (;;) {
-      const uint64_t ours = __ballot(key == int(v)) >> (at - base);
-      const int count = ours == ~0ull ? 64 : __builtin_ctzll(~ours);
-      if (count == 64) {  // a whole run, perhaps many
-        int whole = 0, length = RUN;
-        const float* from = runs;
-        if ((base & (RUN2 - 1)) == 0) {
-          const int64_t i = int64_t(base) + int64_t(lane) * RUN2 + RUN2 - 1;
-          const uint64_t m = __ballot(i < n && sorted.key[i < n ? i : 0] == int(v));
-          whole = m == ~0ull ? 64 : __builtin_ctzll(~m);
-          if (whole > 0) {
-            length = RUN2;
-            from = runs2;
-          }
-        }
-        if (whole == 0) {
-          const int64_t i = int64_t(base) + int64_t(lane) * RUN + RUN - 1;
-          const int until = RUN - (base / RUN & (RUN - 1));  // runs up to the next run of runs
-          const uint64_t m = __ballot(lane < until && i < n && sorted.key[i < n ? i : 0] == int(v));
-          whole = m == ~0ull ? 64 : __builtin_ctzll(~m);
-        }
-        const float* first = from + int64_t(base / length) * p.channels + c;
-        add_rows<VEC>(sum, whole, [&](int i) { return first + int64_t(i) * p.channels; });
-        at = base += whole * length;
-        look();
-        continue;
-      }
-      add_rows<VEC>(sum, count, [&](int i) {
-        return dy + int64_t(__builtin_amdgcn_readlane(pos, at - base + i)) * p.d_y_stride;
-      });
-      at += count;
-      if (at - base < 64) break;  // a position of another token comes next (or none: their keys are the largest)
-      base += RUN;
-      look();
-    }
+  const int before = first > 0 ? sorted.key[first - 1] : -1;
+  const int left = __shfl_up(key, 1);
+  const uint64_t starts = __ballot(lane < OWN && key < vocab && key != (lane == 0 ? before : left));
+  if (starts == 0) return;
+  const int begin = __builtin_ctzll(starts), last = 63 - __builtin_clzll(starts);  // the first and the last list's lanes
+  const int last_key = __builtin_amdgcn_readlane(key, last);
+  const uint64_t of_last = ~(__ballot(key == last_key) >> last);
+  const int end = last + (of_last ? __builtin_ctzll(of_last) : 64 - last);  // of the last list in the window (zeros come in from above)
+  const bool longer = end >= 64 || end - last > 24;
+
+  auto store = [&](int v, Lanes<VEC>& sum) __attribute__((always_inline)) {
 #pragma unroll
     for (int e = 0; e < VEC; ++e) sum.v[e] *= p.scale;
-    st_any<VEC>(out + v * p.channels, sum);
+    st_any<VEC>(out + int64_t(v) * p.channels, sum);
+    sum = zeros<VEC>();
+  };
+  // Lists that end in the window: their positions one after the other, eight under way at a time, a row of the gradient stored
+  // whenever the token changes.
+  const int until = longer ? last : end;
+  Lanes<VEC> sum = zeros<VEC>();
+  int v = __builtin_amdgcn_readlane(key, begin);
+  for (int at = begin; at < until; at += 8) {
+    Held<T, VEC> h[8];
+#pragma unroll
+    for (int q = 0; q < 8; ++q)
+      if (at + q < until) h[q] = ld_any<VEC, false>(dy + int64_t(__builtin_amdgcn_readlane(pos, at + q)) * p.d_y_stride);
+#pragma unroll
+    for (int q = 0; q < 8; ++q)
+      if (at + q < until) {
+        const int token = __builtin_amdgcn_readlane(key, at + q);
+        if (token != v) {
+          store(v, sum);
+          v = token;
+        }
+        add_to(sum, widen(h[q]));
+      }
   }
+  if (until > begin) store(v, sum);
+  if (!longer) return;
+
+  // A long list.
+  v = last_key;
+  int at = first + last;
+  for (;;) {
+    base = at;
+    look();
+    const uint64_t others = ~__ballot(key == v);
+    const int count = others ? __builtin_ctzll(others) : 64;  // of the list, in the window
+    if ((at & (RUN - 1)) != 0 || count < RUN) {  // up to where a run may start, or the end
+      const int ahead = RUN - (at & (RUN - 1)), take = count < ahead ? count : ahead;
+      add_rows<VEC>(sum, take, [&](int i) { return dy + int64_t(__builtin_amdgcn_readlane(pos, i)) * p.d_y_stride; });
+      at += take;
+      if (take < ahead) break;
+      continue;
+    }
+    // whole runs from here on: of runs where one of them may start, else as many as come before that
+    int length = RUN2, whole = 0;
+    if ((at & (RUN2 - 1)) == 0) whole = whole_runs(sorted.key, n, at, RUN2, 64, v, lane);
+    if (whole == 0) {
+      length = RUN;
+      whole = whole_runs(sorted.key, n, at, RUN, RUN - (at / RUN & (RUN - 1)), v, lane);
+    }
+    const float* rows = (length == RUN2 ? runs2 : runs) + int64_t(at / length) * p.channels + c;
+    add_rows<VEC>(sum, whole, [&](int i) { return rows + int64_t(i) * p.channels; });
+    at += whole * length;
+  }
+  store(v, sum);
 }
 
 }  // namespace linrec

@@ -6,6 +6,7 @@ A call whose tensors look like an earlier call's (types, devices, sizes, strides
 only the pointers of that call's argument block in: on small tensors the checks took longer than the kernels.
 """
 import ctypes
+import itertools
 import threading
 
 import torch
@@ -83,13 +84,17 @@ _memory = threading.local()
 _REMEMBERED_MAX = 256
 
 
+_numbers = itertools.count()
+
+
 class _Entry:
     """What is known about calls of one kind: `args`, the argument block, and `ref`, a reference to it; `need`, bytes of
-    workspace; `sizes`, of results and scratch.  args is None where an input has to be copied into another layout first."""
-    __slots__ = ("args", "ref", "need", "sizes")
+    workspace; `sizes`, of results and scratch; `number`, its own.  args is None where an input has to be copied into another
+    layout first."""
+    __slots__ = ("args", "ref", "need", "sizes", "number")
 
     def __init__(self, args=None, need=0, sizes=()):
-        self.args, self.need, self.sizes = args, need, sizes
+        self.args, self.need, self.sizes, self.number = args, need, sizes, next(_numbers)
         self.ref = None if args is None else ctypes.byref(args)
 
 
@@ -220,8 +225,10 @@ def gated_saved_numel(dtype, batch, time, channels):
     return _lib.linrec_gated_saved_floats(DTYPES[dtype], batch, time, channels)
 
 
+# (A forward hands back the number of its kind of call as well: a backward of the same tensors is looked up by that and the
+# strides of the gradient.)
 def gated_fwd(x, gate_a, gate_x, rate, h0, cu_seqlens, reverse, scale, save):
-    """(h, state, saved); saved is None without `save`."""
+    """(h, state, saved, number); saved is None without `save`."""
     key = ("gated", x.dtype, x.device, x.shape, x.stride(), _looks(gate_a), _looks(gate_x), _looks(rate), _looks(h0), _looks(cu_seqlens),
            reverse, scale)
     e = _remembered().get(key)
@@ -240,15 +247,18 @@ def gated_fwd(x, gate_a, gate_x, rate, h0, cu_seqlens, reverse, scale, save):
     a.x, a.gate_a, a.gate_x, a.rate = x.data_ptr(), gate_a.data_ptr(), gate_x.data_ptr(), rate.data_ptr()
     a.h0, a.cu_seqlens, a.h, a.state, a.saved = _p(h0), _p(cu_seqlens), h.data_ptr(), state.data_ptr(), _p(saved)
     _call(x, _lib.linrec_gated_fwd, e, "gated_linrec")
-    return h, state, saved
+    return h, state, saved, e.number
 
 
-def gated_bwd(d_h, d_state, x, gate_a, gate_x, rate, h0, cu_seqlens, saved, reverse, scale):
+def gated_bwd(d_h, d_state, x, gate_a, gate_x, rate, h0, cu_seqlens, saved, reverse, scale, number=None):
     """(d_x, d_gate_a, d_gate_x, d_rate, d_h0); d_h0 is None without h0, d_h or d_state may be None (zeros)."""
     if d_h is None:
         d_h = torch.zeros((), dtype=x.dtype, device=x.device).expand(x.size())
-    key = ("gated_bwd", x.dtype, x.device, x.shape, x.stride(), _looks(d_h), _looks(d_state), _looks(gate_a), _looks(gate_x), _looks(rate),
-           _looks(h0), _looks(cu_seqlens), reverse, scale)
+    if number is not None:
+        key = (number, d_h.stride(), None if d_state is None else d_state.stride())
+    else:
+        key = ("gated_bwd", x.dtype, x.device, x.shape, x.stride(), _looks(d_h), _looks(d_state), _looks(gate_a), _looks(gate_x), _looks(rate),
+               _looks(h0), _looks(cu_seqlens), reverse, scale)
     e = _remembered().get(key)
     if e is None:
         a = _gated_args(x, gate_a, gate_x, rate, h0, cu_seqlens, reverse, scale, d_h)
@@ -381,7 +391,7 @@ def _norm_entry(key, x, groups, weight, bias, eps, act, d_y=None):
 
 
 def norm_fwd(x, groups, weight, bias, eps, act):
-    """(y, stats); stats is (2, batch, groups): the means, and the reciprocal deviations"""
+    """(y, stats, number); stats is (2, batch, groups): the means, and the reciprocal deviations"""
     key = ("norm", x.dtype, x.device, x.shape, x.stride(), groups, _looks(weight), _looks(bias), eps, act)
     e = _remembered().get(key) or _norm_entry(key, x, groups, weight, bias, eps, act)
     a = e.args
@@ -395,12 +405,15 @@ def norm_fwd(x, groups, weight, bias, eps, act):
     a.mean = mean = stats.data_ptr()
     a.rstd = mean + 4 * a.batch * a.groups
     _call(x, _lib.linrec_group_norm_fwd, e, "group_norm_act")
-    return y, stats
+    return y, stats, e.number
 
 
-def norm_bwd(d_y, x, groups, weight, bias, stats, eps, act):
+def norm_bwd(d_y, x, groups, weight, bias, stats, eps, act, number=None):
     """(d_x, d_weight, d_bias), the last two None without a weight"""
-    key = ("norm_bwd", x.dtype, x.device, x.shape, x.stride(), groups, _looks(d_y), _looks(weight), _looks(bias), eps, act)
+    if number is not None:
+        key = (number, d_y.stride())
+    else:
+        key = ("norm_bwd", x.dtype, x.device, x.shape, x.stride(), groups, _looks(d_y), _looks(weight), _looks(bias), eps, act)
     e = _remembered().get(key) or _norm_entry(key, x, groups, weight, bias, eps, act, d_y)
     a = e.args
     if a is None:
@@ -442,6 +455,7 @@ def _embedding_args(tokens, weight, scale, padding_idx):
 
 
 def embedding_fwd(tokens, weight, scale, padding_idx):
+    """(y, number)"""
     key = ("embedding", _looks(tokens), weight.dtype, weight.device, weight.shape, weight.stride(), scale, padding_idx)
     e = _remembered().get(key)
     if e is None:
@@ -454,12 +468,15 @@ def embedding_fwd(tokens, weight, scale, padding_idx):
     y = torch.empty(e.sizes[0], dtype=weight.dtype, device=weight.device)
     a.token, a.weight, a.y = tokens.data_ptr(), weight.data_ptr(), y.data_ptr()
     _call(weight, _lib.linrec_embedding_fwd, e, "embedding")
-    return y
+    return y, e.number
 
 
-def embedding_bwd(d_y, tokens, weight, scale, padding_idx):
+def embedding_bwd(d_y, tokens, weight, scale, padding_idx, number=None):
     """The gradient of `weight` (whose values are not read)."""
-    key = ("embedding_bwd", _looks(d_y), _looks(tokens), weight.dtype, weight.device, weight.shape, scale, padding_idx)
+    if number is not None:
+        key = (number, d_y.stride())
+    else:
+        key = ("embedding_bwd", _looks(d_y), _looks(tokens), weight.dtype, weight.device, weight.shape, scale, padding_idx)
     e = _remembered().get(key)
     if e is None:
         a = _embedding_args(tokens, weight, scale, padding_idx)

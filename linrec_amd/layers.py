@@ -34,11 +34,20 @@ def _recorded(*tensors):
     return forward_ad._current_level >= 0
 
 
+def _once(backward):
+    """once_differentiable, whose wrapper is only paid for where a graph of the backward is asked for."""
+    guarded = torch.autograd.function.once_differentiable(backward)
+
+    def call(ctx, *gradients):
+        return guarded(ctx, *gradients) if torch.is_grad_enabled() else backward(ctx, *gradients)
+    return call
+
+
 # ---- gated linear recurrence -------------------------------------------------------------------
 @torch.library.custom_op("linrec_amd::gated_linrec_fwd", mutates_args=(), device_types="cuda")
 def gated_linrec_fwd(x: Tensor, gate_a: Tensor, gate_x: Tensor, rate: Tensor, h0: Optional[Tensor], cu_seqlens: Optional[Tensor],
                      reverse: bool, scale: float) -> Tuple[Tensor, Tensor, Tensor]:
-    return _layers.gated_fwd(x, gate_a, gate_x, rate, h0, cu_seqlens, reverse, scale, True)
+    return _layers.gated_fwd(x, gate_a, gate_x, rate, h0, cu_seqlens, reverse, scale, True)[:3]
 
 
 @torch.library.custom_op("linrec_amd::gated_linrec_bwd", mutates_args=(), device_types="cuda")
@@ -80,17 +89,17 @@ torch.library.register_autograd("linrec_amd::gated_linrec_fwd", _gated_backward,
 class _GatedFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, gate_a, gate_x, rate, h0, cu_seqlens, reverse, scale):
-        h, state, saved = _layers.gated_fwd(x, gate_a, gate_x, rate, h0, cu_seqlens, reverse, scale, True)
+        h, state, saved, ctx.number = _layers.gated_fwd(x, gate_a, gate_x, rate, h0, cu_seqlens, reverse, scale, True)
         ctx.save_for_backward(x, gate_a, gate_x, rate, h0, cu_seqlens, saved)
         ctx.set_materialize_grads(False)
         ctx.reverse, ctx.scale = reverse, scale
         return h, state
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
+    @_once
     def backward(ctx, d_h, d_state):
         x, gate_a, gate_x, rate, h0, cu_seqlens, saved = ctx.saved_tensors
-        return (*_layers.gated_bwd(d_h, d_state, x, gate_a, gate_x, rate, h0, cu_seqlens, saved, ctx.reverse, ctx.scale),
+        return (*_layers.gated_bwd(d_h, d_state, x, gate_a, gate_x, rate, h0, cu_seqlens, saved, ctx.reverse, ctx.scale, ctx.number),
                 None, None, None)
 
 
@@ -114,7 +123,7 @@ def gated_linrec(x: Tensor, gate_a: Tensor, gate_x: Tensor, rate: Tensor, *, h0:
     elif _recorded(x, gate_a, gate_x, rate, h0):
         h, state = _GatedFn.apply(x, gate_a, gate_x, rate, h0, cu_seqlens, reverse, scale)
     else:
-        h, state, _ = _layers.gated_fwd(x, gate_a, gate_x, rate, h0, cu_seqlens, reverse, scale, False)
+        h, state, *_ = _layers.gated_fwd(x, gate_a, gate_x, rate, h0, cu_seqlens, reverse, scale, False)
     return (h, state) if return_state else h
 
 
@@ -147,7 +156,7 @@ def gated_linrec_step(x: Tensor, gate_a: Tensor, gate_x: Tensor, rate: Tensor, s
 @torch.library.custom_op("linrec_amd::group_norm_act_fwd", mutates_args=(), device_types="cuda")
 def group_norm_act_fwd(x: Tensor, groups: int, weight: Optional[Tensor], bias: Optional[Tensor], eps: float,
                        act: str) -> Tuple[Tensor, Tensor]:
-    return _layers.norm_fwd(x, groups, weight, bias, eps, act)
+    return _layers.norm_fwd(x, groups, weight, bias, eps, act)[:2]
 
 
 @torch.library.custom_op("linrec_amd::group_norm_act_bwd", mutates_args=(), device_types="cuda")
@@ -188,16 +197,16 @@ torch.library.register_autograd("linrec_amd::group_norm_act_fwd", _norm_backward
 class _NormFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, groups, weight, bias, eps, act):
-        y, stats = _layers.norm_fwd(x, groups, weight, bias, eps, act)
+        y, stats, ctx.number = _layers.norm_fwd(x, groups, weight, bias, eps, act)
         ctx.save_for_backward(x, weight, bias, stats)
         ctx.groups, ctx.eps, ctx.act = groups, eps, act
         return y
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
+    @_once
     def backward(ctx, d_y):
         x, weight, bias, stats = ctx.saved_tensors
-        d_x, d_weight, d_bias = _layers.norm_bwd(d_y, x, ctx.groups, weight, bias, stats, ctx.eps, ctx.act)
+        d_x, d_weight, d_bias = _layers.norm_bwd(d_y, x, ctx.groups, weight, bias, stats, ctx.eps, ctx.act, ctx.number)
         return d_x, None, d_weight, d_bias, None, None
 
 
@@ -219,7 +228,7 @@ def group_norm_act(x: Tensor, groups: int, weight: Optional[Tensor] = None, bias
 # ---- embedding ---------------------------------------------------------------------------------
 @torch.library.custom_op("linrec_amd::embedding_fwd", mutates_args=(), device_types="cuda")
 def embedding_fwd(tokens: Tensor, weight: Tensor, scale: float, padding_idx: Optional[int]) -> Tensor:
-    return _layers.embedding_fwd(tokens, weight, scale, padding_idx)
+    return _layers.embedding_fwd(tokens, weight, scale, padding_idx)[0]
 
 
 @torch.library.custom_op("linrec_amd::embedding_bwd", mutates_args=(), device_types="cuda")
@@ -255,12 +264,13 @@ class _EmbeddingFn(torch.autograd.Function):
     def forward(ctx, tokens, weight, scale, padding_idx):
         ctx.save_for_backward(tokens)
         ctx.like, ctx.scale, ctx.padding_idx = weight.detach(), scale, padding_idx
-        return _layers.embedding_fwd(tokens, weight, scale, padding_idx)
+        y, ctx.number = _layers.embedding_fwd(tokens, weight, scale, padding_idx)
+        return y
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
+    @_once
     def backward(ctx, d_y):
-        return None, _layers.embedding_bwd(d_y, ctx.saved_tensors[0], ctx.like, ctx.scale, ctx.padding_idx), None, None
+        return None, _layers.embedding_bwd(d_y, ctx.saved_tensors[0], ctx.like, ctx.scale, ctx.padding_idx, ctx.number), None, None
 
 
 def embedding(tokens: Tensor, weight: Tensor, *, scale: float = 1.0, padding_idx: Optional[int] = None) -> Tensor:
@@ -274,4 +284,4 @@ def embedding(tokens: Tensor, weight: Tensor, *, scale: float = 1.0, padding_idx
         return embedding_fwd(tokens, weight, scale, padding_idx)
     if _recorded(weight):
         return _EmbeddingFn.apply(tokens, weight, scale, padding_idx)
-    return _layers.embedding_fwd(tokens, weight, scale, padding_idx)
+    return _layers.embedding_fwd(tokens, weight, scale, padding_idx)[0]

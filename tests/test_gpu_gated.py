@@ -242,7 +242,7 @@ def test_the_same_bits_every_time_and_in_a_graph():
 
     # both passes without autograd, whose nodes would tie the capture to the stream that they were made on
     def run():
-        h, state, saved = _layers.gated_fwd(x, gate_a, gate_x, rate, h0, None, False, 8.0, True)
+        h, state, saved, _ = _layers.gated_fwd(x, gate_a, gate_x, rate, h0, None, False, 8.0, True)
         return (h, state, *_layers.gated_bwd(d_h, d_state, x, gate_a, gate_x, rate, h0, None, saved, False, 8.0))
     same_bits_in_a_graph(run)
 

@@ -162,7 +162,7 @@ def test_the_same_bits_every_time_and_in_a_graph(shape, groups):
     x, d_y, weight, bias = (t.to(DEV) for t in make(shape, torch.bfloat16, seed=7))
 
     def run():
-        y, stats = _layers.norm_fwd(x, groups, weight, bias, 1e-5, "silu")
+        y, stats, _ = _layers.norm_fwd(x, groups, weight, bias, 1e-5, "silu")
         return (y, stats, *_layers.norm_bwd(d_y, x, groups, weight, bias, stats, 1e-5, "silu"))
     same_bits_in_a_graph(run)
 

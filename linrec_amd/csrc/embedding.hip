@@ -50,7 +50,7 @@ Scratch scratch_layout(int64_t tokens, int64_t channels) {
   s.blocks = cdiv(tokens, SORT_BLOCK);
   s.counts = take(small ? 0 : size_t(s.blocks) * DIGITS * 4);
   s.n_runs = tokens / RUN;
-  s.n_runs2 = tokens / RUN2;
+  s.n_runs2 = tokens < 16384 ? 0 : tokens / RUN2;  // (fewer: the launch costs more than the few sums it saves)
   s.runs = take(size_t(s.n_runs) * size_t(channels) * 4);
   s.runs2 = take(size_t(s.n_runs2) * size_t(channels) * 4);
   s.bytes = at;
@@ -140,7 +140,7 @@ int linrec_embedding_bwd(const linrec_embedding_t* p) {
     constexpr int VEC = decltype(vec)::value;
     const int64_t column_waves = cdiv(p->channels, 64 * VEC);
     float* runs = reinterpret_cast<float*>(scratch + s.runs);
-    float* runs2 = reinterpret_cast<float*>(scratch + s.runs2);
+    float* runs2 = s.n_runs2 ? reinterpret_cast<float*>(scratch + s.runs2) : nullptr;
     if (const int rc = launch_kernel(run_sums_kernel<T, VEC, false>, cdiv(s.n_runs * column_waves, 4), 1, 256, p->stream, *p, sorted, nullptr, runs,
                                      s.n_runs, column_waves))
       return rc;

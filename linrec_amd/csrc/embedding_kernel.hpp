@@ -359,10 +359,10 @@ __global__ __launch_bounds__(256) void list_sums_kernel(linrec_embedding_t p, So
     }
     // whole runs from here on: of runs where one of them may start, else as many as come before that
     int length = RUN2, whole = 0;
-    if ((at & (RUN2 - 1)) == 0) whole = whole_runs(sorted.key, n, at, RUN2, 64, v, lane);
+    if (runs2 && (at & (RUN2 - 1)) == 0) whole = whole_runs(sorted.key, n, at, RUN2, 64, v, lane);
     if (whole == 0) {
       length = RUN;
-      whole = whole_runs(sorted.key, n, at, RUN, RUN - (at / RUN & (RUN - 1)), v, lane);
+      whole = whole_runs(sorted.key, n, at, RUN, runs2 ? RUN - (at / RUN & (RUN - 1)) : 64, v, lane);
     }
     const float* rows = (length == RUN2 ? runs2 : runs) + int64_t(at / length) * p.channels + c;
     add_rows<VEC>(sum, whole, [&](int i) { return rows + int64_t(i) * p.channels; });

@@ -263,7 +263,7 @@ class _EmbeddingFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, tokens, weight, scale, padding_idx):
         ctx.save_for_backward(tokens)
-        ctx.like, ctx.scale, ctx.padding_idx = weight.detach(), scale, padding_idx
+        ctx.like, ctx.scale, ctx.padding_idx = weight, scale, padding_idx  # (its sizes; the values are not read again)
         y, ctx.number = _layers.embedding_fwd(tokens, weight, scale, padding_idx)
         return y
 

@@ -327,3 +327,70 @@ def test_refusals():
             ((x.clone().requires_grad_(), gate_a, gate_x, rate, h0), {}, "no gradient")]:
         with pytest.raises(RuntimeError, match=text):
             step(*args, **kw)
+
+
+@pytest.mark.parametrize("bounds", [None, [0, 1, 700, 700, 1500, 1501, 2300]])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_waits_that_run_out(dtype, bounds):
+    """With a limit of one poll most segments give up on the ones before them and walk their channels themselves."""
+    shape = (1, 2300, 96) if bounds is None else (2300, 96)
+    x, gate_a, gate_x, rate, h0, d_h, d_state = (t.to(DEV) for t in make(shape, dtype, seed=15, sequences=None if bounds is None else len(bounds) - 1))
+    cu = None if bounds is None else torch.tensor(bounds, dtype=torch.int32, device=DEV)
+
+    def run():
+        h, state, saved, _ = _layers.gated_fwd(x, gate_a, gate_x, rate, h0, cu, False, 8.0, True)
+        return (h, state, *_layers.gated_bwd(d_h, d_state, x, gate_a, gate_x, rate, h0, cu, saved, False, 8.0))
+    want = run()
+    before = nat.gave_up_count()
+    old = nat.lib().linrec_set_spin_limit(1)
+    try:
+        got = run()
+        torch.cuda.synchronize()
+    finally:
+        nat.lib().linrec_set_spin_limit(old)
+    assert nat.gave_up_count() > before
+    _, _, a = ref.gated(x.cpu(), gate_a.cpu(), gate_x.cpu(), rate.cpu(), bounds=bounds)
+    for w, g in zip(want, got):
+        tol = ref.gated_tolerance(a, g.dtype)
+        ref.assert_within(g, w.cpu(), 8 * tol * max(1.0, ref.largest(w.cpu())), "after waits that ran out")
+    after = run()
+    assert all(torch.equal(a, b) for a, b in zip(after, want))
+
+
+def test_many_segments_and_channels():
+    """More groups of segments than are looked at at a time, more blocks of channels than one."""
+    data = make((2, 3000, 200), torch.bfloat16, seed=16)
+    check_on_device(data, torch.bfloat16)
+    data = make((1, 6000, 130), torch.float32, seed=17)
+    check_on_device(data, torch.float32)
+
+
+def check_on_device(data, dtype):
+    """As `check`, the float64 loop on the device (over positions, all channels at once)."""
+    x, gate_a, gate_x, rate, h0, d_h, d_state = (t.to(DEV) for t in data)
+    leaves = [t.requires_grad_() for t in (x, gate_a, gate_x, rate, h0)]
+    h, state = linrec_amd.gated_linrec(*leaves[:4], h0=leaves[4], return_state=True)
+    grads = torch.autograd.grad((h, state), leaves, (d_h, d_state))
+    xs, gas, gxs, r = (t.detach().double() for t in leaves[:4])
+    sig_a, sig_x = torch.sigmoid(gas), torch.sigmoid(gxs)
+    log_a = -8.0 * torch.nn.functional.softplus(r) * sig_a
+    a, m = torch.exp(log_a), torch.sqrt(-torch.expm1(2 * log_a))
+    time = x.shape[1]
+    before, value = torch.empty_like(a), h0.detach().double()
+    for t in range(time):
+        before[:, t] = value
+        value = a[:, t] * value + m[:, t] * sig_x[:, t] * xs[:, t]
+    after = a * before + m * sig_x * xs
+    g, carry = torch.empty_like(a), d_state.double()
+    for t in reversed(range(time)):
+        g[:, t] = d_h[:, t].double() + carry
+        carry = a[:, t] * g[:, t]
+    p = g * (log_a * a * before - sig_x * xs * a * a * log_a / m)
+    tol, tol32 = ref.gated_tolerance(a.cpu(), dtype), ref.gated_tolerance(a.cpu(), torch.float32)
+    ref.assert_within(h, after.cpu(), tol * ref.largest(after.cpu()), "h")
+    ref.assert_within(state, value.cpu(), tol32 * ref.largest(after.cpu()), "state")
+    for got, want, name in zip(grads[:3], (g * m * sig_x, p * (1 - sig_a), g * m * xs * sig_x * (1 - sig_x)), ("d_x", "d_gate_a", "d_gate_x")):
+        ref.assert_within(got, want.cpu(), 4 * tol * ref.largest(want.cpu()), name)
+    ratio = ref.sigmoid_over_softplus(r.cpu())
+    ref.assert_within(grads[3], p.sum((0, 1)).cpu() * ratio, 4 * tol32 * p.abs().sum((0, 1)).cpu() * ratio, "d_rate")
+    ref.assert_within(grads[4], carry.cpu(), 4 * tol32 * max(1.0, ref.largest(carry.cpu()), ref.largest(g.cpu())), "d_h0")

@@ -349,6 +349,9 @@ def test_waits_that_run_out(dtype, bounds):
     finally:
         nat.lib().linrec_set_spin_limit(old)
     assert nat.gave_up_count() > before
+    # the other tests take a count of zero as the sign that nobody had to fall back: start over
+    for ws in list(nat._workspaces.values()):
+        ws[:16].view(torch.int32)[1] = 0
     _, _, a = ref.gated(x.cpu(), gate_a.cpu(), gate_x.cpu(), rate.cpu(), bounds=bounds)
     for w, g in zip(want, got):
         tol = ref.gated_tolerance(a, g.dtype)

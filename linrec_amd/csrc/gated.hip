@@ -97,7 +97,7 @@ Geometry geometry(int dtype, int64_t batch, int64_t time, int64_t channels, bool
   g.save = kBwdRun * (dtype == LINREC_DTYPE_F32 ? kBwdWaves<float> : kBwdWaves<__bf16>);
   g.segments = cdiv(time, bwd ? g.save : kFwdWaves * kFwdRun);
   g.grid = g.segments * blocks;
-  g.tiles = (g.segments + cdiv(g.segments, GROUP)) * blocks * rows;  // places of words
+  g.tiles = chain_places(g.segments) * blocks * rows;  // places of words
   return g;
 }
 
@@ -107,6 +107,8 @@ int fill_args(const linrec_gated_t* p, const Geometry& g, GatedArgs* a) {
   a->segments = int(g.segments);
   a->channel_blocks = int(g.channel_blocks);
   a->save = g.save;
+  a->side = p->channels * (p->dtype == LINREC_DTYPE_F32 ? 4 : 2) % 128 ? 8 : GROUP;
+  if (a->side > g.segments) a->side = int(g.segments);
   if (g.grid > 2147483647LL) return LINREC_E_TOO_LARGE;
   if (g.segments <= 1) return LINREC_OK;
   if (!p->workspace || (reinterpret_cast<uintptr_t>(p->workspace) & 15u)) return LINREC_E_WORKSPACE;

@@ -3,22 +3,34 @@
 //   log a = -decay sigmoid(gate_a),  decay = scale softplus(rate)
 //   h[t] = a h[t-1] + m sigmoid(gate_x) x,  m = sqrt(1 - a^2) = sqrt(-expm1(2 log a))
 //
-// The shape is that of the look-back segments (collook_kernel.hpp): the scan axis is cut into segments of NW * U positions, a
-// workgroup takes one segment of 64 * VEC channels, wave w the run [w*U, w*U + U), and the segments of a channel are chained
-// through descriptors in global memory.  The gates are evaluated on the way in, so forward reads three tensors and writes one,
-// where coefficients and inputs made by elementwise kernels first are written and read once more each.
+// The scan axis is cut into segments of NW * U positions; a workgroup takes one segment of 64 * VEC channels, wave w the run
+// [w*U, w*U + U), and the segments of a channel are chained through descriptors in global memory.  The gates are evaluated on the
+// way in, so forward reads three tensors and writes one, where coefficients and inputs made by elementwise kernels first are
+// written and read once more each.
 //
 // Backward, g[t] = d_h[t] + a[t+1] g[t+1] in the opposite direction over the same segments:
 //   d_x = g m sx,  d_gate_x = g m x sx (1 - sx)                         (sx, sa: the gates' sigmoids)
 //   P = g (log a a h[t-1] - sx x a^2 log a / m),  d_gate_a = P (1 - sa),  d_rate = sigmoid(rate) / softplus(rate) sum P
 // (log a and log a / m both go to zero with sigmoid(gate_a), where 1 / m alone does not: every term stays finite.)  h[t-1] is
-// not read: the forward saves the value that enters every 64th position in fp32 (4 bytes for 64 positions of a channel), and the
-// backward goes on from there with the same operations, so the gradient sees the unrounded values and four tensors are read
+// not read: the forward saves the value that enters every backward segment (32 positions in 16-bit storage, 64 in fp32) as 4 bytes,
+// and the backward goes on from there with the same operations, so the gradient sees the unrounded values and four tensors are read
 // where the saved output would make it five.
 //
+// What bounds it: memory where channels are many.  8 x 4096 x 2048 in bf16: 124 us forward (537 MB, 4.3 TB/s of the 5.2 TB/s that
+// a copy reaches) and 222 us backward (940 MB, 4.2 TB/s); 16 x 2048 x 512 in fp32 out of a projection's rows 58 and 105 us (4.6 and
+// 4.5 TB/s).  Without the wait for what enters a segment the former takes 111 and 200 us: the wait is the larger part of the rest,
+// the gates' arithmetic the smaller.  With few channels the chain bounds it: 1 x 32768 x 2048 134 and 248 us, 1 x 131072 x 64 51
+// and 94 us (floors 103, 181; 13, 23).
+//
+// Waves and runs: workgroups wait, so that several to a CU have to hide each other's waits, with all that a segment holds in
+// registers: at most 128 a lane for four workgroups of four waves, and nothing spilled (a handful of registers that are cost 2 to
+// 6 %).  Forward keeps a and the input of 16 positions of two channels, backward a, m and h[t-1] of 8, and the sigmoids in LDS,
+// which saves evaluating them twice.  Eight waves in 16-bit storage instead of four, and longer segments so: 131 and 258 us instead
+// of 125 and 220 for 8 x 4096 x 2048, with twice the links.  fp32, a channel to a lane, needs half the registers a position and
+// takes eight waves in the backward.
+//
 // The value that enters a segment is always the same chain of multiply-adds over the segments before, whichever of them had
-// published what when they were looked at (a window is folded from its farthest segment to its nearest, and a segment's own
-// value by the same operation): results are the same bits in every run.
+// published what when they were looked at: results are the same bits in every run.
 //
 // A position at which a packed sequence starts takes the sequence's own initial value instead of what comes from before it, so
 // nothing passes from one sequence to the next, not even by 0 * inf.  A segment that holds a start does not wait at all.
@@ -34,14 +46,31 @@
 
 namespace linrec {
 
-
 struct GatedArgs {
   linrec_gated_t p;
   TileArgs chain;
   int segments;         // of the scan axis
   int channel_blocks;
+  int side;             // segments side by side
   int save;             // positions from one saved value to the next: those of a backward segment
 };
+
+// Workgroups go through the segments in sets of `side`, through the blocks of channels within a set and the set's segments within
+// a block, so that waits are for smaller numbers.  Sets of a group: its segments run side by side, and what they read is near, 8 x
+// 4096 x 2048 bf16 124 and 221 us (one by one 128 and 221), 1 x 32768 x 2048 134 and 247 (154 and 293).  Workgroups are dealt to the
+// eight XCDs in turn, so that in sets of eight neighbouring blocks of a segment run on the same one; where rows are not whole lines
+// of 128 bytes they write parts of the same lines, which one L2 puts together: 16 x 6250 x 250 bf16 73 and 130 us instead of 81 and
+// 144, 1 x 100001 x 250 82 and 150 instead of 88 and 162 (for whole lines eight are slower: 127 and 235, 136 and 248 above).
+struct Place {
+  int segment;
+  unsigned block;
+};
+__device__ __forceinline__ Place place_of(const GatedArgs& args, unsigned blocks) {
+  const unsigned per_set = blocks * unsigned(args.side), set = blockIdx.x / per_set, in_set = blockIdx.x - set * per_set;
+  const unsigned first = set * unsigned(args.side), width = min(unsigned(args.side), unsigned(args.segments) - first);
+  const unsigned block = in_set / width;
+  return {__builtin_amdgcn_readfirstlane(int(first + in_set - block * width)), unsigned(__builtin_amdgcn_readfirstlane(int(block)))};
+}
 
 // ---- arithmetic -------------------------------------------------------------------------------
 constexpr float LOG2E = 1.4426950408889634f;
@@ -216,19 +245,29 @@ __device__ __forceinline__ P* plus_bytes(P* p, uint32_t bytes) {
 
 // ---- the chain of segments --------------------------------------------------------------------
 // What enters a segment is a chain of multiply-adds over the maps of the segments before, and every link costs a store and a load
-// through memory, about 1.5 us, however many lanes do it side by side.  So the chain goes over groups of GROUP segments: a
-// segment publishes its map; the last one of a group composes the group's maps and publishes that; and what enters a segment is
-// what enters its group, which the chain of groups says, taken through the maps of the segments before it in the group.
-// LOOK groups are looked at at a time, so the value advances by LOOK * GROUP segments a link.  Which groups had published what
-// does not matter to the result: the value that leaves a group is the same multiply-add whoever makes it.
+// through memory, 4 to 5 us with the wait between two looks, however many lanes do it side by side.  So the chain goes over blocks
+// of GROUP groups of GROUP segments: a segment publishes its map; the last one of a group composes the group's maps and publishes
+// that; the last one of a block those of the block's groups; and what enters a segment is what enters its block, which the chain of
+// blocks says, taken through the maps of the groups before it in the block and of the segments before it in the group.  LOOK blocks
+// are looked at at a time, so the value advances by LOOK * GROUP * GROUP segments a link.  Which of them had published what does not
+// matter to the result: the value that leaves a block is the same multiply-add whoever makes it.
 //
-// Words of a place (a segment's, a group's): first the factors of the block's channels, then the addends, RPB each, with the
+// 1 x 100001 x 250 bf16, forward and backward: groups of 8 without blocks over them 119 and 226 us, with blocks 100 and 192; groups
+// of 4 / 5 / 6 with blocks 103, 197 / 90, 167 / 96, 187.  1 x 131072 x 64, groups of 4 / 5 / 6 / 8: 66, 125 / 50, 93 / 53, 100 / 59,
+// 117 (a link of 4 advances by 64 segments, one of 5 by 100; larger groups take registers that the data needs).  LOOK of 6 instead
+// of 4: 8 x 4096 x 2048 130 and 230 us instead of 128 and 221, 50 and 98 here.  The groups before by other waves, while the first
+// look at the segments before: no faster here, 240 us instead of 223 for 8 x 4096 x 2048 backward (registers).
+//
+// Words of a place (a segment's, a group's, a block's): first the factors of the block's channels, then the addends, RPB each, with the
 // launch's number; an addend marked `done` leaves the place whatever enters it (a sequence starts inside, or what entered is in it).
-constexpr int LOOK = 4;   // groups looked at at a time
-constexpr int GROUP = 8;  // segments of a group
+constexpr int LOOK = 4;   // blocks looked at at a time
+constexpr int SLEEP = 32;  // between two looks, 64 cycles each (8: 1 x 32768 x 2048 bf16 159 and 301 us instead of 154 and 293)
+constexpr int GROUP = 5;  // segments of a group, groups of a block
+// Places of a chain of `segments`: theirs, their groups', their blocks'.
+constexpr int64_t chain_places(int64_t segments) { return segments + segments / GROUP + segments / (GROUP * GROUP); }
 struct Chain {
-  uint64_t* segment_words;  // of segment 0, this lane's
-  uint64_t* group_words;    // of group 0
+  uint64_t* segment_words;  // of segment 0, the wave's (the same for all lanes, as all places are here)
+  uint32_t lane_bytes;      // the lane's, from there
   long long per_place;      // from one place's words to the next one's
   int k, segments;
   uint32_t seq;
@@ -238,12 +277,20 @@ struct Chain {
 struct Words {
   uint64_t a, b;
 };
+template <typename P>
+__device__ __forceinline__ P* scalar(P* p) {  // (the same for all lanes, which the compiler need not know)
+  const uint64_t v = reinterpret_cast<uint64_t>(p);
+  return reinterpret_cast<P*>(uint64_t(uint32_t(__builtin_amdgcn_readfirstlane(int(v)))) |
+                              (uint64_t(uint32_t(__builtin_amdgcn_readfirstlane(int(v >> 32)))) << 32));
+}
 template <int RPB>
-__device__ __forceinline__ Words load_words(const uint64_t* d) {
+__device__ __forceinline__ Words load_words(const Chain& c, const uint64_t* place) {
+  const uint64_t* d = plus_bytes(scalar(place), c.lane_bytes);
   return {ld_desc(d), ld_desc(d + RPB)};
 }
 template <int RPB>
-__device__ __forceinline__ void publish(const Chain& c, uint64_t* d, float a, float b, bool constant) {
+__device__ __forceinline__ void publish(const Chain& c, uint64_t* place, float a, float b, bool constant) {
+  uint64_t* d = plus_bytes(scalar(place), c.lane_bytes);
   if (!constant) st_desc(d, pack_desc(c.map(), a));
   st_desc(d + RPB, pack_desc(constant ? c.done() : c.map(), b));
 }
@@ -256,81 +303,101 @@ __device__ __forceinline__ float through(const Chain& c, const Words& w, float v
   return is_done(c, w) ? word_value(w.b) : fmaf(word_value(w.a), v, word_value(w.b));
 }
 
+// The map of the `count` < GROUP places before `place`; a constant one needs nothing of what enters the farthest.
+struct Before {
+  float a = 1.0f, b = 0.0f;
+  bool constant = false, there = true;
+};
+template <int RPB>
+__device__ __forceinline__ Before maps_before(const TileArgs& args, const Chain& c, const uint64_t* place, int count) {
+  Before m;
+  m.there = count == 0;
+  for (int polls = 0; !m.there && polls < args.spin_limit; ++polls) {
+    if (polls > 0) __builtin_amdgcn_s_sleep(SLEEP);
+    Words w[GROUP - 1];  // the farthest first
+#pragma unroll
+    for (int q = 0; q < GROUP - 1; ++q)
+      if (q < count) w[q] = load_words<RPB>(c, place - (count - q) * c.per_place);
+    m.there = true;
+#pragma unroll
+    for (int q = 0; q < GROUP - 1; ++q)
+      if (q < count && __ballot(!is_there(c, w[q])) != 0) m.there = false;
+    if (m.there) {
+#pragma unroll
+      for (int q = 0; q < GROUP - 1; ++q)
+        if (q < count) {
+          const bool cuts = __ballot(!is_done(c, w[q])) == 0;
+          m.b = through(c, w[q], m.b);
+          m.a = cuts ? 1.0f : never_zero(m.a * word_value(w[q].a));
+          m.constant = m.constant || cuts;
+        }
+    }
+  }
+  return m;
+}
+
 // One wave, a channel to a lane: publishes the segment's map (ta, tb; cut: a sequence starts inside) and returns what enters it.
 // `walk` computes that from the channel's own data.
 template <int RPB, typename W>
 __device__ __forceinline__ float enter_segment(const TileArgs& args, const Chain& c, int lane, float first, float ta, float tb, bool cut, W&& walk) {
-  const int in_group = c.k % GROUP, g = c.k / GROUP;
-  const bool last = c.k + 1 >= c.segments, closes = !last && in_group == GROUP - 1;
+  const int in_group = c.k % GROUP, g = c.k / GROUP, in_block = g % GROUP, s = g / GROUP;
+  const bool more = c.k + 1 < c.segments, closes = more && in_group == GROUP - 1, closes_block = closes && in_block == GROUP - 1;
   uint64_t* mine = c.segment_words + c.k * c.per_place;
-  uint64_t* of_group = c.group_words + g * c.per_place;
-  if (!last && !closes) publish<RPB>(c, mine, ta, tb, cut);
-  // The map of the segments before this one in its group; a constant one needs nothing of what enters the group.  (Asking for
-  // what enters the group in the same round trip takes registers that the data needs: 8 x 4096 x 2048 bf16 164 / 281 us against
-  // 127 / 220.)
-  float ga = 1.0f, gb = 0.0f;
-  bool constant = false, there = in_group == 0;
-  for (int polls = 0; !there && polls < args.spin_limit; ++polls) {
-    if (polls > 0) __builtin_amdgcn_s_sleep(1);
-    Words w[GROUP - 1];  // the farthest first
-#pragma unroll
-    for (int q = 0; q < GROUP - 1; ++q)
-      if (q < in_group) w[q] = load_words<RPB>(mine - (in_group - q) * c.per_place);
-    there = true;
-#pragma unroll
-    for (int q = 0; q < GROUP - 1; ++q)
-      if (q < in_group && __ballot(!is_there(c, w[q])) != 0) there = false;
-    if (there) {
-#pragma unroll
-      for (int q = 0; q < GROUP - 1; ++q)
-        if (q < in_group) {
-          const bool cuts = __ballot(!is_done(c, w[q])) == 0;
-          gb = through(c, w[q], gb);
-          ga = cuts ? 1.0f : never_zero(ga * word_value(w[q].a));
-          constant = constant || cuts;
-        }
-    }
+  uint64_t* of_group = c.segment_words + (c.segments + g) * c.per_place;
+  uint64_t* of_block = c.segment_words + (c.segments + c.segments / GROUP + s) * c.per_place;
+  if (more && !closes) publish<RPB>(c, mine, ta, tb, cut);
+  const Before seg = maps_before<RPB>(args, c, mine, in_group);
+  // the maps of the whole group and block, by their last segments
+  float whole_a = never_zero(seg.a * ta), whole_b = cut ? tb : fmaf(ta, seg.b, tb);
+  bool whole_constant = seg.constant || cut;
+  if (seg.there && closes && !closes_block) publish<RPB>(c, of_group, whole_a, whole_b, whole_constant);
+  Before grp;
+  if (seg.there && !seg.constant) grp = maps_before<RPB>(args, c, of_group, in_block);
+  if (!whole_constant) {
+    whole_b = fmaf(whole_a, grp.b, whole_b);
+    whole_a = never_zero(whole_a * grp.a);
+    whole_constant = grp.constant;
   }
-  // that of the whole group, by its last segment (the first group never shows a map: who looks beyond it sees it again, and must
-  // not take it twice)
-  const float whole_a = never_zero(ga * ta), whole_b = cut ? tb : fmaf(ta, gb, tb);
-  const bool whole_constant = constant || cut;
-  if (there && closes && (g > 0 || whole_constant)) publish<RPB>(c, of_group, whole_a, whole_b, whole_constant);
-  float v = first;  // what enters the group
-  bool known = there && (g == 0 || constant);
-  for (int polls = 0; there && !known && polls < args.spin_limit; ++polls) {
-    if (polls > 0) __builtin_amdgcn_s_sleep(1);
-    Words x[LOOK];
+  // (the first block never shows a map: who looks beyond it sees it again, and must not take it twice)
+  bool known = seg.there && grp.there;
+  if (known && closes_block && (s > 0 || whole_constant)) publish<RPB>(c, of_block, whole_a, whole_b, whole_constant);
+  float v = first;  // what enters the block
+  if (known && s > 0 && !seg.constant && !grp.constant) {
+    known = false;
+    for (int polls = 0; !known && polls < args.spin_limit; ++polls) {
+      if (polls > 0) __builtin_amdgcn_s_sleep(SLEEP);
+      Words x[LOOK];
 #pragma unroll
-    for (int q = 0; q < LOOK; ++q) x[q] = load_words<RPB>(of_group - (q < g ? q + 1 : g) * c.per_place);  // (beyond group 0: not used)
-    int from = -1;
-    bool blocked = false;
+      for (int q = 0; q < LOOK; ++q) x[q] = load_words<RPB>(c, of_block - (q < s ? q + 1 : s) * c.per_place);  // (beyond block 0: not used)
+      int from = -1;
+      bool blocked = false;
 #pragma unroll
-    for (int q = 0; q < LOOK; ++q) {
-      if (from < 0 && !blocked) {
-        if (__ballot(!is_done(c, x[q])) == 0) from = q;
-        else blocked = __ballot(!is_there(c, x[q])) != 0;
+      for (int q = 0; q < LOOK; ++q) {
+        if (from < 0 && !blocked) {
+          if (__ballot(!is_done(c, x[q])) == 0) from = q;
+          else blocked = __ballot(!is_there(c, x[q])) != 0;
+        }
       }
-    }
-    if (from >= 0) {
+      if (from >= 0) {
 #pragma unroll
-      for (int q = LOOK - 1; q >= 0; --q) {
-        if (q == from) v = word_value(x[q].b);
-        else if (q < from) v = through(c, x[q], v);
+        for (int q = LOOK - 1; q >= 0; --q) {
+          if (q == from) v = word_value(x[q].b);
+          else if (q < from) v = through(c, x[q], v);
+        }
+        known = true;
       }
-      known = true;
     }
   }
   if (known) {
-    if (closes && !whole_constant) st_desc(of_group + RPB, pack_desc(c.done(), fmaf(whole_a, v, whole_b)));
-    v = constant ? gb : in_group == 0 ? v : fmaf(ga, v, gb);
+    if (closes_block && !whole_constant) st_desc(plus_bytes(scalar(of_block + RPB), c.lane_bytes), pack_desc(c.done(), fmaf(whole_a, v, whole_b)));
+    v = grp.constant ? grp.b : in_block == 0 ? v : fmaf(grp.a, v, grp.b);
+    v = seg.constant ? seg.b : in_group == 0 ? v : fmaf(seg.a, v, seg.b);
   }
   if (__builtin_expect(!known, 0)) {
     if (lane == 0) __hip_atomic_fetch_add(&args.ws->gave_up, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     v = walk();
-    // (whoever looks for what leaves the group waits for it: it leaves through this segment)
-    if (closes && !cut) st_desc(of_group + RPB, pack_desc(c.done(), fmaf(ta, v, tb)));
-    else if (closes) st_desc(of_group + RPB, pack_desc(c.done(), tb));
+    // (whoever looks for what leaves the group or block waits for it: it leaves through this segment)
+    if (closes) st_desc(plus_bytes(scalar((closes_block ? of_block : of_group) + RPB), c.lane_bytes), pack_desc(c.done(), cut ? tb : fmaf(ta, v, tb)));
   }
   return v;
 }
@@ -345,11 +412,6 @@ struct Walk {
   int64_t step;  // elements
   __device__ __forceinline__ Walk(P* tensor, int64_t stride, int n0, int time, bool reverse)
       : at(tensor + int64_t(reverse ? time - 1 - n0 : n0) * stride), step(reverse ? -stride : stride) {}
-  static __device__ __forceinline__ P* scalar(P* p) {  // (the same for all lanes, which the compiler need not know)
-    const uint64_t v = reinterpret_cast<uint64_t>(p);
-    return reinterpret_cast<P*>(uint64_t(uint32_t(__builtin_amdgcn_readfirstlane(int(v)))) |
-                                (uint64_t(uint32_t(__builtin_amdgcn_readfirstlane(int(v >> 32)))) << 32));
-  }
   __device__ __forceinline__ P* lane(uint32_t bytes) const { return plus_bytes(scalar(at), bytes); }
   __device__ __forceinline__ void next() { at += step; }
   __device__ __forceinline__ void back() { at -= step; }
@@ -368,8 +430,9 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(4))) vo
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const unsigned blocks = unsigned(args.channel_blocks) * unsigned(p.batch);
-  const int k = __builtin_amdgcn_readfirstlane(int(blockIdx.x / blocks));
-  const unsigned block = blockIdx.x - unsigned(k) * blocks;
+  const Place at = place_of(args, blocks);
+  const int k = at.segment;
+  const unsigned block = at.block;
   const int batch = __builtin_amdgcn_readfirstlane(int(block / unsigned(args.channel_blocks)));
   const int channels = int(p.channels), time = int(p.time);
   const Channels<VEC> ch = lane_channels<VEC>(int(block) - batch * args.channel_blocks, lane, channels);
@@ -393,27 +456,27 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(4))) vo
   // PLAIN: every position of the segment exists and no sequence starts or ends in it.
   auto segment = [&](auto plain_tag, auto whole_tag) __attribute__((always_inline)) {
     constexpr bool PLAIN = decltype(plain_tag)::value, WHOLE = decltype(whole_tag)::value, CUTS = PACKED && !PLAIN;
-  Held<T, VEC> hx[U], ha[U], hg[U];
-  {
-    Walk<const T> wx(x, p.x_stride[1], n0, time, reverse), wa(ga, p.gate_a_stride[1], n0, time, reverse),
-        wg(gx, p.gate_x_stride[1], n0, time, reverse);
+    Held<T, VEC> hx[U], ha[U], hg[U];
+    {
+      Walk<const T> wx(x, p.x_stride[1], n0, time, reverse), wa(ga, p.gate_a_stride[1], n0, time, reverse),
+          wg(gx, p.gate_x_stride[1], n0, time, reverse);
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      if (PLAIN || n0 + u < time) {
-        hx[u] = ld_any<VEC, true>(wx.lane(lane_bytes));
-        ha[u] = ld_any<VEC, true>(wa.lane(lane_bytes));
-        hg[u] = ld_any<VEC, true>(wg.lane(lane_bytes));
+      for (int u = 0; u < U; ++u) {
+        if (PLAIN || n0 + u < time) {
+          hx[u] = ld_any<VEC, true>(wx.lane(lane_bytes));
+          ha[u] = ld_any<VEC, true>(wa.lane(lane_bytes));
+          hg[u] = ld_any<VEC, true>(wg.lane(lane_bytes));
+        }
+        wx.next();
+        wa.next();
+        wg.next();
       }
-      wx.next();
-      wa.next();
-      wg.next();
     }
-  }
-  if (wave < VEC) {  // a channel to a lane
-    const float rate = p.rate[ch.base + int(ch.rel) + wave];
-    sh_decay[wave * 64 + lane] = LOG2E * p.scale * fast_softplus(rate);
-  }
-  __syncthreads();
+    if (wave < VEC) {  // a channel to a lane
+      const float rate = p.rate[ch.base + int(ch.rel) + wave];
+      sh_decay[wave * 64 + lane] = LOG2E * p.scale * fast_softplus(rate);
+    }
+    __syncthreads();
 
     unsigned starts = 0, ends = 0;
     if constexpr (CUTS) {
@@ -475,8 +538,8 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(4))) vo
         }
       }
       const long long per_segment = 2ll * blocks * RPB;
-      uint64_t* words = args.chain.desc + 2ll * block * RPB + i;
-      const Chain chain{words, words + args.segments * per_segment, per_segment, k, args.segments, seq};
+      uint64_t* words = args.chain.desc + 2ll * block * RPB + e * 64;
+      const Chain chain{words, uint32_t(lane) * 8, per_segment, k, args.segments, seq};
       const float first = !PACKED && p.h0 ? p.h0[int64_t(batch) * channels + c] : 0.0f;
       auto walk = [&] {
         int from = 0;
@@ -565,9 +628,10 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(4))) vo
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const unsigned blocks = unsigned(args.channel_blocks) * unsigned(p.batch);
-  const int kk = __builtin_amdgcn_readfirstlane(int(blockIdx.x / blocks));  // segments from the far end
+  const Place at = place_of(args, blocks);
+  const int kk = at.segment;  // from the far end
   const int k = args.segments - 1 - kk;
-  const unsigned block = blockIdx.x - unsigned(kk) * blocks;
+  const unsigned block = at.block;
   const int batch = __builtin_amdgcn_readfirstlane(int(block / unsigned(args.channel_blocks)));
   const int channels = int(p.channels), time = int(p.time);
   const Channels<VEC> ch = lane_channels<VEC>(int(block) - batch * args.channel_blocks, lane, channels);
@@ -591,29 +655,29 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(4))) vo
 
   auto segment = [&](auto plain_tag, auto whole_tag) __attribute__((always_inline)) {
     constexpr bool PLAIN = decltype(plain_tag)::value, WHOLE = decltype(whole_tag)::value, CUTS = PACKED && !PLAIN;
-  Held<T, VEC> hx[U], ha[U], hg[U], hd[U];
-  {
-    Walk<const T> wx(x, p.x_stride[1], n0, time, reverse), wa(ga, p.gate_a_stride[1], n0, time, reverse),
-        wg(gx, p.gate_x_stride[1], n0, time, reverse), wd(dh, p.d_h_stride[1], n0, time, reverse);
+    Held<T, VEC> hx[U], ha[U], hg[U], hd[U];
+    {
+      Walk<const T> wx(x, p.x_stride[1], n0, time, reverse), wa(ga, p.gate_a_stride[1], n0, time, reverse),
+          wg(gx, p.gate_x_stride[1], n0, time, reverse), wd(dh, p.d_h_stride[1], n0, time, reverse);
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      if (PLAIN || n0 + u < time) {
-        hx[u] = ld_any<VEC, true>(wx.lane(lane_bytes));
-        ha[u] = ld_any<VEC, true>(wa.lane(lane_bytes));
-        hg[u] = ld_any<VEC, true>(wg.lane(lane_bytes));
-        hd[u] = ld_any<VEC, true>(wd.lane(lane_bytes));
+      for (int u = 0; u < U; ++u) {
+        if (PLAIN || n0 + u < time) {
+          hx[u] = ld_any<VEC, true>(wx.lane(lane_bytes));
+          ha[u] = ld_any<VEC, true>(wa.lane(lane_bytes));
+          hg[u] = ld_any<VEC, true>(wg.lane(lane_bytes));
+          hd[u] = ld_any<VEC, true>(wd.lane(lane_bytes));
+        }
+        wx.next();
+        wa.next();
+        wg.next();
+        wd.next();
       }
-      wx.next();
-      wa.next();
-      wg.next();
-      wd.next();
     }
-  }
-  if (wave < VEC) {
-    const float rate = p.rate[ch.base + int(ch.rel) + wave];
-    sh_decay[wave * 64 + lane] = LOG2E * p.scale * fast_softplus(rate);
-  }
-  __syncthreads();
+    if (wave < VEC) {
+      const float rate = p.rate[ch.base + int(ch.rel) + wave];
+      sh_decay[wave * 64 + lane] = LOG2E * p.scale * fast_softplus(rate);
+    }
+    __syncthreads();
 
     unsigned starts = 0, ends = 0;
     if constexpr (CUTS) {
@@ -704,8 +768,8 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(4))) vo
         }
       }
       const long long per_segment = 2ll * blocks * RPB;
-      uint64_t* words = args.chain.desc + 2ll * block * RPB + i;
-      const Chain chain{words, words + args.segments * per_segment, per_segment, kk, args.segments, seq};
+      uint64_t* words = args.chain.desc + 2ll * block * RPB + e * 64;
+      const Chain chain{words, uint32_t(lane) * 8, per_segment, kk, args.segments, seq};
       const float first = !PACKED && p.d_state ? p.d_state[int64_t(batch) * channels + c] : 0.0f;
       auto walk = [&] {
         int from = time;

@@ -397,3 +397,13 @@ def check_on_device(data, dtype):
     ratio = ref.sigmoid_over_softplus(r.cpu())
     ref.assert_within(grads[3], p.sum((0, 1)).cpu() * ratio, 4 * tol32 * p.abs().sum((0, 1)).cpu() * ratio, "d_rate")
     ref.assert_within(grads[4], carry.cpu(), 4 * tol32 * max(1.0, ref.largest(carry.cpu()), ref.largest(g.cpu())), "d_h0")
+
+
+@pytest.mark.parametrize("bounds", [None, [0, 9000, 9001, 24000]])
+def test_long_chains(bounds):
+    """More blocks of groups of segments than are looked at at a time; sequences that start inside one."""
+    if bounds is None:
+        check(make((1, 24000, 3), torch.bfloat16, seed=18), torch.bfloat16)
+        check(make((1, 24000, 2), torch.float32, seed=19), torch.float32, reverse=True)
+    else:
+        check(make((24000, 3), torch.bfloat16, seed=20, sequences=3), torch.bfloat16, bounds=bounds)

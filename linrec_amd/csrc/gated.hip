@@ -82,9 +82,7 @@ int check_gated(const linrec_gated_t* p) {
 // Channels of a lane: 4 bytes' worth, one where there are no two.
 int lane_width(int dtype, int64_t channels) { return dtype == LINREC_DTYPE_F32 || channels < 2 ? 1 : 2; }
 
-constexpr int kFwdRun = 16, kFwdWaves = 4, kBwdRun = 8;
-template <typename T>
-constexpr int kBwdWaves = sizeof(T) == 4 ? 8 : 4;
+constexpr int kFwdRun = 16, kFwdWaves = 4, kBwdRun = 8, kBwdWaves = 8;
 struct Geometry {
   int64_t segments, channel_blocks, grid, tiles;
   int save;
@@ -94,7 +92,7 @@ Geometry geometry(int dtype, int64_t batch, int64_t time, int64_t channels, bool
   const int64_t rows = 64 * lane_width(dtype, channels);
   g.channel_blocks = cdiv(channels, rows);
   const int64_t blocks = g.channel_blocks * batch;
-  g.save = kBwdRun * (dtype == LINREC_DTYPE_F32 ? kBwdWaves<float> : kBwdWaves<__bf16>);
+  g.save = kBwdRun * kBwdWaves;
   g.segments = cdiv(time, bwd ? g.save : kFwdWaves * kFwdRun);
   g.grid = g.segments * blocks;
   g.tiles = chain_places(g.segments) * blocks * rows;  // places of words
@@ -125,7 +123,7 @@ int fill_args(const linrec_gated_t* p, const Geometry& g, GatedArgs* a) {
 
 template <typename T, int VEC, bool PACKED>
 int launch_pass(const GatedArgs& a, const Geometry& g, bool bwd) {
-  return bwd ? launch_kernel(gated_bwd_kernel<T, VEC, kBwdRun, kBwdWaves<T>, PACKED>, g.grid, 1, 64 * kBwdWaves<T>, a.p.stream, a)
+  return bwd ? launch_kernel(gated_bwd_kernel<T, VEC, kBwdRun, kBwdWaves, PACKED>, g.grid, 1, 64 * kBwdWaves, a.p.stream, a)
              : launch_kernel(gated_fwd_kernel<T, VEC, kFwdRun, kFwdWaves, PACKED>, g.grid, 1, 64 * kFwdWaves, a.p.stream, a);
 }
 

@@ -12,22 +12,23 @@
 //   d_x = g m sx,  d_gate_x = g m x sx (1 - sx)                         (sx, sa: the gates' sigmoids)
 //   P = g (log a a h[t-1] - sx x a^2 log a / m),  d_gate_a = P (1 - sa),  d_rate = sigmoid(rate) / softplus(rate) sum P
 // (log a and log a / m both go to zero with sigmoid(gate_a), where 1 / m alone does not: every term stays finite.)  h[t-1] is
-// not read: the forward saves the value that enters every backward segment (32 positions in 16-bit storage, 64 in fp32) as 4 bytes,
-// and the backward goes on from there with the same operations, so the gradient sees the unrounded values and four tensors are read
-// where the saved output would make it five.
+// not read: the forward saves the value that enters every backward segment of 64 positions as 4 bytes, and the backward goes on
+// from there with the same operations, so the gradient sees the unrounded values and four tensors are read where the saved output
+// would make it five.
 //
 // What bounds it: memory where channels are many.  8 x 4096 x 2048 in bf16: 124 us forward (537 MB, 4.3 TB/s of the 5.2 TB/s that
 // a copy reaches) and 222 us backward (940 MB, 4.2 TB/s); 16 x 2048 x 512 in fp32 out of a projection's rows 58 and 105 us (4.6 and
 // 4.5 TB/s).  Without the wait for what enters a segment the former takes 111 and 200 us: the wait is the larger part of the rest,
-// the gates' arithmetic the smaller.  With few channels the chain bounds it: 1 x 32768 x 2048 134 and 248 us, 1 x 131072 x 64 51
-// and 94 us (floors 103, 181; 13, 23).
+// the gates' arithmetic the smaller.  With few channels the chain bounds it: 1 x 32768 x 2048 133 and 234 us, 1 x 131072 x 64 50
+// and 84 us (floors 103, 181; 13, 23).
 //
 // Waves and runs: workgroups wait, so that several to a CU have to hide each other's waits, with all that a segment holds in
-// registers: at most 128 a lane for four workgroups of four waves, and nothing spilled (a handful of registers that are cost 2 to
-// 6 %).  Forward keeps a and the input of 16 positions of two channels, backward a, m and h[t-1] of 8, and the sigmoids in LDS,
-// which saves evaluating them twice.  Eight waves in 16-bit storage instead of four, and longer segments so: 131 and 258 us instead
-// of 125 and 220 for 8 x 4096 x 2048, with twice the links.  fp32, a channel to a lane, needs half the registers a position and
-// takes eight waves in the backward.
+// registers: at most 128 a lane for sixteen waves to a CU, and as little spilled as can be (32 registers that are cost 7 to 20 %).
+// Forward keeps a and the input of 16 positions of two channels, backward a, m and h[t-1] of 8, and the sigmoids in LDS, which
+// saves evaluating them twice.  Forward and backward, 8 x 4096 x 2048 and 1 x 100001 x 250 bf16:
+//   forward, positions of a wave x waves    16 x 4  123 and 81 us    16 x 8  130 and 76    8 x 4  144 and 105    8 x 8  159 and 100
+//   backward                                 8 x 8  222 and 138       8 x 4  222 and 151    4 x 8  299 and 184
+// (longer segments make fewer links, more of them hide each other's waits; shorter runs do more links for what is under way).
 //
 // The value that enters a segment is always the same chain of multiply-adds over the segments before, whichever of them had
 // published what when they were looked at: results are the same bits in every run.
@@ -511,6 +512,9 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(4))) vo
           mb.v[e] = fmaf(g.a, mb.v[e], b[u].v[e]);
           ma.v[e] *= g.a;
         }
+        if constexpr (CUTS) {
+          if (starts >> u & 1u) b[u] = mb;  // (whatever is before)
+        }
       }
     }
 #pragma unroll
@@ -581,11 +585,12 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(4))) vo
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       if (PLAIN || n0 + u < time) {
-        if constexpr (CUTS) {
-          if (starts >> u & 1u) val = initial(u);
-        }
+        if (CUTS && (starts >> u & 1u)) {
+          val = b[u];
+        } else {
 #pragma unroll
-        for (int e = 0; e < VEC; ++e) val.v[e] = fmaf(a[u].v[e], val.v[e], b[u].v[e]);
+          for (int e = 0; e < VEC; ++e) val.v[e] = fmaf(a[u].v[e], val.v[e], b[u].v[e]);
+        }
         T* to = wh.lane(lane_bytes);
         wh.next();
         store_channels<WHOLE>(to, val, ch);

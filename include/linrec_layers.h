@@ -131,7 +131,7 @@ int linrec_group_norm_bwd(const linrec_group_norm_t* args);
 
 /*
  * Embedding: y[n] = scale * weight[token[n]], and its gradient d_weight[v] = scale * sum of d_y[n] over the n with
- * token[n] == v, in ascending order of n.  Tokens are int32 or int64 (token_bytes 4 or 8).  A token outside [0, vocab) gives
+ * token[n] == v, in an order that depends on the tokens alone.  Tokens are int32 or int64 (token_bytes 4 or 8).  A token outside [0, vocab) gives
  * a row of zeros and no gradient; `padding` (negative: none) names a token that is looked up but gets no gradient.
  * weight, y, d_y and d_weight are of type dtype; d_y has a row stride, the others are dense.
  */

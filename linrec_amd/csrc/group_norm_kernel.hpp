@@ -474,6 +474,21 @@ __device__ __forceinline__ void sum_all(float (&v)[N], float* sh, const BlockArg
       v[i] = 0.0f;
       for (int w = 0; w < waves; ++w) v[i] += sh[w * total + i * groups + l.g];
     }
+  } else if (a.columns == a.per_group) {
+    // all waves have the one group
+#pragma unroll
+    for (int i = 0; i < N; ++i) v[i] = team_sum(v[i], 64);
+    __syncthreads();
+    if (lane == 0) {
+#pragma unroll
+      for (int i = 0; i < N; ++i) sh[i * waves + wave] = v[i];
+    }
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      v[i] = 0.0f;
+      for (int w = 0; w < waves; ++w) v[i] += sh[i * waves + w];
+    }
   } else if ((a.per_group & 63) == 0) {
     // a wave has one group
     const int per_row = a.columns >> 6, per_group = a.per_group >> 6, first = l.g * per_group;
@@ -753,7 +768,8 @@ __global__ __launch_bounds__(LANES) void norm_bwd_kernel(BlockArgs args, float* 
         }
       }
     }
-    if (!columns_in_wave(args) && (args.per_group & 63) == 0) sum_all<2>(s, sh, args, l);  // (nothing in the rows but the first)
+    if (!columns_in_wave(args) && (args.columns == args.per_group || (args.per_group & 63) == 0))
+      sum_all<2>(s, sh, args, l);  // (nothing in the rows but the first)
     else sum_group<2>(s, sh, args, l);
   };
   const float inv_count = 1.0f / (float(p.positions) * float(args.whole * VEC));

@@ -275,9 +275,8 @@ class _EmbeddingFn(torch.autograd.Function):
 
 def embedding(tokens: Tensor, weight: Tensor, *, scale: float = 1.0, padding_idx: Optional[int] = None) -> Tensor:
     """scale * weight[tokens], (*tokens.shape, channels), for int32 or int64 tokens and a (vocabulary, channels) table.  The
-    gradient of the table is dense; each of its rows is summed in float32 in the order of the tokens and rounded once, the
-    same in every run.  A token outside the table gives a row of zeros and no gradient; the row `padding_idx` is looked up but
-    gets no gradient.
+    gradient of the table is dense; each of its rows is summed in float32 and rounded once, the same in every run.  A token
+    outside the table gives a row of zeros and no gradient; the row `padding_idx` is looked up but gets no gradient.
     """
     scale = float(scale)
     if _traced(tokens, weight):

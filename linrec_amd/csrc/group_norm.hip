@@ -46,7 +46,8 @@ NormPlan make_norm_plan(int dtype, int64_t batch, int64_t positions, int64_t cha
   while (width % pl.vec) pl.vec >>= 1;
   const int64_t columns = width / pl.vec;  // of a group
 
-  // 16 channels to a lane, at most eight waves to a group
+  // 16 channels to a lane, at most eight waves to a group (32768 x 1024 in 16 groups bf16 31 and 49 us, as a workgroup's columns 61
+  // and 165)
   if (positions == 1 && width <= 16 * 64 * TOKEN_WAVES) {
     pl.shape = Shape::tokens;
     TokenArgs& t = pl.tokens;
@@ -77,7 +78,8 @@ NormPlan make_norm_plan(int dtype, int64_t batch, int64_t positions, int64_t cha
 
   BlockArgs& a = pl.block;
   a.whole = int(columns);
-  // held: whole groups in registers, side by side where one is narrower than a line
+  // held: whole groups in registers, side by side where one is narrower than a line (16 x 2048 x 512 in 32 groups fp32 40 and 66 us,
+  // in chunks 49 and 92; 512 x 64 x 256 in 8 groups bf16 12 and 27, in chunks 16 and 29)
   const int bytes = pl.vec * size;
   const int keep = (bwd && size == 2 ? 24 : 32) / (bytes >= 4 ? bytes / 4 : 1);
   auto rows_of = [](int lanes, int64_t wide) { return wide <= lanes ? lanes / wide : int64_t(0); };
@@ -90,6 +92,9 @@ NormPlan make_norm_plan(int dtype, int64_t batch, int64_t positions, int64_t cha
       if (rounds(lanes, g * columns) > keep) continue;
       // few workgroups: more lanes to each
       if (lanes == 256 && cdiv(groups, g) * batch <= 256 && rounds(lanes, g * columns) > 2) continue;
+      // a backward whose few workgroups hold much is better shared out (1 x 700 x 512 in 8 groups bf16 26 us held, 20 in chunks,
+      // 2 x 2048 x 512 in 32 fp32 26 and 23; of 24 values to a lane 22 and 22, of 128 workgroups and 24 values 24 and 25)
+      if (bwd && cdiv(groups, g) * batch <= 64 && rounds(lanes, g * columns) * pl.vec > 24) continue;
       int64_t items = 1;
       // lanes that have nothing to do take more groups, or more batch items; so do short walks while the chip stays full
       auto grows = [&](int64_t gg, int64_t it) {

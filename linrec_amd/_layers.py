@@ -227,8 +227,8 @@ def gated_saved_numel(dtype, batch, time, channels):
 
 # (A forward hands back the number of its kind of call as well: a backward of the same tensors is looked up by that and the
 # strides of the gradient.)
-def gated_fwd(x, gate_a, gate_x, rate, h0, cu_seqlens, reverse, scale, save):
-    """(h, state, saved, number); saved is None without `save`."""
+def gated_fwd(x, gate_a, gate_x, rate, h0, cu_seqlens, reverse, scale, save, with_state=True):
+    """(h, state, saved, number); state is None without `with_state`, saved without `save`."""
     key = ("gated", x.dtype, x.device, x.shape, x.stride(), _looks(gate_a), _looks(gate_x), _looks(rate), _looks(h0), _looks(cu_seqlens),
            reverse, scale)
     e = _remembered().get(key)
@@ -239,13 +239,13 @@ def gated_fwd(x, gate_a, gate_x, rate, h0, cu_seqlens, reverse, scale, save):
             ((a.sequences, a.channels), gated_saved_numel(x.dtype, a.batch, a.time, a.channels))))
     a = e.args
     if a is None:
-        return gated_fwd(*_with_adjacent_channels(x, gate_a, gate_x), *_dense(rate, h0, cu_seqlens), reverse, scale, save)
+        return gated_fwd(*_with_adjacent_channels(x, gate_a, gate_x), *_dense(rate, h0, cu_seqlens), reverse, scale, save, with_state)
     device = x.device
     h = torch.empty(x.shape, dtype=x.dtype, device=device)
-    state = _floats(e.sizes[0], device)
+    state = _floats(e.sizes[0], device) if with_state else None
     saved = _floats(e.sizes[1], device) if save else None
     a.x, a.gate_a, a.gate_x, a.rate = x.data_ptr(), gate_a.data_ptr(), gate_x.data_ptr(), rate.data_ptr()
-    a.h0, a.cu_seqlens, a.h, a.state, a.saved = _p(h0), _p(cu_seqlens), h.data_ptr(), state.data_ptr(), _p(saved)
+    a.h0, a.cu_seqlens, a.h, a.state, a.saved = _p(h0), _p(cu_seqlens), h.data_ptr(), _p(state), _p(saved)
     _call(x, _lib.linrec_gated_fwd, e, "gated_linrec")
     return h, state, saved, e.number
 

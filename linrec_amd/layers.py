@@ -88,19 +88,19 @@ torch.library.register_autograd("linrec_amd::gated_linrec_fwd", _gated_backward,
 
 class _GatedFn(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, x, gate_a, gate_x, rate, h0, cu_seqlens, reverse, scale):
-        h, state, saved, ctx.number = _layers.gated_fwd(x, gate_a, gate_x, rate, h0, cu_seqlens, reverse, scale, True)
+    def forward(ctx, x, gate_a, gate_x, rate, h0, cu_seqlens, reverse, scale, with_state):
+        h, state, saved, ctx.number = _layers.gated_fwd(x, gate_a, gate_x, rate, h0, cu_seqlens, reverse, scale, True, with_state)
         ctx.save_for_backward(x, gate_a, gate_x, rate, h0, cu_seqlens, saved)
         ctx.set_materialize_grads(False)
         ctx.reverse, ctx.scale = reverse, scale
-        return h, state
+        return (h, state) if with_state else h
 
     @staticmethod
     @_once
-    def backward(ctx, d_h, d_state):
+    def backward(ctx, d_h, d_state=None):
         x, gate_a, gate_x, rate, h0, cu_seqlens, saved = ctx.saved_tensors
         return (*_layers.gated_bwd(d_h, d_state, x, gate_a, gate_x, rate, h0, cu_seqlens, saved, ctx.reverse, ctx.scale, ctx.number),
-                None, None, None)
+                None, None, None, None)
 
 
 def gated_linrec(x: Tensor, gate_a: Tensor, gate_x: Tensor, rate: Tensor, *, h0: Optional[Tensor] = None,
@@ -121,9 +121,9 @@ def gated_linrec(x: Tensor, gate_a: Tensor, gate_x: Tensor, rate: Tensor, *, h0:
     if _traced(x, gate_a, gate_x, rate, h0):
         h, state, _ = gated_linrec_fwd(x, gate_a, gate_x, rate, h0, cu_seqlens, bool(reverse), scale)
     elif _recorded(x, gate_a, gate_x, rate, h0):
-        h, state = _GatedFn.apply(x, gate_a, gate_x, rate, h0, cu_seqlens, reverse, scale)
+        return _GatedFn.apply(x, gate_a, gate_x, rate, h0, cu_seqlens, reverse, scale, return_state)
     else:
-        h, state, *_ = _layers.gated_fwd(x, gate_a, gate_x, rate, h0, cu_seqlens, reverse, scale, False)
+        h, state, *_ = _layers.gated_fwd(x, gate_a, gate_x, rate, h0, cu_seqlens, reverse, scale, False, return_state)
     return (h, state) if return_state else h
 
 

@@ -99,13 +99,16 @@ Geometry geometry(int dtype, int64_t batch, int64_t time, int64_t channels, bool
   return g;
 }
 
+// Rows are whole lines of 128 bytes.
+bool whole_lines(const linrec_gated_t& p) { return p.channels * (p.dtype == LINREC_DTYPE_F32 ? 4 : 2) % 128 == 0; }
+
 int fill_args(const linrec_gated_t* p, const Geometry& g, GatedArgs* a) {
   a->p = *p;
   a->chain = TileArgs{};
   a->segments = int(g.segments);
   a->channel_blocks = int(g.channel_blocks);
   a->save = g.save;
-  a->side = p->channels * (p->dtype == LINREC_DTYPE_F32 ? 4 : 2) % 128 ? 8 : GROUP;
+  a->side = whole_lines(*p) ? GROUP : 8;
   if (a->side > g.segments) a->side = int(g.segments);
   if (g.grid > 2147483647LL) return LINREC_E_TOO_LARGE;
   if (g.segments <= 1) return LINREC_OK;
@@ -121,20 +124,27 @@ int fill_args(const linrec_gated_t* p, const Geometry& g, GatedArgs* a) {
   return LINREC_OK;
 }
 
-template <typename T, int VEC, bool PACKED>
+template <typename T, int VEC, bool PACKED, bool LINES>
 int launch_pass(const GatedArgs& a, const Geometry& g, bool bwd) {
-  return bwd ? launch_kernel(gated_bwd_kernel<T, VEC, kBwdRun, kBwdWaves, PACKED>, g.grid, 1, 64 * kBwdWaves, a.p.stream, a)
-             : launch_kernel(gated_fwd_kernel<T, VEC, kFwdRun, kFwdWaves, PACKED>, g.grid, 1, 64 * kFwdWaves, a.p.stream, a);
+  return bwd ? launch_kernel(gated_bwd_kernel<T, VEC, kBwdRun, kBwdWaves, PACKED, LINES>, g.grid, 1, 64 * kBwdWaves, a.p.stream, a)
+             : launch_kernel(gated_fwd_kernel<T, VEC, kFwdRun, kFwdWaves, PACKED, LINES>, g.grid, 1, 64 * kFwdWaves, a.p.stream, a);
+}
+template <typename T, int VEC>
+int launch_pass(const GatedArgs& a, const Geometry& g, bool bwd) {
+  if constexpr (VEC * sizeof(T) == 2)  // (rows of one value)
+    return a.p.cu_seqlens ? launch_pass<T, VEC, true, false>(a, g, bwd) : launch_pass<T, VEC, false, false>(a, g, bwd);
+  else if (a.p.cu_seqlens) return whole_lines(a.p) ? launch_pass<T, VEC, true, true>(a, g, bwd) : launch_pass<T, VEC, true, false>(a, g, bwd);
+  else
+    return whole_lines(a.p) ? launch_pass<T, VEC, false, true>(a, g, bwd) : launch_pass<T, VEC, false, false>(a, g, bwd);
 }
 
 int launch_pass(const GatedArgs& a, const Geometry& g, bool bwd) {
   return with_dtype(a.p.dtype, [&](auto t) {
     using T = decltype(t);
-    const bool packed = a.p.cu_seqlens != nullptr;
     if constexpr (sizeof(T) == 2) {
-      if (lane_width(a.p.dtype, a.p.channels) == 2) return packed ? launch_pass<T, 2, true>(a, g, bwd) : launch_pass<T, 2, false>(a, g, bwd);
+      if (lane_width(a.p.dtype, a.p.channels) == 2) return launch_pass<T, 2>(a, g, bwd);
     }
-    return packed ? launch_pass<T, 1, true>(a, g, bwd) : launch_pass<T, 1, false>(a, g, bwd);
+    return launch_pass<T, 1>(a, g, bwd);
   });
 }
 

@@ -16,11 +16,11 @@
 // from there with the same operations, so the gradient sees the unrounded values and four tensors are read where the saved output
 // would make it five.
 //
-// What bounds it: memory where channels are many.  8 x 4096 x 2048 in bf16: 124 us forward (537 MB, 4.3 TB/s of the 5.2 TB/s that
-// a copy reaches) and 222 us backward (940 MB, 4.2 TB/s); 16 x 2048 x 512 in fp32 out of a projection's rows 58 and 105 us (4.6 and
+// What bounds it: memory where channels are many.  8 x 4096 x 2048 in bf16: 122 us forward (537 MB, 4.4 TB/s of the 5.2 TB/s that
+// a copy reaches) and 221 us backward (940 MB, 4.2 TB/s); 16 x 2048 x 512 in fp32 out of a projection's rows 57 and 104 us (4.7 and
 // 4.5 TB/s).  Without the wait for what enters a segment the former takes 111 and 200 us: the wait is the larger part of the rest,
-// the gates' arithmetic the smaller.  With few channels the chain bounds it: 1 x 32768 x 2048 133 and 234 us, 1 x 131072 x 64 50
-// and 84 us (floors 103, 181; 13, 23).
+// the gates' arithmetic the smaller.  With few channels the chain bounds it: 1 x 32768 x 2048 132 and 231 us, 1 x 131072 x 64 49
+// and 81 us (floors 103, 181; 13, 23).
 //
 // Waves and runs: workgroups wait, so that several to a CU have to hide each other's waits, with all that a segment holds in
 // registers: at most 128 a lane for sixteen waves to a CU, and as little spilled as can be (32 registers that are cost 7 to 20 %).
@@ -61,7 +61,7 @@ struct GatedArgs {
 // 4096 x 2048 bf16 124 and 221 us (one by one 128 and 221), 1 x 32768 x 2048 134 and 247 (154 and 293).  Workgroups are dealt to the
 // eight XCDs in turn, so that in sets of eight neighbouring blocks of a segment run on the same one; where rows are not whole lines
 // of 128 bytes they write parts of the same lines, which one L2 puts together: 16 x 6250 x 250 bf16 73 and 130 us instead of 81 and
-// 144, 1 x 100001 x 250 82 and 150 instead of 88 and 162 (for whole lines eight are slower: 127 and 235, 136 and 248 above).
+// 144, 4 x 4096 x 1000 43 and 76 instead of 49 and 86 (for whole lines eight are slower: 127 and 235, 136 and 248 above).
 struct Place {
   int segment;
   unsigned block;
@@ -210,14 +210,30 @@ __device__ __forceinline__ Channels<VEC> lane_channels(int block, int lane, int 
   ch.whole = c0 + 64 * VEC <= channels;
   return ch;
 }
-// WHOLE: every lane of the block stores all its channels.
-template <bool WHOLE, int VEC, typename T>
+// WHOLE: every lane of the block stores all its channels.  LINES: rows are whole lines of 128 bytes, and stored past the caches (8 x
+// 4096 x 2048 bf16 backward 220 us, through them 227); others go through them, where the parts of a line that neighbouring blocks
+// and rows write come together (16 x 6250 x 250 bf16 69 and 113 us, past them 74 and 132; 8 x 4096 x 1001 fp32 123 and 233, past them
+// 140 and 274).
+template <bool LINES, bool WHOLE, int VEC, typename T>
 __device__ __forceinline__ void store_channels(T* p, const Lanes<VEC>& v, const Channels<VEC>& ch) {
+  auto store = [&]() __attribute__((always_inline)) {
+    if constexpr (LINES) {
+      st_any<VEC>(p, v);
+    } else if constexpr (VEC == 1) {
+      *p = T(v.v[0]);
+    } else {
+      using A = typename AnyPack<T, VEC>::type;
+      A q;
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) q[e] = T(v.v[e]);
+      *reinterpret_cast<A*>(p) = q;
+    }
+  };
   if constexpr (WHOLE) {
-    st_any<VEC>(p, v);
+    store();
   } else {
     if (ch.own == 0) {
-      st_any<VEC>(p, v);
+      store();
     } else {
 #pragma unroll
       for (int e = 1; e < VEC; ++e)
@@ -262,7 +278,7 @@ __device__ __forceinline__ P* plus_bytes(P* p, uint32_t bytes) {
 // Words of a place (a segment's, a group's, a block's): first the factors of the block's channels, then the addends, RPB each, with the
 // launch's number; an addend marked `done` leaves the place whatever enters it (a sequence starts inside, or what entered is in it).
 constexpr int LOOK = 4;   // blocks looked at at a time
-constexpr int SLEEP = 32;  // between two looks, 64 cycles each (8: 1 x 32768 x 2048 bf16 159 and 301 us instead of 154 and 293)
+constexpr int SLEEP = 16;  // between two looks, 64 cycles each (32: 1 x 32768 x 2048 bf16 133 and 234 us instead of 132 and 231; 64: 136 and 244)
 constexpr int GROUP = 5;  // segments of a group, groups of a block
 // Places of a chain of `segments`: theirs, their groups', their blocks'.
 constexpr int64_t chain_places(int64_t segments) { return segments + segments / GROUP + segments / (GROUP * GROUP); }
@@ -419,7 +435,7 @@ struct Walk {
 };
 
 // ---- forward ----------------------------------------------------------------------------------
-template <typename T, int VEC, int U, int NW, bool PACKED>
+template <typename T, int VEC, int U, int NW, bool PACKED, bool LINES>
 __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(4))) void gated_fwd_kernel(GatedArgs args) {
   constexpr int RPB = 64 * VEC, SEG = NW * U;
   static_assert(VEC <= NW, "a wave per channel of a lane looks back");
@@ -593,7 +609,7 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(4))) vo
         }
         T* to = wh.lane(lane_bytes);
         wh.next();
-        store_channels<WHOLE>(to, val, ch);
+        store_channels<LINES, WHOLE>(to, val, ch);
         if (CUTS && p.state && (ends >> u & 1u))
           store_floats(p.state + int64_t(__builtin_amdgcn_readfirstlane(marks.end[wave * U + u])) * channels + ch.base + ch.rel, val, ch);
         if (!PACKED && (!PLAIN || u == U - 1) && n0 + u == time - 1 && p.state)
@@ -619,7 +635,7 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(4))) vo
 }
 
 // ---- backward ---------------------------------------------------------------------------------
-template <typename T, int VEC, int U, int NW, bool PACKED>
+template <typename T, int VEC, int U, int NW, bool PACKED, bool LINES>
 __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(4))) void gated_bwd_kernel(GatedArgs args) {
   constexpr int RPB = 64 * VEC, SEG = NW * U;
   static_assert(2 * VEC <= NW, "a wave per channel of a lane and direction");
@@ -859,9 +875,9 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(4))) vo
         T* to_x = ox.lane(lane_bytes);
         T* to_a = oa.lane(lane_bytes);
         T* to_g = og.lane(lane_bytes);
-        store_channels<WHOLE>(to_x, rx, ch);
-        store_channels<WHOLE>(to_a, ra, ch);
-        store_channels<WHOLE>(to_g, rg, ch);
+        store_channels<LINES, WHOLE>(to_x, rx, ch);
+        store_channels<LINES, WHOLE>(to_a, ra, ch);
+        store_channels<LINES, WHOLE>(to_g, rg, ch);
         if (CUTS && p.d_h0 && (starts >> u & 1u))
           store_floats(p.d_h0 + int64_t(__builtin_amdgcn_readfirstlane(marks.start[wave * U + u])) * channels + ch.base + ch.rel, back, ch);
         if (!PACKED && u == 0 && n0 == 0 && p.d_h0) store_floats(p.d_h0 + int64_t(batch) * channels + ch.base + ch.rel, back, ch);

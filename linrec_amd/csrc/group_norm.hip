@@ -29,6 +29,7 @@ struct NormPlan {
   int64_t pieces;      // floats of partial statistics
   TokenArgs tokens;
   int items_per_lane;  // tokens: slots of a lane
+  bool parts;          // held: a workgroup's rows are fp32 and not whole lines
   BlockArgs block;
 };
 
@@ -78,7 +79,7 @@ NormPlan make_norm_plan(int dtype, int64_t batch, int64_t positions, int64_t cha
 
   BlockArgs& a = pl.block;
   a.whole = int(columns);
-  // held: whole groups in registers, side by side where one is narrower than a line (16 x 2048 x 512 in 32 groups fp32 40 and 66 us,
+  // held: whole groups in registers, side by side where one is narrower than a line (16 x 2048 x 512 in 32 groups fp32 38 and 62 us,
   // in chunks 49 and 92; 512 x 64 x 256 in 8 groups bf16 12 and 27, in chunks 16 and 29)
   const int bytes = pl.vec * size;
   const int keep = (bwd && size == 2 ? 24 : 32) / (bytes >= 4 ? bytes / 4 : 1);
@@ -112,6 +113,7 @@ NormPlan make_norm_plan(int dtype, int64_t batch, int64_t positions, int64_t cha
       a.columns = int(items * g * columns);
       a.R = int(rows_of(lanes, a.columns));
       a.rows = int(positions);
+      pl.parts = size == 4 && (g * columns * bytes % 128 != 0 || channels * size % 128 != 0);
       pl.param_rows = cdiv(batch, items);
       pl.grid = pl.param_rows * a.blocks;
       return pl;
@@ -156,22 +158,32 @@ int launch_tokens(const linrec_group_norm_t& p, const NormPlan& pl) {
                                 : launch_kernel(norm_tokens_kernel<T, VEC, 16 / VEC, BWD>, pl.grid, 1, pl.lanes, p.stream, a);
 }
 
+template <typename T, int VEC, int LANES, int PHASE>
+int launch_held(const BlockArgs& a, const NormPlan& pl, bool bwd, float* sums) {
+  return bwd ? launch_kernel(norm_bwd_kernel<T, VEC, LANES, PHASE>, pl.grid, 1, LANES, a.p.stream, a, sums)
+             : launch_kernel(norm_fwd_kernel<T, VEC, LANES, PHASE>, pl.grid, 1, LANES, a.p.stream, a);
+}
+template <typename T, int VEC, int PHASE>
+int launch_held(const BlockArgs& a, const NormPlan& pl, bool bwd, float* sums) {
+  return pl.lanes == 256 ? launch_held<T, VEC, 256, PHASE>(a, pl, bwd, sums) : launch_held<T, VEC, 1024, PHASE>(a, pl, bwd, sums);
+}
+
 template <typename T, int VEC>
 int launch_norm(const linrec_group_norm_t& p, const NormPlan& pl, bool bwd) {
   if (pl.shape == Shape::tokens) return bwd ? launch_tokens<T, VEC, true>(p, pl) : launch_tokens<T, VEC, false>(p, pl);
   BlockArgs a = pl.block;
   a.p = p;
   float* sums = p.partial + pl.pieces;
+  if (pl.shape == Shape::held) {
+    if constexpr (sizeof(T) == 4) {
+      if (pl.parts) return launch_held<T, VEC, NORM_HELD_PARTS>(a, pl, bwd, sums);
+    }
+    return launch_held<T, VEC, NORM_HELD>(a, pl, bwd, sums);
+  }
   if (!bwd) {
-    if (pl.shape == Shape::held)
-      return pl.lanes == 256 ? launch_kernel(norm_fwd_kernel<T, VEC, 256, NORM_HELD>, pl.grid, 1, 256, p.stream, a)
-                             : launch_kernel(norm_fwd_kernel<T, VEC, 1024, NORM_HELD>, pl.grid, 1, 1024, p.stream, a);
     if (const int rc = launch_kernel(norm_fwd_kernel<T, VEC, 256, NORM_STATS>, pl.grid, 1, 256, p.stream, a)) return rc;
     return launch_kernel(norm_fwd_kernel<T, VEC, 256, NORM_APPLY>, pl.grid, 1, 256, p.stream, a);
   }
-  if (pl.shape == Shape::held)
-    return pl.lanes == 256 ? launch_kernel(norm_bwd_kernel<T, VEC, 256, NORM_HELD>, pl.grid, 1, 256, p.stream, a, sums)
-                           : launch_kernel(norm_bwd_kernel<T, VEC, 1024, NORM_HELD>, pl.grid, 1, 1024, p.stream, a, sums);
   if (const int rc = launch_kernel(norm_bwd_kernel<T, VEC, 256, NORM_STATS>, pl.grid, 1, 256, p.stream, a, sums)) return rc;
   return launch_kernel(norm_bwd_kernel<T, VEC, 256, NORM_APPLY>, pl.grid, 1, 256, p.stream, a, sums);
 }

@@ -6,8 +6,8 @@
 //
 // What bounds it: memory, and the launches where little is normed.  Forward and backward: 32768 x 1024 in 16 groups, bf16, 31 and
 // 49 us (134 and 201 MB: 4.4 and 4.1 TB/s of the 5.2 that a copy reaches), fp32 52 and 76 (5.1 and 5.3); 16 x 2048 x 512 in 32 groups,
-// fp32, gelu 40 and 66 us (3.3 and 3.0 TB/s): one round of workgroups that all load, then add up, then store; 8 x 16384 x 512 in 32
-// groups, bf16, in chunks 95 and 157 us, for three and five tensors' worth of memory traffic.  3 x 333 x 222 in 6 groups: 13 us, of
+// fp32, gelu 38 and 62 us (3.5 and 3.3 TB/s): one round of workgroups that all load, then add up, then store; 8 x 16384 x 512 in 32
+// groups, bf16, in chunks 95 and 157 us, for three and five tensors' worth of memory traffic.  3 x 333 x 222 in 6 groups: 12 us, of
 // which an empty kernel takes 6.  Three shapes, by how much one group is:
 //   tokens  one position: a team of 1 .. 64 adjacent lanes holds a group in registers; waves keep their channels and walk down
 //           the rows, so weights are read once and the sums of d_w and d_b stay in registers.
@@ -559,7 +559,26 @@ __device__ __forceinline__ int64_t piece_index(const BlockArgs& a, int64_t n, in
   return ((n * a.chunks * a.parts + piece) * a.p.groups + group) * 2;
 }
 
-constexpr int NORM_HELD = 0, NORM_STATS = 1, NORM_APPLY = 2;
+// NORM_HELD_PARTS: the workgroup's rows are fp32 and not whole lines of 128 bytes.  Its results go through the caches, where the parts
+// of a line that neighbours write come together, all others past them: 16 x 2048 x 512 in 32 groups fp32 38 and 62 us, past the caches 40
+// and 66; whole lines, 512 x 64 x 256 in 8 groups bf16, 11 and 27 us past them and 14 and 29 through them; parts of 16 bits gain nothing,
+// 16 x 2048 x 510 in 30 groups bf16 39 and 52 us through them and 38 and 52 past them, 32 x 1024 x 256 in 32 groups 15 and 27, 13 and 27.
+constexpr int NORM_HELD = 0, NORM_STATS = 1, NORM_APPLY = 2, NORM_HELD_PARTS = 3;
+constexpr bool holds(int phase) { return phase == NORM_HELD || phase == NORM_HELD_PARTS; }
+template <int PHASE, int VEC, typename T>
+__device__ __forceinline__ void store_result(T* to, const Lanes<VEC>& v) {
+  if constexpr (PHASE != NORM_HELD_PARTS) {
+    st_any<VEC>(to, v);
+  } else if constexpr (VEC == 1) {
+    *to = T(v.v[0]);
+  } else {
+    using A = typename AnyPack<T, VEC>::type;
+    A q;
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) q[e] = T(v.v[e]);
+    *reinterpret_cast<A*>(to) = q;
+  }
+}
 template <int VEC, typename T>
 constexpr int held_rows(bool two) {  // of a lane: 32 registers' worth, 24 of each of two 16-bit tensors (what they widen to needs more)
   return (two && sizeof(T) == 2 ? 24 : 32) / (VEC * int(sizeof(T)) >= 4 ? VEC * int(sizeof(T)) / 4 : 1);
@@ -568,7 +587,7 @@ constexpr int held_rows(bool two) {  // of a lane: 32 registers' worth, 24 of ea
 template <typename T, int VEC, int LANES, int PHASE>
 __global__ __launch_bounds__(LANES) void norm_fwd_kernel(BlockArgs args) {
   constexpr int KEEP = held_rows<VEC, T>(false);
-  __shared__ float sh[(PHASE == NORM_HELD ? 1 : 3) * LANES];
+  __shared__ float sh[(holds(PHASE) ? 1 : 3) * LANES];
   const linrec_group_norm_t& p = args.p;
   const BlockLane l = block_lane<VEC>(args);
   const T* x = static_cast<const T*>(p.x) + l.n * p.x_stride[0] + l.channel;
@@ -586,11 +605,11 @@ __global__ __launch_bounds__(LANES) void norm_fwd_kernel(BlockArgs args) {
 #pragma unroll
     for (int e = 0; e < VEC; ++e) v.v[e] = fmaf((v.v[e] - mean) * rstd, w[e], b[e]);
     activate<VEC>(p.act, v.v);
-    st_any<VEC>(y + pos * p.channels, v);
+    store_result<PHASE>(y + pos * p.channels, v);
   };
   const bool writes = l.there && l.r == 0 && l.q == 0 && (PHASE != NORM_APPLY || (l.first == 0 && l.channel == l.group * args.whole * VEC));
 
-  if constexpr (PHASE == NORM_HELD) {
+  if constexpr (holds(PHASE)) {
     Held<T, VEC> held[KEEP];
     float s[1] = {0.0f};
 #pragma unroll
@@ -741,7 +760,7 @@ __global__ __launch_bounds__(LANES) void norm_bwd_kernel(BlockArgs args, float* 
     Lanes<VEC> out;
 #pragma unroll
     for (int i = 0; i < VEC; ++i) out.v[i] = rstd * (fmaf(e[i], w[i], -s[0]) - xh[i] * s[1]);
-    st_any<VEC>(dx + pos * p.channels, out);
+    store_result<PHASE>(dx + pos * p.channels, out);
   };
   // the columns' sums, from there those of d_weight and d_bias and the group's
   auto finish_sums = [&]() __attribute__((always_inline)) {
@@ -778,7 +797,7 @@ __global__ __launch_bounds__(LANES) void norm_bwd_kernel(BlockArgs args, float* 
   };
   const float inv_count = 1.0f / (float(p.positions) * float(args.whole * VEC));
 
-  if constexpr (PHASE == NORM_HELD) {
+  if constexpr (holds(PHASE)) {
     Held<T, VEC> hx[KEEP], hd[KEEP];
 #pragma unroll
     for (int i = 0; i < KEEP; ++i) {

@@ -28,7 +28,8 @@
 // saves evaluating them twice.  Forward and backward, 8 x 4096 x 2048 and 1 x 100001 x 250 bf16:
 //   forward, positions of a wave x waves    16 x 4  123 and 81 us    16 x 8  130 and 76    8 x 4  144 and 105    8 x 8  159 and 100
 //   backward                                 8 x 8  222 and 138       8 x 4  222 and 151    4 x 8  299 and 184
-// (longer segments make fewer links, more of them hide each other's waits; shorter runs do more links for what is under way).
+// (longer segments make fewer links, more of them hide each other's waits; shorter runs do more links for what is under way; the rows
+// of 250 were stored past the caches then, and take 79 and 129 us through them).
 //
 // The value that enters a segment is always the same chain of multiply-adds over the segments before, whichever of them had
 // published what when they were looked at: results are the same bits in every run.
@@ -269,7 +270,7 @@ __device__ __forceinline__ P* plus_bytes(P* p, uint32_t bytes) {
 // are looked at at a time, so the value advances by LOOK * GROUP * GROUP segments a link.  Which of them had published what does not
 // matter to the result: the value that leaves a block is the same multiply-add whoever makes it.
 //
-// 1 x 100001 x 250 bf16, forward and backward: groups of 8 without blocks over them 119 and 226 us, with blocks 100 and 192; groups
+// Steps that led here, 1 x 100001 x 250 bf16, forward and backward: groups of 8 without blocks over them 119 and 226 us, with blocks 100 and 192; groups
 // of 4 / 5 / 6 with blocks 103, 197 / 90, 167 / 96, 187.  1 x 131072 x 64, groups of 4 / 5 / 6 / 8: 66, 125 / 50, 93 / 53, 100 / 59,
 // 117 (a link of 4 advances by 64 segments, one of 5 by 100; larger groups take registers that the data needs).  LOOK of 6 instead
 // of 4: 8 x 4096 x 2048 130 and 230 us instead of 128 and 221, 50 and 98 here.  The groups before by other waves, while the first

@@ -117,6 +117,10 @@ def _looks(t):
     return None if t is None else (t.dtype, t.device, t.shape, t.stride())
 
 
+def _strides(*tensors):
+    return tuple([None if t is None else t.stride() for t in tensors])
+
+
 def _call(t, fn, entry, what):
     """fn on the entry's arguments, on t's device and current stream."""
     index = t.device.index
@@ -151,11 +155,15 @@ def _p(t):
 
 
 # ---- checks (of calls that are not remembered) --------------------------------------------------
+def _check_device(what, t, name):
+    if not t.is_cuda:
+        raise RuntimeError(f"{what}: needs device tensors, {name} is on {t.device}")
+
+
 def _check_activations(what, x, *others, names=()):
     if x.dtype not in DTYPES:
         raise RuntimeError(f"{what}: x must be float32, float16 or bfloat16, got {x.dtype}")
-    if not x.is_cuda:
-        raise RuntimeError(f"{what}: needs device tensors, x is on {x.device}")
+    _check_device(what, x, "x")
     for t, name in zip(others, names):
         if t.size() != x.size():
             raise RuntimeError(f"{what}: {name} has size {tuple(t.size())}, x has {tuple(x.size())}")
@@ -225,8 +233,9 @@ def gated_saved_numel(dtype, batch, time, channels):
     return _lib.linrec_gated_saved_floats(DTYPES[dtype], batch, time, channels)
 
 
-# (A forward hands back the number of its kind of call as well: a backward of the same tensors is looked up by that and the
-# strides of the gradient.)
+# (A forward hands back the number of its kind of call as well, which stands for sizes, types, devices and options.  It says nothing
+# of how what the backward reads lies in memory: a forward may have copied an input that the backward gets as it was, and hooks
+# of saved tensors may give back another layout.  So a backward is looked up by that number and the strides of all that it reads.)
 def gated_fwd(x, gate_a, gate_x, rate, h0, cu_seqlens, reverse, scale, save, with_state=True):
     """(h, state, saved, number); state is None without `with_state`, saved without `save`."""
     key = ("gated", x.dtype, x.device, x.shape, x.stride(), _looks(gate_a), _looks(gate_x), _looks(rate), _looks(h0), _looks(cu_seqlens),
@@ -255,7 +264,7 @@ def gated_bwd(d_h, d_state, x, gate_a, gate_x, rate, h0, cu_seqlens, saved, reve
     if d_h is None:
         d_h = torch.zeros((), dtype=x.dtype, device=x.device).expand(x.size())
     if number is not None:
-        key = (number, d_h.stride(), None if d_state is None else d_state.stride())
+        key = (number, _strides(d_h, d_state, x, gate_a, gate_x, rate, h0, cu_seqlens))
     else:
         key = ("gated_bwd", x.dtype, x.device, x.shape, x.stride(), _looks(d_h), _looks(d_state), _looks(gate_a), _looks(gate_x), _looks(rate),
                _looks(h0), _looks(cu_seqlens), reverse, scale)
@@ -279,6 +288,7 @@ def gated_bwd(d_h, d_state, x, gate_a, gate_x, rate, h0, cu_seqlens, saved, reve
         d_state, rate, h0, cu_seqlens = _dense(d_state, rate, h0, cu_seqlens)
         return gated_bwd(d_h, d_state, x, gate_a, gate_x, rate, h0, cu_seqlens, saved, reverse, scale)
     device, shape, dtype = x.device, x.shape, x.dtype
+    saved = saved.contiguous()
     d_x, d_gate_a, d_gate_x = (torch.empty(shape, dtype=dtype, device=device), torch.empty(shape, dtype=dtype, device=device),
                                torch.empty(shape, dtype=dtype, device=device))
     d_rate, partial = _floats(rate.shape, device), _floats(e.sizes[0], device)
@@ -411,7 +421,7 @@ def norm_fwd(x, groups, weight, bias, eps, act):
 def norm_bwd(d_y, x, groups, weight, bias, stats, eps, act, number=None):
     """(d_x, d_weight, d_bias), the last two None without a weight"""
     if number is not None:
-        key = (number, d_y.stride())
+        key = (number, _strides(d_y, x, weight, bias))
     else:
         key = ("norm_bwd", x.dtype, x.device, x.shape, x.stride(), groups, _looks(d_y), _looks(weight), _looks(bias), eps, act)
     e = _remembered().get(key) or _norm_entry(key, x, groups, weight, bias, eps, act, d_y)
@@ -419,6 +429,7 @@ def norm_bwd(d_y, x, groups, weight, bias, stats, eps, act, number=None):
     if a is None:
         return norm_bwd(*_dense(d_y, x), groups, *_dense(weight, bias), stats, eps, act)
     device = x.device
+    stats = stats.contiguous()
     d_x = torch.empty(x.shape, dtype=x.dtype, device=device)
     d_weight = d_bias = None
     if weight is not None:
@@ -437,8 +448,7 @@ def _embedding_args(tokens, weight, scale, padding_idx):
     what = "embedding"
     if weight.dtype not in DTYPES:
         raise RuntimeError(f"{what}: weight must be float32, float16 or bfloat16, got {weight.dtype}")
-    if not weight.is_cuda:
-        raise RuntimeError(f"{what}: needs device tensors, weight is on {weight.device}")
+    _check_device(what, weight, "weight")
     if weight.dim() != 2:
         raise RuntimeError(f"{what}: weight must be (vocabulary, channels), got {weight.dim()} dimensions")
     if tokens.dtype not in (torch.int32, torch.int64):
@@ -474,7 +484,7 @@ def embedding_fwd(tokens, weight, scale, padding_idx):
 def embedding_bwd(d_y, tokens, weight, scale, padding_idx, number=None):
     """The gradient of `weight` (whose values are not read)."""
     if number is not None:
-        key = (number, d_y.stride())
+        key = (number, _strides(d_y, tokens))
     else:
         key = ("embedding_bwd", _looks(d_y), _looks(tokens), weight.dtype, weight.device, weight.shape, scale, padding_idx)
     e = _remembered().get(key)

@@ -33,6 +33,11 @@ def kept(tensors):
     return torch.autograd.graph.saved_tensors_hooks(lambda t: t, unpack)
 
 
+def owners_of(inputs, unpacked):
+    """Who has an address in the forward, and in the backward (what a hook gave back may lie where a copy of the forward lay)."""
+    return [{t.data_ptr(): t for t in tensors} for tensors in (inputs, inputs + unpacked)]
+
+
 def check_gated(fields, owners, sizes):
     for name in ("x", "gate_a", "gate_x"):
         got, owner = fields[name + "_stride"], owners.get(fields[name])
@@ -94,8 +99,8 @@ def test_gated_linrec_reads_every_layout_by_its_own_strides(blocks, packed, layo
             del blocks[:]
             owned = gated_step(tensors, hooks)
             assert [name for name, _ in blocks] == ["linrec_gated_fwd", "linrec_gated_bwd"]
-            for name, fields in blocks:
-                check_gated(fields, {t.data_ptr(): t for t in owned + unpacked}, {"x": tensors["x"].shape})
+            for (_, fields), owners in zip(blocks, owners_of(owned, unpacked)):
+                check_gated(fields, owners, {"x": tensors["x"].shape})
 
 
 def norm_inputs(layout):
@@ -124,8 +129,7 @@ def test_group_norm_act_reads_every_layout_by_its_own_strides(blocks, layout, ho
                 y = linrec_amd.group_norm_act(leaves[0], 2, *leaves[1:])
                 torch.autograd.grad(y, leaves, torch.empty(y.shape))
             assert [name for name, _ in blocks] == ["linrec_group_norm_fwd", "linrec_group_norm_bwd"]
-            owners = {t.data_ptr(): t for t in leaves + unpacked}
-            for _, fields in blocks:
+            for (_, fields), owners in zip(blocks, owners_of(leaves, unpacked)):
                 x = owners.get(fields["x"])
                 assert fields["x_stride"] == (dense_strides((2, 5, 8)) if x is None else x.stride())[:2]
                 assert x is None or x.stride(-1) == 1
@@ -148,6 +152,5 @@ def test_embedding_reads_every_layout_of_tokens(blocks, layout, hooked, dense_fi
                 y = linrec_amd.embedding(tokens, weight)
                 torch.autograd.grad(y, weight, torch.empty(y.shape))
             assert [name for name, _ in blocks] == ["linrec_embedding_fwd", "linrec_embedding_bwd"]
-            owners = {t.data_ptr(): t for t in [tokens] + unpacked}
-            for _, fields in blocks:
+            for (_, fields), owners in zip(blocks, owners_of([tokens], unpacked)):
                 assert fields["token"] not in owners or owners[fields["token"]].is_contiguous()

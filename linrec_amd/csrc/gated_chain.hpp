@@ -16,6 +16,9 @@
 //
 // Words of a place (a segment's, a group's, a block's): first the factors of the block's channels, then the addends, RPB each, with the
 // launch's number; an addend marked `done` leaves the place whatever enters it (a sequence starts inside, or what entered is in it).
+// The words of a segment or a group are written once a launch: maps_before takes a place as constant for all lanes of a wave or none,
+// and a wave that looks while another one writes sees some lanes' words before and some after.  Those of a block may turn from a
+// map to `done`; what leaves blocks is taken lane by lane.
 #pragma once
 #include <stdint.h>
 
@@ -171,8 +174,8 @@ __device__ __forceinline__ float enter_segment(const TileArgs& args, const Chain
   if (__builtin_expect(!known, 0)) {
     if (lane == 0) __hip_atomic_fetch_add(&args.ws->gave_up, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     v = walk();
-    // (whoever looks for what leaves the group or block waits for it: it leaves through this segment)
-    if (closes) st_desc(plus_bytes(scalar((closes_block ? of_block : of_group) + RPB), c.lane_bytes), pack_desc(c.done(), cut ? tb : fmaf(ta, v, tb)));
+    // (whoever looks for what leaves the block, or a group whose map is not there, waits for it: it leaves through this segment)
+    if (closes_block || (closes && !seg.there)) st_desc(plus_bytes(scalar((closes_block ? of_block : of_group) + RPB), c.lane_bytes), pack_desc(c.done(), cut ? tb : fmaf(ta, v, tb)));
   }
   return v;
 }

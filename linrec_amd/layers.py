@@ -143,13 +143,18 @@ def gated_linrec_step(x: Tensor, gate_a: Tensor, gate_x: Tensor, rate: Tensor, s
     """One position of gated_linrec for a batch of rows, for serving: x, gate_a and gate_x are (batch, channels), `state`
     (rows, channels) float32 holds the values before this position and is updated in place.  `slots` (int32, on the device)
     names the row of `state` that each row of x uses; a row whose slot is negative or not in `state` takes no part: its
-    result is zero.  No row of `state` may be named twice.  Records no gradient.
+    result is zero.  No row of `state` may be named twice.  Records no gradient, in neither direction.
     """
     if torch.is_grad_enabled() and any(t.requires_grad for t in (x, gate_a, gate_x, rate, state)):
         raise RuntimeError("gated_linrec_step: records no gradient; call it under torch.no_grad(), or gated_linrec for training")
+    if forward_ad._current_level >= 0 and any(forward_ad.unpack_dual(t).tangent is not None for t in (x, gate_a, gate_x, rate, state)):
+        raise RuntimeError("gated_linrec_step: records no gradient, a tangent of its inputs would be lost")
     if _traced(x, gate_a, gate_x, rate, state):
         return _gated_linrec_step(x, gate_a, gate_x, rate, state, slots, float(scale))
-    return _layers.gated_step(x, gate_a, gate_x, rate, state, slots, float(scale))
+    h = _layers.gated_step(x, gate_a, gate_x, rate, state, slots, float(scale))
+    if not state.is_inference():
+        torch.autograd.graph.increment_version(state)  # (as the registered operator does: whoever saved `state` has to know)
+    return h
 
 
 # ---- group norm with an activation -------------------------------------------------------------

@@ -34,6 +34,14 @@ def _recorded(*tensors):
     return forward_ad._current_level >= 0
 
 
+def _refuse_tangents(what, *tensors):
+    """Neither the registered operators nor the kernels know a derivative forward; they would drop the tangent."""
+    if forward_ad._current_level >= 0:
+        for t in tensors:
+            if t is not None and forward_ad.unpack_dual(t).tangent is not None:
+                raise RuntimeError(f"{what}: records no gradient forward (jvp), a tangent of its inputs would be lost")
+
+
 def _once(backward):
     """once_differentiable, whose wrapper is only paid for where a graph of the backward is asked for."""
     guarded = torch.autograd.function.once_differentiable(backward)
@@ -118,6 +126,7 @@ def gated_linrec(x: Tensor, gate_a: Tensor, gate_x: Tensor, rate: Tensor, *, h0:
     positions or gated_linrec_step goes on from.  Differentiable in x, gate_a, gate_x, rate and h0.
     """
     scale = float(scale)
+    _refuse_tangents("gated_linrec", x, gate_a, gate_x, rate, h0)
     if _traced(x, gate_a, gate_x, rate, h0):
         h, state, _ = gated_linrec_fwd(x, gate_a, gate_x, rate, h0, cu_seqlens, bool(reverse), scale)
     elif _recorded(x, gate_a, gate_x, rate, h0):
@@ -147,8 +156,7 @@ def gated_linrec_step(x: Tensor, gate_a: Tensor, gate_x: Tensor, rate: Tensor, s
     """
     if torch.is_grad_enabled() and any(t.requires_grad for t in (x, gate_a, gate_x, rate, state)):
         raise RuntimeError("gated_linrec_step: records no gradient; call it under torch.no_grad(), or gated_linrec for training")
-    if forward_ad._current_level >= 0 and any(forward_ad.unpack_dual(t).tangent is not None for t in (x, gate_a, gate_x, rate, state)):
-        raise RuntimeError("gated_linrec_step: records no gradient, a tangent of its inputs would be lost")
+    _refuse_tangents("gated_linrec_step", x, gate_a, gate_x, rate, state)
     if _traced(x, gate_a, gate_x, rate, state):
         return _gated_linrec_step(x, gate_a, gate_x, rate, state, slots, float(scale))
     h = _layers.gated_step(x, gate_a, gate_x, rate, state, slots, float(scale))
@@ -223,6 +231,7 @@ def group_norm_act(x: Tensor, groups: int, weight: Optional[Tensor] = None, bias
     "gelu" (the exact one).  Statistics are float32.  Differentiable in x, weight and bias.
     """
     groups, eps = int(groups), float(eps)
+    _refuse_tangents("group_norm_act", x, weight, bias)
     if _traced(x, weight, bias):
         return group_norm_act_fwd(x, groups, weight, bias, eps, act)[0]
     if _recorded(x, weight, bias):
@@ -284,6 +293,7 @@ def embedding(tokens: Tensor, weight: Tensor, *, scale: float = 1.0, padding_idx
     outside the table gives a row of zeros and no gradient; the row `padding_idx` is looked up but gets no gradient.
     """
     scale = float(scale)
+    _refuse_tangents("embedding", weight)
     if _traced(tokens, weight):
         return embedding_fwd(tokens, weight, scale, padding_idx)
     if _recorded(weight):

@@ -230,7 +230,9 @@ def _with_adjacent_channels(*tensors):
 
 
 def gated_saved_numel(dtype, batch, time, channels):
-    return _lib.linrec_gated_saved_floats(DTYPES[dtype], batch, time, channels)
+    """linrec_gated_saved_floats, for sizes that may be symbols of a traced call."""
+    every = (1 << 20) // _lib.linrec_gated_saved_floats(DTYPES[dtype], 1, 1 << 20, 1)
+    return batch * ((time + every - 1) // every) * channels
 
 
 # (A forward hands back the number of its kind of call as well, which stands for sizes, types, devices and options.  It says nothing

@@ -69,7 +69,7 @@ __device__ __forceinline__ void activate_slope(int act, const float (&z)[N], flo
   switch (act) {
     case LINREC_ACT_RELU:
 #pragma unroll
-      for (int i = 0; i < N; ++i) e[i] = z[i] > 0.0f ? e[i] : 0.0f * z[i] * e[i];
+      for (int i = 0; i < N; ++i) e[i] = z[i] > 0.0f ? e[i] : (z[i] != z[i] ? z[i] : 0.0f) * e[i];  // (NaN stays, not what -inf hides)
       break;
     case LINREC_ACT_SILU:
 #pragma unroll

@@ -117,8 +117,8 @@ def _looks(t):
     return None if t is None else (t.dtype, t.device, t.shape, t.stride())
 
 
-def _strides(*tensors):
-    return tuple([None if t is None else t.stride() for t in tensors])
+def _stride(t):
+    return None if t is None else t.stride()
 
 
 def _call(t, fn, entry, what):
@@ -266,7 +266,7 @@ def gated_bwd(d_h, d_state, x, gate_a, gate_x, rate, h0, cu_seqlens, saved, reve
     if d_h is None:
         d_h = torch.zeros((), dtype=x.dtype, device=x.device).expand(x.size())
     if number is not None:
-        key = (number, _strides(d_h, d_state, x, gate_a, gate_x, rate, h0, cu_seqlens))
+        key = (number, d_h.stride(), _stride(d_state), x.stride(), gate_a.stride(), gate_x.stride(), rate.stride(), _stride(h0), _stride(cu_seqlens))
     else:
         key = ("gated_bwd", x.dtype, x.device, x.shape, x.stride(), _looks(d_h), _looks(d_state), _looks(gate_a), _looks(gate_x), _looks(rate),
                _looks(h0), _looks(cu_seqlens), reverse, scale)
@@ -290,7 +290,8 @@ def gated_bwd(d_h, d_state, x, gate_a, gate_x, rate, h0, cu_seqlens, saved, reve
         d_state, rate, h0, cu_seqlens = _dense(d_state, rate, h0, cu_seqlens)
         return gated_bwd(d_h, d_state, x, gate_a, gate_x, rate, h0, cu_seqlens, saved, reverse, scale)
     device, shape, dtype = x.device, x.shape, x.dtype
-    saved = saved.contiguous()
+    if not saved.is_contiguous():
+        saved = saved.contiguous()
     d_x, d_gate_a, d_gate_x = (torch.empty(shape, dtype=dtype, device=device), torch.empty(shape, dtype=dtype, device=device),
                                torch.empty(shape, dtype=dtype, device=device))
     d_rate, partial = _floats(rate.shape, device), _floats(e.sizes[0], device)
@@ -423,7 +424,7 @@ def norm_fwd(x, groups, weight, bias, eps, act):
 def norm_bwd(d_y, x, groups, weight, bias, stats, eps, act, number=None):
     """(d_x, d_weight, d_bias), the last two None without a weight"""
     if number is not None:
-        key = (number, _strides(d_y, x, weight, bias))
+        key = (number, d_y.stride(), x.stride(), _stride(weight), _stride(bias))
     else:
         key = ("norm_bwd", x.dtype, x.device, x.shape, x.stride(), groups, _looks(d_y), _looks(weight), _looks(bias), eps, act)
     e = _remembered().get(key) or _norm_entry(key, x, groups, weight, bias, eps, act, d_y)
@@ -431,7 +432,8 @@ def norm_bwd(d_y, x, groups, weight, bias, stats, eps, act, number=None):
     if a is None:
         return norm_bwd(*_dense(d_y, x), groups, *_dense(weight, bias), stats, eps, act)
     device = x.device
-    stats = stats.contiguous()
+    if not stats.is_contiguous():
+        stats = stats.contiguous()
     d_x = torch.empty(x.shape, dtype=x.dtype, device=device)
     d_weight = d_bias = None
     if weight is not None:
@@ -486,7 +488,7 @@ def embedding_fwd(tokens, weight, scale, padding_idx):
 def embedding_bwd(d_y, tokens, weight, scale, padding_idx, number=None):
     """The gradient of `weight` (whose values are not read)."""
     if number is not None:
-        key = (number, _strides(d_y, tokens))
+        key = (number, d_y.stride(), tokens.stride())
     else:
         key = ("embedding_bwd", _looks(d_y), _looks(tokens), weight.dtype, weight.device, weight.shape, scale, padding_idx)
     e = _remembered().get(key)

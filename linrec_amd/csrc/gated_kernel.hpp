@@ -19,8 +19,8 @@
 // What bounds it: memory where channels are many.  8 x 4096 x 2048 in bf16: 122 us forward (537 MB, 4.4 TB/s of the 5.2 TB/s that
 // a copy reaches) and 221 us backward (940 MB, 4.2 TB/s); 16 x 2048 x 512 in fp32 out of a projection's rows 57 and 104 us (4.7 and
 // 4.5 TB/s).  Without the wait for what enters a segment the former takes 111 and 200 us: the wait is the larger part of the rest,
-// the gates' arithmetic the smaller.  With few channels the chain bounds it: 1 x 32768 x 2048 132 and 231 us, 1 x 131072 x 64 49
-// and 81 us (floors 103, 181; 13, 23).
+// the gates' arithmetic the smaller.  With few rows the chain bounds it: 1 x 32768 x 2048 132 and 231 us, 1 x 131072 x 64 49
+// and 81 us (floors 103, 181; 13, 23); the former 30 and 35 us less without the wait, 1 x 100001 x 250 22 and 31 of 79 and 129.
 //
 // Waves and runs: workgroups wait, so that several to a CU have to hide each other's waits, with all that a segment holds in
 // registers: at most 128 a lane for sixteen waves to a CU, and as little spilled as can be (32 registers that are cost 7 to 20 %).
@@ -32,13 +32,14 @@
 // of 250 were stored past the caches then, and take 79 and 129 us through them).
 //
 // The value that enters a segment is always the same chain of multiply-adds over the segments before, whichever of them had
-// published what when they were looked at: results are the same bits in every run.
+// published what when they were looked at: results are the same bits in every run in which no wait runs out.
 //
 // A position at which a packed sequence starts takes the sequence's own initial value instead of what comes from before it, so
-// nothing passes from one sequence to the next, not even by 0 * inf.  A segment that holds a start does not wait at all.
+// nothing passes from one sequence to the next, not even by 0 * inf.  A segment that holds a start publishes what leaves it
+// without a wait.
 //
 // A wait is for segments of smaller workgroup number only, and bounded; a lane whose wait runs out walks its channel from the
-// sequence's start.
+// sequence's start, which gives the value by other roundings.
 #pragma once
 #include <hip/hip_runtime.h>
 #include <stdint.h>

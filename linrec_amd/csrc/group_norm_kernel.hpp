@@ -565,7 +565,8 @@ __device__ __forceinline__ int64_t piece_index(const BlockArgs& a, int64_t n, in
 // NORM_HELD_PARTS: the workgroup's rows are fp32 and not whole lines of 128 bytes.  Its results go through the caches, where the parts
 // of a line that neighbours write come together, all others past them: 16 x 2048 x 512 in 32 groups fp32 38 and 62 us, past the caches 40
 // and 66; whole lines, 512 x 64 x 256 in 8 groups bf16, 11 and 27 us past them and 14 and 29 through them; parts of 16 bits gain nothing,
-// 16 x 2048 x 510 in 30 groups bf16 39 and 52 us through them and 38 and 52 past them, 32 x 1024 x 256 in 32 groups 15 and 27, 13 and 27.
+// 16 x 2048 x 510 in 30 groups bf16 39 and 52 us through them and 38 and 52 past them (an odd width, one channel of 2 bytes to a lane: that
+// is what bounds it), 32 x 1024 x 256 in 32 groups 15 and 27, 13 and 27.
 constexpr int NORM_HELD = 0, NORM_STATS = 1, NORM_APPLY = 2, NORM_HELD_PARTS = 3;
 constexpr bool holds(int phase) { return phase == NORM_HELD || phase == NORM_HELD_PARTS; }
 template <int PHASE, int VEC, typename T>

@@ -843,7 +843,7 @@ __global__ __launch_bounds__(LANES) void norm_bwd_kernel(BlockArgs args, float* 
     for (int i = 0; i < KEEP; ++i)
       if (l.there && l.first + i * args.R < l.end) apply(held_again(hx[i]), held_again(hd[i]), l.first + i * args.R);
   } else {
-    auto walk = [&](auto&& f) __attribute__((always_inline)) {
+    auto walk = [&](auto&& f, auto&& then) __attribute__((always_inline)) {
       if (!l.there) return;
       for (int64_t pos = l.first; pos < l.end; pos += 2 * args.R) {
         Held<T, VEC> hx[2], hd[2];
@@ -856,10 +856,27 @@ __global__ __launch_bounds__(LANES) void norm_bwd_kernel(BlockArgs args, float* 
 #pragma unroll
         for (int i = 0; i < 2; ++i)
           if (pos + i * args.R < l.end) f(hx[i], hd[i], pos + i * args.R);
+        then();
       }
     };
     if constexpr (PHASE == NORM_STATS) {
-      walk([&](const Held<T, VEC>& hx, const Held<T, VEC>& hd, int64_t) { add(hx, hd); });
+      // two levels: a sum that adds the same value again and again is off the same way at every step
+      float before[2 * VEC];
+      int n = 0;
+#pragma unroll
+      for (int i = 0; i < 2 * VEC; ++i) before[i] = 0.0f;
+      walk([&](const Held<T, VEC>& hx, const Held<T, VEC>& hd, int64_t) { add(hx, hd); },
+           [&] {
+             if (++n < 32) return;  // (of two positions)
+#pragma unroll
+             for (int i = 0; i < 2 * VEC; ++i) {
+               before[i] += sums[i];
+               sums[i] = 0.0f;
+             }
+             n = 0;
+           });
+#pragma unroll
+      for (int i = 0; i < 2 * VEC; ++i) sums[i] += before[i];
       finish_sums();
       if (l.there && l.r == 0 && l.q == 0) {
         const int64_t piece = piece_of(args);
@@ -879,7 +896,7 @@ __global__ __launch_bounds__(LANES) void norm_bwd_kernel(BlockArgs args, float* 
       sum_all<2>(s, sh, args, l);
       s[0] *= inv_count;
       s[1] *= inv_count;
-      walk([&](const Held<T, VEC>& hx, const Held<T, VEC>& hd, int64_t pos) { apply(hx, hd, pos); });
+      walk([&](const Held<T, VEC>& hx, const Held<T, VEC>& hd, int64_t pos) { apply(hx, hd, pos); }, [] {});
     }
   }
 }

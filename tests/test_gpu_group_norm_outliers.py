@@ -42,3 +42,20 @@ def test_statistics(shape, groups, dtype, where, far):
     want = ((v - mean[:, None, :, None]) / torch.sqrt(var + 1e-5)[:, None, :, None]).view(shape)
     worst = ((y.double() - want).abs() - ref.UNIT[dtype] * want.abs()).max()
     assert float(worst) <= (off + 128 * ref.U32 * float((size / var.sqrt()).max())) * max(1.0, float(want.abs().max()))
+
+
+@pytest.mark.parametrize("value", [0.1, 0.7, 1.0 / 3.0])
+@pytest.mark.parametrize("positions,channels", [(1048576, 131), (262144, 516)])
+def test_sums_of_one_gradient_again_and_again(positions, channels, value):
+    """The gradient of a mean: every rounding of a sum that adds the same value goes the same way."""
+    x = torch.randn((1, positions, channels), device=DEV, generator=torch.Generator(device=DEV).manual_seed(2))
+    d_y = torch.full_like(x, value)
+    weight, bias = torch.ones(channels, device=DEV), torch.zeros(channels, device=DEV)
+    _, stats, _ = _layers.norm_fwd(x, 1, weight, bias, 1e-5, "none")
+    _, d_weight, d_bias = _layers.norm_bwd(d_y, x, 1, weight, bias, stats, 1e-5, "none")
+    # two levels of 64 terms each in a lane, those of the workgroups in a tree of at most 40
+    want = torch.full((channels,), positions * float(d_y[0, 0, 0]), dtype=torch.float64)
+    ref.assert_within(d_bias, want, (64 + 64 + 40) * ref.U32 * want, "d_bias")
+    xh = (x[0].double() - stats[0].double()) * stats[1].double()
+    # (the normalised values carry three roundings each; sums of them in any order are off by what their sizes allow)
+    ref.assert_within(d_weight, (float(d_y[0, 0, 0]) * xh.sum(0)).cpu(), (64 + 64 + 44) * ref.U32 * value * xh.abs().sum(0).cpu(), "d_weight")

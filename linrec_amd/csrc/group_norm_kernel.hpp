@@ -7,7 +7,7 @@
 // What bounds it: memory, and the launches where little is normed.  Forward and backward: 32768 x 1024 in 16 groups, bf16, 31 and
 // 49 us (134 and 201 MB: 4.4 and 4.1 TB/s of the 5.2 that a copy reaches), fp32 52 and 76 (5.1 and 5.3); 16 x 2048 x 512 in 32 groups,
 // fp32, gelu 38 and 62 us (3.5 and 3.3 TB/s): one round of workgroups that all load, then add up, then store; 8 x 16384 x 512 in 32
-// groups, bf16, in chunks 95 and 157 us, for three and five tensors' worth of memory traffic.  3 x 333 x 222 in 6 groups: 12 us, of
+// groups, bf16, in chunks 96 and 157 us, for three and five tensors' worth of memory traffic.  3 x 333 x 222 in 6 groups: 12 us, of
 // which an empty kernel takes 6.  Three shapes, by how much one group is:
 //   tokens  one position: a team of 1 .. 64 adjacent lanes holds a group in registers; waves keep their channels and walk down
 //           the rows, so weights are read once and the sums of d_w and d_b stay in registers.

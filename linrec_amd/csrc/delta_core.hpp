@@ -1,0 +1,313 @@
+// What the kernels of the gated delta rule share: the chunk form, fragments of the matrix instructions, tiles in LDS, scratch.
+//
+// The recurrence S_t = e^{g_t} S_{t-1} + k_t u_t^T, u_t = beta_t (v_t - e^{g_t} S_{t-1}^T k_t), o_t = scale S_t^T q_t is taken 64
+// positions at a time.  With G the sums of g from the chunk's start (inclusive) and S the state before the chunk,
+//
+//   A_ij = beta_i e^{G_i - G_j} k_i.k_j (i > j)       M = (1 + A)^-1                              delta_prepare.hpp
+//   N = M diag(beta) (V - e^G K S)                     the rows u_t of the chunk                   delta_scan.hpp
+//   O = scale (e^G Q S + C N), C_ij = e^{G_i - G_j} q_i.k_j (i >= j);   S' = e^{G_63} S + K^T (e^{G_63 - G} N)
+//
+// and backwards, from dS' behind the chunk,
+//
+//   dN = scale C^T dO + e^{G_63 - G} K dS',  dB = M^T dN,  dV = beta dB                            delta_reverse.hpp
+//   dS = e^{G_63} dS' + Q^T (scale e^G dO) - K^T (e^G dV)
+//   the gradients of Q, K and the gates from S, dS', N, dB and dO, chunk by chunk                  delta_gradient.hpp
+//
+// The columns of S (value channels) are independent of each other in the two passes along the sequence, so a wave owns 16 of them for all
+// of the time axis and keeps its key_dim x 16 part of S in accumulators; what it multiplies them with is the same for all waves and
+// comes through LDS.
+//
+// Precision.  States, sums and accumulators are fp32.  An operand of a matrix instruction that is not an input is split into two
+// bf16 (or, beside fp16 inputs, fp16) numbers, its rounding and the rounding of the rest, which together carry 16 bits and more: a
+// product with an input is two instructions, one of two such operands three, and a state is about 1e-6 off.  One bf16 each would
+// be 2e-3.  fp32 inputs take the fp32 instructions.
+#pragma once
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+#include <type_traits>
+
+#include "../../include/linrec_delta.h"
+#include "layer_common.hpp"
+
+namespace linrec {
+
+constexpr int DELTA_CHUNK = 64;
+constexpr float DELTA_LEAST_LOG = -1e4f;  // e^-10000 is zero, and sums of 64 of them keep their digits in fp64
+
+// Storage of what is computed inside: T for fp32, two bf16 for 16-bit inputs.
+template <typename T>
+using Inner = std::conditional_t<sizeof(T) == 4, float, __bf16>;
+template <typename U>
+constexpr int planes_of() {
+  return sizeof(U) == 4 ? 1 : 2;
+}
+// Planes of Inner<T> that hold a T exactly: fp16 has three bits more than bf16.
+template <typename T>
+constexpr int input_planes() {
+  return std::is_same_v<T, _Float16> ? 2 : 1;
+}
+
+// Eight of the 32 positions that a product sums over at once, for one row (or column): lane 16 q + r holds positions 8 q to 8 q + 7
+// of row r.
+template <typename U>
+using Frag = typename Pack<U, 8>::type;
+template <typename U, int N = planes_of<U>()>
+struct Planes {
+  Frag<U> p[N];
+};
+
+// c += a b^T: lane 16 q + r gets rows 4 q to 4 q + 3 of column r.
+__device__ __forceinline__ v4f mma(const Frag<__bf16>& a, const Frag<__bf16>& b, v4f c) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
+}
+__device__ __forceinline__ v4f mma(const Frag<_Float16>& a, const Frag<_Float16>& b, v4f c) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
+}
+__device__ __forceinline__ v4f mma(const Frag<float>& a, const Frag<float>& b, v4f c) {
+#pragma unroll
+  for (int e = 0; e < 8; ++e) c = __builtin_amdgcn_mfma_f32_16x16x4f32(a[e], b[e], c, 0, 0, 0);
+  return c;
+}
+template <typename U, int NA, int NB>
+__device__ __forceinline__ v4f mma(const Planes<U, NA>& a, const Planes<U, NB>& b, v4f c) {
+#pragma unroll
+  for (int i = NA - 1; i >= 0; --i)
+#pragma unroll
+    for (int j = NB - 1; j >= 0; --j)
+      if (i + j < (NA > NB ? NA : NB)) c = mma(a.p[i], b.p[j], c);  // (the product of two rests is below what is kept)
+  return c;
+}
+template <typename U, int N>
+__device__ __forceinline__ v4f mma(const Frag<U>& a, const Planes<U, N>& b, v4f c) {
+#pragma unroll
+  for (int j = N - 1; j >= 0; --j) c = mma(a, b.p[j], c);
+  return c;
+}
+
+// Results of two products side by side are one operand of the next.  Row r of tile t of an operand whose products' rows are summed
+// over next stands for row_of_tile(t, r): then lane 16 q + r holds, of tiles 2 p and 2 p + 1, rows 32 p + 8 q to 32 p + 8 q + 7.
+__device__ __forceinline__ int row_of_tile(int t, int r) { return 32 * (t >> 1) + 8 * (r >> 2) + 4 * (t & 1) + (r & 3); }
+__device__ __forceinline__ int row_of_result(int t, int q) { return 32 * (t >> 1) + 8 * q + 4 * (t & 1); }  // (the first of four)
+
+template <typename U>
+__device__ __forceinline__ Planes<U> split(const v4f& lo, const v4f& hi) {
+  Planes<U> out;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    const float x = e < 4 ? lo[e & 3] : hi[e & 3];
+    out.p[0][e] = U(x);
+    if constexpr (planes_of<U>() == 2) out.p[1][e] = U(x - float(out.p[0][e]));
+  }
+  return out;
+}
+
+// A factor 2^n that brings a column's largest value near 2^13, where two fp16 numbers hold 22 bits of it; 1 for types with the
+// exponents of fp32.
+template <typename T, int N>
+__device__ __forceinline__ float column_factor(const v4f (&x)[N], float* inverse) {
+  if constexpr (!std::is_same_v<T, _Float16>) {
+    *inverse = 1.0f;
+    return 1.0f;
+  } else {
+    float most = 0.0f;
+#pragma unroll
+    for (int t = 0; t < N; ++t)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) most = fmaxf(most, fabsf(x[t][e]));
+    most = fmaxf(most, __shfl_xor(most, 16));
+    most = fmaxf(most, __shfl_xor(most, 32));
+    int ex = int(__float_as_uint(most) >> 23);
+    ex = ex < 14 ? 14 : ex > 253 ? 253 : ex;
+    *inverse = __uint_as_float(unsigned(ex - 13) << 23);
+    return __uint_as_float(unsigned(267 - ex) << 23);
+  }
+}
+template <typename T, int N>
+__device__ __forceinline__ void split_scaled(const v4f (&x)[N], Planes<T> (&out)[N / 2], float* inverse) {
+  const float f = column_factor<T>(x, inverse);
+#pragma unroll
+  for (int p = 0; p < N / 2; ++p) {
+    if constexpr (std::is_same_v<T, _Float16>) out[p] = split<T>(x[2 * p] * f, x[2 * p + 1] * f);
+    else out[p] = split<T>(x[2 * p], x[2 * p + 1]);
+  }
+}
+
+// A row-major tile of COLS columns in LDS, in units of 16 bytes; a unit's place is changed by its row, so that eight lanes that read
+// a unit of rows 0..3, 8..11 (fragments) and sixteen that read halves of units of four rows (transposed ones) spread over the banks.
+template <typename U, int COLS>
+struct Tile {
+  static constexpr int ROW = COLS * int(sizeof(U)), UNITS = ROW / 16, BYTES = 64 * ROW;
+  static constexpr int MASK = UNITS >= 8 ? 7 : UNITS - 1;
+  static constexpr int VEC = 16 / int(sizeof(U));
+  static __device__ __forceinline__ int at(int row, int unit) {
+    const int f = (((row & 1) << 2) | ((row >> 1) & 1) | (((row >> 3) & 1) << 1)) & MASK;
+    return row * ROW + ((unit ^ f) << 4);
+  }
+  static __device__ __forceinline__ float value(const char* tile, int row, int col) {
+    return float(*reinterpret_cast<const U*>(tile + at(row, col / VEC) + (col % VEC) * int(sizeof(U))));
+  }
+  // columns 32 p + 8 q and up of a row
+  static __device__ __forceinline__ Frag<U> frag(const char* tile, int row, int p, int q) {
+    if constexpr (sizeof(U) == 2) {
+      return *reinterpret_cast<const Frag<U>*>(tile + at(row, 4 * p + q));
+    } else {
+      Frag<U> f;
+      const v4f a = *reinterpret_cast<const v4f*>(tile + at(row, 8 * p + 2 * q)), b = *reinterpret_cast<const v4f*>(tile + at(row, 8 * p + 2 * q + 1));
+#pragma unroll
+      for (int e = 0; e < 4; ++e) f[e] = a[e], f[4 + e] = b[e];
+      return f;
+    }
+  }
+  // four rows from `row` of the column that is this lane's (r = lane % 16) of the 16 columns that start at col(0), col(1), col(2),
+  // col(3), four each
+  template <typename F>
+  static __device__ __forceinline__ typename Pack<U, 4>::type column4(const char* tile, int row, F&& col) {
+    const int r = threadIdx.x & 15;
+    typename Pack<U, 4>::type out;
+    if constexpr (sizeof(U) == 2) {
+      typedef short s4 __attribute__((ext_vector_type(4)));
+      typedef __attribute__((address_space(3))) s4* lds_t;
+      const int from = row + (r >> 2), c = col(r & 3);
+      const s4 raw = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_t)(tile + at(from, c / VEC) + (c % VEC) * 2));
+      __builtin_memcpy(&out, &raw, 8);
+    } else {
+      const int c = col(r >> 2) + (r & 3);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) out[e] = *reinterpret_cast<const U*>(tile + at(row + e, c / VEC) + (c % VEC) * 4);
+    }
+    return out;
+  }
+  template <typename F>
+  static __device__ __forceinline__ Frag<U> column_frag(const char* tile, int p, int q, F&& col) {
+    const auto a = column4(tile, 32 * p + 8 * q, col), b = column4(tile, 32 * p + 8 * q + 4, col);
+    Frag<U> f;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) f[e] = a[e], f[4 + e] = b[e];
+    return f;
+  }
+};
+
+// 16 bytes from `col` on of a row of `cols` values; zeros behind its end.
+template <typename T>
+__device__ __forceinline__ typename Slot16<T>::type load_unit(const T* row, int col, int cols) {
+  constexpr int VEC = 16 / int(sizeof(T));
+  typename Slot16<T>::type v;
+  typedef T any __attribute__((ext_vector_type(16 / sizeof(T)), aligned(sizeof(T))));
+  if (col + VEC <= cols) return *reinterpret_cast<const any*>(row + col);
+#pragma unroll
+  for (int e = 0; e < VEC; ++e) v[e] = col + e < cols ? row[col + e] : T(0.0f);
+  return v;
+}
+template <typename T>
+__device__ __forceinline__ typename Slot16<T>::type zero_unit() {
+  typename Slot16<T>::type v;
+#pragma unroll
+  for (int e = 0; e < 16 / int(sizeof(T)); ++e) v[e] = T(0.0f);
+  return v;
+}
+
+// COLS columns of ROWS rows to a tile; zeros for rows from `rows` and columns from `cols` on.
+template <typename T, int COLS, int LANES, int ROWS = 64>
+__device__ __forceinline__ void stage(char* tile, const T* from, int64_t stride, int rows, int cols) {
+  using L = Tile<T, COLS>;
+  constexpr int UNITS = ROWS * L::UNITS;
+#pragma unroll
+  for (int n = 0; n < (UNITS + LANES - 1) / LANES; ++n) {
+    const int i = n * LANES + int(threadIdx.x), row = i / L::UNITS, u = i % L::UNITS;
+    if (UNITS % LANES && i >= UNITS) break;
+    auto v = zero_unit<T>();
+    if (row < rows) v = load_unit(from + row * stride, u * L::VEC, cols);
+    *reinterpret_cast<decltype(v)*>(tile + L::at(row, u)) = v;
+  }
+}
+// The same from dense scratch rows of COLS columns.
+template <typename U, int COLS, int LANES, int ROWS>
+__device__ __forceinline__ void stage_dense(char* tile, const U* from) {
+  using L = Tile<U, COLS>;
+  constexpr int UNITS = ROWS * L::UNITS;
+#pragma unroll
+  for (int n = 0; n < (UNITS + LANES - 1) / LANES; ++n) {
+    const int i = n * LANES + int(threadIdx.x), row = i / L::UNITS, u = i % L::UNITS;
+    if (UNITS % LANES && i >= UNITS) break;
+    *reinterpret_cast<typename Slot16<U>::type*>(tile + L::at(row, u)) = reinterpret_cast<const typename Slot16<U>::type*>(from)[i];
+  }
+}
+
+// ---- chunks and scratch ----------------------------------------------------------------------------------------------------------
+// A chunk has a slot: those of a sequence follow each other, a packed sequence's start at cu_seqlens[n] / 64 + n (so that no two
+// sequences meet, whatever their lengths), a batch item's at n * ceil(time / 64).
+struct DeltaArgs {
+  linrec_delta_t p;
+  int64_t slots;
+  int shared;    // value heads of a key head
+  int columns;   // value_dim rounded up to 32: rows of the planes of S, dS', N and dB
+  int blocks;    // workgroups side by side over the columns
+  int64_t pairs; // sequences x heads
+  // scratch, for every (slot, head): m[planes][64][64] and so on
+  char* m;
+  char* m_t;
+  char* c;       // C scale, transposed in the backward
+  float* gates;  // [3][64]: e^G, e^{G_63 - G}, beta
+  char* s;       // [planes][columns][DK], the state before the chunk
+  char* d_s;     // the same of dS' behind it
+  char* n;       // [planes][columns][64]
+  char* d_b;
+  float* dots;   // [192], sums of the gates' gradients where key_dim comes in turns
+};
+
+struct Span {
+  int64_t batch, first, end;  // positions of a sequence in its batch item
+  int64_t slot;               // of its first chunk
+};
+__device__ __forceinline__ int64_t bound_of(const linrec_delta_t& p, int64_t n) {
+  const int64_t b = p.cu_seqlens[n];
+  return b < 0 ? 0 : b > p.time ? p.time : b;
+}
+__device__ __forceinline__ Span span_of(const linrec_delta_t& p, int64_t n) {
+  if (!p.cu_seqlens) return Span{n, 0, p.time, n * ((p.time + DELTA_CHUNK - 1) / DELTA_CHUNK)};
+  const int64_t a = bound_of(p, n), b = bound_of(p, n + 1);
+  return Span{0, a, b < a ? a : b, a / DELTA_CHUNK + n};
+}
+// The first position and the length of the chunk in a slot; a length of zero where there is none.
+struct Chunk {
+  int64_t batch, first;
+  int length;
+};
+__device__ __forceinline__ Chunk chunk_of(const linrec_delta_t& p, int64_t slot) {
+  if (!p.cu_seqlens) {
+    const int64_t each = (p.time + DELTA_CHUNK - 1) / DELTA_CHUNK, n = slot / each, first = (slot - n * each) * DELTA_CHUNK;
+    return Chunk{n, first, int(p.time - first < DELTA_CHUNK ? p.time - first : DELTA_CHUNK)};
+  }
+  // the last sequence that starts at or before the slot, 64 bounds at a time
+  int lo = 0, hi = int(p.sequences);
+  const int lane = threadIdx.x & 63;
+  while (hi - lo > 1) {
+    const int step = (hi - lo + 63) / 64, at = lo + lane * step;
+    const bool before = at < hi && bound_of(p, at) / DELTA_CHUNK + at <= slot;
+    const int n = __popcll(__ballot(before));
+    lo += (n > 0 ? n - 1 : 0) * step;
+    hi = lo + step < hi ? lo + step : hi;
+  }
+  lo = __builtin_amdgcn_readfirstlane(lo);
+  const Span s = span_of(p, lo);
+  const int64_t first = s.first + (slot - s.slot) * DELTA_CHUNK, left = s.end - first;
+  if (slot < s.slot || left <= 0) return Chunk{0, 0, 0};
+  return Chunk{0, first, int(left < DELTA_CHUNK ? left : DELTA_CHUNK)};
+}
+
+template <typename T>
+__device__ __forceinline__ const T* head_rows(const void* base, const int64_t (&stride)[3], int64_t batch, int64_t first, int64_t head) {
+  return static_cast<const T*>(base) + batch * stride[0] + first * stride[1] + head * stride[2];
+}
+
+// Workgroups of one (sequence, head), which read the same keys and queries, lie on one XCD (workgroups go round the eight in turn).
+__device__ __forceinline__ bool scan_place(const DeltaArgs& a, int64_t* pair, int* block) {
+  const int64_t group = blockIdx.x / unsigned(8 * a.blocks);
+  const int in = int(blockIdx.x - group * unsigned(8 * a.blocks));
+  *block = in >> 3;
+  *pair = group * 8 + (in & 7);
+  return *pair < a.pairs;
+}
+
+}  // namespace linrec

@@ -1,0 +1,196 @@
+// Gated delta rule, the backward's pass against the sequence: dV, dB and the gradient of the state, chunk by chunk (delta_core.hpp).
+//
+// As the forward's: a workgroup has a (sequence, head), a wave 16 columns of dS.
+#pragma once
+#include "delta_scan.hpp"
+
+namespace linrec {
+
+template <typename T, int DK, int WAVES>
+struct ReverseShared {
+  using U = Inner<T>;
+  static constexpr int KEYS = Tile<T, DK>::BYTES, VALUES = Tile<T, 16 * WAVES>::BYTES;
+  static constexpr bool QUERIES = 2 * KEYS + VALUES + 2 * square_bytes<U>() + 1024 <= 160 * 1024;
+  static constexpr int K = 0, Q = K + KEYS, O = Q + (QUERIES ? KEYS : 0), M = O + VALUES, C = M + square_bytes<U>(),
+                       GATES = C + square_bytes<U>(), BYTES = GATES + 3 * 64 * 4;
+};
+
+template <typename T, int DK, int WAVES>
+__global__ __launch_bounds__(64 * WAVES) void delta_reverse_kernel(DeltaArgs a) {
+  using U = Inner<T>;
+  using Sh = ReverseShared<T, DK, WAVES>;
+  using TK = Tile<T, DK>;
+  using TV = Tile<T, 16 * WAVES>;
+  using TS = Tile<U, 64>;
+  constexpr int P = planes_of<U>(), LANES = 64 * WAVES, SQUARE = square_bytes<U>(), IN = input_planes<T>();
+  __shared__ __align__(16) char smem[Sh::BYTES];
+  const linrec_delta_t& p = a.p;
+  int64_t pair;
+  int cb;
+  if (!scan_place(a, &pair, &cb)) return;
+  const int64_t n = pair / p.heads;
+  const int head = int(pair - n * p.heads), key_head = head / a.shared;
+  const Span span = span_of(p, n);
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r = lane & 15, q = lane >> 4;
+  const int c0 = cb * 16 * WAVES, col = c0 + 16 * wave + r;
+  const bool mine = col < p.value_dim, kept_column = col < a.columns;  // (of a whole wave)
+  float* gates = reinterpret_cast<float*>(smem + Sh::GATES);
+
+  v4f s[DK / 16];  // dS'
+  const int64_t at0 = (pair * p.key_dim) * int64_t(p.value_dim) + col;
+#pragma unroll
+  for (int t = 0; t < DK / 16; ++t)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const int d = row_of_result(t, q) + e;
+      s[t][e] = p.d_state && mine && d < p.key_dim ? p.d_state[at0 + d * int64_t(p.value_dim)] : 0.0f;
+    }
+
+  const int64_t chunks = (span.end - span.first + DELTA_CHUNK - 1) / DELTA_CHUNK;
+  for (int64_t c = chunks - 1; c >= 0; --c) {
+    const int64_t first = span.first + c * DELTA_CHUNK, slot = span.slot + c;
+    const int length = int(span.end - first < DELTA_CHUNK ? span.end - first : DELTA_CHUNK);
+    const int64_t block = slot * p.heads + head;
+    __syncthreads();
+    const T* qq = head_rows<T>(p.q, p.q_stride, span.batch, first, key_head);
+    stage<T, DK, LANES>(smem + Sh::K, head_rows<T>(p.k, p.k_stride, span.batch, first, key_head), p.k_stride[1], length, p.key_dim);
+    if constexpr (Sh::QUERIES) stage<T, DK, LANES>(smem + Sh::Q, qq, p.q_stride[1], length, p.key_dim);
+    stage<T, 16 * WAVES, LANES>(smem + Sh::O, head_rows<T>(p.d_o, p.d_o_stride, span.batch, first, head) + c0, p.d_o_stride[1], length,
+                                p.value_dim - c0);
+#pragma unroll
+    for (int k2 = 0; k2 < P; ++k2) {
+      stage_dense<U, 64, LANES, 64>(smem + Sh::M + k2 * TS::BYTES, reinterpret_cast<const U*>(a.m_t + block * SQUARE) + k2 * 4096);
+      stage_dense<U, 64, LANES, 64>(smem + Sh::C + k2 * TS::BYTES, reinterpret_cast<const U*>(a.c + block * SQUARE) + k2 * 4096);
+    }
+    for (int i = threadIdx.x; i < 192; i += LANES) gates[i] = a.gates[block * 192 + i];
+    __syncthreads();
+
+    Planes<T> sp[DK / 32];
+    float un_s;
+    split_scaled<T>(s, sp, &un_s);
+    {
+      U* to = reinterpret_cast<U*>(a.d_s) + block * P * a.columns * DK;
+#pragma unroll
+      for (int b = 0; b < DK / 32; ++b) {
+        if (!kept_column) break;
+        Planes<U> kept;
+        if constexpr (std::is_same_v<T, _Float16>) kept = split<U>(s[2 * b], s[2 * b + 1]);
+        else kept = sp[b];
+#pragma unroll
+        for (int k2 = 0; k2 < P; ++k2) *reinterpret_cast<Frag<U>*>(to + (int64_t(k2) * a.columns + col) * DK + 32 * b + 8 * q) = kept.p[k2];
+      }
+    }
+    auto square = [&](int at, int t, int b) __attribute__((always_inline)) {
+      Planes<U> f;
+#pragma unroll
+      for (int k2 = 0; k2 < P; ++k2) f.p[k2] = TS::frag(smem + at + k2 * TS::BYTES, row_of_tile(t, r), b, q);
+      return f;
+    };
+    // dO of this wave's columns, a result's layout; fp16 as two bf16
+    v4f d_o[4];
+    Planes<U, IN> dop[2];
+#pragma unroll
+    for (int t = 0; t < 4; ++t) {
+      const auto v = TV::column4(smem + Sh::O, row_of_result(t, q), [&](int j) { return 16 * wave + 4 * j; });
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        d_o[t][e] = float(v[e]);
+        const int i = 4 * (t & 1) + e;
+        dop[t >> 1].p[0][i] = U(d_o[t][e]);
+        if constexpr (IN == 2) dop[t >> 1].p[1][i] = U(d_o[t][e] - float(dop[t >> 1].p[0][i]));
+      }
+    }
+    v4f x[4];  // dN
+#pragma unroll
+    for (int t = 0; t < 4; ++t) {
+      x[t] = v4f{0, 0, 0, 0};
+#pragma unroll
+      for (int b = 0; b < DK / 32; ++b) x[t] = mma(TK::frag(smem + Sh::K, row_of_tile(t, r), b, q), sp[b], x[t]);
+      const v4f rest = *reinterpret_cast<const v4f*>(gates + 64 + row_of_result(t, q));
+#pragma unroll
+      for (int e = 0; e < 4; ++e) x[t][e] *= rest[e] * un_s;
+#pragma unroll
+      for (int b = t / 2; b < 2; ++b) x[t] = mma(square(Sh::C, t, b), dop[b], x[t]);
+    }
+    Planes<U> xp[2];
+#pragma unroll
+    for (int b = 0; b < 2; ++b) xp[b] = split<U>(x[2 * b], x[2 * b + 1]);
+    v4f db[4];
+#pragma unroll
+    for (int t = 0; t < 4; ++t) {
+      db[t] = v4f{0, 0, 0, 0};
+#pragma unroll
+      for (int b = t / 2; b < 2; ++b) db[t] = mma(square(Sh::M, t, b), xp[b], db[t]);
+    }
+    if (kept_column) {
+      U* to = reinterpret_cast<U*>(a.d_b) + block * P * a.columns * 64;
+#pragma unroll
+      for (int b = 0; b < 2; ++b) {
+        const Planes<U> kept = split<U>(db[2 * b], db[2 * b + 1]);
+#pragma unroll
+        for (int k2 = 0; k2 < P; ++k2) *reinterpret_cast<Frag<U>*>(to + (int64_t(k2) * a.columns + col) * 64 + 32 * b + 8 * q) = kept.p[k2];
+      }
+    }
+    T* d_v = static_cast<T*>(p.d_v) + ((span.batch * p.time + first) * p.heads + head) * int64_t(p.value_dim) + col;
+#pragma unroll
+    for (int t = 0; t < 4; ++t) {
+      const int row = row_of_result(t, q);
+      const v4f gamma = *reinterpret_cast<const v4f*>(gates + row), beta = *reinterpret_cast<const v4f*>(gates + 128 + row);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const float v = beta[e] * db[t][e];
+        if (mine && row + e < length) d_v[(row + e) * int64_t(p.heads) * p.value_dim] = T(v);
+        db[t][e] = -gamma[e] * v;
+        d_o[t][e] *= gamma[e] * p.scale;
+      }
+    }
+    Planes<T> vp[2], op[2];
+    float un_v, un_o;
+    split_scaled<T>(db, vp, &un_v);
+    split_scaled<T>(d_o, op, &un_o);
+    const float keep = gates[63];
+#pragma unroll
+    for (int t = 0; t < DK / 16; ++t) {
+      auto with_keys = [&](v4f to) __attribute__((always_inline)) {
+#pragma unroll
+        for (int b = 0; b < 2; ++b) to = mma(TK::column_frag(smem + Sh::K, b, q, [&](int j) { return row_of_result(t, j); }), vp[b], to);
+        return to;
+      };
+      auto with_queries = [&](v4f to) __attribute__((always_inline)) {
+#pragma unroll
+        for (int b = 0; b < 2; ++b) {
+          if constexpr (Sh::QUERIES) {
+            to = mma(TK::column_frag(smem + Sh::Q, b, q, [&](int j) { return row_of_result(t, j); }), op[b], to);
+          } else {
+            Frag<T> f;
+            const int d = row_of_tile(t, r);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+              const int row = 32 * b + 8 * q + e;
+              f[e] = row < length && d < p.key_dim ? qq[row * p.q_stride[1] + d] : T(0.0f);
+            }
+            to = mma(f, op[b], to);
+          }
+        }
+        return to;
+      };
+      s[t] *= keep;
+      if constexpr (std::is_same_v<T, _Float16>) {
+        s[t] += un_v * with_keys(v4f{0, 0, 0, 0});
+        s[t] += un_o * with_queries(v4f{0, 0, 0, 0});
+      } else {
+        s[t] = with_queries(with_keys(s[t]));
+      }
+    }
+  }
+  if (p.d_h0 && mine)
+#pragma unroll
+    for (int t = 0; t < DK / 16; ++t)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int d = row_of_result(t, q) + e;
+        if (d < p.key_dim) p.d_h0[at0 + d * int64_t(p.value_dim)] = s[t][e];
+      }
+}
+
+}  // namespace linrec

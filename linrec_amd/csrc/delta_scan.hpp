@@ -1,0 +1,192 @@
+// Gated delta rule, the pass along the sequence: N, O and the state, chunk by chunk (delta_core.hpp).
+//
+// A workgroup has a (sequence, head) and 16 columns of the state for each of its waves.
+#pragma once
+#include "delta_core.hpp"
+
+namespace linrec {
+
+template <typename U>
+constexpr int square_bytes() {
+  return 64 * 64 * int(sizeof(U)) * planes_of<U>();
+}
+
+template <typename T, int DK, int WAVES, bool STATES>
+struct ScanShared {
+  using U = Inner<T>;
+  static constexpr int KEYS = Tile<T, DK>::BYTES, VALUES = Tile<T, 16 * WAVES>::BYTES;
+  // (fp32 of 256 channels: queries are read from memory where they are used)
+  static constexpr bool QUERIES = !STATES && 2 * KEYS + VALUES + 2 * square_bytes<U>() + 1024 <= 160 * 1024;
+  static constexpr int K = 0, Q = K + KEYS, V = Q + (QUERIES ? KEYS : 0), M = V + VALUES, C = M + square_bytes<U>(),
+                       GATES = C + (STATES ? 0 : square_bytes<U>()), BYTES = GATES + 3 * 64 * 4;
+};
+
+// STATES: a backward's first pass, which keeps the states before the chunks and N and has no O.
+template <typename T, int DK, int WAVES, bool STATES>
+__global__ __launch_bounds__(64 * WAVES) void delta_scan_kernel(DeltaArgs a) {
+  using U = Inner<T>;
+  using Sh = ScanShared<T, DK, WAVES, STATES>;
+  using TK = Tile<T, DK>;
+  using TV = Tile<T, 16 * WAVES>;
+  using TS = Tile<U, 64>;
+  constexpr int P = planes_of<U>(), LANES = 64 * WAVES, SQUARE = square_bytes<U>();
+  __shared__ __align__(16) char smem[Sh::BYTES];
+  const linrec_delta_t& p = a.p;
+  int64_t pair;
+  int cb;
+  if (!scan_place(a, &pair, &cb)) return;
+  const int64_t n = pair / p.heads;
+  const int head = int(pair - n * p.heads), key_head = head / a.shared;
+  const Span span = span_of(p, n);
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r = lane & 15, q = lane >> 4;
+  const int c0 = cb * 16 * WAVES, col = c0 + 16 * wave + r;
+  const bool mine = col < p.value_dim, kept_column = col < a.columns;  // (of a whole wave)
+  float* gates = reinterpret_cast<float*>(smem + Sh::GATES);
+
+  v4f s[DK / 16];
+  const int64_t at0 = (pair * p.key_dim) * int64_t(p.value_dim) + col;
+#pragma unroll
+  for (int t = 0; t < DK / 16; ++t)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const int d = row_of_result(t, q) + e;
+      s[t][e] = p.h0 && mine && d < p.key_dim ? p.h0[at0 + d * int64_t(p.value_dim)] : 0.0f;
+    }
+
+  int64_t slot = span.slot;
+  for (int64_t first = span.first; first < span.end; first += DELTA_CHUNK, ++slot) {
+    const int length = int(span.end - first < DELTA_CHUNK ? span.end - first : DELTA_CHUNK);
+    const int64_t block = slot * p.heads + head;
+    __syncthreads();
+    const T* k = head_rows<T>(p.k, p.k_stride, span.batch, first, key_head);
+    const T* qq = head_rows<T>(p.q, p.q_stride, span.batch, first, key_head);
+    stage<T, DK, LANES>(smem + Sh::K, k, p.k_stride[1], length, p.key_dim);
+    if constexpr (Sh::QUERIES) stage<T, DK, LANES>(smem + Sh::Q, qq, p.q_stride[1], length, p.key_dim);
+    stage<T, 16 * WAVES, LANES>(smem + Sh::V, head_rows<T>(p.v, p.v_stride, span.batch, first, head) + c0, p.v_stride[1], length, p.value_dim - c0);
+#pragma unroll
+    for (int k2 = 0; k2 < P; ++k2) {
+      stage_dense<U, 64, LANES, 64>(smem + Sh::M + k2 * TS::BYTES, reinterpret_cast<const U*>(a.m + block * SQUARE) + k2 * 4096);
+      if constexpr (!STATES) stage_dense<U, 64, LANES, 64>(smem + Sh::C + k2 * TS::BYTES, reinterpret_cast<const U*>(a.c + block * SQUARE) + k2 * 4096);
+    }
+    for (int i = threadIdx.x; i < 192; i += LANES) gates[i] = a.gates[block * 192 + i];
+    __syncthreads();
+
+    Planes<T> sp[DK / 32];
+    float un_s;
+    split_scaled<T>(s, sp, &un_s);
+    if constexpr (STATES) {
+      U* to = reinterpret_cast<U*>(a.s) + block * P * a.columns * DK;
+#pragma unroll
+      for (int b = 0; b < DK / 32; ++b) {
+        if (!kept_column) break;
+        Planes<U> kept;
+        if constexpr (std::is_same_v<T, _Float16>) kept = split<U>(s[2 * b], s[2 * b + 1]);
+        else kept = sp[b];
+#pragma unroll
+        for (int k2 = 0; k2 < P; ++k2) *reinterpret_cast<Frag<U>*>(to + (int64_t(k2) * a.columns + col) * DK + 32 * b + 8 * q) = kept.p[k2];
+      }
+    }
+    v4f x[4];  // K S, then beta (V - e^G K S)
+#pragma unroll
+    for (int t = 0; t < 4; ++t) {
+      x[t] = v4f{0, 0, 0, 0};
+#pragma unroll
+      for (int b = 0; b < DK / 32; ++b) x[t] = mma(TK::frag(smem + Sh::K, row_of_tile(t, r), b, q), sp[b], x[t]);
+    }
+    auto square = [&](int at, int t, int b) __attribute__((always_inline)) {
+      Planes<U> f;
+#pragma unroll
+      for (int k2 = 0; k2 < P; ++k2) f.p[k2] = TS::frag(smem + at + k2 * TS::BYTES, row_of_tile(t, r), b, q);
+      return f;
+    };
+#pragma unroll
+    for (int t = 0; t < 4; ++t) {
+      const int row = row_of_result(t, q);
+      const auto v = TV::column4(smem + Sh::V, row, [&](int j) { return 16 * wave + 4 * j; });
+      const v4f gamma = *reinterpret_cast<const v4f*>(gates + row), beta = *reinterpret_cast<const v4f*>(gates + 128 + row);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) x[t][e] = beta[e] * fmaf(-gamma[e] * un_s, x[t][e], float(v[e]));
+    }
+    Planes<U> xp[2];
+#pragma unroll
+    for (int b = 0; b < 2; ++b) xp[b] = split<U>(x[2 * b], x[2 * b + 1]);
+    v4f nn[4];
+#pragma unroll
+    for (int t = 0; t < 4; ++t) {
+      nn[t] = v4f{0, 0, 0, 0};
+#pragma unroll
+      for (int b = 0; b <= t / 2; ++b) nn[t] = mma(square(Sh::M, t, b), xp[b], nn[t]);
+    }
+    Planes<U> np[2];
+#pragma unroll
+    for (int b = 0; b < 2; ++b) np[b] = split<U>(nn[2 * b], nn[2 * b + 1]);
+    if constexpr (STATES) {
+      U* to = reinterpret_cast<U*>(a.n) + block * P * a.columns * 64;
+#pragma unroll
+      for (int b = 0; b < 2; ++b)
+#pragma unroll
+        for (int k2 = 0; k2 < P; ++k2)
+          if (kept_column) *reinterpret_cast<Frag<U>*>(to + (int64_t(k2) * a.columns + col) * 64 + 32 * b + 8 * q) = np[b].p[k2];
+    } else {
+      T* o = static_cast<T*>(p.o) + ((span.batch * p.time + first) * p.heads + head) * int64_t(p.value_dim) + col;
+#pragma unroll
+      for (int t = 0; t < 4; ++t) {
+        v4f y = v4f{0, 0, 0, 0};
+        const int from = row_of_tile(t, r);
+#pragma unroll
+        for (int b = 0; b < DK / 32; ++b) {
+          if constexpr (Sh::QUERIES) {
+            y = mma(TK::frag(smem + Sh::Q, from, b, q), sp[b], y);
+          } else {
+            Frag<T> f;
+#pragma unroll
+            for (int e = 0; e < 8; e += 16 / int(sizeof(T))) {
+              auto part = zero_unit<T>();
+              if (from < length) part = load_unit(qq + from * p.q_stride[1], 32 * b + 8 * q + e, p.key_dim);
+#pragma unroll
+              for (int i = 0; i < 16 / int(sizeof(T)); ++i) f[e + i] = part[i];
+            }
+            y = mma(f, sp[b], y);
+          }
+        }
+        const int row = row_of_result(t, q);
+        const v4f gamma = *reinterpret_cast<const v4f*>(gates + row);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) y[e] *= gamma[e] * un_s * p.scale;
+#pragma unroll
+        for (int b = 0; b <= t / 2; ++b) y = mma(square(Sh::C, t, b), np[b], y);
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if (mine && row + e < length) o[(row + e) * int64_t(p.heads) * p.value_dim] = T(y[e]);
+      }
+    }
+#pragma unroll
+    for (int t = 0; t < 4; ++t) nn[t] *= *reinterpret_cast<const v4f*>(gates + 64 + row_of_result(t, q));
+    Planes<T> nt[2];
+    float un_n;
+    split_scaled<T>(nn, nt, &un_n);
+    const float keep = gates[63];
+#pragma unroll
+    for (int t = 0; t < DK / 16; ++t) {
+      auto added = [&](v4f to) __attribute__((always_inline)) {
+#pragma unroll
+        for (int b = 0; b < 2; ++b)
+          to = mma(TK::column_frag(smem + Sh::K, b, q, [&](int j) { return row_of_result(t, j); }), nt[b], to);
+        return to;
+      };
+      s[t] *= keep;
+      if constexpr (std::is_same_v<T, _Float16>) s[t] += un_n * added(v4f{0, 0, 0, 0});
+      else s[t] = added(s[t]);
+    }
+  }
+  if (!STATES && p.state && mine)
+#pragma unroll
+    for (int t = 0; t < DK / 16; ++t)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int d = row_of_result(t, q) + e;
+        if (d < p.key_dim) p.state[at0 + d * int64_t(p.value_dim)] = s[t][e];
+      }
+}
+
+}  // namespace linrec

@@ -1,6 +1,7 @@
 /*
  * linrec_layers -- C ABI of the layer operators around the scan (linrec_hip.h): the gated linear recurrence and its
- * single-token step, group norm with an activation, and the token embedding with its gradient.
+ * single-token step, group norm with an activation, root-mean-square norm with a residual, and the token embedding with its
+ * gradient.
  *
  * The conventions are those of linrec_hip.h: device pointers, sizes and strides in elements, a HIP stream handle passed as
  * void*; every call only enqueues work on its stream, none synchronises, allocates or frees.  0 on success, a negative
@@ -128,6 +129,49 @@ typedef struct linrec_group_norm {
 int64_t linrec_group_norm_partial_floats(int dtype, int64_t batch, int64_t positions, int64_t channels, int64_t groups, int is_bwd);
 int linrec_group_norm_fwd(const linrec_group_norm_t* args);
 int linrec_group_norm_bwd(const linrec_group_norm_t* args);
+
+/*
+ * Root-mean-square norm of rows of `channels` values, after the residual's addition if there is one:
+ *
+ *   s = x + residual, rounded to dtype and stored to `total`;   y = s * weight / sqrt(mean(s^2) + eps)
+ *
+ * Row n of x, residual, d_y and d_total starts at (n / inner) * stride[0] + (n % inner) * stride[1], channels have unit stride; what
+ * is written is dense.  weight (channels), of weight_dtype, may be NULL (ones).  `quantized` asks for y in 8 bits with a scale a row,
+ * the row's largest |y| over 127 or 448: y = round(y / scale), as int8 or as fp8 of 4 exponent bits without infinities (e4m3);
+ * a row of zeros has the scale 0, one with a value that is not finite the scale NaN and zeros for values.
+ *
+ * The backward reads what was normalised as x (the forward's `total` where there was a residual) and the forward's rstd; d_x is
+ * the gradient of x and of the residual alike.
+ */
+#define LINREC_QUANTIZED_NONE 0
+#define LINREC_QUANTIZED_INT8 1
+#define LINREC_QUANTIZED_E4M3 2
+#define LINREC_RMS_NORM_CHANNELS_MAX 16384
+typedef struct linrec_rms_norm {
+  int32_t dtype, weight_dtype, quantized;
+  float eps;
+  int64_t rows, inner, channels;
+  const void* x;
+  int64_t x_stride[2];
+  const void* residual; /* or NULL */
+  int64_t residual_stride[2];
+  const void* weight;
+  void* y;     /* forward */
+  void* total; /* forward, with a residual */
+  float* rstd; /* (rows): written by the forward unless NULL, read by the backward */
+  float* scales; /* (rows), 8 bits only */
+  const void* d_y;
+  int64_t d_y_stride[2];
+  const void* d_total; /* gradient of `total`, or NULL */
+  int64_t d_total_stride[2];
+  void* d_x;
+  void* d_weight;  /* of weight_dtype, or NULL */
+  float* partial;  /* backward with d_weight: scratch of linrec_rms_norm_partial_floats() */
+  void* stream;
+} linrec_rms_norm_t;
+int64_t linrec_rms_norm_partial_floats(int dtype, int64_t rows, int64_t channels);
+int linrec_rms_norm_fwd(const linrec_rms_norm_t* args);
+int linrec_rms_norm_bwd(const linrec_rms_norm_t* args);
 
 /*
  * Embedding: y[n] = scale * weight[token[n]], and its gradient d_weight[v] = scale * sum of d_y[n] over the n with

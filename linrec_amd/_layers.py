@@ -15,6 +15,8 @@ from . import _native
 from ._native import DTYPES, _raw_stream, check, lib
 
 ACTIVATIONS = {"none": 0, "relu": 1, "silu": 2, "gelu": 3}  # LINREC_ACT_*
+QUANTIZED = {None: 0, torch.int8: 1, torch.float8_e4m3fn: 2}  # LINREC_QUANTIZED_*
+RMS_NORM_CHANNELS_MAX = 16384  # LINREC_RMS_NORM_CHANNELS_MAX
 
 _i32, _i64, _f32, _ptr, _u64 = ctypes.c_int32, ctypes.c_int64, ctypes.c_float, ctypes.c_void_p, ctypes.c_uint64
 _pair = _i64 * 2
@@ -45,6 +47,14 @@ class GroupNorm(ctypes.Structure):
                 ("d_bias", _ptr), ("partial", _ptr), ("stream", _ptr)]
 
 
+class RmsNorm(ctypes.Structure):
+    """linrec_rms_norm_t"""
+    _fields_ = [("dtype", _i32), ("weight_dtype", _i32), ("quantized", _i32), ("eps", _f32), ("rows", _i64), ("inner", _i64),
+                ("channels", _i64), ("x", _ptr), ("x_stride", _pair), ("residual", _ptr), ("residual_stride", _pair), ("weight", _ptr),
+                ("y", _ptr), ("total", _ptr), ("rstd", _ptr), ("scales", _ptr), ("d_y", _ptr), ("d_y_stride", _pair),
+                ("d_total", _ptr), ("d_total_stride", _pair), ("d_x", _ptr), ("d_weight", _ptr), ("partial", _ptr), ("stream", _ptr)]
+
+
 class Embedding(ctypes.Structure):
     """linrec_embedding_t"""
     _fields_ = [("dtype", _i32), ("token_bytes", _i32), ("scale", _f32), ("reserved", _i32), ("tokens", _i64), ("vocab", _i64),
@@ -62,6 +72,9 @@ EXPORTS = {
     "linrec_group_norm_partial_floats": (_i64, [ctypes.c_int] + [_i64] * 4 + [ctypes.c_int]),
     "linrec_group_norm_fwd": (ctypes.c_int, [ctypes.POINTER(GroupNorm)]),
     "linrec_group_norm_bwd": (ctypes.c_int, [ctypes.POINTER(GroupNorm)]),
+    "linrec_rms_norm_partial_floats": (_i64, [ctypes.c_int] + [_i64] * 2),
+    "linrec_rms_norm_fwd": (ctypes.c_int, [ctypes.POINTER(RmsNorm)]),
+    "linrec_rms_norm_bwd": (ctypes.c_int, [ctypes.POINTER(RmsNorm)]),
     "linrec_embedding_scratch_bytes": (ctypes.c_size_t, [_i64] * 3),
     "linrec_embedding_fwd": (ctypes.c_int, [ctypes.POINTER(Embedding)]),
     "linrec_embedding_bwd": (ctypes.c_int, [ctypes.POINTER(Embedding)]),
@@ -445,6 +458,114 @@ def norm_bwd(d_y, x, groups, weight, bias, stats, eps, act, number=None):
     a.d_x, a.d_weight, a.d_bias = d_x.data_ptr(), _p(d_weight), _p(d_bias)
     _call(x, _lib.linrec_group_norm_bwd, e, "group_norm_act")
     return d_x, d_weight, d_bias
+
+
+# ---- root-mean-square norm ---------------------------------------------------------------------
+def _collapse(dims):
+    """Stride of `dims`, (size, stride) pairs, taken as one dimension, or None."""
+    dims = [d for d in dims if d[0] != 1]
+    for (_, s0), (n1, s1) in zip(dims[:-1], dims[1:]):
+        if s0 != s1 * n1:
+            return None
+    return dims[-1][1] if dims else 0
+
+
+def _row_layout(tensors):
+    """(inner, strides of each): rows as (outer, inner) with a stride each, the same for all tensors; None if there is no such way."""
+    shape = tensors[0].shape[:-1]
+    if tensors[0].numel() == 0:
+        return 1, [_pair(0, 0) for _ in tensors]
+    if not all(_adjacent_channels(t) for t in tensors):
+        return None
+    for cut in range(len(shape) + 1):
+        strides = []
+        for t in tensors:
+            dims = list(zip(shape, t.stride()[:-1]))
+            strides.append((_collapse(dims[:cut]), _collapse(dims[cut:])))
+        if all(s is not None for pair in strides for s in pair):
+            inner = 1
+            for n in shape[cut:]:
+                inner *= n
+            return inner, [_pair(*pair) for pair in strides]
+    return None
+
+
+def _rms_entry(key, what, x, weight, eps, others, dtype=None, bwd=False):
+    """others: tensors of x's size, with the names of their fields; None where there is none."""
+    _check_activations(what, x)
+    if x.dim() < 1:
+        raise RuntimeError(f"{what}: x must be (..., channels)")
+    others = {name: t for name, t in others.items() if t is not None}
+    _check_activations(what, x, *others.values(), names=tuple(others))
+    channels = x.size(-1)
+    if not 1 <= channels <= RMS_NORM_CHANNELS_MAX:
+        raise RuntimeError(f"{what}: rows must have 1 to {RMS_NORM_CHANNELS_MAX} channels, got {channels}")
+    if dtype not in QUANTIZED:
+        raise RuntimeError(f"{what}: dtype must be torch.int8 or torch.float8_e4m3fn, got {dtype}")
+    a = RmsNorm(dtype=DTYPES[x.dtype], quantized=QUANTIZED[dtype], eps=eps, rows=x.numel() // channels, channels=channels)
+    if weight is not None:
+        if tuple(weight.size()) != (channels,):
+            raise RuntimeError(f"{what}: weight has size {tuple(weight.size())}, expected ({channels},)")
+        if weight.device != x.device:
+            raise RuntimeError(f"{what}: weight is on {weight.device}, x on {x.device}")
+        if weight.dtype not in (torch.float32, x.dtype):
+            raise RuntimeError(f"{what}: weight must be float32 or {x.dtype}, got {weight.dtype}")
+        a.weight_dtype = DTYPES[weight.dtype]
+    layout = _row_layout([x, *others.values()])
+    if layout is None or not (weight is None or weight.is_contiguous()):
+        return _remember(key, _Entry())
+    a.inner, strides = layout
+    a.x_stride = strides[0]
+    for name, stride in zip(others, strides[1:]):
+        setattr(a, name + "_stride", stride)
+    partial = _lib.linrec_rms_norm_partial_floats(a.dtype, a.rows, channels) if bwd and weight is not None else 0
+    return _remember(key, _Entry(a, 0, (x.shape[:-1], partial)))
+
+
+def rms_fwd(x, weight, residual, eps, dtype=None, save=True):
+    """(y, total, rstd or scales, number): total is None without a residual, rstd None without `save`; scales with a dtype"""
+    what = "rms_norm" if dtype is None else "rms_norm_quantize"
+    key = (what, _looks(x), _looks(weight), _looks(residual), eps, dtype)
+    e = _remembered().get(key) or _rms_entry(key, what, x, weight, eps, {"residual": residual}, dtype)
+    a = e.args
+    if a is None:
+        return rms_fwd(*_dense(x, weight, residual), eps, dtype, save)
+    device, shape = x.device, x.shape
+    y = torch.empty(shape, dtype=dtype or x.dtype, device=device)
+    total = None if residual is None else torch.empty(shape, dtype=x.dtype, device=device)
+    rows = _floats(e.sizes[0], device) if save or dtype is not None else None
+    a.x, a.residual, a.weight, a.y, a.total = x.data_ptr(), _p(residual), _p(weight), y.data_ptr(), _p(total)
+    if dtype is None:
+        a.rstd = _p(rows)
+    else:
+        a.scales = rows.data_ptr()
+    _call(x, _lib.linrec_rms_norm_fwd, e, what)
+    return y, total, rows, e.number
+
+
+def rms_bwd(d_y, d_total, x, weight, rstd, eps, number=None):
+    """(d_x, d_weight), the last None without a weight; x: what was normalised; d_y or d_total may be None (zeros)."""
+    if d_y is None:
+        d_y = torch.zeros((), dtype=x.dtype, device=x.device).expand(x.size())
+    if number is not None:
+        key = ("rms_bwd", number, d_y.stride(), _stride(d_total), x.stride(), _stride(weight))
+    else:
+        key = ("rms_bwd", _looks(x), _looks(weight), _looks(d_y), _looks(d_total), eps)
+    e = _remembered().get(key) or _rms_entry(key, "rms_norm", x, weight, eps, {"d_y": d_y, "d_total": d_total}, bwd=True)
+    a = e.args
+    if a is None:
+        return rms_bwd(*_dense(d_y, d_total, x, weight), rstd, eps)
+    device = x.device
+    if not rstd.is_contiguous():
+        rstd = rstd.contiguous()
+    d_x = torch.empty(x.shape, dtype=x.dtype, device=device)
+    d_weight = partial = None
+    if weight is not None:
+        d_weight, partial = torch.empty(weight.shape, dtype=weight.dtype, device=device), _floats(e.sizes[1], device)
+    a.x, a.d_y, a.d_total, a.weight, a.rstd = x.data_ptr(), d_y.data_ptr(), _p(d_total), _p(weight), rstd.data_ptr()
+    a.d_x, a.d_weight, a.partial = d_x.data_ptr(), _p(d_weight), _p(partial)
+    _call(x, _lib.linrec_rms_norm_bwd, e, "rms_norm")
+    return d_x, d_weight
 
 
 # ---- embedding ---------------------------------------------------------------------------------

@@ -1,5 +1,5 @@
 """Operators of a recurrent layer around the scan: the gated linear recurrence and its single-token step, group norm with an
-activation, and the token embedding.
+activation, root-mean-square norm with a residual, and the token embedding.
 
 As in ops.py each operator is a torch.library custom op (fake function, autograd rule) for tracing and compilation, and an
 equivalent autograd Function, or a plain call where no gradient is recorded, in eager mode.  Device tensors only.
@@ -11,7 +11,7 @@ from torch.autograd import forward_ad
 
 from . import _layers
 
-__all__ = ["gated_linrec", "gated_linrec_step", "group_norm_act", "embedding"]
+__all__ = ["gated_linrec", "gated_linrec_step", "group_norm_act", "rms_norm", "rms_norm_quantize", "embedding"]
 
 Tensor = torch.Tensor
 _PLAIN = (torch.Tensor, torch.nn.Parameter)  # (subclasses, fake ones among them, take the registered operators)
@@ -237,6 +237,111 @@ def group_norm_act(x: Tensor, groups: int, weight: Optional[Tensor] = None, bias
     if _recorded(x, weight, bias):
         return _NormFn.apply(x, groups, weight, bias, eps, act)
     return _layers.norm_fwd(x, groups, weight, bias, eps, act)[0]
+
+
+# ---- root-mean-square norm ---------------------------------------------------------------------
+@torch.library.custom_op("linrec_amd::rms_norm_fwd", mutates_args=(), device_types="cuda")
+def rms_norm_fwd(x: Tensor, weight: Optional[Tensor], residual: Optional[Tensor], eps: float) -> Tuple[Tensor, Tensor, Tensor]:
+    y, total, rstd, _ = _layers.rms_fwd(x, weight, residual, eps)
+    return y, x.new_empty(0) if total is None else total, rstd
+
+
+@torch.library.custom_op("linrec_amd::rms_norm_bwd", mutates_args=(), device_types="cuda")
+def rms_norm_bwd(d_y: Tensor, d_total: Optional[Tensor], x: Tensor, weight: Optional[Tensor], rstd: Tensor,
+                 eps: float) -> Tuple[Tensor, Tensor]:
+    d_x, d_weight = _layers.rms_bwd(d_y, d_total, x, weight, rstd, eps)
+    return d_x, rstd.new_empty(0) if d_weight is None else d_weight
+
+
+@torch.library.custom_op("linrec_amd::rms_norm_quantize", mutates_args=(), device_types="cuda")
+def _rms_norm_quantize(x: Tensor, weight: Optional[Tensor], residual: Optional[Tensor], eps: float,
+                       dtype: torch.dtype) -> Tuple[Tensor, Tensor, Tensor]:
+    q, total, scales, _ = _layers.rms_fwd(x, weight, residual, eps, dtype)
+    return q, scales, x.new_empty(0) if total is None else total
+
+
+@rms_norm_fwd.register_fake
+def _(x, weight, residual, eps):
+    return (x.new_empty(x.size()), x.new_empty(0 if residual is None else x.size()), x.new_empty(x.size()[:-1], dtype=torch.float32))
+
+
+@rms_norm_bwd.register_fake
+def _(d_y, d_total, x, weight, rstd, eps):
+    return x.new_empty(x.size()), rstd.new_empty(0) if weight is None else weight.new_empty(weight.size())
+
+
+@_rms_norm_quantize.register_fake
+def _(x, weight, residual, eps, dtype):
+    return (x.new_empty(x.size(), dtype=dtype), x.new_empty(x.size()[:-1], dtype=torch.float32), x.new_empty(0 if residual is None else x.size()))
+
+
+def _rms_setup(ctx, inputs, output):
+    x, weight, residual, ctx.eps = inputs
+    ctx.with_residual = residual is not None
+    ctx.save_for_backward(output[1] if ctx.with_residual else x, weight, output[2])
+
+
+def _rms_backward(ctx, d_y, d_total, _):
+    x, weight, rstd = ctx.saved_tensors
+    d_x, d_weight = rms_norm_bwd(d_y, d_total if ctx.with_residual else None, x, weight, rstd, ctx.eps)
+    return d_x, None if weight is None else d_weight, d_x if ctx.with_residual else None, None
+
+
+torch.library.register_autograd("linrec_amd::rms_norm_fwd", _rms_backward, setup_context=_rms_setup)
+
+
+class _RmsFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, residual, eps):
+        y, total, rstd, ctx.number = _layers.rms_fwd(x, weight, residual, eps)
+        ctx.save_for_backward(x if total is None else total, weight, rstd)
+        ctx.set_materialize_grads(False)
+        ctx.eps, ctx.with_residual = eps, residual is not None
+        return y if total is None else (y, total)
+
+    @staticmethod
+    @_once
+    def backward(ctx, d_y, d_total=None):
+        x, weight, rstd = ctx.saved_tensors
+        d_x, d_weight = _layers.rms_bwd(d_y, d_total, x, weight, rstd, ctx.eps, ctx.number)
+        return d_x, d_weight, d_x if ctx.with_residual else None, None
+
+
+def rms_norm(x: Tensor, weight: Optional[Tensor] = None, *, residual: Optional[Tensor] = None, eps: float = 1e-6):
+    """x * weight / sqrt(mean(x^2) + eps) over the last dimension of x, (..., channels) with up to 16384 channels.  With a residual, of x's
+    size and type, x + residual is normalised instead, rounded to that type, and returned as well: (y, total), total being what
+    the next layer's residual is.  weight, (channels), is float32 or of x's type, ones if None.  Sums are float32.
+    Differentiable in x, weight and residual.
+    """
+    eps = float(eps)
+    _refuse_tangents("rms_norm", x, weight, residual)
+    if _traced(x, weight, residual):
+        y, total, _ = rms_norm_fwd(x, weight, residual, eps)
+    elif _recorded(x, weight, residual):
+        return _RmsFn.apply(x, weight, residual, eps)
+    else:
+        y, total, *_ = _layers.rms_fwd(x, weight, residual, eps, None, False)
+    return y if residual is None else (y, total)
+
+
+def rms_norm_quantize(x: Tensor, weight: Optional[Tensor] = None, *, residual: Optional[Tensor] = None, eps: float = 1e-6,
+                      dtype: torch.dtype = torch.int8):
+    """rms_norm with an output in 8 bits, for a product in 8 bits: (q, scales), or (q, scales, total) with a residual.  q is int8 or
+    float8_e4m3fn of x's size, scales (float32, x's size without channels) one a row, its largest |y| over 127 or 448: the norm is
+    q * scales[..., None].  A row of zeros has the scale 0; one whose norm is not finite has NaN, and zeros for values.
+    Records no gradient, in neither direction.
+    """
+    eps = float(eps)
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, weight, residual)):
+        raise RuntimeError("rms_norm_quantize: records no gradient; call it under torch.no_grad(), or rms_norm for training")
+    _refuse_tangents("rms_norm_quantize", x, weight, residual)
+    if dtype is None:
+        raise RuntimeError("rms_norm_quantize: dtype must be torch.int8 or torch.float8_e4m3fn, got None")
+    if _traced(x, weight, residual):
+        q, scales, total = _rms_norm_quantize(x, weight, residual, eps, dtype)
+    else:
+        q, total, scales, _ = _layers.rms_fwd(x, weight, residual, eps, dtype)
+    return (q, scales) if residual is None else (q, scales, total)
 
 
 # ---- embedding ---------------------------------------------------------------------------------

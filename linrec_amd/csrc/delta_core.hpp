@@ -188,51 +188,82 @@ struct Tile {
   }
 };
 
-// 16 bytes from `col` on of a row of `cols` values; zeros behind its end.
-template <typename T>
-__device__ __forceinline__ typename Slot16<T>::type load_unit(const T* row, int col, int cols) {
-  constexpr int VEC = 16 / int(sizeof(T));
-  typename Slot16<T>::type v;
-  typedef T any __attribute__((ext_vector_type(16 / sizeof(T)), aligned(sizeof(T))));
-  if (col + VEC <= cols) return *reinterpret_cast<const any*>(row + col);
-#pragma unroll
-  for (int e = 0; e < VEC; ++e) v[e] = col + e < cols ? row[col + e] : T(0.0f);
-  return v;
-}
-template <typename T>
-__device__ __forceinline__ typename Slot16<T>::type zero_unit() {
-  typename Slot16<T>::type v;
-#pragma unroll
-  for (int e = 0; e < 16 / int(sizeof(T)); ++e) v[e] = T(0.0f);
-  return v;
-}
-
-// COLS columns of ROWS rows to a tile; zeros for rows from `rows` and columns from `cols` on.
+// ROWS rows of COLS columns on their way from memory to a tile, by LANES lanes of which this is number `lane`: all loads first, so that
+// their latencies are one, and stores to LDS when they are due.
 template <typename T, int COLS, int LANES, int ROWS = 64>
-__device__ __forceinline__ void stage(char* tile, const T* from, int64_t stride, int rows, int cols) {
+struct Stager {
   using L = Tile<T, COLS>;
-  constexpr int UNITS = ROWS * L::UNITS;
+  using V = typename Slot16<T>::type;
+  static constexpr int VEC = L::VEC, STEP = LANES / L::UNITS, N = (ROWS + STEP - 1) / STEP;  // rows side by side, units of a lane
+  static_assert(LANES % L::UNITS == 0, "a lane has one column of units");
+  V v[N];
+
+  static __device__ __forceinline__ V zero() {
+    V z;
 #pragma unroll
-  for (int n = 0; n < (UNITS + LANES - 1) / LANES; ++n) {
-    const int i = n * LANES + int(threadIdx.x), row = i / L::UNITS, u = i % L::UNITS;
-    if (UNITS % LANES && i >= UNITS) break;
-    auto v = zero_unit<T>();
-    if (row < rows) v = load_unit(from + row * stride, u * L::VEC, cols);
-    *reinterpret_cast<decltype(v)*>(tile + L::at(row, u)) = v;
+    for (int e = 0; e < VEC; ++e) z[e] = T(0.0f);
+    return z;
   }
-}
-// The same from dense scratch rows of COLS columns.
-template <typename U, int COLS, int LANES, int ROWS>
-__device__ __forceinline__ void stage_dense(char* tile, const U* from) {
-  using L = Tile<U, COLS>;
-  constexpr int UNITS = ROWS * L::UNITS;
+  // `back` values down (the same for all lanes), zeros behind them
+  static __device__ __forceinline__ V moved(const V& x, int back) {
+    uint64_t w[2];
+    __builtin_memcpy(w, &x, 16);
+    const int bits = back * 8 * int(sizeof(T));
+    if (bits >= 64) {
+      w[0] = w[1] >> (bits - 64);
+      w[1] = 0;
+    } else if (bits > 0) {
+      w[0] = (w[0] >> bits) | (w[1] << (64 - bits));
+      w[1] >>= bits;
+    }
+    V out;
+    __builtin_memcpy(&out, w, 16);
+    return out;
+  }
+  // zeros for rows from `rows` and columns from `cols` (at least one) on
+  __device__ __forceinline__ void fetch(const T* from, int64_t stride, int rows, int cols, int lane) {
+    typedef T any __attribute__((ext_vector_type(16 / sizeof(T)), aligned(sizeof(T))));
+    const int row = lane / L::UNITS, col = lane % L::UNITS * VEC;
+    if (rows >= ROWS && cols >= COLS) {
+      const T* p = from + row * stride + col;
 #pragma unroll
-  for (int n = 0; n < (UNITS + LANES - 1) / LANES; ++n) {
-    const int i = n * LANES + int(threadIdx.x), row = i / L::UNITS, u = i % L::UNITS;
-    if (UNITS % LANES && i >= UNITS) break;
-    *reinterpret_cast<typename Slot16<U>::type*>(tile + L::at(row, u)) = reinterpret_cast<const typename Slot16<U>::type*>(from)[i];
+      for (int n = 0; n < N; ++n)
+        if (ROWS % STEP == 0 || n * STEP + row < ROWS) v[n] = *reinterpret_cast<const any*>(p + n * STEP * stride);
+      return;
+    }
+#pragma unroll
+    for (int n = 0; n < N; ++n) v[n] = zero();
+    if (cols >= VEC) {  // the last columns by a load that ends with the row
+      const int at = col <= cols - VEC ? col : cols - VEC;
+      const T* p = from + row * stride + at;
+#pragma unroll
+      for (int n = 0; n < N; ++n)
+        if (n * STEP + row < rows && col < cols) v[n] = *reinterpret_cast<const any*>(p + n * STEP * stride);
+      if (cols < COLS && cols % VEC)
+#pragma unroll
+        for (int n = 0; n < N; ++n) {
+          const V m = moved(v[n], VEC - cols % VEC);
+          v[n] = at != col ? m : v[n];
+        }
+    } else {
+      for (int n = 0; n < N; ++n)
+        if (n * STEP + row < rows && col == 0)
+          for (int e = 0; e < cols; ++e) v[n][e] = from[(n * STEP + row) * stride + e];
+    }
   }
-}
+  // dense rows of scratch
+  __device__ __forceinline__ void fetch_dense(const T* from, int lane) {
+#pragma unroll
+    for (int n = 0; n < N; ++n)
+      if (ROWS % STEP == 0 || n * STEP + lane / L::UNITS < ROWS) v[n] = reinterpret_cast<const V*>(from)[n * LANES + lane];
+  }
+  __device__ __forceinline__ void put(char* tile, int lane) const {
+#pragma unroll
+    for (int n = 0; n < N; ++n)
+      if (ROWS % STEP == 0 || n * STEP + lane / L::UNITS < ROWS)
+        *reinterpret_cast<V*>(tile + L::at(n * STEP + lane / L::UNITS, lane % L::UNITS)) = v[n];
+  }
+};
 
 // ---- chunks and scratch ----------------------------------------------------------------------------------------------------------
 // A chunk has a slot: those of a sequence follow each other, a packed sequence's start at cu_seqlens[n] / 64 + n (so that no two

@@ -27,32 +27,29 @@ struct GradientShared {
   static constexpr int BYTES = FIRST > SECOND ? FIRST : SECOND;
 };
 
-// COLS columns of 64 rows of an input to IN tiles of the inner type.
+// COLS columns of 64 rows of an input on their way to IN tiles of the inner type.
 template <typename T, int COLS, int LANES>
-__device__ __forceinline__ void stage_input(char* tile, const T* from, int64_t stride, int rows, int cols) {
+struct InputStager {
   using U = Inner<T>;
-  if constexpr (std::is_same_v<T, U>) {
-    stage<T, COLS, LANES>(tile, from, stride, rows, cols);
-  } else {  // fp16 as two bf16
-    using L = Tile<U, COLS>;
-    constexpr int UNITS = 64 * L::UNITS;
+  Stager<T, COLS, LANES> s;
+  __device__ __forceinline__ void fetch(const T* from, int64_t stride, int rows, int cols) { s.fetch(from, stride, rows, cols, threadIdx.x); }
+  __device__ __forceinline__ void put(char* tile) const {
+    if constexpr (std::is_same_v<T, U>) {
+      s.put(tile, threadIdx.x);
+    } else {  // fp16 as two bf16
+      Stager<U, COLS, LANES> hi, lo;
 #pragma unroll
-    for (int n = 0; n < (UNITS + LANES - 1) / LANES; ++n) {
-      const int i = n * LANES + int(threadIdx.x), row = i / L::UNITS, u = i % L::UNITS;
-      if (UNITS % LANES && i >= UNITS) break;
-      auto v = zero_unit<T>();
-      if (row < rows) v = load_unit(from + row * stride, u * 8, cols);
-      Frag<U> hi, lo;
+      for (int n = 0; n < decltype(s)::N; ++n)
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        hi[e] = U(float(v[e]));
-        lo[e] = U(float(v[e]) - float(hi[e]));
-      }
-      *reinterpret_cast<Frag<U>*>(tile + L::at(row, u)) = hi;
-      *reinterpret_cast<Frag<U>*>(tile + 64 * L::ROW + L::at(row, u)) = lo;
+        for (int e = 0; e < 8; ++e) {
+          hi.v[n][e] = U(float(s.v[n][e]));
+          lo.v[n][e] = U(float(s.v[n][e]) - float(hi.v[n][e]));
+        }
+      hi.put(tile, threadIdx.x);
+      lo.put(tile + 64 * Tile<U, COLS>::ROW, threadIdx.x);
     }
   }
-}
+};
 
 __device__ __forceinline__ float sum_of_16(float x) {
   x += __shfl_xor(x, 1);
@@ -109,19 +106,28 @@ __global__ __launch_bounds__(256) void delta_gradient_kernel(DeltaArgs a) {
       const T* v = head_rows<T>(p.v, p.v_stride, ch.batch, ch.first, head);
       for (int v0 = 0; v0 < p.value_dim; v0 += 32) {
         __syncthreads();
-        stage_input<T, 32, 256>(smem + Sh::O, d_o + v0, p.d_o_stride[1], ch.length, p.value_dim - v0);
-        stage_input<T, 32, 256>(smem + Sh::V, v + v0, p.v_stride[1], ch.length, p.value_dim - v0);
+        {
+          InputStager<T, 32, 256> so, sv;
+          Stager<U, 64, 256, 32> sb[P], sn[P];
+          Stager<U, DK, 256, 32> ss[P], sd[P];
+          so.fetch(d_o + v0, p.d_o_stride[1], ch.length, p.value_dim - v0);
+          sv.fetch(v + v0, p.v_stride[1], ch.length, p.value_dim - v0);
 #pragma unroll
-        for (int k = 0; k < P; ++k) {
-          const int64_t row = (block * P + k) * a.columns + v0;
-          stage_dense<U, 64, 256, 32>(smem + Sh::B + k * Sh::BY_V, reinterpret_cast<const U*>(a.d_b) + row * 64);
-          stage_dense<U, 64, 256, 32>(smem + Sh::N + k * Sh::BY_V, reinterpret_cast<const U*>(a.n) + row * 64);
-          if constexpr (WIDE) {
-            stage<U, DK, 256, 32>(smem + Sh::S + k * Sh::STATE, reinterpret_cast<const U*>(a.s) + row * ROW + d0, ROW, 32, DK);
-            stage<U, DK, 256, 32>(smem + Sh::D + k * Sh::STATE, reinterpret_cast<const U*>(a.d_s) + row * ROW + d0, ROW, 32, DK);
-          } else {
-            stage_dense<U, DK, 256, 32>(smem + Sh::S + k * Sh::STATE, reinterpret_cast<const U*>(a.s) + row * ROW);
-            stage_dense<U, DK, 256, 32>(smem + Sh::D + k * Sh::STATE, reinterpret_cast<const U*>(a.d_s) + row * ROW);
+          for (int k = 0; k < P; ++k) {
+            const int64_t row = (block * P + k) * a.columns + v0;
+            sb[k].fetch_dense(reinterpret_cast<const U*>(a.d_b) + row * 64, threadIdx.x);
+            sn[k].fetch_dense(reinterpret_cast<const U*>(a.n) + row * 64, threadIdx.x);
+            ss[k].fetch(reinterpret_cast<const U*>(a.s) + row * ROW + d0, ROW, 32, DK, threadIdx.x);
+            sd[k].fetch(reinterpret_cast<const U*>(a.d_s) + row * ROW + d0, ROW, 32, DK, threadIdx.x);
+          }
+          so.put(smem + Sh::O);
+          sv.put(smem + Sh::V);
+#pragma unroll
+          for (int k = 0; k < P; ++k) {
+            sb[k].put(smem + Sh::B + k * Sh::BY_V, threadIdx.x);
+            sn[k].put(smem + Sh::N + k * Sh::BY_V, threadIdx.x);
+            ss[k].put(smem + Sh::S + k * Sh::STATE, threadIdx.x);
+            sd[k].put(smem + Sh::D + k * Sh::STATE, threadIdx.x);
           }
         }
         __syncthreads();
@@ -208,8 +214,13 @@ __global__ __launch_bounds__(256) void delta_gradient_kernel(DeltaArgs a) {
       __syncthreads();
       const T* k_rows = head_rows<T>(p.k, p.k_stride, ch.batch, ch.first, key_head) + d0;
       const T* q_rows = head_rows<T>(p.q, p.q_stride, ch.batch, ch.first, key_head) + d0;
-      stage_input<T, DK, 256>(smem + Sh::K, k_rows, p.k_stride[1], ch.length, p.key_dim - d0);
-      stage_input<T, DK, 256>(smem + Sh::Q, q_rows, p.q_stride[1], ch.length, p.key_dim - d0);
+      {
+        InputStager<T, DK, 256> sk, sq;
+        sk.fetch(k_rows, p.k_stride[1], ch.length, p.key_dim - d0);
+        sq.fetch(q_rows, p.q_stride[1], ch.length, p.key_dim - d0);
+        sk.put(smem + Sh::K);
+        sq.put(smem + Sh::Q);
+      }
       __syncthreads();
       float dot_q[4], dot_x[4], dot_y[4], dot_z[4];
 #pragma unroll

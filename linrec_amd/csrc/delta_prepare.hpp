@@ -1,7 +1,7 @@
 // Gated delta rule, what a chunk needs that does not depend on the state: M = (1 + A)^-1, C and the decays.
 //
-// A workgroup for every (chunk, head).  K K^T and Q K^T are matrix instructions whose operands come straight from memory, a wave for
-// 16 rows.  1 + A is unit lower triangular; its inverse is put together in fp32: blocks of 16 by substitution, a lane for a column,
+// A workgroup for every (chunk, head).  K K^T and Q K^T are matrix instructions, a wave for 16 rows; their operands lie in LDS where M
+// and C are put together afterwards.  1 + A is unit lower triangular; its inverse is put together in fp32: blocks of 16 by substitution, a lane for a column,
 // then of 32 and of 64 by M21 = -M22 A21 M11 with the fp32 matrix instruction.  (Substitution over all 64 rows would be 64 dependent
 // steps; powers of A, whose binomials cancel, lose all digits where keys are alike.)
 #pragma once
@@ -27,21 +27,6 @@ __device__ __forceinline__ void store_square(char* to, const float* from) {
   }
 }
 
-// 8 of 32 columns of a row of an input, zeros outside.
-template <typename T>
-__device__ __forceinline__ Frag<T> row_frag(const T* row, bool there, int col, int cols) {
-  Frag<T> f;
-  constexpr int VEC = 16 / int(sizeof(T));
-#pragma unroll
-  for (int h = 0; h < 8 / VEC; ++h) {
-    auto v = zero_unit<T>();
-    if (there) v = load_unit(row, col + h * VEC, cols);
-#pragma unroll
-    for (int e = 0; e < VEC; ++e) f[h * VEC + e] = v[e];
-  }
-  return f;
-}
-
 // e^{G_63 - G} and so on of a chunk by its first wave, a lane for a position; G in fp64, where differences of large sums keep
 // their digits.
 __device__ __forceinline__ double chunk_sum(float g, int lane) {
@@ -55,11 +40,14 @@ __device__ __forceinline__ double chunk_sum(float g, int lane) {
   return sum;
 }
 
-template <typename T, bool BWD>
+template <typename T, int DK, bool BWD>
 __global__ __launch_bounds__(256) void delta_prepare_kernel(DeltaArgs a) {
   using U = Inner<T>;
-  constexpr int S = PREPARE_STRIDE;
-  __shared__ __align__(16) float sh_a[64 * S], sh_m[64 * S], sh_c[64 * S];
+  using TK = Tile<T, DK>;
+  constexpr int S = PREPARE_STRIDE, SQUARES = 2 * 64 * S * 4;
+  __shared__ __align__(16) float sh_a[64 * S];
+  __shared__ __align__(16) char sh_keys[2 * TK::BYTES > SQUARES ? 2 * TK::BYTES : SQUARES];
+  float *sh_m = reinterpret_cast<float*>(sh_keys), *sh_c = sh_m + 64 * S;
   __shared__ double sh_g[64];
   __shared__ float sh_beta[64];
   const linrec_delta_t& p = a.p;
@@ -70,7 +58,13 @@ __global__ __launch_bounds__(256) void delta_prepare_kernel(DeltaArgs a) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r = lane & 15, q = lane >> 4;
   const int64_t block = slot * p.heads + head;
 
-  for (int i = threadIdx.x; i < 64 * S; i += 256) sh_m[i] = 0.0f, sh_c[i] = 0.0f;
+  {
+    Stager<T, DK, 256> k, qq;
+    k.fetch(head_rows<T>(p.k, p.k_stride, ch.batch, ch.first, key_head), p.k_stride[1], ch.length, p.key_dim, threadIdx.x);
+    qq.fetch(head_rows<T>(p.q, p.q_stride, ch.batch, ch.first, key_head), p.q_stride[1], ch.length, p.key_dim, threadIdx.x);
+    k.put(sh_keys, threadIdx.x);
+    qq.put(sh_keys + TK::BYTES, threadIdx.x);
+  }
   if (wave == 0) {
     const bool there = lane < ch.length;
     const float g = there ? *(head_rows<float>(p.log_decay, p.log_decay_stride, ch.batch, ch.first + lane, head)) : 0.0f;
@@ -83,24 +77,24 @@ __global__ __launch_bounds__(256) void delta_prepare_kernel(DeltaArgs a) {
     gates[64 + lane] = expf(float(last - sum));
     gates[128 + lane] = beta;
   }
-  const T* k = head_rows<T>(p.k, p.k_stride, ch.batch, ch.first, key_head);
-  const T* qq = head_rows<T>(p.q, p.q_stride, ch.batch, ch.first, key_head);
+  __syncthreads();
   v4f kk[4], qk[4];
 #pragma unroll
   for (int t = 0; t < 4; ++t) kk[t] = v4f{0, 0, 0, 0}, qk[t] = v4f{0, 0, 0, 0};
-  const int own = 16 * wave + r;
-  for (int c = 0; c < p.key_dim; c += 32) {
-    const Frag<T> rk = row_frag(k + own * p.k_stride[1], own < ch.length, c + 8 * q, p.key_dim);
-    const Frag<T> rq = row_frag(qq + own * p.q_stride[1], own < ch.length, c + 8 * q, p.key_dim);
+  // wave w has rows 16 w and up; tile t of columns from 16 t on, none above the diagonal
+#pragma unroll
+  for (int b = 0; b < DK / 32; ++b) {
+    const Frag<T> rk = TK::frag(sh_keys, 16 * wave + r, b, q), rq = TK::frag(sh_keys + TK::BYTES, 16 * wave + r, b, q);
 #pragma unroll
     for (int t = 0; t < 4; ++t)
       if (t <= wave) {
-        const int other = 16 * t + r;
-        const Frag<T> b = t == wave ? rk : row_frag(k + other * p.k_stride[1], other < ch.length, c + 8 * q, p.key_dim);
-        kk[t] = mma(rk, b, kk[t]);
-        qk[t] = mma(rq, b, qk[t]);
+        const Frag<T> other = TK::frag(sh_keys, 16 * t + r, b, q);
+        kk[t] = mma(rk, other, kk[t]);
+        qk[t] = mma(rq, other, qk[t]);
       }
   }
+  __syncthreads();
+  for (int i = threadIdx.x; i < 64 * S; i += 256) sh_m[i] = 0.0f, sh_c[i] = 0.0f;
   __syncthreads();
 #pragma unroll
   for (int t = 0; t < 4; ++t)

@@ -1,6 +1,6 @@
 // Gated delta rule, the backward's pass against the sequence: dV, dB and the gradient of the state, chunk by chunk (delta_core.hpp).
 //
-// As the forward's: a workgroup has a (sequence, head), a wave 16 columns of dS.
+// As the forward's: a workgroup has a (sequence, head), a wave of its first half 16 columns of dS, and the other half loads.
 #pragma once
 #include "delta_scan.hpp"
 
@@ -13,17 +13,19 @@ struct ReverseShared {
   static constexpr bool QUERIES = 2 * KEYS + VALUES + 2 * square_bytes<U>() + 1024 <= 160 * 1024;
   static constexpr int K = 0, Q = K + KEYS, O = Q + (QUERIES ? KEYS : 0), M = O + VALUES, C = M + square_bytes<U>(),
                        GATES = C + square_bytes<U>(), BYTES = GATES + 3 * 64 * 4;
+  static constexpr bool LOADERS = 2 * BYTES <= 160 * 1024;
+  static constexpr int LANES = 64 * WAVES * (LOADERS ? 2 : 1);
 };
 
 template <typename T, int DK, int WAVES>
-__global__ __launch_bounds__(64 * WAVES) void delta_reverse_kernel(DeltaArgs a) {
+__global__ __launch_bounds__((ReverseShared<T, DK, WAVES>::LANES)) void delta_reverse_kernel(DeltaArgs a) {
   using U = Inner<T>;
   using Sh = ReverseShared<T, DK, WAVES>;
   using TK = Tile<T, DK>;
   using TV = Tile<T, 16 * WAVES>;
   using TS = Tile<U, 64>;
-  constexpr int P = planes_of<U>(), LANES = 64 * WAVES, SQUARE = square_bytes<U>(), IN = input_planes<T>();
-  __shared__ __align__(16) char smem[Sh::BYTES];
+  constexpr int P = planes_of<U>(), STAGING = 64 * WAVES, SQUARE = square_bytes<U>(), IN = input_planes<T>();
+  __shared__ __align__(16) char room[Sh::BYTES * (Sh::LOADERS ? 2 : 1)];
   const linrec_delta_t& p = a.p;
   int64_t pair;
   int cb;
@@ -31,10 +33,43 @@ __global__ __launch_bounds__(64 * WAVES) void delta_reverse_kernel(DeltaArgs a) 
   const int64_t n = pair / p.heads;
   const int head = int(pair - n * p.heads), key_head = head / a.shared;
   const Span span = span_of(p, n);
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r = lane & 15, q = lane >> 4;
+  const int lane = threadIdx.x & 63, r = lane & 15, q = lane >> 4;
+  const bool loader = Sh::LOADERS && threadIdx.x >= 64 * WAVES;
+  const int wave = (threadIdx.x >> 6) - (loader ? WAVES : 0);
   const int c0 = cb * 16 * WAVES, col = c0 + 16 * wave + r;
   const bool mine = col < p.value_dim, kept_column = col < a.columns;  // (of a whole wave)
-  float* gates = reinterpret_cast<float*>(smem + Sh::GATES);
+  const int64_t chunks = (span.end - span.first + DELTA_CHUNK - 1) / DELTA_CHUNK;
+
+  auto load = [&](int64_t c, char* smem) __attribute__((always_inline)) {
+    const int64_t first = span.first + c * DELTA_CHUNK, block = (span.slot + c) * p.heads + head;
+    const int length = int(span.end - first < DELTA_CHUNK ? span.end - first : DELTA_CHUNK), by = wave * 64 + lane;
+    Stager<T, DK, STAGING> k, qq;
+    Stager<T, 16 * WAVES, STAGING> o;
+    Stager<U, 64, STAGING> m[P], cc[P];
+    float gate[(192 + STAGING - 1) / STAGING];
+    k.fetch(head_rows<T>(p.k, p.k_stride, span.batch, first, key_head), p.k_stride[1], length, p.key_dim, by);
+    if constexpr (Sh::QUERIES) qq.fetch(head_rows<T>(p.q, p.q_stride, span.batch, first, key_head), p.q_stride[1], length, p.key_dim, by);
+    o.fetch(head_rows<T>(p.d_o, p.d_o_stride, span.batch, first, head) + c0, p.d_o_stride[1], length, p.value_dim - c0, by);
+#pragma unroll
+    for (int k2 = 0; k2 < P; ++k2) {
+      m[k2].fetch_dense(reinterpret_cast<const U*>(a.m_t + block * SQUARE) + k2 * 4096, by);
+      cc[k2].fetch_dense(reinterpret_cast<const U*>(a.c + block * SQUARE) + k2 * 4096, by);
+    }
+#pragma unroll
+    for (int i = 0; i < (192 + STAGING - 1) / STAGING; ++i)
+      if (i * STAGING + by < 192) gate[i] = a.gates[block * 192 + i * STAGING + by];
+    k.put(smem + Sh::K, by);
+    if constexpr (Sh::QUERIES) qq.put(smem + Sh::Q, by);
+    o.put(smem + Sh::O, by);
+#pragma unroll
+    for (int k2 = 0; k2 < P; ++k2) {
+      m[k2].put(smem + Sh::M + k2 * TS::BYTES, by);
+      cc[k2].put(smem + Sh::C + k2 * TS::BYTES, by);
+    }
+#pragma unroll
+    for (int i = 0; i < (192 + STAGING - 1) / STAGING; ++i)
+      if (i * STAGING + by < 192) reinterpret_cast<float*>(smem + Sh::GATES)[i * STAGING + by] = gate[i];
+  };
 
   v4f s[DK / 16];  // dS'
   const int64_t at0 = (pair * p.key_dim) * int64_t(p.value_dim) + col;
@@ -43,28 +78,14 @@ __global__ __launch_bounds__(64 * WAVES) void delta_reverse_kernel(DeltaArgs a) 
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
       const int d = row_of_result(t, q) + e;
-      s[t][e] = p.d_state && mine && d < p.key_dim ? p.d_state[at0 + d * int64_t(p.value_dim)] : 0.0f;
+      s[t][e] = p.d_state && mine && !loader && d < p.key_dim ? p.d_state[at0 + d * int64_t(p.value_dim)] : 0.0f;
     }
 
-  const int64_t chunks = (span.end - span.first + DELTA_CHUNK - 1) / DELTA_CHUNK;
-  for (int64_t c = chunks - 1; c >= 0; --c) {
-    const int64_t first = span.first + c * DELTA_CHUNK, slot = span.slot + c;
+  auto compute = [&](int64_t c, const char* smem) __attribute__((always_inline)) {
+    const int64_t first = span.first + c * DELTA_CHUNK, block = (span.slot + c) * p.heads + head;
     const int length = int(span.end - first < DELTA_CHUNK ? span.end - first : DELTA_CHUNK);
-    const int64_t block = slot * p.heads + head;
-    __syncthreads();
+    const float* gates = reinterpret_cast<const float*>(smem + Sh::GATES);
     const T* qq = head_rows<T>(p.q, p.q_stride, span.batch, first, key_head);
-    stage<T, DK, LANES>(smem + Sh::K, head_rows<T>(p.k, p.k_stride, span.batch, first, key_head), p.k_stride[1], length, p.key_dim);
-    if constexpr (Sh::QUERIES) stage<T, DK, LANES>(smem + Sh::Q, qq, p.q_stride[1], length, p.key_dim);
-    stage<T, 16 * WAVES, LANES>(smem + Sh::O, head_rows<T>(p.d_o, p.d_o_stride, span.batch, first, head) + c0, p.d_o_stride[1], length,
-                                p.value_dim - c0);
-#pragma unroll
-    for (int k2 = 0; k2 < P; ++k2) {
-      stage_dense<U, 64, LANES, 64>(smem + Sh::M + k2 * TS::BYTES, reinterpret_cast<const U*>(a.m_t + block * SQUARE) + k2 * 4096);
-      stage_dense<U, 64, LANES, 64>(smem + Sh::C + k2 * TS::BYTES, reinterpret_cast<const U*>(a.c + block * SQUARE) + k2 * 4096);
-    }
-    for (int i = threadIdx.x; i < 192; i += LANES) gates[i] = a.gates[block * 192 + i];
-    __syncthreads();
-
     Planes<T> sp[DK / 32];
     float un_s;
     split_scaled<T>(s, sp, &un_s);
@@ -131,16 +152,27 @@ __global__ __launch_bounds__(64 * WAVES) void delta_reverse_kernel(DeltaArgs a) 
         for (int k2 = 0; k2 < P; ++k2) *reinterpret_cast<Frag<U>*>(to + (int64_t(k2) * a.columns + col) * 64 + 32 * b + 8 * q) = kept.p[k2];
       }
     }
+    const int apart = p.heads * p.value_dim;
     T* d_v = static_cast<T*>(p.d_v) + ((span.batch * p.time + first) * p.heads + head) * int64_t(p.value_dim) + col;
 #pragma unroll
     for (int t = 0; t < 4; ++t) {
       const int row = row_of_result(t, q);
       const v4f gamma = *reinterpret_cast<const v4f*>(gates + row), beta = *reinterpret_cast<const v4f*>(gates + 128 + row);
+      T* to = d_v + row * int64_t(apart);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) db[t][e] *= beta[e];
+      if (length == DELTA_CHUNK) {
+        if (mine)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) to[e * apart] = T(db[t][e]);
+      } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if (mine && row + e < length) to[e * apart] = T(db[t][e]);
+      }
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        const float v = beta[e] * db[t][e];
-        if (mine && row + e < length) d_v[(row + e) * int64_t(p.heads) * p.value_dim] = T(v);
-        db[t][e] = -gamma[e] * v;
+        db[t][e] *= -gamma[e];
         d_o[t][e] *= gamma[e] * p.scale;
       }
     }
@@ -182,8 +214,25 @@ __global__ __launch_bounds__(64 * WAVES) void delta_reverse_kernel(DeltaArgs a) 
         s[t] = with_queries(with_keys(s[t]));
       }
     }
+  };
+
+  if constexpr (Sh::LOADERS) {
+    if (loader && chunks > 0) load(chunks - 1, room);
+    __syncthreads();
+    for (int64_t c = chunks - 1, turn = 0; c >= 0; --c, turn ^= 1) {
+      if (!loader) compute(c, room + turn * Sh::BYTES);
+      else if (c > 0) load(c - 1, room + (turn ^ 1) * Sh::BYTES);
+      __syncthreads();
+    }
+  } else {
+    for (int64_t c = chunks - 1; c >= 0; --c) {
+      __syncthreads();
+      load(c, room);
+      __syncthreads();
+      compute(c, room);
+    }
   }
-  if (p.d_h0 && mine)
+  if (p.d_h0 && mine && !loader)
 #pragma unroll
     for (int t = 0; t < DK / 16; ++t)
 #pragma unroll

@@ -1,6 +1,8 @@
 // Gated delta rule, the pass along the sequence: N, O and the state, chunk by chunk (delta_core.hpp).
 //
-// A workgroup has a (sequence, head) and 16 columns of the state for each of its waves.
+// A workgroup has a (sequence, head) and 16 columns of the state for each of half of its waves; the other half loads what the next
+// chunk needs into LDS meanwhile (a state's chunks follow one another, so nothing else hides those loads; where two chunks do not
+// fit into LDS all waves load first and compute then).
 #pragma once
 #include "delta_core.hpp"
 
@@ -19,18 +21,20 @@ struct ScanShared {
   static constexpr bool QUERIES = !STATES && 2 * KEYS + VALUES + 2 * square_bytes<U>() + 1024 <= 160 * 1024;
   static constexpr int K = 0, Q = K + KEYS, V = Q + (QUERIES ? KEYS : 0), M = V + VALUES, C = M + square_bytes<U>(),
                        GATES = C + (STATES ? 0 : square_bytes<U>()), BYTES = GATES + 3 * 64 * 4;
+  static constexpr bool LOADERS = 2 * BYTES <= 160 * 1024;
+  static constexpr int LANES = 64 * WAVES * (LOADERS ? 2 : 1);
 };
 
 // STATES: a backward's first pass, which keeps the states before the chunks and N and has no O.
 template <typename T, int DK, int WAVES, bool STATES>
-__global__ __launch_bounds__(64 * WAVES) void delta_scan_kernel(DeltaArgs a) {
+__global__ __launch_bounds__((ScanShared<T, DK, WAVES, STATES>::LANES)) void delta_scan_kernel(DeltaArgs a) {
   using U = Inner<T>;
   using Sh = ScanShared<T, DK, WAVES, STATES>;
   using TK = Tile<T, DK>;
   using TV = Tile<T, 16 * WAVES>;
   using TS = Tile<U, 64>;
-  constexpr int P = planes_of<U>(), LANES = 64 * WAVES, SQUARE = square_bytes<U>();
-  __shared__ __align__(16) char smem[Sh::BYTES];
+  constexpr int P = planes_of<U>(), STAGING = 64 * WAVES, SQUARE = square_bytes<U>();
+  __shared__ __align__(16) char room[Sh::BYTES * (Sh::LOADERS ? 2 : 1)];
   const linrec_delta_t& p = a.p;
   int64_t pair;
   int cb;
@@ -38,10 +42,43 @@ __global__ __launch_bounds__(64 * WAVES) void delta_scan_kernel(DeltaArgs a) {
   const int64_t n = pair / p.heads;
   const int head = int(pair - n * p.heads), key_head = head / a.shared;
   const Span span = span_of(p, n);
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r = lane & 15, q = lane >> 4;
+  const int lane = threadIdx.x & 63, r = lane & 15, q = lane >> 4;
+  const bool loader = Sh::LOADERS && threadIdx.x >= 64 * WAVES;
+  const int wave = (threadIdx.x >> 6) - (loader ? WAVES : 0);
   const int c0 = cb * 16 * WAVES, col = c0 + 16 * wave + r;
   const bool mine = col < p.value_dim, kept_column = col < a.columns;  // (of a whole wave)
-  float* gates = reinterpret_cast<float*>(smem + Sh::GATES);
+  const int64_t chunks = (span.end - span.first + DELTA_CHUNK - 1) / DELTA_CHUNK;
+
+  auto load = [&](int64_t c, char* smem) __attribute__((always_inline)) {
+    const int64_t first = span.first + c * DELTA_CHUNK, block = (span.slot + c) * p.heads + head;
+    const int length = int(span.end - first < DELTA_CHUNK ? span.end - first : DELTA_CHUNK), by = wave * 64 + lane;
+    Stager<T, DK, STAGING> k, qq;
+    Stager<T, 16 * WAVES, STAGING> v;
+    Stager<U, 64, STAGING> m[P], cc[P];
+    float gate[(192 + STAGING - 1) / STAGING];
+    k.fetch(head_rows<T>(p.k, p.k_stride, span.batch, first, key_head), p.k_stride[1], length, p.key_dim, by);
+    if constexpr (Sh::QUERIES) qq.fetch(head_rows<T>(p.q, p.q_stride, span.batch, first, key_head), p.q_stride[1], length, p.key_dim, by);
+    v.fetch(head_rows<T>(p.v, p.v_stride, span.batch, first, head) + c0, p.v_stride[1], length, p.value_dim - c0, by);
+#pragma unroll
+    for (int k2 = 0; k2 < P; ++k2) {
+      m[k2].fetch_dense(reinterpret_cast<const U*>(a.m + block * SQUARE) + k2 * 4096, by);
+      if constexpr (!STATES) cc[k2].fetch_dense(reinterpret_cast<const U*>(a.c + block * SQUARE) + k2 * 4096, by);
+    }
+#pragma unroll
+    for (int i = 0; i < (192 + STAGING - 1) / STAGING; ++i)
+      if (i * STAGING + by < 192) gate[i] = a.gates[block * 192 + i * STAGING + by];
+    k.put(smem + Sh::K, by);
+    if constexpr (Sh::QUERIES) qq.put(smem + Sh::Q, by);
+    v.put(smem + Sh::V, by);
+#pragma unroll
+    for (int k2 = 0; k2 < P; ++k2) {
+      m[k2].put(smem + Sh::M + k2 * TS::BYTES, by);
+      if constexpr (!STATES) cc[k2].put(smem + Sh::C + k2 * TS::BYTES, by);
+    }
+#pragma unroll
+    for (int i = 0; i < (192 + STAGING - 1) / STAGING; ++i)
+      if (i * STAGING + by < 192) reinterpret_cast<float*>(smem + Sh::GATES)[i * STAGING + by] = gate[i];
+  };
 
   v4f s[DK / 16];
   const int64_t at0 = (pair * p.key_dim) * int64_t(p.value_dim) + col;
@@ -50,27 +87,14 @@ __global__ __launch_bounds__(64 * WAVES) void delta_scan_kernel(DeltaArgs a) {
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
       const int d = row_of_result(t, q) + e;
-      s[t][e] = p.h0 && mine && d < p.key_dim ? p.h0[at0 + d * int64_t(p.value_dim)] : 0.0f;
+      s[t][e] = p.h0 && mine && !loader && d < p.key_dim ? p.h0[at0 + d * int64_t(p.value_dim)] : 0.0f;
     }
 
-  int64_t slot = span.slot;
-  for (int64_t first = span.first; first < span.end; first += DELTA_CHUNK, ++slot) {
+  auto compute = [&](int64_t c, const char* smem) __attribute__((always_inline)) {
+    const int64_t first = span.first + c * DELTA_CHUNK, block = (span.slot + c) * p.heads + head;
     const int length = int(span.end - first < DELTA_CHUNK ? span.end - first : DELTA_CHUNK);
-    const int64_t block = slot * p.heads + head;
-    __syncthreads();
-    const T* k = head_rows<T>(p.k, p.k_stride, span.batch, first, key_head);
+    const float* gates = reinterpret_cast<const float*>(smem + Sh::GATES);
     const T* qq = head_rows<T>(p.q, p.q_stride, span.batch, first, key_head);
-    stage<T, DK, LANES>(smem + Sh::K, k, p.k_stride[1], length, p.key_dim);
-    if constexpr (Sh::QUERIES) stage<T, DK, LANES>(smem + Sh::Q, qq, p.q_stride[1], length, p.key_dim);
-    stage<T, 16 * WAVES, LANES>(smem + Sh::V, head_rows<T>(p.v, p.v_stride, span.batch, first, head) + c0, p.v_stride[1], length, p.value_dim - c0);
-#pragma unroll
-    for (int k2 = 0; k2 < P; ++k2) {
-      stage_dense<U, 64, LANES, 64>(smem + Sh::M + k2 * TS::BYTES, reinterpret_cast<const U*>(a.m + block * SQUARE) + k2 * 4096);
-      if constexpr (!STATES) stage_dense<U, 64, LANES, 64>(smem + Sh::C + k2 * TS::BYTES, reinterpret_cast<const U*>(a.c + block * SQUARE) + k2 * 4096);
-    }
-    for (int i = threadIdx.x; i < 192; i += LANES) gates[i] = a.gates[block * 192 + i];
-    __syncthreads();
-
     Planes<T> sp[DK / 32];
     float un_s;
     split_scaled<T>(s, sp, &un_s);
@@ -140,12 +164,7 @@ __global__ __launch_bounds__(64 * WAVES) void delta_scan_kernel(DeltaArgs a) {
           } else {
             Frag<T> f;
 #pragma unroll
-            for (int e = 0; e < 8; e += 16 / int(sizeof(T))) {
-              auto part = zero_unit<T>();
-              if (from < length) part = load_unit(qq + from * p.q_stride[1], 32 * b + 8 * q + e, p.key_dim);
-#pragma unroll
-              for (int i = 0; i < 16 / int(sizeof(T)); ++i) f[e + i] = part[i];
-            }
+            for (int e = 0; e < 8; ++e) f[e] = from < length && 32 * b + 8 * q + e < p.key_dim ? qq[from * p.q_stride[1] + 32 * b + 8 * q + e] : T(0.0f);
             y = mma(f, sp[b], y);
           }
         }
@@ -155,9 +174,16 @@ __global__ __launch_bounds__(64 * WAVES) void delta_scan_kernel(DeltaArgs a) {
         for (int e = 0; e < 4; ++e) y[e] *= gamma[e] * un_s * p.scale;
 #pragma unroll
         for (int b = 0; b <= t / 2; ++b) y = mma(square(Sh::C, t, b), np[b], y);
+        T* to = o + row * int64_t(p.heads) * p.value_dim;
+        if (length == DELTA_CHUNK) {
+          if (mine)
 #pragma unroll
-        for (int e = 0; e < 4; ++e)
-          if (mine && row + e < length) o[(row + e) * int64_t(p.heads) * p.value_dim] = T(y[e]);
+            for (int e = 0; e < 4; ++e) to[e * (p.heads * p.value_dim)] = T(y[e]);
+        } else {
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            if (mine && row + e < length) to[e * (p.heads * p.value_dim)] = T(y[e]);
+        }
       }
     }
 #pragma unroll
@@ -178,8 +204,25 @@ __global__ __launch_bounds__(64 * WAVES) void delta_scan_kernel(DeltaArgs a) {
       if constexpr (std::is_same_v<T, _Float16>) s[t] += un_n * added(v4f{0, 0, 0, 0});
       else s[t] = added(s[t]);
     }
+  };
+
+  if constexpr (Sh::LOADERS) {
+    if (loader && chunks > 0) load(0, room);
+    __syncthreads();
+    for (int64_t c = 0; c < chunks; ++c) {
+      if (!loader) compute(c, room + (c & 1) * Sh::BYTES);
+      else if (c + 1 < chunks) load(c + 1, room + (~c & 1) * Sh::BYTES);
+      __syncthreads();
+    }
+  } else {
+    for (int64_t c = 0; c < chunks; ++c) {
+      __syncthreads();
+      load(c, room);
+      __syncthreads();
+      compute(c, room);
+    }
   }
-  if (!STATES && p.state && mine)
+  if (!STATES && p.state && mine && !loader)
 #pragma unroll
     for (int t = 0; t < DK / 16; ++t)
 #pragma unroll

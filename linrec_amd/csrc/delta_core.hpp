@@ -134,59 +134,92 @@ __device__ __forceinline__ void split_scaled(const v4f (&x)[N], Planes<T> (&out)
 }
 
 // A row-major tile of COLS columns in LDS, in units of 16 bytes; a unit's place is changed by its row, so that eight lanes that read
-// a unit of rows 0..3, 8..11 (fragments) and sixteen that read halves of units of four rows (transposed ones) spread over the banks.
+// a unit of rows 0..3, 8..11 (fragments) and sixteen that read 32 bytes of four rows (transposed ones) spread over the banks.
+//
+// What a lane reads lies at its view, a place that depends on the lane alone, up to bits that are flipped and bytes that are added
+// as the tile or the step says: constants, so that all of a kernel's reads share a few registers of addresses.
 template <typename U, int COLS>
 struct Tile {
   static constexpr int ROW = COLS * int(sizeof(U)), UNITS = ROW / 16, BYTES = 64 * ROW;
   static constexpr int MASK = UNITS >= 8 ? 7 : UNITS - 1;
   static constexpr int VEC = 16 / int(sizeof(U));
-  static __device__ __forceinline__ int at(int row, int unit) {
-    const int f = (((row & 1) << 2) | ((row >> 1) & 1) | (((row >> 3) & 1) << 1)) & MASK;
-    return row * ROW + ((unit ^ f) << 4);
-  }
-  static __device__ __forceinline__ float value(const char* tile, int row, int col) {
-    return float(*reinterpret_cast<const U*>(tile + at(row, col / VEC) + (col % VEC) * int(sizeof(U))));
-  }
-  // columns 32 p + 8 q and up of a row
-  static __device__ __forceinline__ Frag<U> frag(const char* tile, int row, int p, int q) {
-    if constexpr (sizeof(U) == 2) {
-      return *reinterpret_cast<const Frag<U>*>(tile + at(row, 4 * p + q));
+  static constexpr bool HALF = sizeof(U) == 2;
+  static_assert(HALF ? UNITS >= 4 : UNITS >= 8, "");
+
+  // (of rows that differ in bits 0, 1 and 3 alone)
+  static __device__ __forceinline__ constexpr int flip(int row) { return (((row & 1) << 2) | (row & 2) | ((row >> 3) & 1)) & MASK; }
+  static __device__ __forceinline__ int at(int row, int unit) { return row * ROW + ((unit ^ flip(row)) << 4); }
+
+  // 32 columns of a row: row r of tile t of 16 rows, or row row_of_tile(t, r)
+  static __device__ __forceinline__ int row_view(int row, int q) { return at(row, HALF ? q : 2 * q); }
+  static __device__ __forceinline__ int natural_rows(int r, int q) { return row_view(r, q); }
+  static __device__ __forceinline__ int mapped_rows(int r, int q) { return row_view(row_of_tile(0, r), q); }
+  static __device__ __forceinline__ constexpr int natural_row(int t) { return 16 * t; }
+  static __device__ __forceinline__ constexpr int mapped_row(int t) { return 32 * (t >> 1) + 4 * (t & 1); }
+  // columns 32 p + 8 q and up
+  static __device__ __forceinline__ Frag<U> frag(const char* tile, int view, int rows, int p) {
+    if constexpr (HALF) {
+      return *reinterpret_cast<const Frag<U>*>(tile + (view ^ ((p & 1) << 6)) + (rows * ROW + (p >> 1) * 128));
     } else {
       Frag<U> f;
-      const v4f a = *reinterpret_cast<const v4f*>(tile + at(row, 8 * p + 2 * q)), b = *reinterpret_cast<const v4f*>(tile + at(row, 8 * p + 2 * q + 1));
+      const v4f a = *reinterpret_cast<const v4f*>(tile + view + (rows * ROW + p * 128));
+      const v4f b = *reinterpret_cast<const v4f*>(tile + (view ^ 16) + (rows * ROW + p * 128));
 #pragma unroll
       for (int e = 0; e < 4; ++e) f[e] = a[e], f[4 + e] = b[e];
       return f;
     }
   }
-  // four rows from `row` of the column that is this lane's (r = lane % 16) of the 16 columns that start at col(0), col(1), col(2),
-  // col(3), four each
-  template <typename F>
-  static __device__ __forceinline__ typename Pack<U, 4>::type column4(const char* tile, int row, F&& col) {
-    const int r = threadIdx.x & 15;
+
+  // Four rows of a column: lane 16 q + r has rows 8 q and up of column r of a tile of 16 columns, those as they are (natural) or
+  // 32 (t / 2) + 8 (r / 4) + 4 (t % 2) + r % 4 (mapped).
+  template <bool MAPPED>
+  static __device__ __forceinline__ int columns(int r, int q) {
+    const int j = HALF ? r & 3 : r >> 2;
+    if constexpr (HALF) return at(8 * q + (r >> 2), MAPPED ? j : j >> 1) + (MAPPED ? 0 : (j & 1) * 8);
+    else return at(8 * q, MAPPED ? 2 * j : j) + (r & 3) * 4;
+  }
+  template <bool MAPPED>
+  static __device__ __forceinline__ int column_tile(int view, int t) {
+    if constexpr (HALF) return MAPPED ? (view ^ (((t >> 1) & 1) << 6)) + ((t >> 2) * 128 + (t & 1) * 8) : (view ^ ((t & 3) << 5)) + (t >> 2) * 128;
+    else return (view ^ (MAPPED ? (t & 1) << 4 : (t & 1) << 6)) + (t >> 1) * 128;
+  }
+  template <bool MAPPED>
+  static __device__ __forceinline__ typename Pack<U, 4>::type column4(const char* tile, int view, int rows, int t) {
     typename Pack<U, 4>::type out;
-    if constexpr (sizeof(U) == 2) {
+    if constexpr (HALF) {
       typedef short s4 __attribute__((ext_vector_type(4)));
       typedef __attribute__((address_space(3))) s4* lds_t;
-      const int from = row + (r >> 2), c = col(r & 3);
-      const s4 raw = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_t)(tile + at(from, c / VEC) + (c % VEC) * 2));
+      const s4 raw = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_t)(tile + column_tile<MAPPED>(view, t) + rows * ROW));
       __builtin_memcpy(&out, &raw, 8);
     } else {
-      const int c = col(r >> 2) + (r & 3);
 #pragma unroll
-      for (int e = 0; e < 4; ++e) out[e] = *reinterpret_cast<const U*>(tile + at(row + e, c / VEC) + (c % VEC) * 4);
+      for (int e = 0; e < 4; ++e) out[e] = *reinterpret_cast<const U*>(tile + column_tile<MAPPED>(view ^ (flip(e) << 4), t) + (rows + e) * ROW);
     }
     return out;
   }
-  template <typename F>
-  static __device__ __forceinline__ Frag<U> column_frag(const char* tile, int p, int q, F&& col) {
-    const auto a = column4(tile, 32 * p + 8 * q, col), b = column4(tile, 32 * p + 8 * q + 4, col);
+  // rows 32 p + 8 q and up
+  template <bool MAPPED>
+  static __device__ __forceinline__ Frag<U> column_frag(const char* tile, int view, int p, int t) {
+    const auto a = column4<MAPPED>(tile, view, 32 * p, t), b = column4<MAPPED>(tile, view, 32 * p + 4, t);
     Frag<U> f;
 #pragma unroll
     for (int e = 0; e < 4; ++e) f[e] = a[e], f[4 + e] = b[e];
     return f;
   }
+
+  // a result's values: rows 4 q and up of column r of a tile of 16 columns
+  static __device__ __forceinline__ int points(int r, int q) { return at(4 * q, r / VEC) + r % VEC * int(sizeof(U)); }
+  static __device__ __forceinline__ float point(const char* tile, int view, int rows, int e, int t) {
+    const int at = (view ^ (flip(e) << 4) ^ (HALF ? (t & 3) << 5 : (t & 1) << 6)) + ((HALF ? t >> 2 : t >> 1) * 128);
+    return float(*reinterpret_cast<const U*>(tile + at + (rows + e) * ROW));
+  }
 };
+
+// A view that a loop's body starts from anew: the places made from it are not all kept in registers outside.
+__device__ __forceinline__ int anew(int view) {
+  asm volatile("" : "+v"(view));
+  return view;
+}
 
 // ROWS rows of COLS columns on their way from memory to a tile, by LANES lanes of which this is number `lane`: all loads first, so that
 // their latencies are one, and stores to LDS when they are due.

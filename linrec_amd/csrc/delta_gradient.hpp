@@ -3,18 +3,22 @@
 //   F_ij = scale e^{G_i - G_j} dO_i.N_j (i >= j)      E_ij = -e^{G_i - G_j} dB_i.N_j (i > j)
 //   dQ = scale e^G dO S^T + F K
 //   X  = E K - e^G dB S^T,  Z = e^{G_63 - G} N dS'^T,  Y = Z + F^T Q + E^T (beta K);      dK = beta X + Y
-//   dbeta = dB.V + K.X      dG = Q.dQ + beta K.X - K.Y  (row by row),   dG_63 += sum K.Z + e^{G_63} <S, dS'>
+//   dbeta = dB.V + K.X,  dG = Q.dQ + beta K.X - K.Y (row by row),  dG_63 += sum K.Z + e^{G_63} <S, dS'>
 //
 // and the gradient of log_decay is the sum of dG from a position to the chunk's end.
 //
-// A workgroup has a (chunk, key head) and walks over the value heads that share it, so that nothing is added by atomics; a wave has
-// 16 rows of dQ and dK.  Value channels come 32 at a time through LDS.  The four 64 x 64 products F, F^T, E, E^T are computed as they
-// are needed as operands: what a lane gets of a product is its part of an operand over the product's rows.
+// A workgroup has a (chunk, key head) and walks over the value heads that share it, so that nothing is added by atomics.  Value
+// channels come 32 at a time through LDS, the next ones on their way in registers meanwhile.  Its waves have three parts, four waves
+// of 16 rows each: dQ, X and Y.  (One wave for all three holds twice the registers that three waves to a SIMD leave it, and what
+// then goes through scratch costs more than the products: 2.4 ms instead of the time below.)  The 64 x 64 products F, F^T, E, E^T are
+// computed as they are needed as operands: what a lane gets of a product is its part of an operand over the product's rows.
 #pragma once
 #include "delta_prepare.hpp"
 #include "delta_scan.hpp"
 
 namespace linrec {
+
+constexpr int GRADIENT_LANES = 768, GRADIENT_PART = 256;
 
 template <typename T, int DK>
 struct GradientShared {
@@ -22,9 +26,11 @@ struct GradientShared {
   static constexpr int P = planes_of<U>(), IN = input_planes<T>();
   static constexpr int IN_V = 64 * 32 * int(sizeof(U)), BY_V = 32 * 64 * int(sizeof(U)), STATE = 32 * DK * int(sizeof(U)),
                        KEYS = Tile<U, DK>::BYTES;
-  static constexpr int O = 0, V = O + IN * IN_V, B = V + IN * IN_V, N = B + P * BY_V, S = N + P * BY_V, D = S + P * STATE, FIRST = D + P * STATE;
-  static constexpr int K = 0, Q = K + IN * KEYS, SECOND = Q + IN * KEYS;
-  static constexpr int BYTES = FIRST > SECOND ? FIRST : SECOND;
+  // one step's values, then both inputs of key channels
+  static constexpr int O = 0, V = O + IN * IN_V, B = V + IN * IN_V, N = B + P * BY_V, S = N + P * BY_V, D = S + P * STATE, STEP = D + P * STATE;
+  static constexpr int BUFFERS = 2 * STEP + 2 * IN * KEYS + 4096 <= 160 * 1024 ? 2 : 1;
+  static constexpr int K = BUFFERS * STEP, Q = K + IN * KEYS, BYTES = Q + IN * KEYS;
+  static_assert(64 * DK * 4 <= BUFFERS * STEP, "room to hand dK over");
 };
 
 // COLS columns of 64 rows of an input on their way to IN tiles of the inner type.
@@ -32,10 +38,13 @@ template <typename T, int COLS, int LANES>
 struct InputStager {
   using U = Inner<T>;
   Stager<T, COLS, LANES> s;
-  __device__ __forceinline__ void fetch(const T* from, int64_t stride, int rows, int cols) { s.fetch(from, stride, rows, cols, threadIdx.x); }
+  __device__ __forceinline__ void fetch(const T* from, int64_t stride, int rows, int cols) {
+    s.fetch(from, stride, rows, cols, threadIdx.x & (LANES - 1));
+  }
   __device__ __forceinline__ void put(char* tile) const {
+    const int lane = threadIdx.x & (LANES - 1);
     if constexpr (std::is_same_v<T, U>) {
-      s.put(tile, threadIdx.x);
+      s.put(tile, lane);
     } else {  // fp16 as two bf16
       Stager<U, COLS, LANES> hi, lo;
 #pragma unroll
@@ -45,8 +54,8 @@ struct InputStager {
           hi.v[n][e] = U(float(s.v[n][e]));
           lo.v[n][e] = U(float(s.v[n][e]) - float(hi.v[n][e]));
         }
-      hi.put(tile, threadIdx.x);
-      lo.put(tile + 64 * Tile<U, COLS>::ROW, threadIdx.x);
+      hi.put(tile, lane);
+      lo.put(tile + 64 * Tile<U, COLS>::ROW, lane);
     }
   }
 };
@@ -58,280 +67,322 @@ __device__ __forceinline__ float sum_of_16(float x) {
   return x + __shfl_xor(x, 8);
 }
 
-// DK: columns of dQ and dK at a time; WIDE: key_dim is more than that and they come in turns.
-template <typename T, int DK, bool WIDE>
-__global__ __launch_bounds__(256) void delta_gradient_kernel(DeltaArgs a) {
+enum GradientPart { GRADIENT_Q, GRADIENT_X, GRADIENT_Y };
+
+template <typename T, int DK>
+struct GradientScratch {  // LDS beside GradientShared
+  double g[64];
+  alignas(16) float gamma[64], rest[64], beta[64], q[64], x[64], y[64], bv[64], sum[8];
+};
+
+// What the waves of one part do.  All parts meet at the same barriers.
+template <typename T, int DK, bool WIDE, GradientPart PART>
+__device__ __forceinline__ void gradient_part(const DeltaArgs& a, const Chunk& ch, int64_t slot, int key_head, char* smem, GradientScratch<T, DK>& sh) {
   using U = Inner<T>;
   using Sh = GradientShared<T, DK>;
   using TI = Tile<U, 32>;  // dO, V
   using TB = Tile<U, 64>;  // dB, N: rows are channels
   using TK = Tile<U, DK>;  // K, Q; S, dS': rows are channels
-  constexpr int P = Sh::P, IN = Sh::IN, KT = DK / 16;
+  constexpr int P = Sh::P, IN = Sh::IN, KT = DK / 16, LANES = GRADIENT_PART;
   constexpr int64_t ROW = WIDE ? 2 * DK : DK;  // of the kept states
-  __shared__ __align__(16) char smem[Sh::BYTES];
-  __shared__ double sh_g[64];
-  __shared__ float sh_gamma[64], sh_rest[64], sh_beta[64], sh_total[64], sh_sum[4];
   const linrec_delta_t& p = a.p;
-  const int64_t slot = blockIdx.x / unsigned(p.key_heads);
-  const int key_head = int(blockIdx.x - slot * unsigned(p.key_heads));
-  const Chunk ch = chunk_of(p, slot);
-  if (ch.length == 0) return;
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r = lane & 15, q = lane >> 4;
+  const int lane = threadIdx.x & 63, r = lane & 15, q = lane >> 4, by = threadIdx.x & (LANES - 1);
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) & 3;
   const int row0 = 16 * wave + 4 * q;  // this lane's rows of a result
-  auto natural = [&](int t) { return [t](int j) { return 16 * t + 4 * j; }; };
-  auto mapped = [&](int t) { return [t](int j) { return row_of_result(t, j); }; };
+  const int rows_w0 = TI::natural_rows(r, q) + wave * (16 * TI::ROW), rows_m0 = TI::mapped_rows(r, q);
+  const int cols_w0 = TB::template column_tile<false>(TB::template columns<false>(r, q), wave), cols_m0 = TB::template columns<true>(r, q);
+  const int cols_k0 = TK::template columns<false>(r, q), rows_v0 = TK::natural_rows(r, q) + (wave & 1) * (16 * TK::ROW),
+            points0 = TK::points(r, q) + wave * (16 * TK::ROW);
+
+  // each part loads some of a step: the rows of dO and V with dB and N, S, dS'
+  InputStager<T, 32, LANES> so, sv;
+  Stager<U, 64, LANES, 32> sb[P], sn[P];
+  Stager<U, DK, LANES, 32> ss[P];
+  auto fetch = [&](int head, int v0, int d0) __attribute__((always_inline)) {
+    const int64_t block = slot * p.heads + head;
+    if constexpr (PART == GRADIENT_Q) {
+      so.fetch(head_rows<T>(p.d_o, p.d_o_stride, ch.batch, ch.first, head) + v0, p.d_o_stride[1], ch.length, p.value_dim - v0);
+      sv.fetch(head_rows<T>(p.v, p.v_stride, ch.batch, ch.first, head) + v0, p.v_stride[1], ch.length, p.value_dim - v0);
+    }
+#pragma unroll
+    for (int k = 0; k < P; ++k) {
+      const int64_t row = (block * P + k) * a.columns + v0;
+      if constexpr (PART == GRADIENT_Q) {
+        sb[k].fetch_dense(reinterpret_cast<const U*>(a.d_b) + row * 64, by);
+        sn[k].fetch_dense(reinterpret_cast<const U*>(a.n) + row * 64, by);
+      } else {
+        const U* from = reinterpret_cast<const U*>(PART == GRADIENT_X ? a.s : a.d_s) + row * ROW;
+        if constexpr (WIDE) ss[k].fetch(from + d0, ROW, 32, DK, by);
+        else ss[k].fetch_dense(from, by);
+      }
+    }
+  };
+  auto put = [&](char* to) __attribute__((always_inline)) {
+    if constexpr (PART == GRADIENT_Q) {
+      so.put(to + Sh::O);
+      sv.put(to + Sh::V);
+    }
+#pragma unroll
+    for (int k = 0; k < P; ++k) {
+      if constexpr (PART == GRADIENT_Q) {
+        sb[k].put(to + Sh::B + k * Sh::BY_V, by);
+        sn[k].put(to + Sh::N + k * Sh::BY_V, by);
+      } else {
+        ss[k].put(to + (PART == GRADIENT_X ? Sh::S : Sh::D) + k * Sh::STATE, by);
+      }
+    }
+  };
 
   for (int d0 = 0; d0 < (WIDE ? p.key_dim : 1); d0 += DK) {
-    v4f dq_all[KT], dk_all[KT];
+    v4f all[KT];  // this part's share of dQ or dK over the value heads
 #pragma unroll
-    for (int u = 0; u < KT; ++u) dq_all[u] = v4f{0, 0, 0, 0}, dk_all[u] = v4f{0, 0, 0, 0};
+    for (int u = 0; u < KT; ++u) all[u] = v4f{0, 0, 0, 0};
+    {
+      InputStager<T, DK, LANES> keys;
+      if constexpr (PART == GRADIENT_X)
+        keys.fetch(head_rows<T>(p.k, p.k_stride, ch.batch, ch.first, key_head) + d0, p.k_stride[1], ch.length, p.key_dim - d0);
+      if constexpr (PART == GRADIENT_Y)
+        keys.fetch(head_rows<T>(p.q, p.q_stride, ch.batch, ch.first, key_head) + d0, p.q_stride[1], ch.length, p.key_dim - d0);
+      fetch(key_head * a.shared, 0, d0);
+      __syncthreads();
+      if constexpr (PART != GRADIENT_Q) keys.put(smem + (PART == GRADIENT_X ? Sh::K : Sh::Q));
+    }
+    int turn = 0;
     for (int h = 0; h < a.shared; ++h) {
       const int head = key_head * a.shared + h;
       const int64_t block = slot * p.heads + head;
-      __syncthreads();
-      if (wave == 0) {
+      // (of the head before, these are read before the last barrier, or by the wave that writes them)
+      if (threadIdx.x < 64) {
         const bool there = lane < ch.length;
         const float g = there ? *(head_rows<float>(p.log_decay, p.log_decay_stride, ch.batch, ch.first + lane, head)) : 0.0f;
-        sh_g[lane] = chunk_sum(g, lane);
-        sh_gamma[lane] = a.gates[block * 192 + lane];
-        sh_rest[lane] = a.gates[block * 192 + 64 + lane];
-        sh_beta[lane] = a.gates[block * 192 + 128 + lane];
+        sh.g[lane] = chunk_sum(g, lane);
+        sh.gamma[lane] = a.gates[block * 192 + lane];
+        sh.rest[lane] = a.gates[block * 192 + 64 + lane];
+        sh.beta[lane] = a.gates[block * 192 + 128 + lane];
       }
-      v4f f[4], ft[4], ee[4], et[4], dq[KT], x[KT], y[KT], bv = v4f{0, 0, 0, 0}, inner = v4f{0, 0, 0, 0};
+      // F^T, dQ; E^T, X; F, E, Y
+      v4f f[4], ee[4], acc[KT], bv = v4f{0, 0, 0, 0}, inner = v4f{0, 0, 0, 0};
 #pragma unroll
-      for (int t = 0; t < 4; ++t) f[t] = ft[t] = ee[t] = et[t] = v4f{0, 0, 0, 0};
+      for (int t = 0; t < 4; ++t) f[t] = ee[t] = v4f{0, 0, 0, 0};
 #pragma unroll
-      for (int u = 0; u < KT; ++u) dq[u] = x[u] = y[u] = v4f{0, 0, 0, 0};
-      const T* d_o = head_rows<T>(p.d_o, p.d_o_stride, ch.batch, ch.first, head);
-      const T* v = head_rows<T>(p.v, p.v_stride, ch.batch, ch.first, head);
+      for (int u = 0; u < KT; ++u) acc[u] = v4f{0, 0, 0, 0};
       for (int v0 = 0; v0 < p.value_dim; v0 += 32) {
+        char* at = smem + (Sh::BUFFERS == 2 ? turn * Sh::STEP : 0);
+        if constexpr (Sh::BUFFERS == 1) __syncthreads();
+        put(at);
         __syncthreads();
-        {
-          InputStager<T, 32, 256> so, sv;
-          Stager<U, 64, 256, 32> sb[P], sn[P];
-          Stager<U, DK, 256, 32> ss[P], sd[P];
-          so.fetch(d_o + v0, p.d_o_stride[1], ch.length, p.value_dim - v0);
-          sv.fetch(v + v0, p.v_stride[1], ch.length, p.value_dim - v0);
-#pragma unroll
-          for (int k = 0; k < P; ++k) {
-            const int64_t row = (block * P + k) * a.columns + v0;
-            sb[k].fetch_dense(reinterpret_cast<const U*>(a.d_b) + row * 64, threadIdx.x);
-            sn[k].fetch_dense(reinterpret_cast<const U*>(a.n) + row * 64, threadIdx.x);
-            ss[k].fetch(reinterpret_cast<const U*>(a.s) + row * ROW + d0, ROW, 32, DK, threadIdx.x);
-            sd[k].fetch(reinterpret_cast<const U*>(a.d_s) + row * ROW + d0, ROW, 32, DK, threadIdx.x);
-          }
-          so.put(smem + Sh::O);
-          sv.put(smem + Sh::V);
-#pragma unroll
-          for (int k = 0; k < P; ++k) {
-            sb[k].put(smem + Sh::B + k * Sh::BY_V, threadIdx.x);
-            sn[k].put(smem + Sh::N + k * Sh::BY_V, threadIdx.x);
-            ss[k].put(smem + Sh::S + k * Sh::STATE, threadIdx.x);
-            sd[k].put(smem + Sh::D + k * Sh::STATE, threadIdx.x);
-          }
-        }
-        __syncthreads();
-        auto rows_in = [&](int at, int row) __attribute__((always_inline)) {
+        if (v0 + 32 < p.value_dim) fetch(head, v0 + 32, d0);
+        else if (h + 1 < a.shared) fetch(head + 1, 0, d0);
+        turn ^= 1;
+        const int rows_w = anew(rows_w0), rows_m = anew(rows_m0), cols_w = anew(cols_w0), cols_m = anew(cols_m0), cols_k = anew(cols_k0),
+                  rows_v = anew(rows_v0);
+        auto rows_in = [&](int part, int view, int row) __attribute__((always_inline)) {
           Planes<U, IN> out;
 #pragma unroll
-          for (int k = 0; k < IN; ++k) out.p[k] = TI::frag(smem + at + k * Sh::IN_V, row, 0, q);
+          for (int k = 0; k < IN; ++k) out.p[k] = TI::frag(at + part + k * Sh::IN_V, view, row, 0);
           return out;
         };
-        auto by_v = [&](int at, auto col) __attribute__((always_inline)) {
+        auto by_v = [&](int part) __attribute__((always_inline)) {  // this wave's rows
           Planes<U> out;
 #pragma unroll
-          for (int k = 0; k < P; ++k) out.p[k] = TB::column_frag(smem + at + k * Sh::BY_V, 0, q, col);
+          for (int k = 0; k < P; ++k) out.p[k] = TB::template column_frag<false>(at + part + k * Sh::BY_V, cols_w, 0, 0);
           return out;
         };
-        auto state = [&](int at, auto col) __attribute__((always_inline)) {
+        auto by_v_mapped = [&](int part, int t) __attribute__((always_inline)) {
           Planes<U> out;
 #pragma unroll
-          for (int k = 0; k < P; ++k) out.p[k] = TK::column_frag(smem + at + k * Sh::STATE, 0, q, col);
+          for (int k = 0; k < P; ++k) out.p[k] = TB::template column_frag<true>(at + part + k * Sh::BY_V, cols_m, 0, t);
           return out;
         };
-        const Planes<U, IN> do_w = rows_in(Sh::O, 16 * wave + r), v_w = rows_in(Sh::V, 16 * wave + r);
-        const Planes<U> db_w = by_v(Sh::B, natural(wave)), n_w = by_v(Sh::N, natural(wave));
-        bv = mma(db_w, v_w, bv);
+        auto state = [&](int part, int u) __attribute__((always_inline)) {
+          Planes<U> out;
 #pragma unroll
-        for (int t = 0; t < 4; ++t) {
-          if (t / 2 <= wave / 2) {  // rows j of F^T and E^T up to this wave's columns i
-            const Planes<U> n_t = by_v(Sh::N, mapped(t));
-            ft[t] = mma(n_t, do_w, ft[t]);
-            et[t] = mma(n_t, db_w, et[t]);
-          }
-          if (t / 2 >= wave / 2) {
-            f[t] = mma(rows_in(Sh::O, row_of_tile(t, r)), n_w, f[t]);
-            ee[t] = mma(by_v(Sh::B, mapped(t)), n_w, ee[t]);
-          }
-        }
+          for (int k = 0; k < P; ++k) out.p[k] = TK::template column_frag<false>(at + part + k * Sh::STATE, cols_k, 0, u);
+          return out;
+        };
+        if constexpr (PART == GRADIENT_Q) {
+          const Planes<U, IN> do_w = rows_in(Sh::O, rows_w, 0);
 #pragma unroll
-        for (int u = 0; u < KT; ++u) {
-          const Planes<U> s_u = state(Sh::S, natural(u));
-          dq[u] = mma(do_w, s_u, dq[u]);
-          x[u] = mma(db_w, s_u, x[u]);
-          y[u] = mma(n_w, state(Sh::D, natural(u)), y[u]);
-        }
-        // <S, dS'> on the diagonal of S^T dS', 16 channels at a time
-        {
-          const int row = 16 * (wave & 1) + r;
+          for (int t = 0; t < 4; ++t)
+            if (t / 2 <= wave / 2) f[t] = mma(by_v_mapped(Sh::N, t), do_w, f[t]);  // rows j up to this wave's columns i
+#pragma unroll
+          for (int u = 0; u < KT; ++u) acc[u] = mma(do_w, state(Sh::S, u), acc[u]);
+        } else if constexpr (PART == GRADIENT_X) {
+          const Planes<U> db_w = by_v(Sh::B);
+#pragma unroll
+          for (int t = 0; t < 4; ++t)
+            if (t / 2 <= wave / 2) ee[t] = mma(by_v_mapped(Sh::N, t), db_w, ee[t]);
+#pragma unroll
+          for (int u = 0; u < KT; ++u) acc[u] = mma(db_w, state(Sh::S, u), acc[u]);
+          bv = mma(db_w, rows_in(Sh::V, rows_w, 0), bv);
+          // <S, dS'> on the diagonal of S^T dS', 16 channels at a time
 #pragma unroll
           for (int b = 0; b < DK / 32; ++b)
             if ((b & 1) == wave >> 1) {
               Planes<U> s_v, d_v;
 #pragma unroll
               for (int k = 0; k < P; ++k) {
-                s_v.p[k] = TK::frag(smem + Sh::S + k * Sh::STATE, row, b, q);
-                d_v.p[k] = TK::frag(smem + Sh::D + k * Sh::STATE, row, b, q);
+                s_v.p[k] = TK::frag(at + Sh::S + k * Sh::STATE, rows_v, 0, b);
+                d_v.p[k] = TK::frag(at + Sh::D + k * Sh::STATE, rows_v, 0, b);
               }
               inner = mma(s_v, d_v, inner);
             }
+        } else {
+          const Planes<U> n_w = by_v(Sh::N);
+#pragma unroll
+          for (int t = 0; t < 4; ++t)
+            if (t / 2 >= wave / 2) {
+              f[t] = mma(rows_in(Sh::O, rows_m, TI::mapped_row(t)), n_w, f[t]);
+              ee[t] = mma(by_v_mapped(Sh::B, t), n_w, ee[t]);
+            }
+#pragma unroll
+          for (int u = 0; u < KT; ++u) acc[u] = mma(n_w, state(Sh::D, u), acc[u]);
         }
       }
+      const int cols_k = anew(cols_k0), points = anew(points0);
       // the masks and decays; rows of results to operands
-      Planes<U> fp[2], ftp[2], ep[2], etp[2];
+      Planes<U> fp[2], ep[2];
       {
         const int own = 16 * wave + r;
 #pragma unroll
         for (int t = 0; t < 4; ++t)
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
-            const int i = row_of_result(t, q) + e;
-            const float down = i >= own ? expf(float(sh_g[i] - sh_g[own])) : 0.0f;  // i after this lane's column
-            const float up = own >= i ? expf(float(sh_g[own] - sh_g[i])) : 0.0f;
-            f[t][e] = i >= own ? p.scale * down * f[t][e] : 0.0f;
-            ee[t][e] = i > own ? -sh_beta[i] * down * ee[t][e] : 0.0f;
-            ft[t][e] = own >= i ? p.scale * up * ft[t][e] : 0.0f;
-            et[t][e] = own > i ? -up * et[t][e] : 0.0f;
+            const int other = row_of_result(t, q) + e, i = PART == GRADIENT_Y ? other : own, j = PART == GRADIENT_Y ? own : other;
+            const float d = i >= j ? expf(float(sh.g[i] - sh.g[j])) : 0.0f;
+            if constexpr (PART != GRADIENT_X) f[t][e] = i >= j ? p.scale * d * f[t][e] : 0.0f;
+            if constexpr (PART != GRADIENT_Q) ee[t][e] = i > j ? -(PART == GRADIENT_Y ? sh.beta[i] : 1.0f) * d * ee[t][e] : 0.0f;
           }
 #pragma unroll
         for (int b = 0; b < 2; ++b) {
-          fp[b] = split<U>(f[2 * b], f[2 * b + 1]);
-          ftp[b] = split<U>(ft[2 * b], ft[2 * b + 1]);
-          ep[b] = split<U>(ee[2 * b], ee[2 * b + 1]);
-          etp[b] = split<U>(et[2 * b], et[2 * b + 1]);
+          if constexpr (PART != GRADIENT_X) fp[b] = split<U>(f[2 * b], f[2 * b + 1]);
+          if constexpr (PART != GRADIENT_Q) ep[b] = split<U>(ee[2 * b], ee[2 * b + 1]);
         }
       }
-      __syncthreads();
-      const T* k_rows = head_rows<T>(p.k, p.k_stride, ch.batch, ch.first, key_head) + d0;
-      const T* q_rows = head_rows<T>(p.q, p.q_stride, ch.batch, ch.first, key_head) + d0;
-      {
-        InputStager<T, DK, 256> sk, sq;
-        sk.fetch(k_rows, p.k_stride[1], ch.length, p.key_dim - d0);
-        sq.fetch(q_rows, p.q_stride[1], ch.length, p.key_dim - d0);
-        sk.put(smem + Sh::K);
-        sq.put(smem + Sh::Q);
-      }
-      __syncthreads();
-      float dot_q[4], dot_x[4], dot_y[4], dot_z[4];
+      auto keys = [&](int part, int b, int u) __attribute__((always_inline)) {
+        Planes<U, IN> out;
 #pragma unroll
-      for (int e = 0; e < 4; ++e) dot_q[e] = dot_x[e] = dot_y[e] = dot_z[e] = 0.0f;
-      const v4f gamma = *reinterpret_cast<const v4f*>(sh_gamma + row0), rest = *reinterpret_cast<const v4f*>(sh_rest + row0),
-                beta = *reinterpret_cast<const v4f*>(sh_beta + row0);
-#pragma unroll
-      for (int u = 0; u < KT; ++u) {
-        v4f kv = v4f{0, 0, 0, 0}, qv = v4f{0, 0, 0, 0};
+        for (int k = 0; k < IN; ++k) out.p[k] = TK::template column_frag<false>(smem + part + k * Sh::KEYS, cols_k, b, u);
+        return out;
+      };
+      auto values = [&](int part, int u) __attribute__((always_inline)) {
+        v4f out = v4f{0, 0, 0, 0};
 #pragma unroll
         for (int k = 0; k < IN; ++k)
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            kv[e] += TK::value(smem + Sh::K + k * Sh::KEYS, row0 + e, 16 * u + r);
-            qv[e] += TK::value(smem + Sh::Q + k * Sh::KEYS, row0 + e, 16 * u + r);
-          }
-        v4f dqu = dq[u] * gamma * p.scale, xu = -gamma * x[u], yu = rest * y[u];
+          for (int e = 0; e < 4; ++e) out[e] += TK::point(smem + part + k * Sh::KEYS, points, 0, e, u);
+        return out;
+      };
+      v4f dot = v4f{0, 0, 0, 0}, ends = v4f{0, 0, 0, 0};
+      v4f rows = *reinterpret_cast<const v4f*>((PART == GRADIENT_Y ? sh.rest : sh.gamma) + row0);
+      if constexpr (PART == GRADIENT_Q) rows *= p.scale;
+      if constexpr (PART == GRADIENT_X) rows = -rows;
+      const v4f beta = *reinterpret_cast<const v4f*>(sh.beta + row0);
 #pragma unroll
-        for (int e = 0; e < 4; ++e) dot_z[e] = fmaf(kv[e], yu[e], dot_z[e]);
+      for (int u = 0; u < KT; ++u) {
+        v4f z = rows * acc[u];
+        const v4f x = values(PART == GRADIENT_Q ? Sh::Q : Sh::K, u);
+        if constexpr (PART == GRADIENT_Y) ends += x * z;
 #pragma unroll
         for (int b = 0; b < 2; ++b) {
-          Planes<U, IN> k_b, q_b;
-#pragma unroll
-          for (int k = 0; k < IN; ++k) {
-            k_b.p[k] = TK::column_frag(smem + Sh::K + k * Sh::KEYS, b, q, natural(u));
-            q_b.p[k] = TK::column_frag(smem + Sh::Q + k * Sh::KEYS, b, q, natural(u));
-          }
-          if (b <= wave / 2) {
-            dqu = mma(ftp[b], k_b, dqu);
-            xu = mma(etp[b], k_b, xu);
-          }
-          if (b >= wave / 2) {
-            yu = mma(fp[b], q_b, yu);
-            yu = mma(ep[b], k_b, yu);
+          if constexpr (PART == GRADIENT_Q) {
+            if (b <= wave / 2) z = mma(fp[b], keys(Sh::K, b, u), z);
+          } else if constexpr (PART == GRADIENT_X) {
+            if (b <= wave / 2) z = mma(ep[b], keys(Sh::K, b, u), z);
+          } else if (b >= wave / 2) {
+            z = mma(fp[b], keys(Sh::Q, b, u), z);
+            z = mma(ep[b], keys(Sh::K, b, u), z);
           }
         }
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          dot_q[e] = fmaf(qv[e], dqu[e], dot_q[e]);
-          dot_x[e] = fmaf(kv[e], xu[e], dot_x[e]);
-          dot_y[e] = fmaf(kv[e], yu[e], dot_y[e]);
-        }
-        dq_all[u] += dqu;
-        dk_all[u] += beta * xu + yu;
+        dot += x * z;
+        if constexpr (PART == GRADIENT_X) z *= beta;
+        all[u] += z;
       }
-      float z = 0.0f;
-      float* dots = a.dots + block * 192;  // (every place is written and read by one lane)
+      float* to = PART == GRADIENT_Q ? sh.q : PART == GRADIENT_X ? sh.x : sh.y;
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        const float qq = sum_of_16(dot_q[e]), xx = sum_of_16(dot_x[e]), yy = sum_of_16(dot_y[e]);
-        z += sum_of_16(dot_z[e]);
-        // dB.V stands on the diagonal of a product, lane 16 q + 4 q + e
-        const float own = __shfl(bv[e], 16 * q + 4 * q + e);
-        float total = qq + beta[e] * xx - yy, d_beta = xx;
-        if (r == 0) {
-          if (WIDE && d0 > 0) {
-            total += dots[row0 + e];
-            d_beta += dots[64 + row0 + e];
-          } else {
-            d_beta += own;
-          }
-          if (WIDE && d0 + DK < p.key_dim) {
-            dots[row0 + e] = total;
-            dots[64 + row0 + e] = d_beta;
-          } else if (row0 + e < ch.length) {
-            p.d_beta[((ch.batch * p.time + ch.first + row0 + e) * p.heads) + head] = d_beta;
-          }
-          sh_total[row0 + e] = total;
-        }
+        const float d = sum_of_16(dot[e]);
+        if (r == 0) to[row0 + e] = d;
       }
-      // z of four rows in every lane of a group of 16; <S, dS'> on diagonals
-      float sum = r == 0 ? z : 0.0f;
+      if constexpr (PART == GRADIENT_X) {
+        // dB.V and <S, dS'> stand on diagonals, lane 16 q + 4 q + e
 #pragma unroll
-      for (int e = 0; e < 4; ++e)
-        if (r == 4 * q + e) sum = fmaf(sh_gamma[63], inner[e], sum);
-      sum = sum_of_16(sum);
-      sum += __shfl_xor(sum, 16);
-      sum += __shfl_xor(sum, 32);
-      if (lane == 0) sh_sum[wave] = sum;
+        for (int e = 0; e < 4; ++e)
+          if (r == 4 * q + e) {
+            sh.bv[row0 + e] = bv[e];
+            ends[0] = sh.gamma[63] * inner[e];
+          }
+      }
+      if constexpr (PART != GRADIENT_Q) {
+        float sum = sum_of_16((ends[0] + ends[1]) + (ends[2] + ends[3]));
+        sum += __shfl_xor(sum, 16);
+        sum += __shfl_xor(sum, 32);
+        if (lane == 0) sh.sum[PART == GRADIENT_X ? wave : 4 + wave] = sum;
+      }
       __syncthreads();
-      if (wave == 0) {
-        double total = double(sh_total[lane]);
-        if (lane == 63) {
-          float ends = (sh_sum[0] + sh_sum[1]) + (sh_sum[2] + sh_sum[3]);
-          if (WIDE && d0 > 0) ends += dots[128];
-          if (WIDE && d0 + DK < p.key_dim) dots[128] = ends;
-          total += double(ends);
+      if (threadIdx.x < 64) {  // a lane for a position
+        float* dots = a.dots + block * 192;  // (every place is written and read by one lane)
+        float total = sh.q[lane] + sh.beta[lane] * sh.x[lane] - sh.y[lane], d_beta = sh.x[lane] + (d0 == 0 ? sh.bv[lane] : 0.0f);
+        if (lane == 63) total += ((sh.sum[0] + sh.sum[1]) + (sh.sum[2] + sh.sum[3])) + ((sh.sum[4] + sh.sum[5]) + (sh.sum[6] + sh.sum[7]));
+        if (WIDE && d0 > 0) {
+          total += dots[lane];
+          d_beta += dots[64 + lane];
         }
-        if (!WIDE || d0 + DK >= p.key_dim) {
+        if (WIDE && d0 + DK < p.key_dim) {
+          dots[lane] = total;
+          dots[64 + lane] = d_beta;
+        } else {
+          double after = double(total);
 #pragma unroll
           for (int d = 1; d < 64; d <<= 1) {
-            const double up = __shfl_down(total, d);
-            if (lane + d < 64) total += up;
+            const double up = __shfl_down(after, d);
+            if (lane + d < 64) after += up;
           }
-          if (lane < ch.length) p.d_log_decay[((ch.batch * p.time + ch.first + lane) * p.heads) + head] = float(total);
+          if (lane < ch.length) {
+            const int64_t at = (ch.batch * p.time + ch.first + lane) * p.heads + head;
+            p.d_log_decay[at] = float(after);
+            p.d_beta[at] = d_beta;
+          }
         }
       }
     }
-    // what the value heads' shares add up to
+    // the two shares of dK together
+    __syncthreads();
+    float* sh_k = reinterpret_cast<float*>(smem);
+    if constexpr (PART == GRADIENT_Y)
 #pragma unroll
-    for (int e = 0; e < 4; ++e)
-      if (row0 + e < ch.length) {
-        const int64_t at = ((ch.batch * p.time + ch.first + row0 + e) * p.key_heads + key_head) * int64_t(p.key_dim) + d0;
+      for (int u = 0; u < KT; ++u)
 #pragma unroll
-        for (int u = 0; u < KT; ++u)
-          if (d0 + 16 * u + r < p.key_dim) {
-            static_cast<T*>(p.d_q)[at + 16 * u + r] = T(dq_all[u][e]);
-            static_cast<T*>(p.d_k)[at + 16 * u + r] = T(dk_all[u][e]);
-          }
-      }
+        for (int e = 0; e < 4; ++e) sh_k[(row0 + e) * DK + 16 * u + r] = all[u][e];
+    __syncthreads();
+    if constexpr (PART != GRADIENT_Y) {
+      T* out = static_cast<T*>(PART == GRADIENT_Q ? p.d_q : p.d_k);
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        if (row0 + e < ch.length) {
+          const int64_t at = ((ch.batch * p.time + ch.first + row0 + e) * p.key_heads + key_head) * int64_t(p.key_dim) + d0;
+#pragma unroll
+          for (int u = 0; u < KT; ++u)
+            if (d0 + 16 * u + r < p.key_dim)
+              out[at + 16 * u + r] = T(PART == GRADIENT_Q ? all[u][e] : all[u][e] + sh_k[(row0 + e) * DK + 16 * u + r]);
+        }
+    }
   }
+}
+
+// DK: columns of dQ and dK at a time; WIDE: key_dim is more than that and they come in turns.
+template <typename T, int DK, bool WIDE>
+__global__ __launch_bounds__(GRADIENT_LANES) void delta_gradient_kernel(DeltaArgs a) {
+  __shared__ __align__(16) char smem[GradientShared<T, DK>::BYTES];
+  __shared__ GradientScratch<T, DK> sh;
+  const int64_t slot = blockIdx.x / unsigned(a.p.key_heads);
+  const int key_head = int(blockIdx.x - slot * unsigned(a.p.key_heads));
+  const Chunk ch = chunk_of(a.p, slot);
+  if (ch.length == 0) return;
+  const int part = __builtin_amdgcn_readfirstlane(threadIdx.x >> 8);
+  if (part == 0) gradient_part<T, DK, WIDE, GRADIENT_Q>(a, ch, slot, key_head, smem, sh);
+  else if (part == 1) gradient_part<T, DK, WIDE, GRADIENT_X>(a, ch, slot, key_head, smem, sh);
+  else gradient_part<T, DK, WIDE, GRADIENT_Y>(a, ch, slot, key_head, smem, sh);
 }
 
 }  // namespace linrec

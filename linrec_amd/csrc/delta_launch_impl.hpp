@@ -56,9 +56,9 @@ int delta_backward(const DeltaArgs& a, int key_width) {
   });
   if (rc || a.p.time == 0) return rc;
   const int64_t grid = a.slots * a.p.key_heads;
-  if (key_width == 64) return launch_kernel(delta_gradient_kernel<T, 64, false>, grid, 1, 256, a.p.stream, a);
-  if (key_width == 128) return launch_kernel(delta_gradient_kernel<T, 128, false>, grid, 1, 256, a.p.stream, a);
-  return launch_kernel(delta_gradient_kernel<T, 128, true>, grid, 1, 256, a.p.stream, a);
+  if (key_width == 64) return launch_kernel(delta_gradient_kernel<T, 64, false>, grid, 1, GRADIENT_LANES, a.p.stream, a);
+  if (key_width == 128) return launch_kernel(delta_gradient_kernel<T, 128, false>, grid, 1, GRADIENT_LANES, a.p.stream, a);
+  return launch_kernel(delta_gradient_kernel<T, 128, true>, grid, 1, GRADIENT_LANES, a.p.stream, a);
 }
 
 }  // namespace linrec

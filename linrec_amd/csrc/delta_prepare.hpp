@@ -55,7 +55,7 @@ __global__ __launch_bounds__(256) void delta_prepare_kernel(DeltaArgs a) {
   const int head = int(blockIdx.x - slot * unsigned(p.heads)), key_head = head / a.shared;
   const Chunk ch = chunk_of(p, slot);
   if (ch.length == 0) return;
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r = lane & 15, q = lane >> 4;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), r = lane & 15, q = lane >> 4;
   const int64_t block = slot * p.heads + head;
 
   {
@@ -81,14 +81,15 @@ __global__ __launch_bounds__(256) void delta_prepare_kernel(DeltaArgs a) {
   v4f kk[4], qk[4];
 #pragma unroll
   for (int t = 0; t < 4; ++t) kk[t] = v4f{0, 0, 0, 0}, qk[t] = v4f{0, 0, 0, 0};
+  const int rows = TK::natural_rows(r, q);
   // wave w has rows 16 w and up; tile t of columns from 16 t on, none above the diagonal
 #pragma unroll
   for (int b = 0; b < DK / 32; ++b) {
-    const Frag<T> rk = TK::frag(sh_keys, 16 * wave + r, b, q), rq = TK::frag(sh_keys + TK::BYTES, 16 * wave + r, b, q);
+    const Frag<T> rk = TK::frag(sh_keys + wave * (16 * TK::ROW), rows, 0, b), rq = TK::frag(sh_keys + TK::BYTES + wave * (16 * TK::ROW), rows, 0, b);
 #pragma unroll
     for (int t = 0; t < 4; ++t)
       if (t <= wave) {
-        const Frag<T> other = TK::frag(sh_keys, 16 * t + r, b, q);
+        const Frag<T> other = TK::frag(sh_keys, rows, 16 * t, b);
         kk[t] = mma(rk, other, kk[t]);
         qk[t] = mma(rq, other, qk[t]);
       }

@@ -34,8 +34,8 @@ __global__ __launch_bounds__((ReverseShared<T, DK, WAVES>::LANES)) void delta_re
   const int head = int(pair - n * p.heads), key_head = head / a.shared;
   const Span span = span_of(p, n);
   const int lane = threadIdx.x & 63, r = lane & 15, q = lane >> 4;
-  const bool loader = Sh::LOADERS && threadIdx.x >= 64 * WAVES;
-  const int wave = (threadIdx.x >> 6) - (loader ? WAVES : 0);
+  const bool loader = Sh::LOADERS && __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) >= WAVES;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) - (loader ? WAVES : 0);
   const int c0 = cb * 16 * WAVES, col = c0 + 16 * wave + r;
   const bool mine = col < p.value_dim, kept_column = col < a.columns;  // (of a whole wave)
   const int64_t chunks = (span.end - span.first + DELTA_CHUNK - 1) / DELTA_CHUNK;
@@ -81,6 +81,8 @@ __global__ __launch_bounds__((ReverseShared<T, DK, WAVES>::LANES)) void delta_re
       s[t][e] = p.d_state && mine && !loader && d < p.key_dim ? p.d_state[at0 + d * int64_t(p.value_dim)] : 0.0f;
     }
 
+  const int rows_k = TK::mapped_rows(r, q), rows_s = TS::mapped_rows(r, q), cols_k = TK::template columns<true>(r, q),
+            cols_v = TV::template column_tile<false>(TV::template columns<false>(r, q), wave);
   auto compute = [&](int64_t c, const char* smem) __attribute__((always_inline)) {
     const int64_t first = span.first + c * DELTA_CHUNK, block = (span.slot + c) * p.heads + head;
     const int length = int(span.end - first < DELTA_CHUNK ? span.end - first : DELTA_CHUNK);
@@ -104,7 +106,7 @@ __global__ __launch_bounds__((ReverseShared<T, DK, WAVES>::LANES)) void delta_re
     auto square = [&](int at, int t, int b) __attribute__((always_inline)) {
       Planes<U> f;
 #pragma unroll
-      for (int k2 = 0; k2 < P; ++k2) f.p[k2] = TS::frag(smem + at + k2 * TS::BYTES, row_of_tile(t, r), b, q);
+      for (int k2 = 0; k2 < P; ++k2) f.p[k2] = TS::frag(smem + at + k2 * TS::BYTES, rows_s, TS::mapped_row(t), b);
       return f;
     };
     // dO of this wave's columns, a result's layout; fp16 as two bf16
@@ -112,7 +114,7 @@ __global__ __launch_bounds__((ReverseShared<T, DK, WAVES>::LANES)) void delta_re
     Planes<U, IN> dop[2];
 #pragma unroll
     for (int t = 0; t < 4; ++t) {
-      const auto v = TV::column4(smem + Sh::O, row_of_result(t, q), [&](int j) { return 16 * wave + 4 * j; });
+      const auto v = TV::template column4<false>(smem + Sh::O, cols_v, TK::mapped_row(t), 0);
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         d_o[t][e] = float(v[e]);
@@ -126,7 +128,7 @@ __global__ __launch_bounds__((ReverseShared<T, DK, WAVES>::LANES)) void delta_re
     for (int t = 0; t < 4; ++t) {
       x[t] = v4f{0, 0, 0, 0};
 #pragma unroll
-      for (int b = 0; b < DK / 32; ++b) x[t] = mma(TK::frag(smem + Sh::K, row_of_tile(t, r), b, q), sp[b], x[t]);
+      for (int b = 0; b < DK / 32; ++b) x[t] = mma(TK::frag(smem + Sh::K, rows_k, TK::mapped_row(t), b), sp[b], x[t]);
       const v4f rest = *reinterpret_cast<const v4f*>(gates + 64 + row_of_result(t, q));
 #pragma unroll
       for (int e = 0; e < 4; ++e) x[t][e] *= rest[e] * un_s;
@@ -185,14 +187,14 @@ __global__ __launch_bounds__((ReverseShared<T, DK, WAVES>::LANES)) void delta_re
     for (int t = 0; t < DK / 16; ++t) {
       auto with_keys = [&](v4f to) __attribute__((always_inline)) {
 #pragma unroll
-        for (int b = 0; b < 2; ++b) to = mma(TK::column_frag(smem + Sh::K, b, q, [&](int j) { return row_of_result(t, j); }), vp[b], to);
+        for (int b = 0; b < 2; ++b) to = mma(TK::template column_frag<true>(smem + Sh::K, cols_k, b, t), vp[b], to);
         return to;
       };
       auto with_queries = [&](v4f to) __attribute__((always_inline)) {
 #pragma unroll
         for (int b = 0; b < 2; ++b) {
           if constexpr (Sh::QUERIES) {
-            to = mma(TK::column_frag(smem + Sh::Q, b, q, [&](int j) { return row_of_result(t, j); }), op[b], to);
+            to = mma(TK::template column_frag<true>(smem + Sh::Q, cols_k, b, t), op[b], to);
           } else {
             Frag<T> f;
             const int d = row_of_tile(t, r);

@@ -43,8 +43,8 @@ __global__ __launch_bounds__((ScanShared<T, DK, WAVES, STATES>::LANES)) void del
   const int head = int(pair - n * p.heads), key_head = head / a.shared;
   const Span span = span_of(p, n);
   const int lane = threadIdx.x & 63, r = lane & 15, q = lane >> 4;
-  const bool loader = Sh::LOADERS && threadIdx.x >= 64 * WAVES;
-  const int wave = (threadIdx.x >> 6) - (loader ? WAVES : 0);
+  const bool loader = Sh::LOADERS && __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) >= WAVES;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) - (loader ? WAVES : 0);
   const int c0 = cb * 16 * WAVES, col = c0 + 16 * wave + r;
   const bool mine = col < p.value_dim, kept_column = col < a.columns;  // (of a whole wave)
   const int64_t chunks = (span.end - span.first + DELTA_CHUNK - 1) / DELTA_CHUNK;
@@ -90,6 +90,8 @@ __global__ __launch_bounds__((ScanShared<T, DK, WAVES, STATES>::LANES)) void del
       s[t][e] = p.h0 && mine && !loader && d < p.key_dim ? p.h0[at0 + d * int64_t(p.value_dim)] : 0.0f;
     }
 
+  const int rows_k = TK::mapped_rows(r, q), rows_s = TS::mapped_rows(r, q), cols_k = TK::template columns<true>(r, q),
+            cols_v = TV::template column_tile<false>(TV::template columns<false>(r, q), wave);
   auto compute = [&](int64_t c, const char* smem) __attribute__((always_inline)) {
     const int64_t first = span.first + c * DELTA_CHUNK, block = (span.slot + c) * p.heads + head;
     const int length = int(span.end - first < DELTA_CHUNK ? span.end - first : DELTA_CHUNK);
@@ -115,18 +117,18 @@ __global__ __launch_bounds__((ScanShared<T, DK, WAVES, STATES>::LANES)) void del
     for (int t = 0; t < 4; ++t) {
       x[t] = v4f{0, 0, 0, 0};
 #pragma unroll
-      for (int b = 0; b < DK / 32; ++b) x[t] = mma(TK::frag(smem + Sh::K, row_of_tile(t, r), b, q), sp[b], x[t]);
+      for (int b = 0; b < DK / 32; ++b) x[t] = mma(TK::frag(smem + Sh::K, rows_k, TK::mapped_row(t), b), sp[b], x[t]);
     }
     auto square = [&](int at, int t, int b) __attribute__((always_inline)) {
       Planes<U> f;
 #pragma unroll
-      for (int k2 = 0; k2 < P; ++k2) f.p[k2] = TS::frag(smem + at + k2 * TS::BYTES, row_of_tile(t, r), b, q);
+      for (int k2 = 0; k2 < P; ++k2) f.p[k2] = TS::frag(smem + at + k2 * TS::BYTES, rows_s, TS::mapped_row(t), b);
       return f;
     };
 #pragma unroll
     for (int t = 0; t < 4; ++t) {
       const int row = row_of_result(t, q);
-      const auto v = TV::column4(smem + Sh::V, row, [&](int j) { return 16 * wave + 4 * j; });
+      const auto v = TV::template column4<false>(smem + Sh::V, cols_v, TK::mapped_row(t), 0);
       const v4f gamma = *reinterpret_cast<const v4f*>(gates + row), beta = *reinterpret_cast<const v4f*>(gates + 128 + row);
 #pragma unroll
       for (int e = 0; e < 4; ++e) x[t][e] = beta[e] * fmaf(-gamma[e] * un_s, x[t][e], float(v[e]));
@@ -160,7 +162,7 @@ __global__ __launch_bounds__((ScanShared<T, DK, WAVES, STATES>::LANES)) void del
 #pragma unroll
         for (int b = 0; b < DK / 32; ++b) {
           if constexpr (Sh::QUERIES) {
-            y = mma(TK::frag(smem + Sh::Q, from, b, q), sp[b], y);
+            y = mma(TK::frag(smem + Sh::Q, rows_k, TK::mapped_row(t), b), sp[b], y);
           } else {
             Frag<T> f;
 #pragma unroll
@@ -197,7 +199,7 @@ __global__ __launch_bounds__((ScanShared<T, DK, WAVES, STATES>::LANES)) void del
       auto added = [&](v4f to) __attribute__((always_inline)) {
 #pragma unroll
         for (int b = 0; b < 2; ++b)
-          to = mma(TK::column_frag(smem + Sh::K, b, q, [&](int j) { return row_of_result(t, j); }), nt[b], to);
+          to = mma(TK::template column_frag<true>(smem + Sh::K, cols_k, b, t), nt[b], to);
         return to;
       };
       s[t] *= keep;

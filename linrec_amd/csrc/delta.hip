@@ -15,7 +15,22 @@ int check_delta(const linrec_delta_t* p) {
   return LINREC_OK;
 }
 
+constexpr int64_t DELTA_FILL = 256, DELTA_LEAST_SEGMENT = 8;  // workgroups, chunks
+
 size_t aligned(size_t n) { return (n + 255) & ~size_t(255); }
+
+// Chunks of a segment, 0 where sequences are not cut.
+int segment_of(const DeltaArgs& a, int width) {
+  const linrec_delta_t& p = a.p;
+  if (p.sequences == 0 || p.time == 0) return 0;
+  const int64_t side = p.sequences * p.heads, key_blocks = width / (16 * delta_waves(a.columns));
+  const int64_t chunks = cdiv(a.slots, p.sequences);  // of a sequence (of packed ones the mean)
+  // so many that the first pass, which has the columns of the unit matrix as well, fills the chip
+  const int64_t segments = DELTA_FILL / (side * (a.blocks + key_blocks));
+  if (segments < 3 || chunks < 3 * DELTA_LEAST_SEGMENT) return 0;
+  const int64_t each = cdiv(chunks, segments);
+  return int(each < DELTA_LEAST_SEGMENT ? DELTA_LEAST_SEGMENT : each);
+}
 
 // Sizes, and scratch parts from `base` on; returns the bytes of scratch.
 size_t lay_out(const linrec_delta_t& p, bool bwd, char* base, DeltaArgs* a) {
@@ -23,8 +38,11 @@ size_t lay_out(const linrec_delta_t& p, bool bwd, char* base, DeltaArgs* a) {
   a->shared = p.heads / p.key_heads;
   a->columns = int(cdiv(p.value_dim, 32) * 32);
   a->blocks = int(cdiv(a->columns, 16 * delta_waves(a->columns)));
-  a->pairs = p.sequences * p.heads;
   a->slots = p.cu_seqlens ? p.time / DELTA_CHUNK + p.sequences : p.batch * cdiv(p.time, DELTA_CHUNK);
+  const int width = delta_key_width(p.key_dim);
+  a->segment = segment_of(*a, width);
+  a->parts = !a->segment ? p.sequences : p.cu_seqlens ? a->slots / a->segment + p.sequences : p.batch * cdiv(cdiv(p.time, DELTA_CHUNK), a->segment);
+  a->pairs = a->parts * p.heads;
   const size_t blocks = size_t(a->slots) * size_t(p.heads);
   constexpr size_t value = 4;  // bytes of a value of inner type in all its planes
   size_t at = 0;
@@ -37,13 +55,19 @@ size_t lay_out(const linrec_delta_t& p, bool bwd, char* base, DeltaArgs* a) {
   a->c = part(4096 * value);
   a->gates = reinterpret_cast<float*>(part(192 * 4));
   if (bwd) {
-    const size_t state = size_t(a->columns) * size_t(delta_key_width(p.key_dim)) * value, rows = size_t(a->columns) * 64 * value;
+    const size_t state = size_t(a->columns) * size_t(width) * value, rows = size_t(a->columns) * 64 * value;
     a->m_t = part(4096 * value);
     a->s = part(state);
     a->d_s = part(state);
     a->n = part(rows);
     a->d_b = part(rows);
     a->dots = reinterpret_cast<float*>(part(192 * 4));
+  }
+  if (a->segment) {
+    a->carry = reinterpret_cast<float*>(base + at);
+    at += aligned(size_t(a->pairs) * size_t(a->columns + width) * size_t(width) * 4);
+    a->start = reinterpret_cast<float*>(base + at);
+    at += aligned(size_t(a->pairs) * size_t(a->columns) * size_t(width) * 4);
   }
   return at;
 }

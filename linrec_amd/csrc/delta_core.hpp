@@ -284,6 +284,10 @@ struct Stager {
           for (int e = 0; e < cols; ++e) v[n][e] = from[(n * STEP + row) * stride + e];
     }
   }
+  __device__ __forceinline__ void clear() {
+#pragma unroll
+    for (int n = 0; n < N; ++n) v[n] = zero();
+  }
   // dense rows of scratch
   __device__ __forceinline__ void fetch_dense(const T* from, int lane) {
 #pragma unroll
@@ -307,7 +311,9 @@ struct DeltaArgs {
   int shared;    // value heads of a key head
   int columns;   // value_dim rounded up to 32: rows of the planes of S, dS', N and dB
   int blocks;    // workgroups side by side over the columns
-  int64_t pairs; // sequences x heads
+  int64_t pairs; // parts x heads
+  int64_t parts; // sequences, or segments of them
+  int segment;   // chunks of a segment, 0: sequences are not cut
   // scratch, for every (slot, head): m[planes][64][64] and so on
   char* m;
   char* m_t;
@@ -318,6 +324,9 @@ struct DeltaArgs {
   char* n;       // [planes][columns][64]
   char* d_b;
   float* dots;   // [192], sums of the gates' gradients where key_dim comes in turns
+  // for every (part, head), where sequences are cut (delta_segments.hpp)
+  float* carry;  // [columns + DK][DK]: what a segment makes of nothing, and of the unit matrix
+  float* start;  // [columns][DK]: the state that enters a segment
 };
 
 struct Span {
@@ -360,15 +369,58 @@ __device__ __forceinline__ Chunk chunk_of(const linrec_delta_t& p, int64_t slot)
   return Chunk{0, first, int(left < DELTA_CHUNK ? left : DELTA_CHUNK)};
 }
 
+// Part of a sequence: all of it, or a segment.  Segments are numbered as slots are: a packed sequence's from slot / segment + n on.
+struct Part {
+  int64_t n;
+  Span span;
+  int64_t index, count;  // of the sequence's parts; count is 0 where there is none
+  int64_t begin, end;    // chunks
+};
+__device__ __forceinline__ int64_t chunks_of(const Span& s) { return (s.end - s.first + DELTA_CHUNK - 1) / DELTA_CHUNK; }
+__device__ __forceinline__ int64_t first_part(const DeltaArgs& a, int64_t n, const Span& s) {
+  if (!a.segment) return n;
+  if (a.p.cu_seqlens) return s.slot / a.segment + n;
+  return n * ((chunks_of(s) + a.segment - 1) / a.segment);
+}
+__device__ __forceinline__ int64_t count_of_parts(const DeltaArgs& a, const Span& s) {
+  const int64_t chunks = chunks_of(s);
+  return a.segment && chunks > a.segment ? (chunks + a.segment - 1) / a.segment : 1;  // (one of nothing hands the state on)
+}
+__device__ __forceinline__ Part part_of(const DeltaArgs& a, int64_t at) {
+  int64_t n = at;
+  if (a.segment && !a.p.cu_seqlens) {
+    n = at / count_of_parts(a, span_of(a.p, 0));
+  } else if (a.segment) {  // the last sequence whose parts start at or before this one, 64 at a time
+    int lo = 0, hi = int(a.p.sequences);
+    const int lane = threadIdx.x & 63;
+    while (hi - lo > 1) {
+      const int step = (hi - lo + 63) / 64, probe = lo + lane * step;
+      const bool before = probe < hi && first_part(a, probe, span_of(a.p, probe)) <= at;
+      const int found = __popcll(__ballot(before));
+      lo += (found > 0 ? found - 1 : 0) * step;
+      hi = lo + step < hi ? lo + step : hi;
+    }
+    n = __builtin_amdgcn_readfirstlane(lo);
+  }
+  Part part{n, span_of(a.p, n), 0, 0, 0, 0};
+  const int64_t chunks = chunks_of(part.span);
+  part.count = count_of_parts(a, part.span);
+  part.index = at - first_part(a, n, part.span);
+  part.begin = part.index * (a.segment ? a.segment : chunks);
+  part.end = a.segment && part.begin + a.segment < chunks ? part.begin + a.segment : chunks;
+  if (part.index < 0 || part.index >= part.count) part.count = 0;
+  return part;
+}
+
 template <typename T>
 __device__ __forceinline__ const T* head_rows(const void* base, const int64_t (&stride)[3], int64_t batch, int64_t first, int64_t head) {
   return static_cast<const T*>(base) + batch * stride[0] + first * stride[1] + head * stride[2];
 }
 
-// Workgroups of one (sequence, head), which read the same keys and queries, lie on one XCD (workgroups go round the eight in turn).
-__device__ __forceinline__ bool scan_place(const DeltaArgs& a, int64_t* pair, int* block) {
-  const int64_t group = blockIdx.x / unsigned(8 * a.blocks);
-  const int in = int(blockIdx.x - group * unsigned(8 * a.blocks));
+// Workgroups of one (part, head), which read the same keys and queries, lie on one XCD (workgroups go round the eight in turn).
+__device__ __forceinline__ bool scan_place(const DeltaArgs& a, int blocks, int64_t* pair, int* block) {
+  const int64_t group = blockIdx.x / unsigned(8 * blocks);
+  const int in = int(blockIdx.x - group * unsigned(8 * blocks));
   *block = in >> 3;
   *pair = group * 8 + (in & 7);
   return *pair < a.pairs;

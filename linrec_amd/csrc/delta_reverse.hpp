@@ -17,7 +17,8 @@ struct ReverseShared {
   static constexpr int LANES = 64 * WAVES * (LOADERS ? 2 : 1);
 };
 
-template <typename T, int DK, int WAVES>
+// CARRY: only what a segment adds to the gradient of the state before it, for delta_segments.hpp.
+template <typename T, int DK, int WAVES, bool CARRY>
 __global__ __launch_bounds__((ReverseShared<T, DK, WAVES>::LANES)) void delta_reverse_kernel(DeltaArgs a) {
   using U = Inner<T>;
   using Sh = ReverseShared<T, DK, WAVES>;
@@ -29,16 +30,17 @@ __global__ __launch_bounds__((ReverseShared<T, DK, WAVES>::LANES)) void delta_re
   const linrec_delta_t& p = a.p;
   int64_t pair;
   int cb;
-  if (!scan_place(a, &pair, &cb)) return;
-  const int64_t n = pair / p.heads;
-  const int head = int(pair - n * p.heads), key_head = head / a.shared;
-  const Span span = span_of(p, n);
+  if (!scan_place(a, a.blocks, &pair, &cb)) return;
+  const int64_t place = pair / p.heads;
+  const int head = int(pair - place * p.heads), key_head = head / a.shared;
+  const Part part = part_of(a, place);
+  if (part.count == 0 || (CARRY && part.count == 1)) return;
+  const Span span = part.span;
   const int lane = threadIdx.x & 63, r = lane & 15, q = lane >> 4;
   const bool loader = Sh::LOADERS && __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) >= WAVES;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) - (loader ? WAVES : 0);
   const int c0 = cb * 16 * WAVES, col = c0 + 16 * wave + r;
   const bool mine = col < p.value_dim, kept_column = col < a.columns;  // (of a whole wave)
-  const int64_t chunks = (span.end - span.first + DELTA_CHUNK - 1) / DELTA_CHUNK;
 
   auto load = [&](int64_t c, char* smem) __attribute__((always_inline)) {
     const int64_t first = span.first + c * DELTA_CHUNK, block = (span.slot + c) * p.heads + head;
@@ -72,14 +74,21 @@ __global__ __launch_bounds__((ReverseShared<T, DK, WAVES>::LANES)) void delta_re
   };
 
   v4f s[DK / 16];  // dS'
-  const int64_t at0 = (pair * p.key_dim) * int64_t(p.value_dim) + col;
+  const int64_t at0 = ((part.n * p.heads + head) * p.key_dim) * int64_t(p.value_dim) + col;
 #pragma unroll
-  for (int t = 0; t < DK / 16; ++t)
+  for (int t = 0; t < DK / 16; ++t) s[t] = v4f{0, 0, 0, 0};
+  if (loader || CARRY) {
+  } else if (a.segment) {
+    if (kept_column) load_columns<DK>(a.start + (pair * a.columns + col) * DK, q, s);
+  } else if (p.d_state && mine) {
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      const int d = row_of_result(t, q) + e;
-      s[t][e] = p.d_state && mine && !loader && d < p.key_dim ? p.d_state[at0 + d * int64_t(p.value_dim)] : 0.0f;
-    }
+    for (int t = 0; t < DK / 16; ++t)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int d = row_of_result(t, q) + e;
+        if (d < p.key_dim) s[t][e] = p.d_state[at0 + d * int64_t(p.value_dim)];
+      }
+  }
 
   const int rows_k = TK::mapped_rows(r, q), rows_s = TS::mapped_rows(r, q), cols_k = TK::template columns<true>(r, q),
             cols_v = TV::template column_tile<false>(TV::template columns<false>(r, q), wave);
@@ -91,7 +100,7 @@ __global__ __launch_bounds__((ReverseShared<T, DK, WAVES>::LANES)) void delta_re
     Planes<T> sp[DK / 32];
     float un_s;
     split_scaled<T>(s, sp, &un_s);
-    {
+    if constexpr (!CARRY) {
       U* to = reinterpret_cast<U*>(a.d_s) + block * P * a.columns * DK;
 #pragma unroll
       for (int b = 0; b < DK / 32; ++b) {
@@ -145,7 +154,7 @@ __global__ __launch_bounds__((ReverseShared<T, DK, WAVES>::LANES)) void delta_re
 #pragma unroll
       for (int b = t / 2; b < 2; ++b) db[t] = mma(square(Sh::M, t, b), xp[b], db[t]);
     }
-    if (kept_column) {
+    if (!CARRY && kept_column) {
       U* to = reinterpret_cast<U*>(a.d_b) + block * P * a.columns * 64;
 #pragma unroll
       for (int b = 0; b < 2; ++b) {
@@ -163,7 +172,8 @@ __global__ __launch_bounds__((ReverseShared<T, DK, WAVES>::LANES)) void delta_re
       T* to = d_v + row * int64_t(apart);
 #pragma unroll
       for (int e = 0; e < 4; ++e) db[t][e] *= beta[e];
-      if (length == DELTA_CHUNK) {
+      if constexpr (CARRY) {
+      } else if (length == DELTA_CHUNK) {
         if (mine)
 #pragma unroll
           for (int e = 0; e < 4; ++e) to[e * apart] = T(db[t][e]);
@@ -219,22 +229,26 @@ __global__ __launch_bounds__((ReverseShared<T, DK, WAVES>::LANES)) void delta_re
   };
 
   if constexpr (Sh::LOADERS) {
-    if (loader && chunks > 0) load(chunks - 1, room);
+    if (loader && part.begin < part.end) load(part.end - 1, room);
     __syncthreads();
-    for (int64_t c = chunks - 1, turn = 0; c >= 0; --c, turn ^= 1) {
+    int turn = 0;
+    for (int64_t c = part.end - 1; c >= part.begin; --c, turn ^= 1) {
       if (!loader) compute(c, room + turn * Sh::BYTES);
-      else if (c > 0) load(c - 1, room + (turn ^ 1) * Sh::BYTES);
+      else if (c > part.begin) load(c - 1, room + (turn ^ 1) * Sh::BYTES);
       __syncthreads();
     }
   } else {
-    for (int64_t c = chunks - 1; c >= 0; --c) {
+    for (int64_t c = part.end - 1; c >= part.begin; --c) {
       __syncthreads();
       load(c, room);
       __syncthreads();
       compute(c, room);
     }
   }
-  if (p.d_h0 && mine && !loader)
+  if (loader) return;
+  if constexpr (CARRY) {
+    if (kept_column) store_columns<DK>(a.carry + (pair * (a.columns + DK) + col) * DK, q, s);
+  } else if (p.d_h0 && mine && part.index == 0) {
 #pragma unroll
     for (int t = 0; t < DK / 16; ++t)
 #pragma unroll
@@ -242,6 +256,7 @@ __global__ __launch_bounds__((ReverseShared<T, DK, WAVES>::LANES)) void delta_re
         const int d = row_of_result(t, q) + e;
         if (d < p.key_dim) p.d_h0[at0 + d * int64_t(p.value_dim)] = s[t][e];
       }
+  }
 }
 
 }  // namespace linrec

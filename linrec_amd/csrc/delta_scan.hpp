@@ -1,6 +1,6 @@
 // Gated delta rule, the pass along the sequence: N, O and the state, chunk by chunk (delta_core.hpp).
 //
-// A workgroup has a (sequence, head) and 16 columns of the state for each of half of its waves; the other half loads what the next
+// A workgroup has a (sequence, head), or a segment of one (delta_segments.hpp), and 16 columns of the state for each of half of its waves; the other half loads what the next
 // chunk needs into LDS meanwhile (a state's chunks follow one another, so nothing else hides those loads; where two chunks do not
 // fit into LDS all waves load first and compute then).
 #pragma once
@@ -13,8 +13,15 @@ constexpr int square_bytes() {
   return 64 * 64 * int(sizeof(U)) * planes_of<U>();
 }
 
-template <typename T, int DK, int WAVES, bool STATES>
+enum ScanMode {
+  SCAN_OUT,     // the forward: O and the last state
+  SCAN_STATES,  // a backward's first pass, which keeps the states before the chunks and N and has no O
+  SCAN_CARRY,   // what a segment makes of nothing, and of the unit matrix (where V is zero)
+};
+
+template <typename T, int DK, int WAVES, ScanMode MODE>
 struct ScanShared {
+  static constexpr bool STATES = MODE != SCAN_OUT;
   using U = Inner<T>;
   static constexpr int KEYS = Tile<T, DK>::BYTES, VALUES = Tile<T, 16 * WAVES>::BYTES;
   // (fp32 of 256 channels: queries are read from memory where they are used)
@@ -25,11 +32,22 @@ struct ScanShared {
   static constexpr int LANES = 64 * WAVES * (LOADERS ? 2 : 1);
 };
 
-// STATES: a backward's first pass, which keeps the states before the chunks and N and has no O.
-template <typename T, int DK, int WAVES, bool STATES>
-__global__ __launch_bounds__((ScanShared<T, DK, WAVES, STATES>::LANES)) void delta_scan_kernel(DeltaArgs a) {
+// Where a lane's part of a state lies that is kept as [columns][DK].
+template <int DK>
+__device__ __forceinline__ void load_columns(const float* from, int q, v4f (&s)[DK / 16]) {
+#pragma unroll
+  for (int t = 0; t < DK / 16; ++t) s[t] = *reinterpret_cast<const v4f*>(from + row_of_result(t, q));
+}
+template <int DK>
+__device__ __forceinline__ void store_columns(float* to, int q, const v4f (&s)[DK / 16]) {
+#pragma unroll
+  for (int t = 0; t < DK / 16; ++t) *reinterpret_cast<v4f*>(to + row_of_result(t, q)) = s[t];
+}
+
+template <typename T, int DK, int WAVES, ScanMode MODE>
+__global__ __launch_bounds__((ScanShared<T, DK, WAVES, MODE>::LANES)) void delta_scan_kernel(DeltaArgs a) {
   using U = Inner<T>;
-  using Sh = ScanShared<T, DK, WAVES, STATES>;
+  using Sh = ScanShared<T, DK, WAVES, MODE>;
   using TK = Tile<T, DK>;
   using TV = Tile<T, 16 * WAVES>;
   using TS = Tile<U, 64>;
@@ -38,16 +56,18 @@ __global__ __launch_bounds__((ScanShared<T, DK, WAVES, STATES>::LANES)) void del
   const linrec_delta_t& p = a.p;
   int64_t pair;
   int cb;
-  if (!scan_place(a, &pair, &cb)) return;
-  const int64_t n = pair / p.heads;
-  const int head = int(pair - n * p.heads), key_head = head / a.shared;
-  const Span span = span_of(p, n);
+  if (!scan_place(a, MODE == SCAN_CARRY ? a.blocks + DK / (16 * WAVES) : a.blocks, &pair, &cb)) return;
+  const int64_t place = pair / p.heads;
+  const int head = int(pair - place * p.heads), key_head = head / a.shared;
+  const Part part = part_of(a, place);
+  if (part.count == 0 || (MODE == SCAN_CARRY && part.count == 1)) return;
+  const Span span = part.span;
   const int lane = threadIdx.x & 63, r = lane & 15, q = lane >> 4;
   const bool loader = Sh::LOADERS && __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) >= WAVES;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) - (loader ? WAVES : 0);
-  const int c0 = cb * 16 * WAVES, col = c0 + 16 * wave + r;
+  const bool unit = MODE == SCAN_CARRY && cb >= a.blocks;  // columns of the unit matrix
+  const int c0 = (unit ? cb - a.blocks : cb) * 16 * WAVES, col = c0 + 16 * wave + r;
   const bool mine = col < p.value_dim, kept_column = col < a.columns;  // (of a whole wave)
-  const int64_t chunks = (span.end - span.first + DELTA_CHUNK - 1) / DELTA_CHUNK;
 
   auto load = [&](int64_t c, char* smem) __attribute__((always_inline)) {
     const int64_t first = span.first + c * DELTA_CHUNK, block = (span.slot + c) * p.heads + head;
@@ -58,11 +78,12 @@ __global__ __launch_bounds__((ScanShared<T, DK, WAVES, STATES>::LANES)) void del
     float gate[(192 + STAGING - 1) / STAGING];
     k.fetch(head_rows<T>(p.k, p.k_stride, span.batch, first, key_head), p.k_stride[1], length, p.key_dim, by);
     if constexpr (Sh::QUERIES) qq.fetch(head_rows<T>(p.q, p.q_stride, span.batch, first, key_head), p.q_stride[1], length, p.key_dim, by);
-    v.fetch(head_rows<T>(p.v, p.v_stride, span.batch, first, head) + c0, p.v_stride[1], length, p.value_dim - c0, by);
+    if (!unit) v.fetch(head_rows<T>(p.v, p.v_stride, span.batch, first, head) + c0, p.v_stride[1], length, p.value_dim - c0, by);
+    else v.clear();
 #pragma unroll
     for (int k2 = 0; k2 < P; ++k2) {
       m[k2].fetch_dense(reinterpret_cast<const U*>(a.m + block * SQUARE) + k2 * 4096, by);
-      if constexpr (!STATES) cc[k2].fetch_dense(reinterpret_cast<const U*>(a.c + block * SQUARE) + k2 * 4096, by);
+      if constexpr (MODE == SCAN_OUT) cc[k2].fetch_dense(reinterpret_cast<const U*>(a.c + block * SQUARE) + k2 * 4096, by);
     }
 #pragma unroll
     for (int i = 0; i < (192 + STAGING - 1) / STAGING; ++i)
@@ -73,7 +94,7 @@ __global__ __launch_bounds__((ScanShared<T, DK, WAVES, STATES>::LANES)) void del
 #pragma unroll
     for (int k2 = 0; k2 < P; ++k2) {
       m[k2].put(smem + Sh::M + k2 * TS::BYTES, by);
-      if constexpr (!STATES) cc[k2].put(smem + Sh::C + k2 * TS::BYTES, by);
+      if constexpr (MODE == SCAN_OUT) cc[k2].put(smem + Sh::C + k2 * TS::BYTES, by);
     }
 #pragma unroll
     for (int i = 0; i < (192 + STAGING - 1) / STAGING; ++i)
@@ -81,14 +102,27 @@ __global__ __launch_bounds__((ScanShared<T, DK, WAVES, STATES>::LANES)) void del
   };
 
   v4f s[DK / 16];
-  const int64_t at0 = (pair * p.key_dim) * int64_t(p.value_dim) + col;
+  const int64_t at0 = ((part.n * p.heads + head) * p.key_dim) * int64_t(p.value_dim) + col;
 #pragma unroll
-  for (int t = 0; t < DK / 16; ++t)
+  for (int t = 0; t < DK / 16; ++t) s[t] = v4f{0, 0, 0, 0};
+  if (loader) {
+  } else if constexpr (MODE == SCAN_CARRY) {
+    if (unit)
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      const int d = row_of_result(t, q) + e;
-      s[t][e] = p.h0 && mine && !loader && d < p.key_dim ? p.h0[at0 + d * int64_t(p.value_dim)] : 0.0f;
-    }
+      for (int t = 0; t < DK / 16; ++t)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) s[t][e] = row_of_result(t, q) + e == col ? 1.0f : 0.0f;
+  } else if (a.segment) {
+    if (kept_column) load_columns<DK>(a.start + (pair * a.columns + col) * DK, q, s);
+  } else if (p.h0 && mine) {
+#pragma unroll
+    for (int t = 0; t < DK / 16; ++t)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int d = row_of_result(t, q) + e;
+        if (d < p.key_dim) s[t][e] = p.h0[at0 + d * int64_t(p.value_dim)];
+      }
+  }
 
   const int rows_k = TK::mapped_rows(r, q), rows_s = TS::mapped_rows(r, q), cols_k = TK::template columns<true>(r, q),
             cols_v = TV::template column_tile<false>(TV::template columns<false>(r, q), wave);
@@ -100,7 +134,7 @@ __global__ __launch_bounds__((ScanShared<T, DK, WAVES, STATES>::LANES)) void del
     Planes<T> sp[DK / 32];
     float un_s;
     split_scaled<T>(s, sp, &un_s);
-    if constexpr (STATES) {
+    if constexpr (MODE == SCAN_STATES) {
       U* to = reinterpret_cast<U*>(a.s) + block * P * a.columns * DK;
 #pragma unroll
       for (int b = 0; b < DK / 32; ++b) {
@@ -146,7 +180,8 @@ __global__ __launch_bounds__((ScanShared<T, DK, WAVES, STATES>::LANES)) void del
     Planes<U> np[2];
 #pragma unroll
     for (int b = 0; b < 2; ++b) np[b] = split<U>(nn[2 * b], nn[2 * b + 1]);
-    if constexpr (STATES) {
+    if constexpr (MODE == SCAN_CARRY) {
+    } else if constexpr (MODE == SCAN_STATES) {
       U* to = reinterpret_cast<U*>(a.n) + block * P * a.columns * 64;
 #pragma unroll
       for (int b = 0; b < 2; ++b)
@@ -209,22 +244,26 @@ __global__ __launch_bounds__((ScanShared<T, DK, WAVES, STATES>::LANES)) void del
   };
 
   if constexpr (Sh::LOADERS) {
-    if (loader && chunks > 0) load(0, room);
+    if (loader && part.begin < part.end) load(part.begin, room);
     __syncthreads();
-    for (int64_t c = 0; c < chunks; ++c) {
-      if (!loader) compute(c, room + (c & 1) * Sh::BYTES);
-      else if (c + 1 < chunks) load(c + 1, room + (~c & 1) * Sh::BYTES);
+    int turn = 0;
+    for (int64_t c = part.begin; c < part.end; ++c, turn ^= 1) {
+      if (!loader) compute(c, room + turn * Sh::BYTES);
+      else if (c + 1 < part.end) load(c + 1, room + (turn ^ 1) * Sh::BYTES);
       __syncthreads();
     }
   } else {
-    for (int64_t c = 0; c < chunks; ++c) {
+    for (int64_t c = part.begin; c < part.end; ++c) {
       __syncthreads();
       load(c, room);
       __syncthreads();
       compute(c, room);
     }
   }
-  if (!STATES && p.state && mine && !loader)
+  if (loader) return;
+  if constexpr (MODE == SCAN_CARRY) {
+    if (unit || kept_column) store_columns<DK>(a.carry + (pair * (a.columns + DK) + (unit ? a.columns : 0) + col) * DK, q, s);
+  } else if (MODE == SCAN_OUT && p.state && mine && part.index == part.count - 1) {
 #pragma unroll
     for (int t = 0; t < DK / 16; ++t)
 #pragma unroll
@@ -232,6 +271,7 @@ __global__ __launch_bounds__((ScanShared<T, DK, WAVES, STATES>::LANES)) void del
         const int d = row_of_result(t, q) + e;
         if (d < p.key_dim) p.state[at0 + d * int64_t(p.value_dim)] = s[t][e];
       }
+  }
 }
 
 }  // namespace linrec

@@ -51,16 +51,19 @@ size_t lay_out(const linrec_delta_t& p, bool bwd, char* base, DeltaArgs* a) {
     at += aligned(blocks * bytes_of_block);
     return to;
   };
-  a->m = part(4096 * value);
-  a->c = part(4096 * value);
+  a->square = 4096 * value;
+  a->state = int64_t(a->columns) * width * value;
+  a->rows = int64_t(a->columns) * 64 * value;
+  a->m = part(a->square);
+  a->c = part(a->square);
   a->gates = reinterpret_cast<float*>(part(192 * 4));
   if (bwd) {
-    const size_t state = size_t(a->columns) * size_t(width) * value, rows = size_t(a->columns) * 64 * value;
-    a->m_t = part(4096 * value);
-    a->s = part(state);
-    a->d_s = part(state);
-    a->n = part(rows);
-    a->d_b = part(rows);
+    a->sums = reinterpret_cast<double*>(part(64 * 8));
+    a->m_t = part(a->square);
+    a->s = part(a->state);
+    a->d_s = part(a->state);
+    a->n = part(a->rows);
+    a->d_b = part(a->rows);
     a->dots = reinterpret_cast<float*>(part(192 * 4));
   }
   if (a->segment) {

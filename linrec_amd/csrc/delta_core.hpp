@@ -48,6 +48,20 @@ constexpr int input_planes() {
   return std::is_same_v<T, _Float16> ? 2 : 1;
 }
 
+// e^x; the rounding of x log2(e) is |x| 2^-24 of the result, no more than 2^-25 of one.
+__device__ __forceinline__ float fast_exp(float x) { return __builtin_amdgcn_exp2f(x * 1.44269504f); }
+
+// Sum over 16 neighbouring lanes, in each of them.
+__device__ __forceinline__ float sum_of_16(float x) {
+  auto turned = [&](auto n) __attribute__((always_inline)) {  // lane l has lane l - n of its 16
+    return __uint_as_float(unsigned(__builtin_amdgcn_update_dpp(0, int(__float_as_uint(x)), 0x120 + n(), 0xf, 0xf, true)));
+  };
+  x += turned(std::integral_constant<int, 8>{});
+  x += turned(std::integral_constant<int, 4>{});
+  x += turned(std::integral_constant<int, 2>{});
+  return x + turned(std::integral_constant<int, 1>{});
+}
+
 // Eight of the 32 positions that a product sums over at once, for one row (or column): lane 16 q + r holds positions 8 q to 8 q + 7
 // of row r.
 template <typename U>
@@ -221,6 +235,12 @@ __device__ __forceinline__ int anew(int view) {
   return view;
 }
 
+// The same, not before `result` is there.
+__device__ __forceinline__ int anew_after(int view, v4f& result) {
+  asm volatile("" : "+v"(view), "+v"(result));
+  return view;
+}
+
 // ROWS rows of COLS columns on their way from memory to a tile, by LANES lanes of which this is number `lane`: all loads first, so that
 // their latencies are one, and stores to LDS when they are due.
 template <typename T, int COLS, int LANES, int ROWS = 64>
@@ -314,11 +334,13 @@ struct DeltaArgs {
   int64_t pairs; // parts x heads
   int64_t parts; // sequences, or segments of them
   int segment;   // chunks of a segment, 0: sequences are not cut
-  // scratch, for every (slot, head): m[planes][64][64] and so on
+  // scratch, for every (slot, head): m[planes][64][64] and so on.  Bytes from one to the next:
+  int64_t square, state, rows;
   char* m;
   char* m_t;
   char* c;       // C scale, transposed in the backward
   float* gates;  // [3][64]: e^G, e^{G_63 - G}, beta
+  double* sums;  // [64]: G
   char* s;       // [planes][columns][DK], the state before the chunk
   char* d_s;     // the same of dS' behind it
   char* n;       // [planes][columns][64]

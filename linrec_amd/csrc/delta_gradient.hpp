@@ -38,11 +38,8 @@ template <typename T, int COLS, int LANES>
 struct InputStager {
   using U = Inner<T>;
   Stager<T, COLS, LANES> s;
-  __device__ __forceinline__ void fetch(const T* from, int64_t stride, int rows, int cols) {
-    s.fetch(from, stride, rows, cols, threadIdx.x & (LANES - 1));
-  }
-  __device__ __forceinline__ void put(char* tile) const {
-    const int lane = threadIdx.x & (LANES - 1);
+  __device__ __forceinline__ void fetch(const T* from, int64_t stride, int rows, int cols, int lane) { s.fetch(from, stride, rows, cols, lane); }
+  __device__ __forceinline__ void put(char* tile, int lane) const {
     if constexpr (std::is_same_v<T, U>) {
       s.put(tile, lane);
     } else {  // fp16 as two bf16
@@ -59,13 +56,6 @@ struct InputStager {
     }
   }
 };
-
-__device__ __forceinline__ float sum_of_16(float x) {
-  x += __shfl_xor(x, 1);
-  x += __shfl_xor(x, 2);
-  x += __shfl_xor(x, 4);
-  return x + __shfl_xor(x, 8);
-}
 
 enum GradientPart { GRADIENT_Q, GRADIENT_X, GRADIENT_Y };
 
@@ -86,7 +76,7 @@ __device__ __forceinline__ void gradient_part(const DeltaArgs& a, const Chunk& c
   constexpr int P = Sh::P, IN = Sh::IN, KT = DK / 16, LANES = GRADIENT_PART;
   constexpr int64_t ROW = WIDE ? 2 * DK : DK;  // of the kept states
   const linrec_delta_t& p = a.p;
-  const int lane = threadIdx.x & 63, r = lane & 15, q = lane >> 4, by = threadIdx.x & (LANES - 1);
+  const int lane = threadIdx.x & 63, r = lane & 15, q = lane >> 4, by0 = threadIdx.x & (LANES - 1);
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) & 3;
   const int row0 = 16 * wave + 4 * q;  // this lane's rows of a result
   const int rows_w0 = TI::natural_rows(r, q) + wave * (16 * TI::ROW), rows_m0 = TI::mapped_rows(r, q);
@@ -98,29 +88,42 @@ __device__ __forceinline__ void gradient_part(const DeltaArgs& a, const Chunk& c
   InputStager<T, 32, LANES> so, sv;
   Stager<U, 64, LANES, 32> sb[P], sn[P];
   Stager<U, DK, LANES, 32> ss[P];
+  // one wave has what belongs to the positions, a lane for each
+  const bool keeper = PART == GRADIENT_Y && wave == 0;
+  double sum = 0.0;
+  float gamma = 0.0f, rest = 0.0f, beta = 0.0f;
   auto fetch = [&](int head, int v0, int d0) __attribute__((always_inline)) {
     const int64_t block = slot * p.heads + head;
+    const int by = anew(by0);
+    if (keeper && v0 == 0) {
+      const int own = anew(lane);
+      sum = a.sums[block * 64 + own];
+      gamma = a.gates[block * 192 + own];
+      rest = a.gates[block * 192 + 64 + own];
+      beta = a.gates[block * 192 + 128 + own];
+    }
     if constexpr (PART == GRADIENT_Q) {
-      so.fetch(head_rows<T>(p.d_o, p.d_o_stride, ch.batch, ch.first, head) + v0, p.d_o_stride[1], ch.length, p.value_dim - v0);
-      sv.fetch(head_rows<T>(p.v, p.v_stride, ch.batch, ch.first, head) + v0, p.v_stride[1], ch.length, p.value_dim - v0);
+      so.fetch(head_rows<T>(p.d_o, p.d_o_stride, ch.batch, ch.first, head) + v0, p.d_o_stride[1], ch.length, p.value_dim - v0, by);
+      sv.fetch(head_rows<T>(p.v, p.v_stride, ch.batch, ch.first, head) + v0, p.v_stride[1], ch.length, p.value_dim - v0, by);
     }
 #pragma unroll
     for (int k = 0; k < P; ++k) {
-      const int64_t row = (block * P + k) * a.columns + v0;
+      const int64_t row = int64_t(k) * a.columns + v0;
       if constexpr (PART == GRADIENT_Q) {
-        sb[k].fetch_dense(reinterpret_cast<const U*>(a.d_b) + row * 64, by);
-        sn[k].fetch_dense(reinterpret_cast<const U*>(a.n) + row * 64, by);
+        sb[k].fetch_dense(reinterpret_cast<const U*>(a.d_b + block * a.rows) + row * 64, by);
+        sn[k].fetch_dense(reinterpret_cast<const U*>(a.n + block * a.rows) + row * 64, by);
       } else {
-        const U* from = reinterpret_cast<const U*>(PART == GRADIENT_X ? a.s : a.d_s) + row * ROW;
+        const U* from = reinterpret_cast<const U*>((PART == GRADIENT_X ? a.s : a.d_s) + block * a.state) + row * ROW;
         if constexpr (WIDE) ss[k].fetch(from + d0, ROW, 32, DK, by);
         else ss[k].fetch_dense(from, by);
       }
     }
   };
   auto put = [&](char* to) __attribute__((always_inline)) {
+    const int by = anew(by0);
     if constexpr (PART == GRADIENT_Q) {
-      so.put(to + Sh::O);
-      sv.put(to + Sh::V);
+      so.put(to + Sh::O, by);
+      sv.put(to + Sh::V, by);
     }
 #pragma unroll
     for (int k = 0; k < P; ++k) {
@@ -135,37 +138,39 @@ __device__ __forceinline__ void gradient_part(const DeltaArgs& a, const Chunk& c
 
   for (int d0 = 0; d0 < (WIDE ? p.key_dim : 1); d0 += DK) {
     v4f all[KT];  // this part's share of dQ or dK over the value heads
+    v4f before = v4f{0, 0, 0, 0};  // Y: K times what it was before this head, row by row
 #pragma unroll
     for (int u = 0; u < KT; ++u) all[u] = v4f{0, 0, 0, 0};
     {
       InputStager<T, DK, LANES> keys;
       if constexpr (PART == GRADIENT_X)
-        keys.fetch(head_rows<T>(p.k, p.k_stride, ch.batch, ch.first, key_head) + d0, p.k_stride[1], ch.length, p.key_dim - d0);
+        keys.fetch(head_rows<T>(p.k, p.k_stride, ch.batch, ch.first, key_head) + d0, p.k_stride[1], ch.length, p.key_dim - d0, by0);
       if constexpr (PART == GRADIENT_Y)
-        keys.fetch(head_rows<T>(p.q, p.q_stride, ch.batch, ch.first, key_head) + d0, p.q_stride[1], ch.length, p.key_dim - d0);
+        keys.fetch(head_rows<T>(p.q, p.q_stride, ch.batch, ch.first, key_head) + d0, p.q_stride[1], ch.length, p.key_dim - d0, by0);
       fetch(key_head * a.shared, 0, d0);
       __syncthreads();
-      if constexpr (PART != GRADIENT_Q) keys.put(smem + (PART == GRADIENT_X ? Sh::K : Sh::Q));
+      if constexpr (PART != GRADIENT_Q) keys.put(smem + (PART == GRADIENT_X ? Sh::K : Sh::Q), by0);
     }
     int turn = 0;
     for (int h = 0; h < a.shared; ++h) {
       const int head = key_head * a.shared + h;
       const int64_t block = slot * p.heads + head;
-      // (of the head before, these are read before the last barrier, or by the wave that writes them)
-      if (threadIdx.x < 64) {
-        const bool there = lane < ch.length;
-        const float g = there ? *(head_rows<float>(p.log_decay, p.log_decay_stride, ch.batch, ch.first + lane, head)) : 0.0f;
-        sh.g[lane] = chunk_sum(g, lane);
-        sh.gamma[lane] = a.gates[block * 192 + lane];
-        sh.rest[lane] = a.gates[block * 192 + 64 + lane];
-        sh.beta[lane] = a.gates[block * 192 + 128 + lane];
+      // (of the head before, others read these before the last barrier)
+      if (keeper) {
+        const int own = anew(lane);
+        sh.g[own] = sum;
+        sh.gamma[own] = gamma;
+        sh.rest[own] = rest;
+        sh.beta[own] = beta;
       }
       // F^T, dQ; E^T, X; F, E, Y
-      v4f f[4], ee[4], acc[KT], bv = v4f{0, 0, 0, 0}, inner = v4f{0, 0, 0, 0};
+      // (Y has the most operands: its rows of N are scaled on their way, so that it adds to the share itself)
+      v4f f[4], ee[4], acc[PART == GRADIENT_Y ? 1 : KT], bv = v4f{0, 0, 0, 0}, inner = v4f{0, 0, 0, 0};
 #pragma unroll
       for (int t = 0; t < 4; ++t) f[t] = ee[t] = v4f{0, 0, 0, 0};
+      if constexpr (PART != GRADIENT_Y)
 #pragma unroll
-      for (int u = 0; u < KT; ++u) acc[u] = v4f{0, 0, 0, 0};
+        for (int u = 0; u < KT; ++u) acc[u] = v4f{0, 0, 0, 0};
       for (int v0 = 0; v0 < p.value_dim; v0 += 32) {
         char* at = smem + (Sh::BUFFERS == 2 ? turn * Sh::STEP : 0);
         if constexpr (Sh::BUFFERS == 1) __syncthreads();
@@ -235,21 +240,34 @@ __device__ __forceinline__ void gradient_part(const DeltaArgs& a, const Chunk& c
               f[t] = mma(rows_in(Sh::O, rows_m, TI::mapped_row(t)), n_w, f[t]);
               ee[t] = mma(by_v_mapped(Sh::B, t), n_w, ee[t]);
             }
+          Planes<U> scaled;
+          {
+            const float by = sh.rest[16 * wave + anew(r)];
+            v4f n[2];
 #pragma unroll
-          for (int u = 0; u < KT; ++u) acc[u] = mma(n_w, state(Sh::D, u), acc[u]);
+            for (int e = 0; e < 8; ++e) {
+              float x = float(n_w.p[0][e]);
+              if constexpr (P == 2) x += float(n_w.p[1][e]);
+              n[e >> 2][e & 3] = by * x;
+            }
+            scaled = split<U>(n[0], n[1]);
+          }
+#pragma unroll
+          for (int u = 0; u < KT; ++u) all[u] = mma(scaled, state(Sh::D, u), all[u]);
         }
       }
-      const int cols_k = anew(cols_k0), points = anew(points0);
+      int cols_k = anew(cols_k0), points = anew(points0);
+      const int r1 = anew(r), row1 = 16 * wave + 4 * anew(q);
       // the masks and decays; rows of results to operands
       Planes<U> fp[2], ep[2];
       {
-        const int own = 16 * wave + r;
+        const int own = 16 * wave + anew(r), q1 = anew(q);
 #pragma unroll
         for (int t = 0; t < 4; ++t)
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
-            const int other = row_of_result(t, q) + e, i = PART == GRADIENT_Y ? other : own, j = PART == GRADIENT_Y ? own : other;
-            const float d = i >= j ? expf(float(sh.g[i] - sh.g[j])) : 0.0f;
+            const int other = row_of_result(t, q1) + e, i = PART == GRADIENT_Y ? other : own, j = PART == GRADIENT_Y ? own : other;
+            const float d = i >= j ? fast_exp(float(sh.g[i] - sh.g[j])) : 0.0f;
             if constexpr (PART != GRADIENT_X) f[t][e] = i >= j ? p.scale * d * f[t][e] : 0.0f;
             if constexpr (PART != GRADIENT_Q) ee[t][e] = i > j ? -(PART == GRADIENT_Y ? sh.beta[i] : 1.0f) * d * ee[t][e] : 0.0f;
           }
@@ -274,13 +292,15 @@ __device__ __forceinline__ void gradient_part(const DeltaArgs& a, const Chunk& c
         return out;
       };
       v4f dot = v4f{0, 0, 0, 0}, ends = v4f{0, 0, 0, 0};
-      v4f rows = *reinterpret_cast<const v4f*>((PART == GRADIENT_Y ? sh.rest : sh.gamma) + row0);
-      if constexpr (PART == GRADIENT_Q) rows *= p.scale;
-      if constexpr (PART == GRADIENT_X) rows = -rows;
-      const v4f beta = *reinterpret_cast<const v4f*>(sh.beta + row0);
+      v4f by_row = *reinterpret_cast<const v4f*>(sh.gamma + row1);
+      if constexpr (PART == GRADIENT_Q) by_row *= p.scale;
+      if constexpr (PART == GRADIENT_X) by_row = -by_row;
+      const v4f beta_of = *reinterpret_cast<const v4f*>(sh.beta + row1);
 #pragma unroll
       for (int u = 0; u < KT; ++u) {
-        v4f z = rows * acc[u];
+        v4f z;
+        if constexpr (PART == GRADIENT_Y) z = all[u];
+        else z = by_row * acc[u];
         const v4f x = values(PART == GRADIENT_Q ? Sh::Q : Sh::K, u);
         if constexpr (PART == GRADIENT_Y) ends += x * z;
 #pragma unroll
@@ -295,51 +315,62 @@ __device__ __forceinline__ void gradient_part(const DeltaArgs& a, const Chunk& c
           }
         }
         dot += x * z;
-        if constexpr (PART == GRADIENT_X) z *= beta;
-        all[u] += z;
+        // (reads of the next columns, all ahead of their products, would push other values out of the registers)
+        points = anew_after(points, dot);
+        cols_k = anew_after(cols_k, z);
+        if constexpr (PART == GRADIENT_X) z *= beta_of;
+        if constexpr (PART == GRADIENT_Y) all[u] = z;
+        else all[u] += z;
+      }
+      if constexpr (PART == GRADIENT_Y) {
+        const v4f now = dot;
+        dot -= before;
+        ends -= before;
+        before = now;
       }
       float* to = PART == GRADIENT_Q ? sh.q : PART == GRADIENT_X ? sh.x : sh.y;
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         const float d = sum_of_16(dot[e]);
-        if (r == 0) to[row0 + e] = d;
+        if (r1 == 0) to[row1 + e] = d;
       }
       if constexpr (PART == GRADIENT_X) {
         // dB.V and <S, dS'> stand on diagonals, lane 16 q + 4 q + e
 #pragma unroll
         for (int e = 0; e < 4; ++e)
-          if (r == 4 * q + e) {
-            sh.bv[row0 + e] = bv[e];
+          if (r1 == row1 - 16 * wave + e) {
+            sh.bv[row1 + e] = bv[e];
             ends[0] = sh.gamma[63] * inner[e];
           }
       }
       if constexpr (PART != GRADIENT_Q) {
-        float sum = sum_of_16((ends[0] + ends[1]) + (ends[2] + ends[3]));
-        sum += __shfl_xor(sum, 16);
-        sum += __shfl_xor(sum, 32);
-        if (lane == 0) sh.sum[PART == GRADIENT_X ? wave : 4 + wave] = sum;
+        float whole = sum_of_16((ends[0] + ends[1]) + (ends[2] + ends[3]));
+        whole += __shfl_xor(whole, 16);
+        whole += __shfl_xor(whole, 32);
+        if (lane == 0) sh.sum[PART == GRADIENT_X ? wave : 4 + wave] = whole;
       }
       __syncthreads();
-      if (threadIdx.x < 64) {  // a lane for a position
-        float* dots = a.dots + block * 192;  // (every place is written and read by one lane)
-        float total = sh.q[lane] + sh.beta[lane] * sh.x[lane] - sh.y[lane], d_beta = sh.x[lane] + (d0 == 0 ? sh.bv[lane] : 0.0f);
-        if (lane == 63) total += ((sh.sum[0] + sh.sum[1]) + (sh.sum[2] + sh.sum[3])) + ((sh.sum[4] + sh.sum[5]) + (sh.sum[6] + sh.sum[7]));
+      if (keeper) {
+        const int own = anew(lane);
+        float* dots = a.dots + block * 192;  // (every place is written and read by one own)
+        float total = sh.q[own] + sh.beta[own] * sh.x[own] - sh.y[own], d_beta = sh.x[own] + (d0 == 0 ? sh.bv[own] : 0.0f);
+        if (own == 63) total += ((sh.sum[0] + sh.sum[1]) + (sh.sum[2] + sh.sum[3])) + ((sh.sum[4] + sh.sum[5]) + (sh.sum[6] + sh.sum[7]));
         if (WIDE && d0 > 0) {
-          total += dots[lane];
-          d_beta += dots[64 + lane];
+          total += dots[own];
+          d_beta += dots[64 + own];
         }
         if (WIDE && d0 + DK < p.key_dim) {
-          dots[lane] = total;
-          dots[64 + lane] = d_beta;
+          dots[own] = total;
+          dots[64 + own] = d_beta;
         } else {
           double after = double(total);
 #pragma unroll
           for (int d = 1; d < 64; d <<= 1) {
             const double up = __shfl_down(after, d);
-            if (lane + d < 64) after += up;
+            if (own + d < 64) after += up;
           }
-          if (lane < ch.length) {
-            const int64_t at = (ch.batch * p.time + ch.first + lane) * p.heads + head;
+          if (own < ch.length) {
+            const int64_t at = (ch.batch * p.time + ch.first + own) * p.heads + head;
             p.d_log_decay[at] = float(after);
             p.d_beta[at] = d_beta;
           }

@@ -76,6 +76,7 @@ __global__ __launch_bounds__(256) void delta_prepare_kernel(DeltaArgs a) {
     gates[lane] = expf(float(sum));
     gates[64 + lane] = expf(float(last - sum));
     gates[128 + lane] = beta;
+    if constexpr (BWD) a.sums[block * 64 + lane] = sum;
   }
   __syncthreads();
   v4f kk[4], qk[4];
@@ -104,7 +105,7 @@ __global__ __launch_bounds__(256) void delta_prepare_kernel(DeltaArgs a) {
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         const int i = 16 * wave + 4 * q + e;
-        const float d = i >= j ? expf(float(sh_g[i] - sh_g[j])) : 0.0f;
+        const float d = i >= j ? fast_exp(float(sh_g[i] - sh_g[j])) : 0.0f;
         sh_a[i * S + j] = i > j ? sh_beta[i] * d * kk[t][e] : 0.0f;
         sh_c[i * S + j] = i >= j ? p.scale * d * qk[t][e] : 0.0f;
       }
@@ -157,10 +158,9 @@ __global__ __launch_bounds__(256) void delta_prepare_kernel(DeltaArgs a) {
     for (int e = 0; e < 4; ++e) sh_m[(32 + 16 * rt + 4 * q + e) * S + 16 * ct + r] = -y[e];
   }
   __syncthreads();
-  constexpr int64_t SQUARE = 64 * 64 * int64_t(sizeof(U)) * planes_of<U>();
-  store_square<U, false>(a.m + block * SQUARE, sh_m);
-  if constexpr (BWD) store_square<U, true>(a.m_t + block * SQUARE, sh_m);
-  store_square<U, BWD>(a.c + block * SQUARE, sh_c);
+  store_square<U, false>(a.m + block * a.square, sh_m);
+  if constexpr (BWD) store_square<U, true>(a.m_t + block * a.square, sh_m);
+  store_square<U, BWD>(a.c + block * a.square, sh_c);
 }
 
 }  // namespace linrec

@@ -25,7 +25,7 @@ __global__ __launch_bounds__((ReverseShared<T, DK, WAVES>::LANES)) void delta_re
   using TK = Tile<T, DK>;
   using TV = Tile<T, 16 * WAVES>;
   using TS = Tile<U, 64>;
-  constexpr int P = planes_of<U>(), STAGING = 64 * WAVES, SQUARE = square_bytes<U>(), IN = input_planes<T>();
+  constexpr int P = planes_of<U>(), STAGING = 64 * WAVES, IN = input_planes<T>();
   __shared__ __align__(16) char room[Sh::BYTES * (Sh::LOADERS ? 2 : 1)];
   const linrec_delta_t& p = a.p;
   int64_t pair;
@@ -54,8 +54,8 @@ __global__ __launch_bounds__((ReverseShared<T, DK, WAVES>::LANES)) void delta_re
     o.fetch(head_rows<T>(p.d_o, p.d_o_stride, span.batch, first, head) + c0, p.d_o_stride[1], length, p.value_dim - c0, by);
 #pragma unroll
     for (int k2 = 0; k2 < P; ++k2) {
-      m[k2].fetch_dense(reinterpret_cast<const U*>(a.m_t + block * SQUARE) + k2 * 4096, by);
-      cc[k2].fetch_dense(reinterpret_cast<const U*>(a.c + block * SQUARE) + k2 * 4096, by);
+      m[k2].fetch_dense(reinterpret_cast<const U*>(a.m_t + block * a.square) + k2 * 4096, by);
+      cc[k2].fetch_dense(reinterpret_cast<const U*>(a.c + block * a.square) + k2 * 4096, by);
     }
 #pragma unroll
     for (int i = 0; i < (192 + STAGING - 1) / STAGING; ++i)
@@ -101,7 +101,7 @@ __global__ __launch_bounds__((ReverseShared<T, DK, WAVES>::LANES)) void delta_re
     float un_s;
     split_scaled<T>(s, sp, &un_s);
     if constexpr (!CARRY) {
-      U* to = reinterpret_cast<U*>(a.d_s) + block * P * a.columns * DK;
+      U* to = reinterpret_cast<U*>(a.d_s + block * a.state);
 #pragma unroll
       for (int b = 0; b < DK / 32; ++b) {
         if (!kept_column) break;
@@ -155,7 +155,7 @@ __global__ __launch_bounds__((ReverseShared<T, DK, WAVES>::LANES)) void delta_re
       for (int b = t / 2; b < 2; ++b) db[t] = mma(square(Sh::M, t, b), xp[b], db[t]);
     }
     if (!CARRY && kept_column) {
-      U* to = reinterpret_cast<U*>(a.d_b) + block * P * a.columns * 64;
+      U* to = reinterpret_cast<U*>(a.d_b + block * a.rows);
 #pragma unroll
       for (int b = 0; b < 2; ++b) {
         const Planes<U> kept = split<U>(db[2 * b], db[2 * b + 1]);

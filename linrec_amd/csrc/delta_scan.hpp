@@ -51,7 +51,7 @@ __global__ __launch_bounds__((ScanShared<T, DK, WAVES, MODE>::LANES)) void delta
   using TK = Tile<T, DK>;
   using TV = Tile<T, 16 * WAVES>;
   using TS = Tile<U, 64>;
-  constexpr int P = planes_of<U>(), STAGING = 64 * WAVES, SQUARE = square_bytes<U>();
+  constexpr int P = planes_of<U>(), STAGING = 64 * WAVES;
   __shared__ __align__(16) char room[Sh::BYTES * (Sh::LOADERS ? 2 : 1)];
   const linrec_delta_t& p = a.p;
   int64_t pair;
@@ -82,8 +82,8 @@ __global__ __launch_bounds__((ScanShared<T, DK, WAVES, MODE>::LANES)) void delta
     else v.clear();
 #pragma unroll
     for (int k2 = 0; k2 < P; ++k2) {
-      m[k2].fetch_dense(reinterpret_cast<const U*>(a.m + block * SQUARE) + k2 * 4096, by);
-      if constexpr (MODE == SCAN_OUT) cc[k2].fetch_dense(reinterpret_cast<const U*>(a.c + block * SQUARE) + k2 * 4096, by);
+      m[k2].fetch_dense(reinterpret_cast<const U*>(a.m + block * a.square) + k2 * 4096, by);
+      if constexpr (MODE == SCAN_OUT) cc[k2].fetch_dense(reinterpret_cast<const U*>(a.c + block * a.square) + k2 * 4096, by);
     }
 #pragma unroll
     for (int i = 0; i < (192 + STAGING - 1) / STAGING; ++i)
@@ -135,7 +135,7 @@ __global__ __launch_bounds__((ScanShared<T, DK, WAVES, MODE>::LANES)) void delta
     float un_s;
     split_scaled<T>(s, sp, &un_s);
     if constexpr (MODE == SCAN_STATES) {
-      U* to = reinterpret_cast<U*>(a.s) + block * P * a.columns * DK;
+      U* to = reinterpret_cast<U*>(a.s + block * a.state);
 #pragma unroll
       for (int b = 0; b < DK / 32; ++b) {
         if (!kept_column) break;
@@ -182,7 +182,7 @@ __global__ __launch_bounds__((ScanShared<T, DK, WAVES, MODE>::LANES)) void delta
     for (int b = 0; b < 2; ++b) np[b] = split<U>(nn[2 * b], nn[2 * b + 1]);
     if constexpr (MODE == SCAN_CARRY) {
     } else if constexpr (MODE == SCAN_STATES) {
-      U* to = reinterpret_cast<U*>(a.n) + block * P * a.columns * 64;
+      U* to = reinterpret_cast<U*>(a.n + block * a.rows);
 #pragma unroll
       for (int b = 0; b < 2; ++b)
 #pragma unroll

@@ -8,17 +8,18 @@
 // and the gradient of log_decay is the sum of dG from a position to the chunk's end.
 //
 // A workgroup has a (chunk, key head) and walks over the value heads that share it, so that nothing is added by atomics.  Value
-// channels come 32 at a time through LDS, the next ones on their way in registers meanwhile.  Its waves have three parts, four waves
-// of 16 rows each: dQ, X and Y.  (One wave for all three holds twice the registers that three waves to a SIMD leave it, and what
-// then goes through scratch costs more than the products: 2.4 ms instead of the time below.)  The 64 x 64 products F, F^T, E, E^T are
-// computed as they are needed as operands: what a lane gets of a product is its part of an operand over the product's rows.
+// channels come 32 at a time through LDS, the next ones on their way in registers meanwhile.  Its waves have two parts, four waves
+// of 16 rows each: dQ and X, which multiply S, and Y, which multiplies dS'.  One wave for all three would hold more than its share of the
+// registers (what then goes through scratch costs more than the products: 2.4 ms for 8 x 4096 x 16 heads of 128 x 128 bf16), three
+// parts read S from LDS twice (0.79 ms).  The 64 x 64 products F, F^T, E, E^T are computed as they are needed as operands: what a
+// lane gets of a product is its part of an operand over the product's rows.
 #pragma once
 #include "delta_prepare.hpp"
 #include "delta_scan.hpp"
 
 namespace linrec {
 
-constexpr int GRADIENT_LANES = 768, GRADIENT_PART = 256;
+constexpr int GRADIENT_LANES = 512, GRADIENT_PART = 256;
 
 template <typename T, int DK>
 struct GradientShared {
@@ -57,16 +58,27 @@ struct InputStager {
   }
 };
 
-enum GradientPart { GRADIENT_Q, GRADIENT_X, GRADIENT_Y };
-
 template <typename T, int DK>
 struct GradientScratch {  // LDS beside GradientShared
   double g[64];
-  alignas(16) float gamma[64], rest[64], beta[64], q[64], x[64], y[64], bv[64], sum[8];
+  alignas(16) float gamma[64], rest[64], beta[64], q[64], x[64], y[64], bv[64], sum[4];
 };
 
-// What the waves of one part do.  All parts meet at the same barriers.
-template <typename T, int DK, bool WIDE, GradientPart PART>
+// An operand with its rows scaled.
+template <typename U, int N>
+__device__ __forceinline__ Planes<U> scaled(const Planes<U, N>& f, float by) {
+  v4f x[2];
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    float v = float(f.p[0][e]);
+    if constexpr (N == 2) v += float(f.p[1][e]);
+    x[e >> 2][e & 3] = by * v;
+  }
+  return split<U>(x[0], x[1]);
+}
+
+// What the waves of one part do: dQ and X, or (BEHIND) Y.  Both parts meet at the same barriers.
+template <typename T, int DK, bool WIDE, bool BEHIND>
 __device__ __forceinline__ void gradient_part(const DeltaArgs& a, const Chunk& ch, int64_t slot, int key_head, char* smem, GradientScratch<T, DK>& sh) {
   using U = Inner<T>;
   using Sh = GradientShared<T, DK>;
@@ -78,18 +90,17 @@ __device__ __forceinline__ void gradient_part(const DeltaArgs& a, const Chunk& c
   const linrec_delta_t& p = a.p;
   const int lane = threadIdx.x & 63, r = lane & 15, q = lane >> 4, by0 = threadIdx.x & (LANES - 1);
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) & 3;
-  const int row0 = 16 * wave + 4 * q;  // this lane's rows of a result
   const int rows_w0 = TI::natural_rows(r, q) + wave * (16 * TI::ROW), rows_m0 = TI::mapped_rows(r, q);
   const int cols_w0 = TB::template column_tile<false>(TB::template columns<false>(r, q), wave), cols_m0 = TB::template columns<true>(r, q);
   const int cols_k0 = TK::template columns<false>(r, q), rows_v0 = TK::natural_rows(r, q) + (wave & 1) * (16 * TK::ROW),
             points0 = TK::points(r, q) + wave * (16 * TK::ROW);
 
-  // each part loads some of a step: the rows of dO and V with dB and N, S, dS'
+  // what a step needs on its way: the rows of dO and V with dB and N, or S and dS'
   InputStager<T, 32, LANES> so, sv;
   Stager<U, 64, LANES, 32> sb[P], sn[P];
-  Stager<U, DK, LANES, 32> ss[P];
+  Stager<U, DK, LANES, 32> ss[P], sd[P];
   // one wave has what belongs to the positions, a lane for each
-  const bool keeper = PART == GRADIENT_Y && wave == 0;
+  const bool keeper = BEHIND && wave == 0;
   double sum = 0.0;
   float gamma = 0.0f, rest = 0.0f, beta = 0.0f;
   auto fetch = [&](int head, int v0, int d0) __attribute__((always_inline)) {
@@ -102,54 +113,63 @@ __device__ __forceinline__ void gradient_part(const DeltaArgs& a, const Chunk& c
       rest = a.gates[block * 192 + 64 + own];
       beta = a.gates[block * 192 + 128 + own];
     }
-    if constexpr (PART == GRADIENT_Q) {
+    if constexpr (!BEHIND) {
       so.fetch(head_rows<T>(p.d_o, p.d_o_stride, ch.batch, ch.first, head) + v0, p.d_o_stride[1], ch.length, p.value_dim - v0, by);
       sv.fetch(head_rows<T>(p.v, p.v_stride, ch.batch, ch.first, head) + v0, p.v_stride[1], ch.length, p.value_dim - v0, by);
     }
 #pragma unroll
     for (int k = 0; k < P; ++k) {
       const int64_t row = int64_t(k) * a.columns + v0;
-      if constexpr (PART == GRADIENT_Q) {
+      if constexpr (!BEHIND) {
         sb[k].fetch_dense(reinterpret_cast<const U*>(a.d_b + block * a.rows) + row * 64, by);
         sn[k].fetch_dense(reinterpret_cast<const U*>(a.n + block * a.rows) + row * 64, by);
       } else {
-        const U* from = reinterpret_cast<const U*>((PART == GRADIENT_X ? a.s : a.d_s) + block * a.state) + row * ROW;
-        if constexpr (WIDE) ss[k].fetch(from + d0, ROW, 32, DK, by);
-        else ss[k].fetch_dense(from, by);
+        const U* s = reinterpret_cast<const U*>(a.s + block * a.state) + row * ROW;
+        const U* d = reinterpret_cast<const U*>(a.d_s + block * a.state) + row * ROW;
+        if constexpr (WIDE) {
+          ss[k].fetch(s + d0, ROW, 32, DK, by);
+          sd[k].fetch(d + d0, ROW, 32, DK, by);
+        } else {
+          ss[k].fetch_dense(s, by);
+          sd[k].fetch_dense(d, by);
+        }
       }
     }
   };
   auto put = [&](char* to) __attribute__((always_inline)) {
     const int by = anew(by0);
-    if constexpr (PART == GRADIENT_Q) {
+    if constexpr (!BEHIND) {
       so.put(to + Sh::O, by);
       sv.put(to + Sh::V, by);
     }
 #pragma unroll
     for (int k = 0; k < P; ++k) {
-      if constexpr (PART == GRADIENT_Q) {
+      if constexpr (!BEHIND) {
         sb[k].put(to + Sh::B + k * Sh::BY_V, by);
         sn[k].put(to + Sh::N + k * Sh::BY_V, by);
       } else {
-        ss[k].put(to + (PART == GRADIENT_X ? Sh::S : Sh::D) + k * Sh::STATE, by);
+        ss[k].put(to + Sh::S + k * Sh::STATE, by);
+        sd[k].put(to + Sh::D + k * Sh::STATE, by);
       }
     }
   };
 
   for (int d0 = 0; d0 < (WIDE ? p.key_dim : 1); d0 += DK) {
-    v4f all[KT];  // this part's share of dQ or dK over the value heads
-    v4f before = v4f{0, 0, 0, 0};  // Y: K times what it was before this head, row by row
+    // dQ, or Y, over the value heads (their rows are scaled on their way, so that products add to the sums themselves), and beta X
+    v4f all[KT], all_x[BEHIND ? 1 : KT];
+    v4f before = v4f{0, 0, 0, 0};  // Q dQ, or K Y, before this head, row by row
 #pragma unroll
     for (int u = 0; u < KT; ++u) all[u] = v4f{0, 0, 0, 0};
+    if constexpr (!BEHIND)
+#pragma unroll
+      for (int u = 0; u < KT; ++u) all_x[u] = v4f{0, 0, 0, 0};
     {
       InputStager<T, DK, LANES> keys;
-      if constexpr (PART == GRADIENT_X)
-        keys.fetch(head_rows<T>(p.k, p.k_stride, ch.batch, ch.first, key_head) + d0, p.k_stride[1], ch.length, p.key_dim - d0, by0);
-      if constexpr (PART == GRADIENT_Y)
-        keys.fetch(head_rows<T>(p.q, p.q_stride, ch.batch, ch.first, key_head) + d0, p.q_stride[1], ch.length, p.key_dim - d0, by0);
+      const T* from = BEHIND ? head_rows<T>(p.q, p.q_stride, ch.batch, ch.first, key_head) : head_rows<T>(p.k, p.k_stride, ch.batch, ch.first, key_head);
+      keys.fetch(from + d0, BEHIND ? p.q_stride[1] : p.k_stride[1], ch.length, p.key_dim - d0, by0);
       fetch(key_head * a.shared, 0, d0);
       __syncthreads();
-      if constexpr (PART != GRADIENT_Q) keys.put(smem + (PART == GRADIENT_X ? Sh::K : Sh::Q), by0);
+      keys.put(smem + (BEHIND ? Sh::Q : Sh::K), by0);
     }
     int turn = 0;
     for (int h = 0; h < a.shared; ++h) {
@@ -163,14 +183,12 @@ __device__ __forceinline__ void gradient_part(const DeltaArgs& a, const Chunk& c
         sh.rest[own] = rest;
         sh.beta[own] = beta;
       }
-      // F^T, dQ; E^T, X; F, E, Y
-      // (Y has the most operands: its rows of N are scaled on their way, so that it adds to the share itself)
-      v4f f[4], ee[4], acc[PART == GRADIENT_Y ? 1 : KT], bv = v4f{0, 0, 0, 0}, inner = v4f{0, 0, 0, 0};
+      v4f f[4], ee[4], x[BEHIND ? 1 : KT], bv = v4f{0, 0, 0, 0}, inner = v4f{0, 0, 0, 0};
 #pragma unroll
       for (int t = 0; t < 4; ++t) f[t] = ee[t] = v4f{0, 0, 0, 0};
-      if constexpr (PART != GRADIENT_Y)
+      if constexpr (!BEHIND)
 #pragma unroll
-        for (int u = 0; u < KT; ++u) acc[u] = v4f{0, 0, 0, 0};
+        for (int u = 0; u < KT; ++u) x[u] = v4f{0, 0, 0, 0};
       for (int v0 = 0; v0 < p.value_dim; v0 += 32) {
         char* at = smem + (Sh::BUFFERS == 2 ? turn * Sh::STEP : 0);
         if constexpr (Sh::BUFFERS == 1) __syncthreads();
@@ -205,21 +223,36 @@ __device__ __forceinline__ void gradient_part(const DeltaArgs& a, const Chunk& c
           for (int k = 0; k < P; ++k) out.p[k] = TK::template column_frag<false>(at + part + k * Sh::STATE, cols_k, 0, u);
           return out;
         };
-        if constexpr (PART == GRADIENT_Q) {
+        const Planes<U> db_w = by_v(Sh::B);
+        const int own = 16 * wave + anew(r);
+        if constexpr (!BEHIND) {
           const Planes<U, IN> do_w = rows_in(Sh::O, rows_w, 0);
 #pragma unroll
           for (int t = 0; t < 4; ++t)
-            if (t / 2 <= wave / 2) f[t] = mma(by_v_mapped(Sh::N, t), do_w, f[t]);  // rows j up to this wave's columns i
+            if (t / 2 <= wave / 2) {  // rows j of F^T and E^T up to this wave's columns i
+              const Planes<U> n_t = by_v_mapped(Sh::N, t);
+              f[t] = mma(n_t, do_w, f[t]);
+              ee[t] = mma(n_t, db_w, ee[t]);
+            }
+          const Planes<U> do_s = scaled<U>(do_w, p.scale * sh.gamma[own]);
 #pragma unroll
-          for (int u = 0; u < KT; ++u) acc[u] = mma(do_w, state(Sh::S, u), acc[u]);
-        } else if constexpr (PART == GRADIENT_X) {
-          const Planes<U> db_w = by_v(Sh::B);
+          for (int u = 0; u < KT; ++u) {
+            const Planes<U> s_u = state(Sh::S, u);
+            all[u] = mma(do_s, s_u, all[u]);
+            x[u] = mma(db_w, s_u, x[u]);
+          }
+        } else {
+          const Planes<U> n_w = by_v(Sh::N);
 #pragma unroll
           for (int t = 0; t < 4; ++t)
-            if (t / 2 <= wave / 2) ee[t] = mma(by_v_mapped(Sh::N, t), db_w, ee[t]);
-#pragma unroll
-          for (int u = 0; u < KT; ++u) acc[u] = mma(db_w, state(Sh::S, u), acc[u]);
+            if (t / 2 >= wave / 2) {
+              f[t] = mma(rows_in(Sh::O, rows_m, TI::mapped_row(t)), n_w, f[t]);
+              ee[t] = mma(by_v_mapped(Sh::B, t), n_w, ee[t]);
+            }
           bv = mma(db_w, rows_in(Sh::V, rows_w, 0), bv);
+          const Planes<U> n_s = scaled<U>(n_w, sh.rest[own]);
+#pragma unroll
+          for (int u = 0; u < KT; ++u) all[u] = mma(n_s, state(Sh::D, u), all[u]);
           // <S, dS'> on the diagonal of S^T dS', 16 channels at a time
 #pragma unroll
           for (int b = 0; b < DK / 32; ++b)
@@ -232,28 +265,6 @@ __device__ __forceinline__ void gradient_part(const DeltaArgs& a, const Chunk& c
               }
               inner = mma(s_v, d_v, inner);
             }
-        } else {
-          const Planes<U> n_w = by_v(Sh::N);
-#pragma unroll
-          for (int t = 0; t < 4; ++t)
-            if (t / 2 >= wave / 2) {
-              f[t] = mma(rows_in(Sh::O, rows_m, TI::mapped_row(t)), n_w, f[t]);
-              ee[t] = mma(by_v_mapped(Sh::B, t), n_w, ee[t]);
-            }
-          Planes<U> scaled;
-          {
-            const float by = sh.rest[16 * wave + anew(r)];
-            v4f n[2];
-#pragma unroll
-            for (int e = 0; e < 8; ++e) {
-              float x = float(n_w.p[0][e]);
-              if constexpr (P == 2) x += float(n_w.p[1][e]);
-              n[e >> 2][e & 3] = by * x;
-            }
-            scaled = split<U>(n[0], n[1]);
-          }
-#pragma unroll
-          for (int u = 0; u < KT; ++u) all[u] = mma(scaled, state(Sh::D, u), all[u]);
         }
       }
       int cols_k = anew(cols_k0), points = anew(points0);
@@ -266,15 +277,15 @@ __device__ __forceinline__ void gradient_part(const DeltaArgs& a, const Chunk& c
         for (int t = 0; t < 4; ++t)
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
-            const int other = row_of_result(t, q1) + e, i = PART == GRADIENT_Y ? other : own, j = PART == GRADIENT_Y ? own : other;
+            const int other = row_of_result(t, q1) + e, i = BEHIND ? other : own, j = BEHIND ? own : other;
             const float d = i >= j ? fast_exp(float(sh.g[i] - sh.g[j])) : 0.0f;
-            if constexpr (PART != GRADIENT_X) f[t][e] = i >= j ? p.scale * d * f[t][e] : 0.0f;
-            if constexpr (PART != GRADIENT_Q) ee[t][e] = i > j ? -(PART == GRADIENT_Y ? sh.beta[i] : 1.0f) * d * ee[t][e] : 0.0f;
+            f[t][e] = i >= j ? p.scale * d * f[t][e] : 0.0f;
+            ee[t][e] = i > j ? -(BEHIND ? sh.beta[i] : 1.0f) * d * ee[t][e] : 0.0f;
           }
 #pragma unroll
         for (int b = 0; b < 2; ++b) {
-          if constexpr (PART != GRADIENT_X) fp[b] = split<U>(f[2 * b], f[2 * b + 1]);
-          if constexpr (PART != GRADIENT_Q) ep[b] = split<U>(ee[2 * b], ee[2 * b + 1]);
+          fp[b] = split<U>(f[2 * b], f[2 * b + 1]);
+          ep[b] = split<U>(ee[2 * b], ee[2 * b + 1]);
         }
       }
       auto keys = [&](int part, int b, int u) __attribute__((always_inline)) {
@@ -291,70 +302,74 @@ __device__ __forceinline__ void gradient_part(const DeltaArgs& a, const Chunk& c
           for (int e = 0; e < 4; ++e) out[e] += TK::point(smem + part + k * Sh::KEYS, points, 0, e, u);
         return out;
       };
-      v4f dot = v4f{0, 0, 0, 0}, ends = v4f{0, 0, 0, 0};
-      v4f by_row = *reinterpret_cast<const v4f*>(sh.gamma + row1);
-      if constexpr (PART == GRADIENT_Q) by_row *= p.scale;
-      if constexpr (PART == GRADIENT_X) by_row = -by_row;
-      const v4f beta_of = *reinterpret_cast<const v4f*>(sh.beta + row1);
+      v4f dot = v4f{0, 0, 0, 0}, dot_x = v4f{0, 0, 0, 0}, ends = v4f{0, 0, 0, 0};
+      const v4f down = -*reinterpret_cast<const v4f*>(sh.gamma + row1), beta_of = *reinterpret_cast<const v4f*>(sh.beta + row1);
 #pragma unroll
       for (int u = 0; u < KT; ++u) {
-        v4f z;
-        if constexpr (PART == GRADIENT_Y) z = all[u];
-        else z = by_row * acc[u];
-        const v4f x = values(PART == GRADIENT_Q ? Sh::Q : Sh::K, u);
-        if constexpr (PART == GRADIENT_Y) ends += x * z;
+        const v4f kv = values(Sh::K, u);
+        v4f z = all[u];
+        if constexpr (!BEHIND) {
+          const v4f qv = values(Sh::Q, u);
+          v4f xu = down * x[u];
 #pragma unroll
-        for (int b = 0; b < 2; ++b) {
-          if constexpr (PART == GRADIENT_Q) {
-            if (b <= wave / 2) z = mma(fp[b], keys(Sh::K, b, u), z);
-          } else if constexpr (PART == GRADIENT_X) {
-            if (b <= wave / 2) z = mma(ep[b], keys(Sh::K, b, u), z);
-          } else if (b >= wave / 2) {
-            z = mma(fp[b], keys(Sh::Q, b, u), z);
-            z = mma(ep[b], keys(Sh::K, b, u), z);
-          }
+          for (int b = 0; b < 2; ++b)
+            if (b <= wave / 2) {
+              const Planes<U, IN> k_b = keys(Sh::K, b, u);
+              z = mma(fp[b], k_b, z);
+              xu = mma(ep[b], k_b, xu);
+            }
+          dot += qv * z;
+          dot_x += kv * xu;
+          all_x[u] += beta_of * xu;
+        } else {
+          ends += kv * z;
+#pragma unroll
+          for (int b = 0; b < 2; ++b)
+            if (b >= wave / 2) {
+              z = mma(fp[b], keys(Sh::Q, b, u), z);
+              z = mma(ep[b], keys(Sh::K, b, u), z);
+            }
+          dot += kv * z;
         }
-        dot += x * z;
         // (reads of the next columns, all ahead of their products, would push other values out of the registers)
         points = anew_after(points, dot);
         cols_k = anew_after(cols_k, z);
-        if constexpr (PART == GRADIENT_X) z *= beta_of;
-        if constexpr (PART == GRADIENT_Y) all[u] = z;
-        else all[u] += z;
+        all[u] = z;
       }
-      if constexpr (PART == GRADIENT_Y) {
-        const v4f now = dot;
-        dot -= before;
-        ends -= before;
-        before = now;
-      }
-      float* to = PART == GRADIENT_Q ? sh.q : PART == GRADIENT_X ? sh.x : sh.y;
+      const v4f now = dot;
+      dot -= before;
+      ends -= before;
+      before = now;
+      float* to = BEHIND ? sh.y : sh.q;
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         const float d = sum_of_16(dot[e]);
         if (r1 == 0) to[row1 + e] = d;
+        if constexpr (!BEHIND) {
+          const float dx = sum_of_16(dot_x[e]);
+          if (r1 == 0) sh.x[row1 + e] = dx;
+        }
       }
-      if constexpr (PART == GRADIENT_X) {
+      if constexpr (BEHIND) {
+        float whole = (ends[0] + ends[1]) + (ends[2] + ends[3]);
         // dB.V and <S, dS'> stand on diagonals, lane 16 q + 4 q + e
 #pragma unroll
         for (int e = 0; e < 4; ++e)
           if (r1 == row1 - 16 * wave + e) {
             sh.bv[row1 + e] = bv[e];
-            ends[0] = sh.gamma[63] * inner[e];
+            whole = fmaf(sh.gamma[63], inner[e], whole);
           }
-      }
-      if constexpr (PART != GRADIENT_Q) {
-        float whole = sum_of_16((ends[0] + ends[1]) + (ends[2] + ends[3]));
+        whole = sum_of_16(whole);
         whole += __shfl_xor(whole, 16);
         whole += __shfl_xor(whole, 32);
-        if (lane == 0) sh.sum[PART == GRADIENT_X ? wave : 4 + wave] = whole;
+        if (lane == 0) sh.sum[wave] = whole;
       }
       __syncthreads();
       if (keeper) {
         const int own = anew(lane);
-        float* dots = a.dots + block * 192;  // (every place is written and read by one own)
+        float* dots = a.dots + block * 192;  // (every place is written and read by one lane)
         float total = sh.q[own] + sh.beta[own] * sh.x[own] - sh.y[own], d_beta = sh.x[own] + (d0 == 0 ? sh.bv[own] : 0.0f);
-        if (own == 63) total += ((sh.sum[0] + sh.sum[1]) + (sh.sum[2] + sh.sum[3])) + ((sh.sum[4] + sh.sum[5]) + (sh.sum[6] + sh.sum[7]));
+        if (own == 63) total += (sh.sum[0] + sh.sum[1]) + (sh.sum[2] + sh.sum[3]);
         if (WIDE && d0 > 0) {
           total += dots[own];
           d_beta += dots[64 + own];
@@ -380,24 +395,25 @@ __device__ __forceinline__ void gradient_part(const DeltaArgs& a, const Chunk& c
     // the two shares of dK together
     __syncthreads();
     float* sh_k = reinterpret_cast<float*>(smem);
-    if constexpr (PART == GRADIENT_Y)
+    const int r2 = anew(r), row2 = 16 * wave + 4 * anew(q);
+    if constexpr (BEHIND)
 #pragma unroll
       for (int u = 0; u < KT; ++u)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) sh_k[(row0 + e) * DK + 16 * u + r] = all[u][e];
+        for (int e = 0; e < 4; ++e) sh_k[(row2 + e) * DK + 16 * u + r2] = all[u][e];
     __syncthreads();
-    if constexpr (PART != GRADIENT_Y) {
-      T* out = static_cast<T*>(PART == GRADIENT_Q ? p.d_q : p.d_k);
+    if constexpr (!BEHIND)
 #pragma unroll
       for (int e = 0; e < 4; ++e)
-        if (row0 + e < ch.length) {
-          const int64_t at = ((ch.batch * p.time + ch.first + row0 + e) * p.key_heads + key_head) * int64_t(p.key_dim) + d0;
+        if (row2 + e < ch.length) {
+          const int64_t at = ((ch.batch * p.time + ch.first + row2 + e) * p.key_heads + key_head) * int64_t(p.key_dim) + d0;
 #pragma unroll
           for (int u = 0; u < KT; ++u)
-            if (d0 + 16 * u + r < p.key_dim)
-              out[at + 16 * u + r] = T(PART == GRADIENT_Q ? all[u][e] : all[u][e] + sh_k[(row0 + e) * DK + 16 * u + r]);
+            if (d0 + 16 * u + r2 < p.key_dim) {
+              static_cast<T*>(p.d_q)[at + 16 * u + r2] = T(all[u][e]);
+              static_cast<T*>(p.d_k)[at + 16 * u + r2] = T(all_x[u][e] + sh_k[(row2 + e) * DK + 16 * u + r2]);
+            }
         }
-    }
   }
 }
 
@@ -410,10 +426,8 @@ __global__ __launch_bounds__(GRADIENT_LANES) void delta_gradient_kernel(DeltaArg
   const int key_head = int(blockIdx.x - slot * unsigned(a.p.key_heads));
   const Chunk ch = chunk_of(a.p, slot);
   if (ch.length == 0) return;
-  const int part = __builtin_amdgcn_readfirstlane(threadIdx.x >> 8);
-  if (part == 0) gradient_part<T, DK, WIDE, GRADIENT_Q>(a, ch, slot, key_head, smem, sh);
-  else if (part == 1) gradient_part<T, DK, WIDE, GRADIENT_X>(a, ch, slot, key_head, smem, sh);
-  else gradient_part<T, DK, WIDE, GRADIENT_Y>(a, ch, slot, key_head, smem, sh);
+  if (__builtin_amdgcn_readfirstlane(threadIdx.x >> 8) == 0) gradient_part<T, DK, WIDE, false>(a, ch, slot, key_head, smem, sh);
+  else gradient_part<T, DK, WIDE, true>(a, ch, slot, key_head, smem, sh);
 }
 
 }  // namespace linrec

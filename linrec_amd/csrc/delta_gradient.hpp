@@ -332,8 +332,10 @@ __device__ __forceinline__ void gradient_part(const DeltaArgs& a, const Chunk& c
           dot += kv * z;
         }
         // (reads of the next columns, all ahead of their products, would push other values out of the registers)
-        points = anew_after(points, dot);
-        cols_k = anew_after(cols_k, z);
+        if constexpr (!BEHIND) {
+          points = anew_after(points, dot);
+          cols_k = anew_after(cols_k, z);
+        }
         all[u] = z;
       }
       const v4f now = dot;

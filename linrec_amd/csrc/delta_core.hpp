@@ -99,6 +99,25 @@ __device__ __forceinline__ v4f mma(const Frag<U>& a, const Planes<U, N>& b, v4f 
   return c;
 }
 
+// The same for several tiles: one instruction of each before the next of any, whose results it would wait for.  COUNT tiles from FIRST.
+template <int FIRST, int COUNT, typename U, int NB, int N>
+__device__ __forceinline__ void mma_tiles(const Frag<U> (&a)[N], const Planes<U, NB>& b, v4f* c) {
+#pragma unroll
+  for (int j = NB - 1; j >= 0; --j)
+#pragma unroll
+    for (int t = FIRST; t < FIRST + COUNT; ++t) c[t] = mma(a[t], b.p[j], c[t]);
+}
+template <int FIRST, int COUNT, typename U, int NA, int NB, int N>
+__device__ __forceinline__ void mma_tiles(const Planes<U, NA> (&a)[N], const Planes<U, NB>& b, v4f* c) {
+#pragma unroll
+  for (int i = NA - 1; i >= 0; --i)
+#pragma unroll
+    for (int j = NB - 1; j >= 0; --j)
+      if (i + j < (NA > NB ? NA : NB))
+#pragma unroll
+        for (int t = FIRST; t < FIRST + COUNT; ++t) c[t] = mma(a[t].p[i], b.p[j], c[t]);
+}
+
 // Results of two products side by side are one operand of the next.  Row r of tile t of an operand whose products' rows are summed
 // over next stands for row_of_tile(t, r): then lane 16 q + r holds, of tiles 2 p and 2 p + 1, rows 32 p + 8 q to 32 p + 8 q + 7.
 __device__ __forceinline__ int row_of_tile(int t, int r) { return 32 * (t >> 1) + 8 * (r >> 2) + 4 * (t & 1) + (r & 3); }
@@ -168,7 +187,6 @@ struct Tile {
   static __device__ __forceinline__ int row_view(int row, int q) { return at(row, HALF ? q : 2 * q); }
   static __device__ __forceinline__ int natural_rows(int r, int q) { return row_view(r, q); }
   static __device__ __forceinline__ int mapped_rows(int r, int q) { return row_view(row_of_tile(0, r), q); }
-  static __device__ __forceinline__ constexpr int natural_row(int t) { return 16 * t; }
   static __device__ __forceinline__ constexpr int mapped_row(int t) { return 32 * (t >> 1) + 4 * (t & 1); }
   // columns 32 p + 8 q and up
   static __device__ __forceinline__ Frag<U> frag(const char* tile, int view, int rows, int p) {

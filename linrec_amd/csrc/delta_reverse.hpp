@@ -112,11 +112,18 @@ __global__ __launch_bounds__((ReverseShared<T, DK, WAVES>::LANES)) void delta_re
         for (int k2 = 0; k2 < P; ++k2) *reinterpret_cast<Frag<U>*>(to + (int64_t(k2) * a.columns + col) * DK + 32 * b + 8 * q) = kept.p[k2];
       }
     }
-    auto square = [&](int at, int t, int b) __attribute__((always_inline)) {
-      Planes<U> f;
+    // upper triangular: the first 32 positions have no part in rows from 32 on
+    auto upper = [&](int at, const auto(&by)[2], v4f* to) __attribute__((always_inline)) {
+      Planes<U> f[4];
 #pragma unroll
-      for (int k2 = 0; k2 < P; ++k2) f.p[k2] = TS::frag(smem + at + k2 * TS::BYTES, rows_s, TS::mapped_row(t), b);
-      return f;
+      for (int b = 0; b < 2; ++b) {
+#pragma unroll
+        for (int t = 0; t < 2 + 2 * b; ++t)
+#pragma unroll
+          for (int k2 = 0; k2 < P; ++k2) f[t].p[k2] = TS::frag(smem + at + k2 * TS::BYTES, rows_s, TS::mapped_row(t), b);
+        if (b == 0) mma_tiles<0, 2>(f, by[b], to);
+        else mma_tiles<0, 4>(f, by[b], to);
+      }
     };
     // dO of this wave's columns, a result's layout; fp16 as two bf16
     v4f d_o[4];
@@ -134,26 +141,24 @@ __global__ __launch_bounds__((ReverseShared<T, DK, WAVES>::LANES)) void delta_re
     }
     v4f x[4];  // dN
 #pragma unroll
-    for (int t = 0; t < 4; ++t) {
-      x[t] = v4f{0, 0, 0, 0};
+    for (int t = 0; t < 4; ++t) x[t] = v4f{0, 0, 0, 0};
 #pragma unroll
-      for (int b = 0; b < DK / 32; ++b) x[t] = mma(TK::frag(smem + Sh::K, rows_k, TK::mapped_row(t), b), sp[b], x[t]);
-      const v4f rest = *reinterpret_cast<const v4f*>(gates + 64 + row_of_result(t, q));
+    for (int b = 0; b < DK / 32; ++b) {
+      Frag<T> f[4];
 #pragma unroll
-      for (int e = 0; e < 4; ++e) x[t][e] *= rest[e] * un_s;
-#pragma unroll
-      for (int b = t / 2; b < 2; ++b) x[t] = mma(square(Sh::C, t, b), dop[b], x[t]);
+      for (int t = 0; t < 4; ++t) f[t] = TK::frag(smem + Sh::K, rows_k, TK::mapped_row(t), b);
+      mma_tiles<0, 4>(f, sp[b], x);
     }
+#pragma unroll
+    for (int t = 0; t < 4; ++t) x[t] *= *reinterpret_cast<const v4f*>(gates + 64 + row_of_result(t, q)) * un_s;
+    upper(Sh::C, dop, x);
     Planes<U> xp[2];
 #pragma unroll
     for (int b = 0; b < 2; ++b) xp[b] = split<U>(x[2 * b], x[2 * b + 1]);
     v4f db[4];
 #pragma unroll
-    for (int t = 0; t < 4; ++t) {
-      db[t] = v4f{0, 0, 0, 0};
-#pragma unroll
-      for (int b = t / 2; b < 2; ++b) db[t] = mma(square(Sh::M, t, b), xp[b], db[t]);
-    }
+    for (int t = 0; t < 4; ++t) db[t] = v4f{0, 0, 0, 0};
+    upper(Sh::M, xp, db);
     if (!CARRY && kept_column) {
       U* to = reinterpret_cast<U*>(a.d_b + block * a.rows);
 #pragma unroll

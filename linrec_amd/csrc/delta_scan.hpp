@@ -148,16 +148,26 @@ __global__ __launch_bounds__((ScanShared<T, DK, WAVES, MODE>::LANES)) void delta
     }
     v4f x[4];  // K S, then beta (V - e^G K S)
 #pragma unroll
-    for (int t = 0; t < 4; ++t) {
-      x[t] = v4f{0, 0, 0, 0};
+    for (int t = 0; t < 4; ++t) x[t] = v4f{0, 0, 0, 0};
 #pragma unroll
-      for (int b = 0; b < DK / 32; ++b) x[t] = mma(TK::frag(smem + Sh::K, rows_k, TK::mapped_row(t), b), sp[b], x[t]);
+    for (int b = 0; b < DK / 32; ++b) {
+      Frag<T> f[4];
+#pragma unroll
+      for (int t = 0; t < 4; ++t) f[t] = TK::frag(smem + Sh::K, rows_k, TK::mapped_row(t), b);
+      mma_tiles<0, 4>(f, sp[b], x);
     }
-    auto square = [&](int at, int t, int b) __attribute__((always_inline)) {
-      Planes<U> f;
+    // lower triangular: positions from 32 on have no part in the first 32 rows
+    auto lower = [&](int at, const Planes<U>(&by)[2], v4f* to) __attribute__((always_inline)) {
+      Planes<U> f[4];
 #pragma unroll
-      for (int k2 = 0; k2 < P; ++k2) f.p[k2] = TS::frag(smem + at + k2 * TS::BYTES, rows_s, TS::mapped_row(t), b);
-      return f;
+      for (int b = 0; b < 2; ++b) {
+#pragma unroll
+        for (int t = 2 * b; t < 4; ++t)
+#pragma unroll
+          for (int k2 = 0; k2 < P; ++k2) f[t].p[k2] = TS::frag(smem + at + k2 * TS::BYTES, rows_s, TS::mapped_row(t), b);
+        if (b == 0) mma_tiles<0, 4>(f, by[b], to);
+        else mma_tiles<2, 2>(f, by[b], to);
+      }
     };
 #pragma unroll
     for (int t = 0; t < 4; ++t) {
@@ -172,11 +182,8 @@ __global__ __launch_bounds__((ScanShared<T, DK, WAVES, MODE>::LANES)) void delta
     for (int b = 0; b < 2; ++b) xp[b] = split<U>(x[2 * b], x[2 * b + 1]);
     v4f nn[4];
 #pragma unroll
-    for (int t = 0; t < 4; ++t) {
-      nn[t] = v4f{0, 0, 0, 0};
-#pragma unroll
-      for (int b = 0; b <= t / 2; ++b) nn[t] = mma(square(Sh::M, t, b), xp[b], nn[t]);
-    }
+    for (int t = 0; t < 4; ++t) nn[t] = v4f{0, 0, 0, 0};
+    lower(Sh::M, xp, nn);
     Planes<U> np[2];
 #pragma unroll
     for (int b = 0; b < 2; ++b) np[b] = split<U>(nn[2 * b], nn[2 * b + 1]);
@@ -190,36 +197,39 @@ __global__ __launch_bounds__((ScanShared<T, DK, WAVES, MODE>::LANES)) void delta
           if (kept_column) *reinterpret_cast<Frag<U>*>(to + (int64_t(k2) * a.columns + col) * 64 + 32 * b + 8 * q) = np[b].p[k2];
     } else {
       T* o = static_cast<T*>(p.o) + ((span.batch * p.time + first) * p.heads + head) * int64_t(p.value_dim) + col;
+      v4f y[4];
 #pragma unroll
-      for (int t = 0; t < 4; ++t) {
-        v4f y = v4f{0, 0, 0, 0};
-        const int from = row_of_tile(t, r);
+      for (int t = 0; t < 4; ++t) y[t] = v4f{0, 0, 0, 0};
 #pragma unroll
-        for (int b = 0; b < DK / 32; ++b) {
+      for (int b = 0; b < DK / 32; ++b) {
+        Frag<T> f[4];
+#pragma unroll
+        for (int t = 0; t < 4; ++t) {
           if constexpr (Sh::QUERIES) {
-            y = mma(TK::frag(smem + Sh::Q, rows_k, TK::mapped_row(t), b), sp[b], y);
+            f[t] = TK::frag(smem + Sh::Q, rows_k, TK::mapped_row(t), b);
           } else {
-            Frag<T> f;
+            const int from = row_of_tile(t, r);
 #pragma unroll
-            for (int e = 0; e < 8; ++e) f[e] = from < length && 32 * b + 8 * q + e < p.key_dim ? qq[from * p.q_stride[1] + 32 * b + 8 * q + e] : T(0.0f);
-            y = mma(f, sp[b], y);
+            for (int e = 0; e < 8; ++e) f[t][e] = from < length && 32 * b + 8 * q + e < p.key_dim ? qq[from * p.q_stride[1] + 32 * b + 8 * q + e] : T(0.0f);
           }
         }
+        mma_tiles<0, 4>(f, sp[b], y);
+      }
+#pragma unroll
+      for (int t = 0; t < 4; ++t) y[t] *= *reinterpret_cast<const v4f*>(gates + row_of_result(t, q)) * (un_s * p.scale);
+      lower(Sh::C, np, y);
+#pragma unroll
+      for (int t = 0; t < 4; ++t) {
         const int row = row_of_result(t, q);
-        const v4f gamma = *reinterpret_cast<const v4f*>(gates + row);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) y[e] *= gamma[e] * un_s * p.scale;
-#pragma unroll
-        for (int b = 0; b <= t / 2; ++b) y = mma(square(Sh::C, t, b), np[b], y);
         T* to = o + row * int64_t(p.heads) * p.value_dim;
         if (length == DELTA_CHUNK) {
           if (mine)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) to[e * (p.heads * p.value_dim)] = T(y[e]);
+            for (int e = 0; e < 4; ++e) to[e * (p.heads * p.value_dim)] = T(y[t][e]);
         } else {
 #pragma unroll
           for (int e = 0; e < 4; ++e)
-            if (mine && row + e < length) to[e * (p.heads * p.value_dim)] = T(y[e]);
+            if (mine && row + e < length) to[e * (p.heads * p.value_dim)] = T(y[t][e]);
         }
       }
     }
@@ -230,16 +240,19 @@ __global__ __launch_bounds__((ScanShared<T, DK, WAVES, MODE>::LANES)) void delta
     split_scaled<T>(nn, nt, &un_n);
     const float keep = gates[63];
 #pragma unroll
-    for (int t = 0; t < DK / 16; ++t) {
-      auto added = [&](v4f to) __attribute__((always_inline)) {
+    for (int t0 = 0; t0 < DK / 16; t0 += 4) {
+      v4f to[4];
 #pragma unroll
-        for (int b = 0; b < 2; ++b)
-          to = mma(TK::template column_frag<true>(smem + Sh::K, cols_k, b, t), nt[b], to);
-        return to;
-      };
-      s[t] *= keep;
-      if constexpr (std::is_same_v<T, _Float16>) s[t] += un_n * added(v4f{0, 0, 0, 0});
-      else s[t] = added(s[t]);
+      for (int t = 0; t < 4; ++t) to[t] = std::is_same_v<T, _Float16> ? v4f{0, 0, 0, 0} : s[t0 + t] * keep;
+#pragma unroll
+      for (int b = 0; b < 2; ++b) {
+        Frag<T> f[4];
+#pragma unroll
+        for (int t = 0; t < 4; ++t) f[t] = TK::template column_frag<true>(smem + Sh::K, cols_k, b, t0 + t);
+        mma_tiles<0, 4>(f, nt[b], to);
+      }
+#pragma unroll
+      for (int t = 0; t < 4; ++t) s[t0 + t] = std::is_same_v<T, _Float16> ? s[t0 + t] * keep + un_n * to[t] : to[t];
     }
   };
 

@@ -332,6 +332,26 @@ struct Stager {
     for (int n = 0; n < N; ++n)
       if (ROWS % STEP == 0 || n * STEP + lane / L::UNITS < ROWS) v[n] = reinterpret_cast<const V*>(from)[n * LANES + lane];
   }
+  // pieces of store_rows: PIECES of a group of 16 rows from FROM_PIECE on, of EVERY that it has
+  template <int EVERY = L::UNITS / 4>
+  __device__ __forceinline__ void fetch_pieces(const T* from, int from_piece, int lane) {
+    constexpr int GROUP = L::UNITS / 4 * 64;  // units of a group here
+    static_assert(LANES % 64 == 0 && ROWS % 16 == 0, "");
+#pragma unroll
+    for (int n = 0; n < N; ++n) {
+      const int i = n * LANES + lane, g = i / GROUP;
+      if (ROWS % STEP == 0 || i < ROWS * L::UNITS) v[n] = reinterpret_cast<const V*>(from)[(g * EVERY + from_piece) * 64 + i - g * GROUP];
+    }
+  }
+  __device__ __forceinline__ void put_pieces(char* tile, int lane) const {
+    constexpr int GROUP = L::UNITS / 4 * 64;
+#pragma unroll
+    for (int n = 0; n < N; ++n) {
+      const int i = n * LANES + lane, g = i / GROUP, k = (i - g * GROUP) >> 6, r = i & 15, q = (i >> 4) & 3;
+      if (ROWS % STEP == 0 || i < ROWS * L::UNITS)
+        *reinterpret_cast<V*>(tile + L::at(16 * g + r, L::HALF ? 4 * k + q : 8 * (k >> 1) + 2 * q + (k & 1))) = v[n];
+    }
+  }
   __device__ __forceinline__ void put(char* tile, int lane) const {
 #pragma unroll
     for (int n = 0; n < N; ++n)
@@ -339,6 +359,26 @@ struct Stager {
         *reinterpret_cast<V*>(tile + L::at(n * STEP + lane / L::UNITS, lane % L::UNITS)) = v[n];
   }
 };
+
+// Operands of 16 rows, a lane's as it has them: pieces of 1 KB that a wave stores and loads whole (rows of their own would be stored 64
+// bytes at a time).  `to`: of plane k at to + k * plane; b: which 32 columns.
+template <typename U>
+__device__ __forceinline__ void store_rows(U* to, int64_t plane, int b, int lane, const Planes<U>& f) {
+#pragma unroll
+  for (int k = 0; k < planes_of<U>(); ++k) {
+    if constexpr (sizeof(U) == 2) {
+      *reinterpret_cast<Frag<U>*>(to + k * plane + b * 512 + lane * 8) = f.p[k];
+    } else {
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        v4f x;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) x[e] = f.p[k][4 * h + e];
+        *reinterpret_cast<v4f*>(to + k * plane + (2 * b + h) * 256 + lane * 4) = x;
+      }
+    }
+  }
+}
 
 // ---- chunks and scratch ----------------------------------------------------------------------------------------------------------
 // A chunk has a slot: those of a sequence follow each other, a packed sequence's start at cu_seqlens[n] / 64 + n (so that no two
@@ -359,9 +399,9 @@ struct DeltaArgs {
   char* c;       // C scale, transposed in the backward
   float* gates;  // [3][64]: e^G, e^{G_63 - G}, beta
   double* sums;  // [64]: G
-  char* s;       // [planes][columns][DK], the state before the chunk
+  char* s;       // [planes][columns][DK] in pieces of 16 columns (store_rows), the state before the chunk
   char* d_s;     // the same of dS' behind it
-  char* n;       // [planes][columns][64]
+  char* n;       // [planes][columns][64] in such pieces
   char* d_b;
   float* dots;   // [192], sums of the gates' gradients where key_dim comes in turns
   // for every (part, head), where sequences are cut (delta_segments.hpp)

@@ -121,18 +121,14 @@ __device__ __forceinline__ void gradient_part(const DeltaArgs& a, const Chunk& c
     for (int k = 0; k < P; ++k) {
       const int64_t row = int64_t(k) * a.columns + v0;
       if constexpr (!BEHIND) {
-        sb[k].fetch_dense(reinterpret_cast<const U*>(a.d_b + block * a.rows) + row * 64, by);
-        sn[k].fetch_dense(reinterpret_cast<const U*>(a.n + block * a.rows) + row * 64, by);
+        sb[k].fetch_pieces(reinterpret_cast<const U*>(a.d_b + block * a.rows) + row * 64, 0, by);
+        sn[k].fetch_pieces(reinterpret_cast<const U*>(a.n + block * a.rows) + row * 64, 0, by);
       } else {
         const U* s = reinterpret_cast<const U*>(a.s + block * a.state) + row * ROW;
         const U* d = reinterpret_cast<const U*>(a.d_s + block * a.state) + row * ROW;
-        if constexpr (WIDE) {
-          ss[k].fetch(s + d0, ROW, 32, DK, by);
-          sd[k].fetch(d + d0, ROW, 32, DK, by);
-        } else {
-          ss[k].fetch_dense(s, by);
-          sd[k].fetch_dense(d, by);
-        }
+        constexpr int EVERY = int(ROW * int64_t(sizeof(U)) / 64);
+        ss[k].template fetch_pieces<EVERY>(s, WIDE ? d0 * int(sizeof(U)) / 64 : 0, by);
+        sd[k].template fetch_pieces<EVERY>(d, WIDE ? d0 * int(sizeof(U)) / 64 : 0, by);
       }
     }
   };
@@ -145,11 +141,11 @@ __device__ __forceinline__ void gradient_part(const DeltaArgs& a, const Chunk& c
 #pragma unroll
     for (int k = 0; k < P; ++k) {
       if constexpr (!BEHIND) {
-        sb[k].put(to + Sh::B + k * Sh::BY_V, by);
-        sn[k].put(to + Sh::N + k * Sh::BY_V, by);
+        sb[k].put_pieces(to + Sh::B + k * Sh::BY_V, by);
+        sn[k].put_pieces(to + Sh::N + k * Sh::BY_V, by);
       } else {
-        ss[k].put(to + Sh::S + k * Sh::STATE, by);
-        sd[k].put(to + Sh::D + k * Sh::STATE, by);
+        ss[k].put_pieces(to + Sh::S + k * Sh::STATE, by);
+        sd[k].put_pieces(to + Sh::D + k * Sh::STATE, by);
       }
     }
   };

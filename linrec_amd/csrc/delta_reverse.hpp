@@ -101,15 +101,14 @@ __global__ __launch_bounds__((ReverseShared<T, DK, WAVES>::LANES)) void delta_re
     float un_s;
     split_scaled<T>(s, sp, &un_s);
     if constexpr (!CARRY) {
-      U* to = reinterpret_cast<U*>(a.d_s + block * a.state);
+      U* to = reinterpret_cast<U*>(a.d_s + block * a.state) + int64_t(col - r) * DK;
 #pragma unroll
       for (int b = 0; b < DK / 32; ++b) {
         if (!kept_column) break;
         Planes<U> kept;
         if constexpr (std::is_same_v<T, _Float16>) kept = split<U>(s[2 * b], s[2 * b + 1]);
         else kept = sp[b];
-#pragma unroll
-        for (int k2 = 0; k2 < P; ++k2) *reinterpret_cast<Frag<U>*>(to + (int64_t(k2) * a.columns + col) * DK + 32 * b + 8 * q) = kept.p[k2];
+        store_rows<U>(to, int64_t(a.columns) * DK, b, lane, kept);
       }
     }
     // upper triangular: the first 32 positions have no part in rows from 32 on
@@ -160,13 +159,9 @@ __global__ __launch_bounds__((ReverseShared<T, DK, WAVES>::LANES)) void delta_re
     for (int t = 0; t < 4; ++t) db[t] = v4f{0, 0, 0, 0};
     upper(Sh::M, xp, db);
     if (!CARRY && kept_column) {
-      U* to = reinterpret_cast<U*>(a.d_b + block * a.rows);
+      U* to = reinterpret_cast<U*>(a.d_b + block * a.rows) + (col - r) * 64;
 #pragma unroll
-      for (int b = 0; b < 2; ++b) {
-        const Planes<U> kept = split<U>(db[2 * b], db[2 * b + 1]);
-#pragma unroll
-        for (int k2 = 0; k2 < P; ++k2) *reinterpret_cast<Frag<U>*>(to + (int64_t(k2) * a.columns + col) * 64 + 32 * b + 8 * q) = kept.p[k2];
-      }
+      for (int b = 0; b < 2; ++b) store_rows<U>(to, int64_t(a.columns) * 64, b, lane, split<U>(db[2 * b], db[2 * b + 1]));
     }
     const int apart = p.heads * p.value_dim;
     T* d_v = static_cast<T*>(p.d_v) + ((span.batch * p.time + first) * p.heads + head) * int64_t(p.value_dim) + col;

@@ -135,15 +135,14 @@ __global__ __launch_bounds__((ScanShared<T, DK, WAVES, MODE>::LANES)) void delta
     float un_s;
     split_scaled<T>(s, sp, &un_s);
     if constexpr (MODE == SCAN_STATES) {
-      U* to = reinterpret_cast<U*>(a.s + block * a.state);
+      U* to = reinterpret_cast<U*>(a.s + block * a.state) + int64_t(col - r) * DK;
 #pragma unroll
       for (int b = 0; b < DK / 32; ++b) {
         if (!kept_column) break;
         Planes<U> kept;
         if constexpr (std::is_same_v<T, _Float16>) kept = split<U>(s[2 * b], s[2 * b + 1]);
         else kept = sp[b];
-#pragma unroll
-        for (int k2 = 0; k2 < P; ++k2) *reinterpret_cast<Frag<U>*>(to + (int64_t(k2) * a.columns + col) * DK + 32 * b + 8 * q) = kept.p[k2];
+        store_rows<U>(to, int64_t(a.columns) * DK, b, lane, kept);
       }
     }
     v4f x[4];  // K S, then beta (V - e^G K S)
@@ -189,12 +188,10 @@ __global__ __launch_bounds__((ScanShared<T, DK, WAVES, MODE>::LANES)) void delta
     for (int b = 0; b < 2; ++b) np[b] = split<U>(nn[2 * b], nn[2 * b + 1]);
     if constexpr (MODE == SCAN_CARRY) {
     } else if constexpr (MODE == SCAN_STATES) {
-      U* to = reinterpret_cast<U*>(a.n + block * a.rows);
+      U* to = reinterpret_cast<U*>(a.n + block * a.rows) + (col - r) * 64;
 #pragma unroll
       for (int b = 0; b < 2; ++b)
-#pragma unroll
-        for (int k2 = 0; k2 < P; ++k2)
-          if (kept_column) *reinterpret_cast<Frag<U>*>(to + (int64_t(k2) * a.columns + col) * 64 + 32 * b + 8 * q) = np[b].p[k2];
+        if (kept_column) store_rows<U>(to, int64_t(a.columns) * 64, b, lane, np[b]);
     } else {
       T* o = static_cast<T*>(p.o) + ((span.batch * p.time + first) * p.heads + head) * int64_t(p.value_dim) + col;
       v4f y[4];

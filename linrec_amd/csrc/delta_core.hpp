@@ -17,10 +17,11 @@
 // of the time axis and keeps its key_dim x 16 part of S in accumulators; what it multiplies them with is the same for all waves and
 // comes through LDS.
 //
-// Precision.  States, sums and accumulators are fp32.  An operand of a matrix instruction that is not an input is split into two
-// bf16 (or, beside fp16 inputs, fp16) numbers, its rounding and the rounding of the rest, which together carry 16 bits and more: a
-// product with an input is two instructions, one of two such operands three, and a state is about 1e-6 off.  One bf16 each would
-// be 2e-3.  fp32 inputs take the fp32 instructions.
+// Precision.  States, sums and accumulators are fp32.  An operand of a matrix instruction that is not an input is split into
+// bf16 (or, beside fp16 inputs, fp16) numbers, its rounding, the rounding of the rest and so on: two bf16 carry 16 to 17 bits, three 24, two
+// fp16 22.  In the chain of products that makes a state from the one before, what meets an input is three bf16 or two fp16, and what meets M
+// three bf16; M, C and all that is kept for the gradients are two.  So a state is 1e-6 off and a gradient 3e-6 (with two bf16 in the
+// chain 5e-6 and 1e-5, with one 2e-3).  fp32 inputs take the fp32 instructions.
 #pragma once
 #include <hip/hip_runtime.h>
 #include <stdint.h>
@@ -83,14 +84,19 @@ __device__ __forceinline__ v4f mma(const Frag<float>& a, const Frag<float>& b, v
   for (int e = 0; e < 8; ++e) c = __builtin_amdgcn_mfma_f32_16x16x4f32(a[e], b[e], c, 0, 0, 0);
   return c;
 }
-template <typename U, int NA, int NB>
-__device__ __forceinline__ v4f mma(const Planes<U, NA>& a, const Planes<U, NB>& b, v4f c) {
+// MOST: planes whose numbers add up to more than this are left out, the product of two rests where both operands have two.
+template <int MOST, typename U, int NA, int NB>
+__device__ __forceinline__ v4f mma_up_to(const Planes<U, NA>& a, const Planes<U, NB>& b, v4f c) {
 #pragma unroll
   for (int i = NA - 1; i >= 0; --i)
 #pragma unroll
     for (int j = NB - 1; j >= 0; --j)
-      if (i + j < (NA > NB ? NA : NB)) c = mma(a.p[i], b.p[j], c);  // (the product of two rests is below what is kept)
+      if (i + j <= MOST) c = mma(a.p[i], b.p[j], c);
   return c;
+}
+template <typename U, int NA, int NB>
+__device__ __forceinline__ v4f mma(const Planes<U, NA>& a, const Planes<U, NB>& b, v4f c) {
+  return mma_up_to<(NA > NB ? NA : NB) - 1>(a, b, c);
 }
 template <typename U, int N>
 __device__ __forceinline__ v4f mma(const Frag<U>& a, const Planes<U, N>& b, v4f c) {
@@ -123,15 +129,30 @@ __device__ __forceinline__ void mma_tiles(const Planes<U, NA> (&a)[N], const Pla
 __device__ __forceinline__ int row_of_tile(int t, int r) { return 32 * (t >> 1) + 8 * (r >> 2) + 4 * (t & 1) + (r & 3); }
 __device__ __forceinline__ int row_of_result(int t, int q) { return 32 * (t >> 1) + 8 * q + 4 * (t & 1); }  // (the first of four)
 
-template <typename U>
-__device__ __forceinline__ Planes<U> split(const v4f& lo, const v4f& hi) {
-  Planes<U> out;
+template <typename U, int N = planes_of<U>()>
+__device__ __forceinline__ Planes<U, N> split(const v4f& lo, const v4f& hi) {
+  Planes<U, N> out;
 #pragma unroll
   for (int e = 0; e < 8; ++e) {
-    const float x = e < 4 ? lo[e & 3] : hi[e & 3];
-    out.p[0][e] = U(x);
-    if constexpr (planes_of<U>() == 2) out.p[1][e] = U(x - float(out.p[0][e]));
+    float x = e < 4 ? lo[e & 3] : hi[e & 3];
+#pragma unroll
+    for (int k = 0; k < N; ++k) {
+      out.p[k][e] = U(x);
+      if (k + 1 < N) x -= float(out.p[k][e]);
+    }
   }
+  return out;
+}
+// Planes of an operand in the chain of products of a state.
+template <typename U>
+constexpr int chain_planes() {
+  return std::is_same_v<U, __bf16> ? 3 : planes_of<U>();
+}
+// The third of them, where two are there.
+__device__ __forceinline__ Planes<__bf16, 1> third_plane(const v4f& lo, const v4f& hi, const Planes<__bf16>& f) {
+  Planes<__bf16, 1> out;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) out.p[0][e] = __bf16((e < 4 ? lo[e & 3] : hi[e & 3]) - float(f.p[0][e]) - float(f.p[1][e]));
   return out;
 }
 
@@ -156,13 +177,13 @@ __device__ __forceinline__ float column_factor(const v4f (&x)[N], float* inverse
     return __uint_as_float(unsigned(267 - ex) << 23);
   }
 }
-template <typename T, int N>
-__device__ __forceinline__ void split_scaled(const v4f (&x)[N], Planes<T> (&out)[N / 2], float* inverse) {
+template <typename T, int N, int P>
+__device__ __forceinline__ void split_scaled(const v4f (&x)[N], Planes<T, P> (&out)[N / 2], float* inverse) {
   const float f = column_factor<T>(x, inverse);
 #pragma unroll
   for (int p = 0; p < N / 2; ++p) {
-    if constexpr (std::is_same_v<T, _Float16>) out[p] = split<T>(x[2 * p] * f, x[2 * p + 1] * f);
-    else out[p] = split<T>(x[2 * p], x[2 * p + 1]);
+    if constexpr (std::is_same_v<T, _Float16>) out[p] = split<T, P>(x[2 * p] * f, x[2 * p + 1] * f);
+    else out[p] = split<T, P>(x[2 * p], x[2 * p + 1]);
   }
 }
 

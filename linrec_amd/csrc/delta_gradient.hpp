@@ -65,8 +65,8 @@ struct GradientScratch {  // LDS beside GradientShared
 };
 
 // An operand with its rows scaled.
-template <typename U, int N>
-__device__ __forceinline__ Planes<U> scaled(const Planes<U, N>& f, float by) {
+template <typename U, int OUT, int N>
+__device__ __forceinline__ Planes<U, OUT> scaled(const Planes<U, N>& f, float by) {
   v4f x[2];
 #pragma unroll
   for (int e = 0; e < 8; ++e) {
@@ -74,7 +74,7 @@ __device__ __forceinline__ Planes<U> scaled(const Planes<U, N>& f, float by) {
     if constexpr (N == 2) v += float(f.p[1][e]);
     x[e >> 2][e & 3] = by * v;
   }
-  return split<U>(x[0], x[1]);
+  return split<U, OUT>(x[0], x[1]);
 }
 
 // What the waves of one part do: dQ and X, or (BEHIND) Y.  Both parts meet at the same barriers.
@@ -228,9 +228,9 @@ __device__ __forceinline__ void gradient_part(const DeltaArgs& a, const Chunk& c
             if (t / 2 <= wave / 2) {  // rows j of F^T and E^T up to this wave's columns i
               const Planes<U> n_t = by_v_mapped(Sh::N, t);
               f[t] = mma(n_t, do_w, f[t]);
-              ee[t] = mma(n_t, db_w, ee[t]);
+              ee[t] = mma_up_to<2>(n_t, db_w, ee[t]);
             }
-          const Planes<U> do_s = scaled<U>(do_w, p.scale * sh.gamma[own]);
+          const Planes<U> do_s = scaled<U, P>(do_w, p.scale * sh.gamma[own]);
 #pragma unroll
           for (int u = 0; u < KT; ++u) {
             const Planes<U> s_u = state(Sh::S, u);
@@ -243,10 +243,11 @@ __device__ __forceinline__ void gradient_part(const DeltaArgs& a, const Chunk& c
           for (int t = 0; t < 4; ++t)
             if (t / 2 >= wave / 2) {
               f[t] = mma(rows_in(Sh::O, rows_m, TI::mapped_row(t)), n_w, f[t]);
-              ee[t] = mma(by_v_mapped(Sh::B, t), n_w, ee[t]);
+              ee[t] = mma_up_to<2>(by_v_mapped(Sh::B, t), n_w, ee[t]);
             }
           bv = mma(db_w, rows_in(Sh::V, rows_w, 0), bv);
-          const Planes<U> n_s = scaled<U>(n_w, sh.rest[own]);
+          // (what goes into the gradient of log_decay through Z is a small sum of large terms: all that two numbers hold counts)
+          const Planes<U, chain_planes<U>()> n_s = scaled<U, chain_planes<U>()>(n_w, sh.rest[own]);
 #pragma unroll
           for (int u = 0; u < KT; ++u) all[u] = mma(n_s, state(Sh::D, u), all[u]);
           // <S, dS'> on the diagonal of S^T dS', 16 channels at a time

@@ -99,7 +99,7 @@ __global__ __launch_bounds__((ReverseShared<T, DK, WAVES>::LANES)) void delta_re
     const T* qq = head_rows<T>(p.q, p.q_stride, span.batch, first, key_head);
     Planes<T> sp[DK / 32];
     float un_s;
-    split_scaled<T>(s, sp, &un_s);
+    split_scaled(s, sp, &un_s);
     if constexpr (!CARRY) {
       U* to = reinterpret_cast<U*>(a.d_s + block * a.state) + int64_t(col - r) * DK;
 #pragma unroll
@@ -146,14 +146,16 @@ __global__ __launch_bounds__((ReverseShared<T, DK, WAVES>::LANES)) void delta_re
       Frag<T> f[4];
 #pragma unroll
       for (int t = 0; t < 4; ++t) f[t] = TK::frag(smem + Sh::K, rows_k, TK::mapped_row(t), b);
+      if constexpr (std::is_same_v<T, __bf16>) mma_tiles<0, 4>(f, third_plane(s[2 * b], s[2 * b + 1], sp[b]), x);
       mma_tiles<0, 4>(f, sp[b], x);
     }
 #pragma unroll
     for (int t = 0; t < 4; ++t) x[t] *= *reinterpret_cast<const v4f*>(gates + 64 + row_of_result(t, q)) * un_s;
     upper(Sh::C, dop, x);
-    Planes<U> xp[2];
+    constexpr int CHAIN = chain_planes<U>();
+    Planes<U, CHAIN> xp[2];
 #pragma unroll
-    for (int b = 0; b < 2; ++b) xp[b] = split<U>(x[2 * b], x[2 * b + 1]);
+    for (int b = 0; b < 2; ++b) xp[b] = split<U, CHAIN>(x[2 * b], x[2 * b + 1]);
     v4f db[4];
 #pragma unroll
     for (int t = 0; t < 4; ++t) db[t] = v4f{0, 0, 0, 0};
@@ -188,10 +190,10 @@ __global__ __launch_bounds__((ReverseShared<T, DK, WAVES>::LANES)) void delta_re
         d_o[t][e] *= gamma[e] * p.scale;
       }
     }
-    Planes<T> vp[2], op[2];
+    Planes<T, chain_planes<T>()> vp[2], op[2];
     float un_v, un_o;
-    split_scaled<T>(db, vp, &un_v);
-    split_scaled<T>(d_o, op, &un_o);
+    split_scaled(db, vp, &un_v);
+    split_scaled(d_o, op, &un_o);
     const float keep = gates[63];
 #pragma unroll
     for (int t = 0; t < DK / 16; ++t) {

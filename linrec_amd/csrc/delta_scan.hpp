@@ -133,7 +133,7 @@ __global__ __launch_bounds__((ScanShared<T, DK, WAVES, MODE>::LANES)) void delta
     const T* qq = head_rows<T>(p.q, p.q_stride, span.batch, first, key_head);
     Planes<T> sp[DK / 32];
     float un_s;
-    split_scaled<T>(s, sp, &un_s);
+    split_scaled(s, sp, &un_s);
     if constexpr (MODE == SCAN_STATES) {
       U* to = reinterpret_cast<U*>(a.s + block * a.state) + int64_t(col - r) * DK;
 #pragma unroll
@@ -153,10 +153,11 @@ __global__ __launch_bounds__((ScanShared<T, DK, WAVES, MODE>::LANES)) void delta
       Frag<T> f[4];
 #pragma unroll
       for (int t = 0; t < 4; ++t) f[t] = TK::frag(smem + Sh::K, rows_k, TK::mapped_row(t), b);
+      if constexpr (std::is_same_v<T, __bf16>) mma_tiles<0, 4>(f, third_plane(s[2 * b], s[2 * b + 1], sp[b]), x);
       mma_tiles<0, 4>(f, sp[b], x);
     }
     // lower triangular: positions from 32 on have no part in the first 32 rows
-    auto lower = [&](int at, const Planes<U>(&by)[2], v4f* to) __attribute__((always_inline)) {
+    auto lower = [&](int at, const auto(&by)[2], v4f* to) __attribute__((always_inline)) {
       Planes<U> f[4];
 #pragma unroll
       for (int b = 0; b < 2; ++b) {
@@ -176,9 +177,10 @@ __global__ __launch_bounds__((ScanShared<T, DK, WAVES, MODE>::LANES)) void delta
 #pragma unroll
       for (int e = 0; e < 4; ++e) x[t][e] = beta[e] * fmaf(-gamma[e] * un_s, x[t][e], float(v[e]));
     }
-    Planes<U> xp[2];
+    constexpr int CHAIN = chain_planes<U>();
+    Planes<U, CHAIN> xp[2];
 #pragma unroll
-    for (int b = 0; b < 2; ++b) xp[b] = split<U>(x[2 * b], x[2 * b + 1]);
+    for (int b = 0; b < 2; ++b) xp[b] = split<U, CHAIN>(x[2 * b], x[2 * b + 1]);
     v4f nn[4];
 #pragma unroll
     for (int t = 0; t < 4; ++t) nn[t] = v4f{0, 0, 0, 0};
@@ -232,9 +234,9 @@ __global__ __launch_bounds__((ScanShared<T, DK, WAVES, MODE>::LANES)) void delta
     }
 #pragma unroll
     for (int t = 0; t < 4; ++t) nn[t] *= *reinterpret_cast<const v4f*>(gates + 64 + row_of_result(t, q));
-    Planes<T> nt[2];
+    Planes<T, chain_planes<T>()> nt[2];
     float un_n;
-    split_scaled<T>(nn, nt, &un_n);
+    split_scaled(nn, nt, &un_n);
     const float keep = gates[63];
 #pragma unroll
     for (int t0 = 0; t0 < DK / 16; t0 += 4) {

@@ -113,13 +113,13 @@ __device__ __forceinline__ void mma_tiles(const Frag<U> (&a)[N], const Planes<U,
 #pragma unroll
     for (int t = FIRST; t < FIRST + COUNT; ++t) c[t] = mma(a[t], b.p[j], c[t]);
 }
-template <int FIRST, int COUNT, typename U, int NA, int NB, int N>
+template <int FIRST, int COUNT, int MOST = -1, typename U, int NA, int NB, int N>
 __device__ __forceinline__ void mma_tiles(const Planes<U, NA> (&a)[N], const Planes<U, NB>& b, v4f* c) {
 #pragma unroll
   for (int i = NA - 1; i >= 0; --i)
 #pragma unroll
     for (int j = NB - 1; j >= 0; --j)
-      if (i + j < (NA > NB ? NA : NB))
+      if (i + j <= (MOST >= 0 ? MOST : (NA > NB ? NA : NB) - 1))
 #pragma unroll
         for (int t = FIRST; t < FIRST + COUNT; ++t) c[t] = mma(a[t].p[i], b.p[j], c[t]);
 }
@@ -147,6 +147,12 @@ __device__ __forceinline__ Planes<U, N> split(const v4f& lo, const v4f& hi) {
 template <typename U>
 constexpr int chain_planes() {
   return std::is_same_v<U, __bf16> ? 3 : planes_of<U>();
+}
+// Planes of N and dS' as they are kept for the gradients.  With up to 64 key channels the gradients of the gates are sums of so few
+// terms that the rounding of two shows: 1e-5 of them for 16 to 32 key channels, 3e-6 with three, which LDS has room for there.
+template <typename U, int DK>
+constexpr int kept_planes() {
+  return DK == 64 ? chain_planes<U>() : planes_of<U>();
 }
 // The third of them, where two are there.
 __device__ __forceinline__ Planes<__bf16, 1> third_plane(const v4f& lo, const v4f& hi, const Planes<__bf16>& f) {
@@ -383,10 +389,10 @@ struct Stager {
 
 // Operands of 16 rows, a lane's as it has them: pieces of 1 KB that a wave stores and loads whole (rows of their own would be stored 64
 // bytes at a time).  `to`: of plane k at to + k * plane; b: which 32 columns.
-template <typename U>
-__device__ __forceinline__ void store_rows(U* to, int64_t plane, int b, int lane, const Planes<U>& f) {
+template <typename U, int N>
+__device__ __forceinline__ void store_rows(U* to, int64_t plane, int b, int lane, const Planes<U, N>& f) {
 #pragma unroll
-  for (int k = 0; k < planes_of<U>(); ++k) {
+  for (int k = 0; k < N; ++k) {
     if constexpr (sizeof(U) == 2) {
       *reinterpret_cast<Frag<U>*>(to + k * plane + b * 512 + lane * 8) = f.p[k];
     } else {
@@ -414,15 +420,15 @@ struct DeltaArgs {
   int64_t parts; // sequences, or segments of them
   int segment;   // chunks of a segment, 0: sequences are not cut
   // scratch, for every (slot, head): m[planes][64][64] and so on.  Bytes from one to the next:
-  int64_t square, state, rows;
+  int64_t square, state, state_d, rows, rows_n;
   char* m;
   char* m_t;
   char* c;       // C scale, transposed in the backward
   float* gates;  // [3][64]: e^G, e^{G_63 - G}, beta
   double* sums;  // [64]: G
   char* s;       // [planes][columns][DK] in pieces of 16 columns (store_rows), the state before the chunk
-  char* d_s;     // the same of dS' behind it
-  char* n;       // [planes][columns][64] in such pieces
+  char* d_s;     // the same of dS' behind it, [kept_planes]
+  char* n;       // [kept_planes][columns][64] in such pieces
   char* d_b;
   float* dots;   // [192], sums of the gates' gradients where key_dim comes in turns
   // for every (part, head), where sequences are cut (delta_segments.hpp)

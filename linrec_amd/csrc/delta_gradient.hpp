@@ -24,11 +24,11 @@ constexpr int GRADIENT_LANES = 512, GRADIENT_PART = 256;
 template <typename T, int DK>
 struct GradientShared {
   using U = Inner<T>;
-  static constexpr int P = planes_of<U>(), IN = input_planes<T>();
+  static constexpr int P = planes_of<U>(), KEPT = kept_planes<U, DK>(), IN = input_planes<T>();
   static constexpr int IN_V = 64 * 32 * int(sizeof(U)), BY_V = 32 * 64 * int(sizeof(U)), STATE = 32 * DK * int(sizeof(U)),
                        KEYS = Tile<U, DK>::BYTES;
   // one step's values, then both inputs of key channels
-  static constexpr int O = 0, V = O + IN * IN_V, B = V + IN * IN_V, N = B + P * BY_V, S = N + P * BY_V, D = S + P * STATE, STEP = D + P * STATE;
+  static constexpr int O = 0, V = O + IN * IN_V, B = V + IN * IN_V, N = B + P * BY_V, S = N + KEPT * BY_V, D = S + P * STATE, STEP = D + KEPT * STATE;
   static constexpr int BUFFERS = 2 * STEP + 2 * IN * KEYS + 4096 <= 160 * 1024 ? 2 : 1;
   static constexpr int K = BUFFERS * STEP, Q = K + IN * KEYS, BYTES = Q + IN * KEYS;
   static_assert(64 * DK * 4 <= BUFFERS * STEP, "room to hand dK over");
@@ -71,7 +71,8 @@ __device__ __forceinline__ Planes<U, OUT> scaled(const Planes<U, N>& f, float by
 #pragma unroll
   for (int e = 0; e < 8; ++e) {
     float v = float(f.p[0][e]);
-    if constexpr (N == 2) v += float(f.p[1][e]);
+    if constexpr (N >= 2) v += float(f.p[1][e]);
+    if constexpr (N >= 3) v += float(f.p[2][e]);
     x[e >> 2][e & 3] = by * v;
   }
   return split<U, OUT>(x[0], x[1]);
@@ -85,7 +86,7 @@ __device__ __forceinline__ void gradient_part(const DeltaArgs& a, const Chunk& c
   using TI = Tile<U, 32>;  // dO, V
   using TB = Tile<U, 64>;  // dB, N: rows are channels
   using TK = Tile<U, DK>;  // K, Q; S, dS': rows are channels
-  constexpr int P = Sh::P, IN = Sh::IN, KT = DK / 16, LANES = GRADIENT_PART;
+  constexpr int P = Sh::P, KEPT = Sh::KEPT, IN = Sh::IN, KT = DK / 16, LANES = GRADIENT_PART;
   constexpr int64_t ROW = WIDE ? 2 * DK : DK;  // of the kept states
   const linrec_delta_t& p = a.p;
   const int lane = threadIdx.x & 63, r = lane & 15, q = lane >> 4, by0 = threadIdx.x & (LANES - 1);
@@ -97,8 +98,8 @@ __device__ __forceinline__ void gradient_part(const DeltaArgs& a, const Chunk& c
 
   // what a step needs on its way: the rows of dO and V with dB and N, or S and dS'
   InputStager<T, 32, LANES> so, sv;
-  Stager<U, 64, LANES, 32> sb[P], sn[P];
-  Stager<U, DK, LANES, 32> ss[P], sd[P];
+  Stager<U, 64, LANES, 32> sb[P], sn[KEPT];
+  Stager<U, DK, LANES, 32> ss[P], sd[KEPT];
   // one wave has what belongs to the positions, a lane for each
   const bool keeper = BEHIND && wave == 0;
   double sum = 0.0;
@@ -118,16 +119,16 @@ __device__ __forceinline__ void gradient_part(const DeltaArgs& a, const Chunk& c
       sv.fetch(head_rows<T>(p.v, p.v_stride, ch.batch, ch.first, head) + v0, p.v_stride[1], ch.length, p.value_dim - v0, by);
     }
 #pragma unroll
-    for (int k = 0; k < P; ++k) {
+    for (int k = 0; k < KEPT; ++k) {
       const int64_t row = int64_t(k) * a.columns + v0;
       if constexpr (!BEHIND) {
-        sb[k].fetch_pieces(reinterpret_cast<const U*>(a.d_b + block * a.rows) + row * 64, 0, by);
-        sn[k].fetch_pieces(reinterpret_cast<const U*>(a.n + block * a.rows) + row * 64, 0, by);
+        if (k < P) sb[k].fetch_pieces(reinterpret_cast<const U*>(a.d_b + block * a.rows) + row * 64, 0, by);
+        sn[k].fetch_pieces(reinterpret_cast<const U*>(a.n + block * a.rows_n) + row * 64, 0, by);
       } else {
         const U* s = reinterpret_cast<const U*>(a.s + block * a.state) + row * ROW;
-        const U* d = reinterpret_cast<const U*>(a.d_s + block * a.state) + row * ROW;
+        const U* d = reinterpret_cast<const U*>(a.d_s + block * a.state_d) + row * ROW;
         constexpr int EVERY = int(ROW * int64_t(sizeof(U)) / 64);
-        ss[k].template fetch_pieces<EVERY>(s, WIDE ? d0 * int(sizeof(U)) / 64 : 0, by);
+        if (k < P) ss[k].template fetch_pieces<EVERY>(s, WIDE ? d0 * int(sizeof(U)) / 64 : 0, by);
         sd[k].template fetch_pieces<EVERY>(d, WIDE ? d0 * int(sizeof(U)) / 64 : 0, by);
       }
     }
@@ -139,12 +140,12 @@ __device__ __forceinline__ void gradient_part(const DeltaArgs& a, const Chunk& c
       sv.put(to + Sh::V, by);
     }
 #pragma unroll
-    for (int k = 0; k < P; ++k) {
+    for (int k = 0; k < KEPT; ++k) {
       if constexpr (!BEHIND) {
-        sb[k].put_pieces(to + Sh::B + k * Sh::BY_V, by);
+        if (k < P) sb[k].put_pieces(to + Sh::B + k * Sh::BY_V, by);
         sn[k].put_pieces(to + Sh::N + k * Sh::BY_V, by);
       } else {
-        ss[k].put_pieces(to + Sh::S + k * Sh::STATE, by);
+        if (k < P) ss[k].put_pieces(to + Sh::S + k * Sh::STATE, by);
         sd[k].put_pieces(to + Sh::D + k * Sh::STATE, by);
       }
     }
@@ -195,61 +196,63 @@ __device__ __forceinline__ void gradient_part(const DeltaArgs& a, const Chunk& c
         turn ^= 1;
         const int rows_w = anew(rows_w0), rows_m = anew(rows_m0), cols_w = anew(cols_w0), cols_m = anew(cols_m0), cols_k = anew(cols_k0),
                   rows_v = anew(rows_v0);
+        constexpr std::integral_constant<int, P> two{};
+        constexpr std::integral_constant<int, KEPT> kept{};
         auto rows_in = [&](int part, int view, int row) __attribute__((always_inline)) {
           Planes<U, IN> out;
 #pragma unroll
           for (int k = 0; k < IN; ++k) out.p[k] = TI::frag(at + part + k * Sh::IN_V, view, row, 0);
           return out;
         };
-        auto by_v = [&](int part) __attribute__((always_inline)) {  // this wave's rows
-          Planes<U> out;
+        auto by_v = [&](int part, auto planes) __attribute__((always_inline)) {  // this wave's rows
+          Planes<U, planes()> out;
 #pragma unroll
-          for (int k = 0; k < P; ++k) out.p[k] = TB::template column_frag<false>(at + part + k * Sh::BY_V, cols_w, 0, 0);
+          for (int k = 0; k < planes(); ++k) out.p[k] = TB::template column_frag<false>(at + part + k * Sh::BY_V, cols_w, 0, 0);
           return out;
         };
-        auto by_v_mapped = [&](int part, int t) __attribute__((always_inline)) {
-          Planes<U> out;
+        auto by_v_mapped = [&](int part, int t, auto planes) __attribute__((always_inline)) {
+          Planes<U, planes()> out;
 #pragma unroll
-          for (int k = 0; k < P; ++k) out.p[k] = TB::template column_frag<true>(at + part + k * Sh::BY_V, cols_m, 0, t);
+          for (int k = 0; k < planes(); ++k) out.p[k] = TB::template column_frag<true>(at + part + k * Sh::BY_V, cols_m, 0, t);
           return out;
         };
-        auto state = [&](int part, int u) __attribute__((always_inline)) {
-          Planes<U> out;
+        auto state = [&](int part, int u, auto planes) __attribute__((always_inline)) {
+          Planes<U, planes()> out;
 #pragma unroll
-          for (int k = 0; k < P; ++k) out.p[k] = TK::template column_frag<false>(at + part + k * Sh::STATE, cols_k, 0, u);
+          for (int k = 0; k < planes(); ++k) out.p[k] = TK::template column_frag<false>(at + part + k * Sh::STATE, cols_k, 0, u);
           return out;
         };
-        const Planes<U> db_w = by_v(Sh::B);
+        const Planes<U> db_w = by_v(Sh::B, two);
         const int own = 16 * wave + anew(r);
         if constexpr (!BEHIND) {
           const Planes<U, IN> do_w = rows_in(Sh::O, rows_w, 0);
 #pragma unroll
           for (int t = 0; t < 4; ++t)
             if (t / 2 <= wave / 2) {  // rows j of F^T and E^T up to this wave's columns i
-              const Planes<U> n_t = by_v_mapped(Sh::N, t);
-              f[t] = mma(n_t, do_w, f[t]);
+              const Planes<U, KEPT> n_t = by_v_mapped(Sh::N, t, kept);
+              f[t] = mma_up_to<2>(n_t, do_w, f[t]);
               ee[t] = mma_up_to<2>(n_t, db_w, ee[t]);
             }
           const Planes<U> do_s = scaled<U, P>(do_w, p.scale * sh.gamma[own]);
 #pragma unroll
           for (int u = 0; u < KT; ++u) {
-            const Planes<U> s_u = state(Sh::S, u);
+            const Planes<U> s_u = state(Sh::S, u, two);
             all[u] = mma(do_s, s_u, all[u]);
             x[u] = mma(db_w, s_u, x[u]);
           }
         } else {
-          const Planes<U> n_w = by_v(Sh::N);
+          const Planes<U, KEPT> n_w = by_v(Sh::N, kept);
 #pragma unroll
           for (int t = 0; t < 4; ++t)
             if (t / 2 >= wave / 2) {
-              f[t] = mma(rows_in(Sh::O, rows_m, TI::mapped_row(t)), n_w, f[t]);
-              ee[t] = mma_up_to<2>(by_v_mapped(Sh::B, t), n_w, ee[t]);
+              f[t] = mma_up_to<2>(rows_in(Sh::O, rows_m, TI::mapped_row(t)), n_w, f[t]);
+              ee[t] = mma_up_to<2>(by_v_mapped(Sh::B, t, two), n_w, ee[t]);
             }
-          bv = mma(db_w, rows_in(Sh::V, rows_w, 0), bv);
+          bv = mma_up_to<2>(db_w, rows_in(Sh::V, rows_w, 0), bv);
           // (what goes into the gradient of log_decay through Z is a small sum of large terms: all that two numbers hold counts)
           const Planes<U, chain_planes<U>()> n_s = scaled<U, chain_planes<U>()>(n_w, sh.rest[own]);
 #pragma unroll
-          for (int u = 0; u < KT; ++u) all[u] = mma(n_s, state(Sh::D, u), all[u]);
+          for (int u = 0; u < KT; ++u) all[u] = mma(n_s, state(Sh::D, u, kept), all[u]);
           // <S, dS'> on the diagonal of S^T dS', 16 channels at a time
 #pragma unroll
           for (int b = 0; b < DK / 32; ++b)
@@ -267,7 +270,7 @@ __device__ __forceinline__ void gradient_part(const DeltaArgs& a, const Chunk& c
       int cols_k = anew(cols_k0), points = anew(points0);
       const int r1 = anew(r), row1 = 16 * wave + 4 * anew(q);
       // the masks and decays; rows of results to operands
-      Planes<U> fp[2], ep[2];
+      Planes<U, KEPT> fp[2], ep[2];
       {
         const int own = 16 * wave + anew(r), q1 = anew(q);
 #pragma unroll
@@ -281,8 +284,8 @@ __device__ __forceinline__ void gradient_part(const DeltaArgs& a, const Chunk& c
           }
 #pragma unroll
         for (int b = 0; b < 2; ++b) {
-          fp[b] = split<U>(f[2 * b], f[2 * b + 1]);
-          ep[b] = split<U>(ee[2 * b], ee[2 * b + 1]);
+          fp[b] = split<U, KEPT>(f[2 * b], f[2 * b + 1]);
+          ep[b] = split<U, KEPT>(ee[2 * b], ee[2 * b + 1]);
         }
       }
       auto keys = [&](int part, int b, int u) __attribute__((always_inline)) {
@@ -312,8 +315,8 @@ __device__ __forceinline__ void gradient_part(const DeltaArgs& a, const Chunk& c
           for (int b = 0; b < 2; ++b)
             if (b <= wave / 2) {
               const Planes<U, IN> k_b = keys(Sh::K, b, u);
-              z = mma(fp[b], k_b, z);
-              xu = mma(ep[b], k_b, xu);
+              z = mma_up_to<2>(fp[b], k_b, z);
+              xu = mma_up_to<2>(ep[b], k_b, xu);
             }
           dot += qv * z;
           dot_x += kv * xu;
@@ -323,8 +326,8 @@ __device__ __forceinline__ void gradient_part(const DeltaArgs& a, const Chunk& c
 #pragma unroll
           for (int b = 0; b < 2; ++b)
             if (b >= wave / 2) {
-              z = mma(fp[b], keys(Sh::Q, b, u), z);
-              z = mma(ep[b], keys(Sh::K, b, u), z);
+              z = mma_up_to<2>(fp[b], keys(Sh::Q, b, u), z);
+              z = mma_up_to<2>(ep[b], keys(Sh::K, b, u), z);
             }
           dot += kv * z;
         }

@@ -101,14 +101,12 @@ __global__ __launch_bounds__((ReverseShared<T, DK, WAVES>::LANES)) void delta_re
     float un_s;
     split_scaled(s, sp, &un_s);
     if constexpr (!CARRY) {
-      U* to = reinterpret_cast<U*>(a.d_s + block * a.state) + int64_t(col - r) * DK;
+      U* to = reinterpret_cast<U*>(a.d_s + block * a.state_d) + int64_t(col - r) * DK;
 #pragma unroll
       for (int b = 0; b < DK / 32; ++b) {
         if (!kept_column) break;
-        Planes<U> kept;
-        if constexpr (std::is_same_v<T, _Float16>) kept = split<U>(s[2 * b], s[2 * b + 1]);
-        else kept = sp[b];
-        store_rows<U>(to, int64_t(a.columns) * DK, b, lane, kept);
+        // (of bf16 inputs the first two are sp[b], which the compiler sees)
+        store_rows(to, int64_t(a.columns) * DK, b, lane, split<U, kept_planes<U, DK>()>(s[2 * b], s[2 * b + 1]));
       }
     }
     // upper triangular: the first 32 positions have no part in rows from 32 on
@@ -120,8 +118,8 @@ __global__ __launch_bounds__((ReverseShared<T, DK, WAVES>::LANES)) void delta_re
         for (int t = 0; t < 2 + 2 * b; ++t)
 #pragma unroll
           for (int k2 = 0; k2 < P; ++k2) f[t].p[k2] = TS::frag(smem + at + k2 * TS::BYTES, rows_s, TS::mapped_row(t), b);
-        if (b == 0) mma_tiles<0, 2>(f, by[b], to);
-        else mma_tiles<0, 4>(f, by[b], to);
+        if (b == 0) mma_tiles<0, 2, 2>(f, by[b], to);
+        else mma_tiles<0, 4, 2>(f, by[b], to);
       }
     };
     // dO of this wave's columns, a result's layout; fp16 as two bf16
@@ -163,7 +161,7 @@ __global__ __launch_bounds__((ReverseShared<T, DK, WAVES>::LANES)) void delta_re
     if (!CARRY && kept_column) {
       U* to = reinterpret_cast<U*>(a.d_b + block * a.rows) + (col - r) * 64;
 #pragma unroll
-      for (int b = 0; b < 2; ++b) store_rows<U>(to, int64_t(a.columns) * 64, b, lane, split<U>(db[2 * b], db[2 * b + 1]));
+      for (int b = 0; b < 2; ++b) store_rows(to, int64_t(a.columns) * 64, b, lane, split<U>(db[2 * b], db[2 * b + 1]));
     }
     const int apart = p.heads * p.value_dim;
     T* d_v = static_cast<T*>(p.d_v) + ((span.batch * p.time + first) * p.heads + head) * int64_t(p.value_dim) + col;

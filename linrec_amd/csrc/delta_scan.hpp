@@ -142,7 +142,7 @@ __global__ __launch_bounds__((ScanShared<T, DK, WAVES, MODE>::LANES)) void delta
         Planes<U> kept;
         if constexpr (std::is_same_v<T, _Float16>) kept = split<U>(s[2 * b], s[2 * b + 1]);
         else kept = sp[b];
-        store_rows<U>(to, int64_t(a.columns) * DK, b, lane, kept);
+        store_rows(to, int64_t(a.columns) * DK, b, lane, kept);
       }
     }
     v4f x[4];  // K S, then beta (V - e^G K S)
@@ -190,10 +190,11 @@ __global__ __launch_bounds__((ScanShared<T, DK, WAVES, MODE>::LANES)) void delta
     for (int b = 0; b < 2; ++b) np[b] = split<U>(nn[2 * b], nn[2 * b + 1]);
     if constexpr (MODE == SCAN_CARRY) {
     } else if constexpr (MODE == SCAN_STATES) {
-      U* to = reinterpret_cast<U*>(a.n + block * a.rows) + (col - r) * 64;
+      constexpr int KEPT = kept_planes<U, DK>();
+      U* to = reinterpret_cast<U*>(a.n + block * a.rows_n) + (col - r) * 64;
 #pragma unroll
       for (int b = 0; b < 2; ++b)
-        if (kept_column) store_rows<U>(to, int64_t(a.columns) * 64, b, lane, np[b]);
+        if (kept_column) store_rows(to, int64_t(a.columns) * 64, b, lane, split<U, KEPT>(nn[2 * b], nn[2 * b + 1]));
     } else {
       T* o = static_cast<T*>(p.o) + ((span.batch * p.time + first) * p.heads + head) * int64_t(p.value_dim) + col;
       v4f y[4];

@@ -52,11 +52,10 @@ size_t lay_out(const linrec_delta_t& p, bool bwd, char* base, DeltaArgs* a) {
     return to;
   };
   a->square = 4096 * value;
-  a->state = int64_t(a->columns) * width * value;
   a->rows = int64_t(a->columns) * 64 * value;
   const int kept = width == 64 && p.dtype != LINREC_DTYPE_F32 ? 6 : value;  // (kept_planes)
-  a->state_d = int64_t(a->columns) * width * kept;
   a->rows_n = int64_t(a->columns) * 64 * kept;
+  a->state = int64_t(a->columns) * width * kept;
   a->m = part(a->square);
   a->c = part(a->square);
   a->gates = reinterpret_cast<float*>(part(192 * 4));
@@ -64,7 +63,7 @@ size_t lay_out(const linrec_delta_t& p, bool bwd, char* base, DeltaArgs* a) {
     a->sums = reinterpret_cast<double*>(part(64 * 8));
     a->m_t = part(a->square);
     a->s = part(a->state);
-    a->d_s = part(a->state_d);
+    a->d_s = part(a->state);
     a->n = part(a->rows_n);
     a->d_b = part(a->rows);
     a->dots = reinterpret_cast<float*>(part(192 * 4));

@@ -148,7 +148,7 @@ template <typename U>
 constexpr int chain_planes() {
   return std::is_same_v<U, __bf16> ? 3 : planes_of<U>();
 }
-// Planes of N and dS' as they are kept for the gradients.  With up to 64 key channels the gradients of the gates are sums of so few
+// Planes of N, S and dS' as they are kept for the gradients.  With up to 64 key channels the gradients of the gates are sums of so few
 // terms that the rounding of two shows: 1e-5 of them for 16 to 32 key channels, 3e-6 with three, which LDS has room for there.
 template <typename U, int DK>
 constexpr int kept_planes() {
@@ -420,14 +420,14 @@ struct DeltaArgs {
   int64_t parts; // sequences, or segments of them
   int segment;   // chunks of a segment, 0: sequences are not cut
   // scratch, for every (slot, head): m[planes][64][64] and so on.  Bytes from one to the next:
-  int64_t square, state, state_d, rows, rows_n;
+  int64_t square, state, rows, rows_n;
   char* m;
   char* m_t;
   char* c;       // C scale, transposed in the backward
   float* gates;  // [3][64]: e^G, e^{G_63 - G}, beta
   double* sums;  // [64]: G
-  char* s;       // [planes][columns][DK] in pieces of 16 columns (store_rows), the state before the chunk
-  char* d_s;     // the same of dS' behind it, [kept_planes]
+  char* s;       // [kept_planes][columns][DK] in pieces of 16 columns (store_rows), the state before the chunk
+  char* d_s;     // the same of dS' behind it
   char* n;       // [kept_planes][columns][64] in such pieces
   char* d_b;
   float* dots;   // [192], sums of the gates' gradients where key_dim comes in turns

@@ -28,7 +28,7 @@ struct GradientShared {
   static constexpr int IN_V = 64 * 32 * int(sizeof(U)), BY_V = 32 * 64 * int(sizeof(U)), STATE = 32 * DK * int(sizeof(U)),
                        KEYS = Tile<U, DK>::BYTES;
   // one step's values, then both inputs of key channels
-  static constexpr int O = 0, V = O + IN * IN_V, B = V + IN * IN_V, N = B + P * BY_V, S = N + KEPT * BY_V, D = S + P * STATE, STEP = D + KEPT * STATE;
+  static constexpr int O = 0, V = O + IN * IN_V, B = V + IN * IN_V, N = B + P * BY_V, S = N + KEPT * BY_V, D = S + KEPT * STATE, STEP = D + KEPT * STATE;
   static constexpr int BUFFERS = 2 * STEP + 2 * IN * KEYS + 4096 <= 160 * 1024 ? 2 : 1;
   static constexpr int K = BUFFERS * STEP, Q = K + IN * KEYS, BYTES = Q + IN * KEYS;
   static_assert(64 * DK * 4 <= BUFFERS * STEP, "room to hand dK over");
@@ -99,7 +99,7 @@ __device__ __forceinline__ void gradient_part(const DeltaArgs& a, const Chunk& c
   // what a step needs on its way: the rows of dO and V with dB and N, or S and dS'
   InputStager<T, 32, LANES> so, sv;
   Stager<U, 64, LANES, 32> sb[P], sn[KEPT];
-  Stager<U, DK, LANES, 32> ss[P], sd[KEPT];
+  Stager<U, DK, LANES, 32> ss[KEPT], sd[KEPT];
   // one wave has what belongs to the positions, a lane for each
   const bool keeper = BEHIND && wave == 0;
   double sum = 0.0;
@@ -126,9 +126,9 @@ __device__ __forceinline__ void gradient_part(const DeltaArgs& a, const Chunk& c
         sn[k].fetch_pieces(reinterpret_cast<const U*>(a.n + block * a.rows_n) + row * 64, 0, by);
       } else {
         const U* s = reinterpret_cast<const U*>(a.s + block * a.state) + row * ROW;
-        const U* d = reinterpret_cast<const U*>(a.d_s + block * a.state_d) + row * ROW;
+        const U* d = reinterpret_cast<const U*>(a.d_s + block * a.state) + row * ROW;
         constexpr int EVERY = int(ROW * int64_t(sizeof(U)) / 64);
-        if (k < P) ss[k].template fetch_pieces<EVERY>(s, WIDE ? d0 * int(sizeof(U)) / 64 : 0, by);
+        ss[k].template fetch_pieces<EVERY>(s, WIDE ? d0 * int(sizeof(U)) / 64 : 0, by);
         sd[k].template fetch_pieces<EVERY>(d, WIDE ? d0 * int(sizeof(U)) / 64 : 0, by);
       }
     }
@@ -145,7 +145,7 @@ __device__ __forceinline__ void gradient_part(const DeltaArgs& a, const Chunk& c
         if (k < P) sb[k].put_pieces(to + Sh::B + k * Sh::BY_V, by);
         sn[k].put_pieces(to + Sh::N + k * Sh::BY_V, by);
       } else {
-        if (k < P) ss[k].put_pieces(to + Sh::S + k * Sh::STATE, by);
+        ss[k].put_pieces(to + Sh::S + k * Sh::STATE, by);
         sd[k].put_pieces(to + Sh::D + k * Sh::STATE, by);
       }
     }
@@ -216,10 +216,10 @@ __device__ __forceinline__ void gradient_part(const DeltaArgs& a, const Chunk& c
           for (int k = 0; k < planes(); ++k) out.p[k] = TB::template column_frag<true>(at + part + k * Sh::BY_V, cols_m, 0, t);
           return out;
         };
-        auto state = [&](int part, int u, auto planes) __attribute__((always_inline)) {
-          Planes<U, planes()> out;
+        auto state = [&](int part, int u) __attribute__((always_inline)) {
+          Planes<U, KEPT> out;
 #pragma unroll
-          for (int k = 0; k < planes(); ++k) out.p[k] = TK::template column_frag<false>(at + part + k * Sh::STATE, cols_k, 0, u);
+          for (int k = 0; k < KEPT; ++k) out.p[k] = TK::template column_frag<false>(at + part + k * Sh::STATE, cols_k, 0, u);
           return out;
         };
         const Planes<U> db_w = by_v(Sh::B, two);
@@ -233,10 +233,10 @@ __device__ __forceinline__ void gradient_part(const DeltaArgs& a, const Chunk& c
               f[t] = mma_up_to<2>(n_t, do_w, f[t]);
               ee[t] = mma_up_to<2>(n_t, db_w, ee[t]);
             }
-          const Planes<U> do_s = scaled<U, P>(do_w, p.scale * sh.gamma[own]);
+          const Planes<U, KEPT> do_s = scaled<U, KEPT>(do_w, p.scale * sh.gamma[own]);
 #pragma unroll
           for (int u = 0; u < KT; ++u) {
-            const Planes<U> s_u = state(Sh::S, u, two);
+            const Planes<U, KEPT> s_u = state(Sh::S, u);
             all[u] = mma(do_s, s_u, all[u]);
             x[u] = mma(db_w, s_u, x[u]);
           }
@@ -252,18 +252,18 @@ __device__ __forceinline__ void gradient_part(const DeltaArgs& a, const Chunk& c
           // (what goes into the gradient of log_decay through Z is a small sum of large terms: all that two numbers hold counts)
           const Planes<U, chain_planes<U>()> n_s = scaled<U, chain_planes<U>()>(n_w, sh.rest[own]);
 #pragma unroll
-          for (int u = 0; u < KT; ++u) all[u] = mma(n_s, state(Sh::D, u, kept), all[u]);
+          for (int u = 0; u < KT; ++u) all[u] = mma(n_s, state(Sh::D, u), all[u]);
           // <S, dS'> on the diagonal of S^T dS', 16 channels at a time
 #pragma unroll
           for (int b = 0; b < DK / 32; ++b)
             if ((b & 1) == wave >> 1) {
-              Planes<U> s_v, d_v;
+              Planes<U, KEPT> s_v, d_v;
 #pragma unroll
-              for (int k = 0; k < P; ++k) {
+              for (int k = 0; k < KEPT; ++k) {
                 s_v.p[k] = TK::frag(at + Sh::S + k * Sh::STATE, rows_v, 0, b);
                 d_v.p[k] = TK::frag(at + Sh::D + k * Sh::STATE, rows_v, 0, b);
               }
-              inner = mma(s_v, d_v, inner);
+              inner = mma_up_to<2>(s_v, d_v, inner);
             }
         }
       }

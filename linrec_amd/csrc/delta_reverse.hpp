@@ -101,7 +101,7 @@ __global__ __launch_bounds__((ReverseShared<T, DK, WAVES>::LANES)) void delta_re
     float un_s;
     split_scaled(s, sp, &un_s);
     if constexpr (!CARRY) {
-      U* to = reinterpret_cast<U*>(a.d_s + block * a.state_d) + int64_t(col - r) * DK;
+      U* to = reinterpret_cast<U*>(a.d_s + block * a.state) + int64_t(col - r) * DK;
 #pragma unroll
       for (int b = 0; b < DK / 32; ++b) {
         if (!kept_column) break;

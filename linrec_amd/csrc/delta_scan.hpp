@@ -139,10 +139,8 @@ __global__ __launch_bounds__((ScanShared<T, DK, WAVES, MODE>::LANES)) void delta
 #pragma unroll
       for (int b = 0; b < DK / 32; ++b) {
         if (!kept_column) break;
-        Planes<U> kept;
-        if constexpr (std::is_same_v<T, _Float16>) kept = split<U>(s[2 * b], s[2 * b + 1]);
-        else kept = sp[b];
-        store_rows(to, int64_t(a.columns) * DK, b, lane, kept);
+        // (of bf16 inputs the first two are sp[b], which the compiler sees)
+        store_rows(to, int64_t(a.columns) * DK, b, lane, split<U, kept_planes<U, DK>()>(s[2 * b], s[2 * b + 1]));
       }
     }
     v4f x[4];  // K S, then beta (V - e^G K S)

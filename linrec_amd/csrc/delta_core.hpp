@@ -20,8 +20,9 @@
 // Precision.  States, sums and accumulators are fp32.  An operand of a matrix instruction that is not an input is split into
 // bf16 (or, beside fp16 inputs, fp16) numbers, its rounding, the rounding of the rest and so on: two bf16 carry 16 to 17 bits, three 24, two
 // fp16 22.  In the chain of products that makes a state from the one before, what meets an input is three bf16 or two fp16, and what meets M
-// three bf16; M, C and all that is kept for the gradients are two.  So a state is 1e-6 off and a gradient 3e-6 (with two bf16 in the
-// chain 5e-6 and 1e-5, with one 2e-3).  fp32 inputs take the fp32 instructions.
+// three bf16; M, C and what is kept for the gradients are two, S, dS' and N up to 64 key channels three (kept_planes).  So a state is
+// 1e-6 off, the gradient of beta 4e-6 and that of log_decay 3e-6 up to 64 key channels, 5e-6 from there on (with two bf16 in the chain and
+// without the products of rests 1e-5 to 1.6e-5, with one bf16 2e-3).  fp32 inputs take the fp32 instructions.
 #pragma once
 #include <hip/hip_runtime.h>
 #include <stdint.h>

@@ -30,16 +30,21 @@ RmsPlan plan_rms(int dtype, int64_t rows, int64_t channels, bool bwd) {
     while (int64_t(team) * items < slots) team <<= 1;
     return team;
   };
-  // a wave to a row, or less, as long as it can hold it
-  pl.items = 1;
-  while (pl.items < most_items && team_of(pl.items) > 64) pl.items *= 2;
+  // Two loads of a lane to a row, and as many more as keep a row within a workgroup of 256: many waves hide the latency better than
+  // many loads of few (20011 x 4096 bf16 with a residual to 8 bits: teams of 256 lanes with 2 loads 147 us, 64 with 8 212, 512 with 1 231,
+  // all three before the weights came as vectors, with which the first is 117; 40000 x 1024: 64 with 2 32, 128 with 1 36, 32 with 4 45)
+  pl.items = slots < 64 ? 1 : 2;
+  while (pl.items < most_items && team_of(pl.items) > RMS_LANES) pl.items *= 2;
   // few rows: more lanes to each, so that one load's latency is all that a row takes
   while (pl.items > 1 && rows * team_of(pl.items) < 65536 && team_of(pl.items / 2) <= RMS_WIDE) pl.items /= 2;
   // a wide workgroup has half the registers for a lane
   while (pl.items > 1 && team_of(pl.items) > RMS_LANES && team_of(pl.items / 2) <= RMS_WIDE) pl.items /= 2;
   pl.team = team_of(pl.items);
-  pl.lanes = pl.team > RMS_LANES ? RMS_WIDE : RMS_LANES;
-  const int64_t needed = cdiv(rows, pl.lanes / pl.team), most = (bwd ? 1024 : 2048) * RMS_LANES / pl.lanes;
+  pl.lanes = pl.team > RMS_LANES ? pl.team : RMS_LANES;
+  // A backward's workgroups each leave a row of sums behind: no more of them than a million sums, but twice the CUs (32768 x 2048 bf16: 512
+  // 106 us, 1024 127, 4096 138; 262144 x 64 fp32: 4096 49 us, 1024 71).
+  const int64_t sums = (int64_t(1) << 20) / channels;
+  const int64_t needed = cdiv(rows, pl.lanes / pl.team), most = (!bwd || sums > 4096 ? 4096 : sums < 512 ? 512 : sums) * RMS_LANES / pl.lanes;
   pl.blocks = int(needed < most ? needed : most);
   return pl;
 }
@@ -67,8 +72,8 @@ int with_items(int items, F&& f) {
 template <typename T, int KIND>
 int launch_fwd(const RmsArgs& a, const RmsPlan& pl) {
   auto go = [&](auto vec, auto items) {
-    if constexpr (vec() > 1 && items() <= 4)
-      if (pl.lanes == RMS_WIDE) return launch_kernel(rms_fwd_kernel<T, vec(), items(), KIND, RMS_WIDE>, pl.blocks, 1, RMS_WIDE, a.p.stream, a);
+    if constexpr (vec() > 1 && vec() * items() <= 16)  // (16384 channels are 16 to each of 1024 lanes)
+      if (pl.lanes > RMS_LANES) return launch_kernel(rms_fwd_kernel<T, vec(), items(), KIND, RMS_WIDE>, pl.blocks, 1, pl.lanes, a.p.stream, a);
     return launch_kernel(rms_fwd_kernel<T, vec(), items(), KIND, RMS_LANES>, pl.blocks, 1, RMS_LANES, a.p.stream, a);
   };
   if (pl.vec == 1) return go(std::integral_constant<int, 1>{}, std::integral_constant<int, 1>{});  // (fewer channels than a lane holds)
@@ -114,8 +119,8 @@ int linrec_rms_norm_bwd(const linrec_rms_norm_t* p) {
     const int rc = with_dtype(p->dtype, [&](auto t) {
       using T = decltype(t);
       auto go = [&](auto vec, auto items) {
-        if constexpr (vec() > 1)
-          if (pl.lanes == RMS_WIDE) return launch_kernel(rms_bwd_kernel<T, vec(), items(), RMS_WIDE>, pl.blocks, 1, RMS_WIDE, p->stream, a);
+        if constexpr (vec() > 1 && vec() * items() <= 16)
+          if (pl.lanes > RMS_LANES) return launch_kernel(rms_bwd_kernel<T, vec(), items(), RMS_WIDE>, pl.blocks, 1, pl.lanes, p->stream, a);
         return launch_kernel(rms_bwd_kernel<T, vec(), items(), RMS_LANES>, pl.blocks, 1, RMS_LANES, p->stream, a);
       };
       if (pl.vec == 1) return go(std::integral_constant<int, 1>{}, std::integral_constant<int, 1>{});

@@ -11,7 +11,7 @@
 // lane's weights stay with it from row to row.  Sums are fp32, in an order that depends on sizes alone.
 //
 // Measured against what the bytes take at the rate of a large copy (5.1 TB/s): 32768 x 2048 bf16 with a residual 95 us (105) and back 102
-// (131, of which 26 were still in the caches), 262144 x 64 fp32 31 (26) and 46 (39), 20011 x 4096 bf16 with a residual to 8 bits 117
+// (105; some of it is still in the caches), 262144 x 64 fp32 31 (26) and 46 (39), 20011 x 4096 bf16 with a residual to 8 bits 117
 // (112); 64 x 4096 5.3 us, the latency of three loads and two meetings of a workgroup.
 #pragma once
 #include "collook_kernel.hpp"

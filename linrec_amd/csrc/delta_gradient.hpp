@@ -60,7 +60,7 @@ struct InputStager {
 
 template <typename T, int DK>
 struct GradientScratch {  // LDS beside GradientShared
-  double g[64];
+  alignas(32) double g[64];
   alignas(16) float gamma[64], rest[64], beta[64], q[64], x[64], y[64], bv[64], sum[4];
 };
 
@@ -273,16 +273,24 @@ __device__ __forceinline__ void gradient_part(const DeltaArgs& a, const Chunk& c
       // the masks and decays; rows of results to operands
       Planes<U, KEPT> fp[2], ep[2];
       {
+        // (all reads ahead of what they are compared for: a read that waits in a branch of its own costs its latency, 16 times over)
+        typedef double v4d __attribute__((ext_vector_type(4)));
         const int own = 16 * wave + anew(r), q1 = anew(q);
+        const double g_own = sh.g[own];
 #pragma unroll
-        for (int t = 0; t < 4; ++t)
+        for (int t = 0; t < 4; ++t) {
+          const int first = row_of_result(t, q1);
+          const v4d g_other = *reinterpret_cast<const v4d*>(sh.g + first);
+          const v4f beta_of = BEHIND ? *reinterpret_cast<const v4f*>(sh.beta + first) : v4f{1, 1, 1, 1};
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
-            const int other = row_of_result(t, q1) + e, i = BEHIND ? other : own, j = BEHIND ? own : other;
-            const float d = i >= j ? fast_exp(float(sh.g[i] - sh.g[j])) : 0.0f;
+            const int i = BEHIND ? first + e : own, j = BEHIND ? own : first + e;
+            const float apart = float(BEHIND ? g_other[e] - g_own : g_own - g_other[e]);
+            const float d = fast_exp(i >= j ? apart : -__builtin_inff());
             f[t][e] = i >= j ? p.scale * d * f[t][e] : 0.0f;
-            ee[t][e] = i > j ? -(BEHIND ? sh.beta[i] : 1.0f) * d * ee[t][e] : 0.0f;
+            ee[t][e] = i > j ? -beta_of[e] * d * ee[t][e] : 0.0f;
           }
+        }
 #pragma unroll
         for (int b = 0; b < 2; ++b) {
           fp[b] = split<U, KEPT>(f[2 * b], f[2 * b + 1]);

@@ -275,6 +275,15 @@ struct Tile {
   }
 };
 
+// f(0) to f(N - 1), constants.
+template <int N, int I = 0, typename F>
+__device__ __forceinline__ void static_for(F&& f) {
+  if constexpr (I < N) {
+    f(std::integral_constant<int, I>{});
+    static_for<N, I + 1>(f);
+  }
+}
+
 // A view that a loop's body starts from anew: the places made from it are not all kept in registers outside.
 __device__ __forceinline__ int anew(int view) {
   asm volatile("" : "+v"(view));

@@ -104,33 +104,36 @@ __device__ __forceinline__ void gradient_part(const DeltaArgs& a, const Chunk& c
   const bool keeper = BEHIND && wave == 0;
   double sum = 0.0;
   float gamma = 0.0f, rest = 0.0f, beta = 0.0f;
-  auto fetch = [&](int head, int v0, int d0) __attribute__((always_inline)) {
-    const int64_t block = slot * p.heads + head;
-    const int by = anew(by0);
-    if (keeper && v0 == 0) {
+  // (loads are issued one part after the other between products: all at once they wait for each other, 2600 of a step's 8000 cycles)
+  constexpr int PARTS = BEHIND ? 2 * KEPT : 2 + P + KEPT;
+  auto fetch_gates = [&](int head) __attribute__((always_inline)) {
+    if (keeper) {
+      const int64_t block = slot * p.heads + head;
       const int own = anew(lane);
       sum = a.sums[block * 64 + own];
       gamma = a.gates[block * 192 + own];
       rest = a.gates[block * 192 + 64 + own];
       beta = a.gates[block * 192 + 128 + own];
     }
+  };
+  auto fetch_part = [&](auto part, int head, int v0, int d0, int by) __attribute__((always_inline)) {
+    const int64_t block = slot * p.heads + head;
     if constexpr (!BEHIND) {
-      so.fetch(head_rows<T>(p.d_o, p.d_o_stride, ch.batch, ch.first, head) + v0, p.d_o_stride[1], ch.length, p.value_dim - v0, by);
-      sv.fetch(head_rows<T>(p.v, p.v_stride, ch.batch, ch.first, head) + v0, p.v_stride[1], ch.length, p.value_dim - v0, by);
-    }
-#pragma unroll
-    for (int k = 0; k < KEPT; ++k) {
-      const int64_t row = int64_t(k) * a.columns + v0;
-      if constexpr (!BEHIND) {
-        if (k < P) sb[k].fetch_pieces(reinterpret_cast<const U*>(a.d_b + block * a.rows) + row * 64, 0, by);
-        sn[k].fetch_pieces(reinterpret_cast<const U*>(a.n + block * a.rows_n) + row * 64, 0, by);
+      if constexpr (part() == 0) {
+        so.fetch(head_rows<T>(p.d_o, p.d_o_stride, ch.batch, ch.first, head) + v0, p.d_o_stride[1], ch.length, p.value_dim - v0, by);
+      } else if constexpr (part() == 1) {
+        sv.fetch(head_rows<T>(p.v, p.v_stride, ch.batch, ch.first, head) + v0, p.v_stride[1], ch.length, p.value_dim - v0, by);
+      } else if constexpr (part() < 2 + P) {
+        constexpr int k = part() - 2;
+        sb[k].fetch_pieces(reinterpret_cast<const U*>(a.d_b + block * a.rows) + (int64_t(k) * a.columns + v0) * 64, 0, by);
       } else {
-        const U* s = reinterpret_cast<const U*>(a.s + block * a.state) + row * ROW;
-        const U* d = reinterpret_cast<const U*>(a.d_s + block * a.state) + row * ROW;
-        constexpr int EVERY = int(ROW * int64_t(sizeof(U)) / 64);
-        ss[k].template fetch_pieces<EVERY>(s, WIDE ? d0 * int(sizeof(U)) / 64 : 0, by);
-        sd[k].template fetch_pieces<EVERY>(d, WIDE ? d0 * int(sizeof(U)) / 64 : 0, by);
+        constexpr int k = part() - 2 - P;
+        sn[k].fetch_pieces(reinterpret_cast<const U*>(a.n + block * a.rows_n) + (int64_t(k) * a.columns + v0) * 64, 0, by);
       }
+    } else {
+      constexpr int k = part() % KEPT, EVERY = int(ROW * int64_t(sizeof(U)) / 64);
+      const U* from = reinterpret_cast<const U*>((part() < KEPT ? a.s : a.d_s) + block * a.state) + (int64_t(k) * a.columns + v0) * ROW;
+      (part() < KEPT ? ss : sd)[k].template fetch_pieces<EVERY>(from, WIDE ? d0 * int(sizeof(U)) / 64 : 0, by);
     }
   };
   auto put = [&](char* to) __attribute__((always_inline)) {
@@ -164,7 +167,8 @@ __device__ __forceinline__ void gradient_part(const DeltaArgs& a, const Chunk& c
       InputStager<T, DK, LANES> keys;
       const T* from = BEHIND ? head_rows<T>(p.q, p.q_stride, ch.batch, ch.first, key_head) : head_rows<T>(p.k, p.k_stride, ch.batch, ch.first, key_head);
       keys.fetch(from + d0, BEHIND ? p.q_stride[1] : p.k_stride[1], ch.length, p.key_dim - d0, by0);
-      fetch(key_head * a.shared, 0, d0);
+      fetch_gates(key_head * a.shared);
+      static_for<PARTS>([&](auto part) __attribute__((always_inline)) { fetch_part(part, key_head * a.shared, 0, d0, anew(by0)); });
       __syncthreads();
       keys.put(smem + (BEHIND ? Sh::Q : Sh::K), by0);
     }
@@ -191,9 +195,19 @@ __device__ __forceinline__ void gradient_part(const DeltaArgs& a, const Chunk& c
         if constexpr (Sh::BUFFERS == 1) __syncthreads();
         put(at);
         __syncthreads();
-        if (v0 + 32 < p.value_dim) fetch(head, v0 + 32, d0);
-        else if (h + 1 < a.shared) fetch(head + 1, 0, d0);
         turn ^= 1;
+        const bool same = v0 + 32 < p.value_dim;
+        const int next = same ? head : head + 1, next_v0 = same ? v0 + 32 : 0;
+        if (!same && h + 1 < a.shared) fetch_gates(next);
+        const bool more = same || h + 1 < a.shared;
+        // the parts that come with column tile u, not before its product is there
+        auto fetch_beside = [&](auto u, v4f& after) __attribute__((always_inline)) {
+          if (more) {
+            static_for<PARTS>([&](auto part) __attribute__((always_inline)) {
+              if constexpr (part() * KT / PARTS == u()) fetch_part(part, next, next_v0, d0, anew_after(by0, after));
+            });
+          }
+        };
         const int rows_w = anew(rows_w0), rows_m = anew(rows_m0), cols_w = anew(cols_w0), cols_m = anew(cols_m0), cols_k = anew(cols_k0),
                   rows_v = anew(rows_v0);
         constexpr std::integral_constant<int, P> two{};
@@ -234,13 +248,13 @@ __device__ __forceinline__ void gradient_part(const DeltaArgs& a, const Chunk& c
               ee[t] = mma_up_to<2>(n_t, db_w, ee[t]);
             }
           const Planes<U, KEPT> do_s = scaled<U, KEPT>(do_w, p.scale * sh.gamma[own]);
-#pragma unroll
-          for (int u = 0; u < KT; ++u) {
+          static_for<KT>([&](auto u) __attribute__((always_inline)) {
             const Planes<U, KEPT> s_u = state(Sh::S, u);
             // (the products of two rests too: without them the gradient of log_decay is a sixth further off, for 46 of 774 us)
             all[u] = mma_up_to<2>(do_s, s_u, all[u]);
             x[u] = mma_up_to<2>(db_w, s_u, x[u]);
-          }
+            fetch_beside(u, all[u]);
+          });
         } else {
           const Planes<U, KEPT> n_w = by_v(Sh::N, kept);
 #pragma unroll
@@ -252,8 +266,10 @@ __device__ __forceinline__ void gradient_part(const DeltaArgs& a, const Chunk& c
           bv = mma_up_to<2>(db_w, rows_in(Sh::V, rows_w, 0), bv);
           // (what goes into the gradient of log_decay through Z is a small sum of large terms: all that two numbers hold counts)
           const Planes<U, chain_planes<U>()> n_s = scaled<U, chain_planes<U>()>(n_w, sh.rest[own]);
-#pragma unroll
-          for (int u = 0; u < KT; ++u) all[u] = mma(n_s, state(Sh::D, u), all[u]);
+          static_for<KT>([&](auto u) __attribute__((always_inline)) {
+            all[u] = mma(n_s, state(Sh::D, u), all[u]);
+            fetch_beside(u, all[u]);
+          });
           // <S, dS'> on the diagonal of S^T dS', 16 channels at a time
 #pragma unroll
           for (int b = 0; b < DK / 32; ++b)

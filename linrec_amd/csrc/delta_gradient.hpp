@@ -61,7 +61,7 @@ struct InputStager {
 template <typename T, int DK>
 struct GradientScratch {  // LDS beside GradientShared
   alignas(32) double g[64];
-  alignas(16) float gamma[64], rest[64], beta[64], q[64], x[64], y[64], bv[64], sum[4];
+  alignas(16) float gamma[64], rest[64], beta[64], q[64], x[64], y[64], bv[64], sum[8];
 };
 
 // An operand with its rows scaled.
@@ -236,9 +236,9 @@ __device__ __forceinline__ void gradient_part(const DeltaArgs& a, const Chunk& c
           for (int k = 0; k < KEPT; ++k) out.p[k] = TK::template column_frag<false>(at + part + k * Sh::STATE, cols_k, 0, u);
           return out;
         };
-        const Planes<U> db_w = by_v(Sh::B, two);
         const int own = 16 * wave + anew(r);
         if constexpr (!BEHIND) {
+          const Planes<U> db_w = by_v(Sh::B, two);
           const Planes<U, IN> do_w = rows_in(Sh::O, rows_w, 0);
 #pragma unroll
           for (int t = 0; t < 4; ++t)
@@ -255,21 +255,7 @@ __device__ __forceinline__ void gradient_part(const DeltaArgs& a, const Chunk& c
             x[u] = mma_up_to<2>(db_w, s_u, x[u]);
             fetch_beside(u, all[u]);
           });
-        } else {
-          const Planes<U, KEPT> n_w = by_v(Sh::N, kept);
-#pragma unroll
-          for (int t = 0; t < 4; ++t)
-            if (t / 2 >= wave / 2) {
-              f[t] = mma_up_to<2>(rows_in(Sh::O, rows_m, TI::mapped_row(t)), n_w, f[t]);
-              ee[t] = mma_up_to<2>(by_v_mapped(Sh::B, t, two), n_w, ee[t]);
-            }
           bv = mma_up_to<2>(db_w, rows_in(Sh::V, rows_w, 0), bv);
-          // (what goes into the gradient of log_decay through Z is a small sum of large terms: all that two numbers hold counts)
-          const Planes<U, chain_planes<U>()> n_s = scaled<U, chain_planes<U>()>(n_w, sh.rest[own]);
-          static_for<KT>([&](auto u) __attribute__((always_inline)) {
-            all[u] = mma(n_s, state(Sh::D, u), all[u]);
-            fetch_beside(u, all[u]);
-          });
           // <S, dS'> on the diagonal of S^T dS', 16 channels at a time
 #pragma unroll
           for (int b = 0; b < DK / 32; ++b)
@@ -282,6 +268,20 @@ __device__ __forceinline__ void gradient_part(const DeltaArgs& a, const Chunk& c
               }
               inner = mma_up_to<2>(s_v, d_v, inner);
             }
+        } else {
+          const Planes<U, KEPT> n_w = by_v(Sh::N, kept);
+#pragma unroll
+          for (int t = 0; t < 4; ++t)
+            if (t / 2 >= wave / 2) {
+              f[t] = mma_up_to<2>(rows_in(Sh::O, rows_m, TI::mapped_row(t)), n_w, f[t]);
+              ee[t] = mma_up_to<2>(by_v_mapped(Sh::B, t, two), n_w, ee[t]);
+            }
+          // (what goes into the gradient of log_decay through Z is a small sum of large terms: all that two numbers hold counts)
+          const Planes<U, chain_planes<U>()> n_s = scaled<U, chain_planes<U>()>(n_w, sh.rest[own]);
+          static_for<KT>([&](auto u) __attribute__((always_inline)) {
+            all[u] = mma(n_s, state(Sh::D, u), all[u]);
+            fetch_beside(u, all[u]);
+          });
         }
       }
       int cols_k = anew(cols_k0), points = anew(points0);
@@ -377,26 +377,28 @@ __device__ __forceinline__ void gradient_part(const DeltaArgs& a, const Chunk& c
           if (r1 == 0) sh.x[row1 + e] = dx;
         }
       }
+      // sum K.Z, or (on the diagonal, lane 16 q + 4 q + e, where dB.V stands too) <S, dS'>
+      float whole = 0.0f;
       if constexpr (BEHIND) {
-        float whole = (ends[0] + ends[1]) + (ends[2] + ends[3]);
-        // dB.V and <S, dS'> stand on diagonals, lane 16 q + 4 q + e
+        whole = (ends[0] + ends[1]) + (ends[2] + ends[3]);
+      } else {
 #pragma unroll
         for (int e = 0; e < 4; ++e)
           if (r1 == row1 - 16 * wave + e) {
             sh.bv[row1 + e] = bv[e];
-            whole = fmaf(sh.gamma[63], inner[e], whole);
+            whole = sh.gamma[63] * inner[e];
           }
-        whole = sum_of_16(whole);
-        whole += __shfl_xor(whole, 16);
-        whole += __shfl_xor(whole, 32);
-        if (lane == 0) sh.sum[wave] = whole;
       }
+      whole = sum_of_16(whole);
+      whole += __shfl_xor(whole, 16);
+      whole += __shfl_xor(whole, 32);
+      if (lane == 0) sh.sum[BEHIND ? 4 + wave : wave] = whole;
       __syncthreads();
       if (keeper) {
         const int own = anew(lane);
         float* dots = a.dots + block * 192;  // (every place is written and read by one lane)
         float total = sh.q[own] + sh.beta[own] * sh.x[own] - sh.y[own], d_beta = sh.x[own] + (d0 == 0 ? sh.bv[own] : 0.0f);
-        if (own == 63) total += (sh.sum[0] + sh.sum[1]) + (sh.sum[2] + sh.sum[3]);
+        if (own == 63) total += ((sh.sum[0] + sh.sum[1]) + (sh.sum[2] + sh.sum[3])) + ((sh.sum[4] + sh.sum[5]) + (sh.sum[6] + sh.sum[7]));
         if (WIDE && d0 > 0) {
           total += dots[own];
           d_beta += dots[64 + own];

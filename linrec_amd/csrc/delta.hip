@@ -15,21 +15,34 @@ int check_delta(const linrec_delta_t* p) {
   return LINREC_OK;
 }
 
-constexpr int64_t DELTA_FILL = 256, DELTA_LEAST_SEGMENT = 8;  // workgroups, chunks
-
 size_t aligned(size_t n) { return (n + 255) & ~size_t(255); }
 
 // Chunks of a segment, 0 where sequences are not cut.
+//
+// A workgroup of a pass fills a CU, so `w` of them take ceil(w / 256) rounds, each as long as its chunks are many.  Cut into n segments a pass becomes
+// two, the first with the columns of the unit matrix as well, and what goes from segment to segment: about half a chunk's time for
+// each, and two chunks' for two launches more.  What counts is n at which a pass's rounds are about to grow, and the most that leaves four
+// chunks to a segment (shorter ones gain nothing: 1 x 2048 with 8 heads of 64 x 64, forward and backward, 172 us with 4, 199 with 2, 214 with 8).
+// 1 x 8192 with 128 x 128 bf16, forward and backward, cut and not: 16 heads (8 segments) 906 and 1696 us, 32 heads (4) 1460 and 1988, 48 heads (2) 2441
+// and 2276, which is not cut.
 int segment_of(const DeltaArgs& a, int width) {
+  constexpr int64_t CUS = 256, LEAST = 4;
   const linrec_delta_t& p = a.p;
   if (p.sequences == 0 || p.time == 0) return 0;
-  const int64_t side = p.sequences * p.heads, key_blocks = width / (16 * delta_waves(a.columns));
+  const int64_t side = p.sequences * p.heads, one = side * a.blocks, both = side * (a.blocks + width / (16 * delta_waves(a.columns)));
   const int64_t chunks = cdiv(a.slots, p.sequences);  // of a sequence (of packed ones the mean)
-  // so many that the first pass, which has the columns of the unit matrix as well, fills the chip
-  const int64_t segments = DELTA_FILL / (side * (a.blocks + key_blocks));
-  if (segments < 3 || chunks < 3 * DELTA_LEAST_SEGMENT) return 0;
-  const int64_t each = cdiv(chunks, segments);
-  return int(each < DELTA_LEAST_SEGMENT ? DELTA_LEAST_SEGMENT : each);
+  int64_t best = 2 * chunks * cdiv(one, CUS), segments = 0;  // (times in half chunks)
+  auto look = [&](int64_t n) {
+    if (n > chunks / LEAST) n = chunks / LEAST;
+    if (n < 2) return;
+    const int64_t time = 2 * cdiv(chunks, n) * (cdiv(both * n, CUS) + cdiv(one * n, CUS)) + n + 4;
+    if (time < best) best = time, segments = n;
+  };
+  for (int64_t rounds = 1; rounds <= 4; ++rounds) {
+    look(CUS * rounds / both);
+    look(CUS * rounds / one);
+  }
+  return segments ? int(cdiv(chunks, segments)) : 0;
 }
 
 // Sizes, and scratch parts from `base` on; returns the bytes of scratch.

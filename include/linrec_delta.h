@@ -20,6 +20,7 @@ extern "C" {
 #endif
 
 #define LINREC_DELTA_KEY_DIM_MAX 256
+#define LINREC_DELTA_ROW_MAX (1 << 28) /* heads x value_dim, of linrec_delta_t */
 
 /*
  * Gated delta rule.  Every value head has a state S of key_dim x value_dim, and at a position

@@ -15,6 +15,7 @@ from ._native import DTYPES, lib
 _i32, _i64, _f32, _ptr, _u64 = ctypes.c_int32, ctypes.c_int64, ctypes.c_float, ctypes.c_void_p, ctypes.c_uint64
 _pair, _three = _i64 * 2, _i64 * 3
 KEY_DIM_MAX = 256  # LINREC_DELTA_KEY_DIM_MAX
+ROW_MAX = 1 << 28  # LINREC_DELTA_ROW_MAX
 
 
 class Delta(ctypes.Structure):
@@ -114,6 +115,8 @@ def _delta_args(q, k, v, log_decay, beta, h0, cu_seqlens, scale, *gradients):
     packed = cu_seqlens is not None
     lead = (time,) if packed else (batch, time)
     key_heads, key_dim, heads, value_dim = _check_heads(what, q, k, v, log_decay, beta, "positions" if packed else "batch, time", lead)
+    if heads * value_dim > ROW_MAX:
+        raise RuntimeError(f"{what}: {heads} heads of {value_dim} values are more than {ROW_MAX} values a position")
     if h0 is not None:
         _check_fp32(what, h0, "h0", (sequences, heads, key_dim, value_dim), q.device)
     whole = all(t is None or t.is_contiguous() for t in (h0, cu_seqlens))

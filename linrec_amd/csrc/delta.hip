@@ -11,7 +11,7 @@ int check_delta(const linrec_delta_t* p) {
   if (p->key_dim > LINREC_DELTA_KEY_DIM_MAX) return LINREC_E_UNSUPPORTED;
   if (p->cu_seqlens ? p->batch != 1 : p->sequences != p->batch) return LINREC_E_INVALID;
   if (p->time > 2147483647LL - 4096 || p->batch > 2147483647LL || p->sequences > 2147483647LL - 64) return LINREC_E_TOO_LARGE;
-  if (p->value_dim > (1 << 20)) return LINREC_E_TOO_LARGE;
+  if (p->value_dim > (1 << 20) || int64_t(p->heads) * p->value_dim > LINREC_DELTA_ROW_MAX) return LINREC_E_TOO_LARGE;
   return LINREC_OK;
 }
 

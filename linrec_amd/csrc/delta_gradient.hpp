@@ -58,7 +58,6 @@ struct InputStager {
   }
 };
 
-template <typename T, int DK>
 struct GradientScratch {  // LDS beside GradientShared
   alignas(32) double g[64];
   alignas(16) float gamma[64], rest[64], beta[64], q[64], x[64], y[64], bv[64], sum[8];
@@ -80,7 +79,7 @@ __device__ __forceinline__ Planes<U, OUT> scaled(const Planes<U, N>& f, float by
 
 // What the waves of one part do: dQ and X, or (BEHIND) Y.  Both parts meet at the same barriers.
 template <typename T, int DK, bool WIDE, bool BEHIND>
-__device__ __forceinline__ void gradient_part(const DeltaArgs& a, const Chunk& ch, int64_t slot, int key_head, char* smem, GradientScratch<T, DK>& sh) {
+__device__ __forceinline__ void gradient_part(const DeltaArgs& a, const Chunk& ch, int64_t slot, int key_head, char* smem, GradientScratch& sh) {
   using U = Inner<T>;
   using Sh = GradientShared<T, DK>;
   using TI = Tile<U, 32>;  // dO, V
@@ -454,7 +453,7 @@ __device__ __forceinline__ void gradient_part(const DeltaArgs& a, const Chunk& c
 template <typename T, int DK, bool WIDE>
 __global__ __launch_bounds__(GRADIENT_LANES) void delta_gradient_kernel(DeltaArgs a) {
   __shared__ __align__(16) char smem[GradientShared<T, DK>::BYTES];
-  __shared__ GradientScratch<T, DK> sh;
+  __shared__ GradientScratch sh;
   const int64_t slot = blockIdx.x / unsigned(a.p.key_heads);
   const int key_head = int(blockIdx.x - slot * unsigned(a.p.key_heads));
   const Chunk ch = chunk_of(a.p, slot);

@@ -129,6 +129,16 @@ def test_bad_arguments_are_rejected_by_the_library():
         assert call(ctypes.byref(args)) == -2
 
 
+def test_positions_of_too_many_values_are_refused(no_launch):
+    library = _delta._lib
+    wide = _delta.Delta(dtype=2, key_heads=1, heads=512, key_dim=4, value_dim=(1 << 19) + 1, batch=1, time=4, sequences=1)
+    assert library.linrec_delta_fwd(ctypes.byref(wide)) == library.linrec_delta_bwd(ctypes.byref(wide)) == -4
+    assert library.linrec_delta_scratch_bytes(ctypes.byref(wide), 0) == 0
+    v = torch.empty(1).expand(1, 1, 512, (1 << 19) + 1)
+    with pytest.raises(RuntimeError, match="values a position"):
+        linrec_amd.gated_delta(torch.empty(1, 1, 1, 4), torch.empty(1, 1, 1, 4), v, torch.empty(1, 1, 512), torch.empty(1, 1, 512))
+
+
 def test_a_step_counts_as_a_change_of_the_states_and_refuses_tangents(no_launch):
     from torch.autograd import forward_ad
     tensors = [t[:, 0] for t in arguments()] + [torch.zeros(2, 2, 8, 4)]

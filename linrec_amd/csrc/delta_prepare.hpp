@@ -4,6 +4,9 @@
 // and C are put together afterwards.  1 + A is unit lower triangular; its inverse is put together in fp32: blocks of 16 by substitution, a lane for a column,
 // then of 32 and of 64 by M21 = -M22 A21 M11 with the fp32 matrix instruction.  (Substitution over all 64 rows would be 64 dependent
 // steps; powers of A, whose binomials cancel, lose all digits where keys are alike.)
+//
+// 8 x 4096, 16 heads of 128 x 128 bf16: 140 us forward and 160 backward for 0.40 and 0.54 GB (79 and 105 us at the rate of a copy); ten meetings
+// of a workgroup, three of which fit into a CU.
 #pragma once
 #include "delta_core.hpp"
 

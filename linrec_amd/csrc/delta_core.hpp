@@ -389,6 +389,16 @@ struct Stager {
         *reinterpret_cast<V*>(tile + L::at(16 * g + r, L::HALF ? 4 * k + q : 8 * (k >> 1) + 2 * q + (k & 1))) = v[n];
     }
   }
+  // a triangle, without its empty quarter
+  template <bool UPPER>
+  __device__ __forceinline__ void put_triangle(char* tile, int lane) const {
+    const int row0 = lane / L::UNITS, unit = lane % L::UNITS;
+#pragma unroll
+    for (int n = 0; n < N; ++n) {
+      const int row = n * STEP + row0;
+      if (UPPER ? row < ROWS / 2 || unit >= L::UNITS / 2 : row >= ROWS / 2 || unit < L::UNITS / 2) *reinterpret_cast<V*>(tile + L::at(row, unit)) = v[n];
+    }
+  }
   __device__ __forceinline__ void put(char* tile, int lane) const {
 #pragma unroll
     for (int n = 0; n < N; ++n)

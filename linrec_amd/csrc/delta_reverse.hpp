@@ -14,7 +14,9 @@ struct ReverseShared {
   static constexpr int KEYS = Tile<T, DK>::BYTES, VALUES = Tile<T, 16 * WAVES>::BYTES;
   static constexpr bool QUERIES = 2 * KEYS + VALUES + 2 * square_bytes<U>() + 1024 <= 160 * 1024;
   static constexpr int K = 0, Q = K + KEYS, O = Q + (QUERIES ? KEYS : 0), M = O + VALUES, C = M + square_bytes<U>(),
-                       GATES = C + square_bytes<U>(), BYTES = GATES + 3 * 64 * 4;
+                       TILES = C + square_bytes<U>();
+  static constexpr GatePlace<U, true> GATES{TILES, C, true};
+  static constexpr int BYTES = GATES.bytes;
   static constexpr bool LOADERS = 2 * BYTES <= 160 * 1024;
   static constexpr int LANES = 64 * WAVES * (LOADERS ? 2 : 1);
 };
@@ -68,11 +70,12 @@ __global__ __launch_bounds__((ReverseShared<T, DK, WAVES>::LANES)) void delta_re
 #pragma unroll
     for (int k2 = 0; k2 < P; ++k2) {
       m[k2].put(smem + Sh::M + k2 * TS::BYTES, by);
-      cc[k2].put(smem + Sh::C + k2 * TS::BYTES, by);
+      if constexpr (Sh::GATES.inside) cc[k2].template put_triangle<true>(smem + Sh::C + k2 * TS::BYTES, by);
+      else cc[k2].put(smem + Sh::C + k2 * TS::BYTES, by);
     }
 #pragma unroll
     for (int i = 0; i < (192 + STAGING - 1) / STAGING; ++i)
-      if (i * STAGING + by < 192) reinterpret_cast<float*>(smem + Sh::GATES)[i * STAGING + by] = gate[i];
+      if (i * STAGING + by < 192) reinterpret_cast<float*>(smem + Sh::GATES.at)[Sh::GATES.place(i * STAGING + by)] = gate[i];
   };
 
   v4f s[DK / 16];  // dS'
@@ -97,7 +100,7 @@ __global__ __launch_bounds__((ReverseShared<T, DK, WAVES>::LANES)) void delta_re
   auto compute = [&](int64_t c, const char* smem) __attribute__((always_inline)) {
     const int64_t first = span.first + c * DELTA_CHUNK, block = (span.slot + c) * p.heads + head;
     const int length = int(span.end - first < DELTA_CHUNK ? span.end - first : DELTA_CHUNK);
-    const float* gates = reinterpret_cast<const float*>(smem + Sh::GATES);
+    const float* gates = reinterpret_cast<const float*>(smem + Sh::GATES.at);
     const T* qq = head_rows<T>(p.q, p.q_stride, span.batch, first, key_head);
     Planes<T> sp[DK / 32];
     float un_s;
@@ -150,7 +153,7 @@ __global__ __launch_bounds__((ReverseShared<T, DK, WAVES>::LANES)) void delta_re
       mma_tiles<0, 4>(f, sp[b], x);
     }
 #pragma unroll
-    for (int t = 0; t < 4; ++t) x[t] *= *reinterpret_cast<const v4f*>(gates + 64 + row_of_result(t, q)) * un_s;
+    for (int t = 0; t < 4; ++t) x[t] *= Sh::GATES.four(gates + 64, 64, row_of_result(t, q)) * un_s;
     upper(Sh::C, dop, x);
     constexpr int CHAIN = chain_planes<U>();
     Planes<U, CHAIN> xp[2];
@@ -170,7 +173,7 @@ __global__ __launch_bounds__((ReverseShared<T, DK, WAVES>::LANES)) void delta_re
 #pragma unroll
     for (int t = 0; t < 4; ++t) {
       const int row = row_of_result(t, q);
-      const v4f gamma = *reinterpret_cast<const v4f*>(gates + row), beta = *reinterpret_cast<const v4f*>(gates + 128 + row);
+      const v4f gamma = Sh::GATES.four(gates, 0, row), beta = Sh::GATES.four(gates + 128, 128, row);
       T* to = d_v + row * int64_t(apart);
 #pragma unroll
       for (int e = 0; e < 4; ++e) db[t][e] *= beta[e];
@@ -194,7 +197,7 @@ __global__ __launch_bounds__((ReverseShared<T, DK, WAVES>::LANES)) void delta_re
     float un_v, un_o;
     split_scaled(db, vp, &un_v);
     split_scaled(d_o, op, &un_o);
-    const float keep = gates[63];
+    const float keep = gates[Sh::GATES.place(63)];
 #pragma unroll
     for (int t = 0; t < DK / 16; ++t) {
       auto with_keys = [&](v4f to) __attribute__((always_inline)) {

@@ -16,6 +16,24 @@ constexpr int square_bytes() {
   return 64 * 64 * int(sizeof(U)) * planes_of<U>();
 }
 
+// Where a chunk's gates lie: behind its tiles, or in the empty quarter of the triangle C, the last of them, where two chunks fit into LDS only so
+// (fp32 of 64 channels, 160 KB to the byte: 8 x 4096 with 16 heads of 64 x 64 575 us forward and 2042 with the backward, 710 and 2303 with one chunk).
+// In bytes; place() in floats.
+template <typename U, bool UPPER>
+struct GatePlace {
+  static constexpr int ALONE = 3 * 64 * 4;
+  bool inside;
+  int at, bytes;
+  constexpr GatePlace(int tiles, int c, bool has_c)
+      : inside(has_c && sizeof(U) == 4 && 2 * (tiles + ALONE) > 160 * 1024 && 2 * tiles <= 160 * 1024),
+        at(!inside ? tiles : c + (UPPER ? 32 * 64 : 32) * 4), bytes(inside ? tiles : tiles + ALONE) {}
+  constexpr __device__ __forceinline__ int place(int gate) const { return inside ? (gate >> 5) * 64 + (gate & 31) : gate; }
+  // four gates of a kind (from the first of them on) of rows from `row` on
+  __device__ __forceinline__ v4f four(const float* kind, int first, int row) const {
+    return *reinterpret_cast<const v4f*>(inside ? kind + (place(first + row) - first) : kind + row);
+  }
+};
+
 enum ScanMode {
   SCAN_OUT,     // the forward: O and the last state
   SCAN_STATES,  // a backward's first pass, which keeps the states before the chunks and N and has no O
@@ -30,7 +48,9 @@ struct ScanShared {
   // (fp32 of 256 channels: queries are read from memory where they are used)
   static constexpr bool QUERIES = !STATES && 2 * KEYS + VALUES + 2 * square_bytes<U>() + 1024 <= 160 * 1024;
   static constexpr int K = 0, Q = K + KEYS, V = Q + (QUERIES ? KEYS : 0), M = V + VALUES, C = M + square_bytes<U>(),
-                       GATES = C + (STATES ? 0 : square_bytes<U>()), BYTES = GATES + 3 * 64 * 4;
+                       TILES = C + (STATES ? 0 : square_bytes<U>());
+  static constexpr GatePlace<U, false> GATES{TILES, C, !STATES};
+  static constexpr int BYTES = GATES.bytes;
   static constexpr bool LOADERS = 2 * BYTES <= 160 * 1024;
   static constexpr int LANES = 64 * WAVES * (LOADERS ? 2 : 1);
 };
@@ -97,11 +117,12 @@ __global__ __launch_bounds__((ScanShared<T, DK, WAVES, MODE>::LANES)) void delta
 #pragma unroll
     for (int k2 = 0; k2 < P; ++k2) {
       m[k2].put(smem + Sh::M + k2 * TS::BYTES, by);
-      if constexpr (MODE == SCAN_OUT) cc[k2].put(smem + Sh::C + k2 * TS::BYTES, by);
+      if constexpr (Sh::GATES.inside) cc[k2].template put_triangle<false>(smem + Sh::C + k2 * TS::BYTES, by);
+      else if constexpr (MODE == SCAN_OUT) cc[k2].put(smem + Sh::C + k2 * TS::BYTES, by);
     }
 #pragma unroll
     for (int i = 0; i < (192 + STAGING - 1) / STAGING; ++i)
-      if (i * STAGING + by < 192) reinterpret_cast<float*>(smem + Sh::GATES)[i * STAGING + by] = gate[i];
+      if (i * STAGING + by < 192) reinterpret_cast<float*>(smem + Sh::GATES.at)[Sh::GATES.place(i * STAGING + by)] = gate[i];
   };
 
   v4f s[DK / 16];
@@ -132,7 +153,7 @@ __global__ __launch_bounds__((ScanShared<T, DK, WAVES, MODE>::LANES)) void delta
   auto compute = [&](int64_t c, const char* smem) __attribute__((always_inline)) {
     const int64_t first = span.first + c * DELTA_CHUNK, block = (span.slot + c) * p.heads + head;
     const int length = int(span.end - first < DELTA_CHUNK ? span.end - first : DELTA_CHUNK);
-    const float* gates = reinterpret_cast<const float*>(smem + Sh::GATES);
+    const float* gates = reinterpret_cast<const float*>(smem + Sh::GATES.at);
     const T* qq = head_rows<T>(p.q, p.q_stride, span.batch, first, key_head);
     Planes<T> sp[DK / 32];
     float un_s;
@@ -174,7 +195,7 @@ __global__ __launch_bounds__((ScanShared<T, DK, WAVES, MODE>::LANES)) void delta
     for (int t = 0; t < 4; ++t) {
       const int row = row_of_result(t, q);
       const auto v = TV::template column4<false>(smem + Sh::V, cols_v, TK::mapped_row(t), 0);
-      const v4f gamma = *reinterpret_cast<const v4f*>(gates + row), beta = *reinterpret_cast<const v4f*>(gates + 128 + row);
+      const v4f gamma = Sh::GATES.four(gates, 0, row), beta = Sh::GATES.four(gates + 128, 128, row);
 #pragma unroll
       for (int e = 0; e < 4; ++e) x[t][e] = beta[e] * fmaf(-gamma[e] * un_s, x[t][e], float(v[e]));
     }
@@ -217,7 +238,7 @@ __global__ __launch_bounds__((ScanShared<T, DK, WAVES, MODE>::LANES)) void delta
         mma_tiles<0, 4>(f, sp[b], y);
       }
 #pragma unroll
-      for (int t = 0; t < 4; ++t) y[t] *= *reinterpret_cast<const v4f*>(gates + row_of_result(t, q)) * (un_s * p.scale);
+      for (int t = 0; t < 4; ++t) y[t] *= Sh::GATES.four(gates, 0, row_of_result(t, q)) * (un_s * p.scale);
       lower(Sh::C, np, y);
 #pragma unroll
       for (int t = 0; t < 4; ++t) {
@@ -235,11 +256,11 @@ __global__ __launch_bounds__((ScanShared<T, DK, WAVES, MODE>::LANES)) void delta
       }
     }
 #pragma unroll
-    for (int t = 0; t < 4; ++t) nn[t] *= *reinterpret_cast<const v4f*>(gates + 64 + row_of_result(t, q));
+    for (int t = 0; t < 4; ++t) nn[t] *= Sh::GATES.four(gates + 64, 64, row_of_result(t, q));
     Planes<T, chain_planes<T>()> nt[2];
     float un_n;
     split_scaled(nn, nt, &un_n);
-    const float keep = gates[63];
+    const float keep = gates[Sh::GATES.place(63)];
 #pragma unroll
     for (int t0 = 0; t0 < DK / 16; t0 += 4) {
       v4f to[4];

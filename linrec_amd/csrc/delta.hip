@@ -66,8 +66,8 @@ size_t lay_out(const linrec_delta_t& p, bool bwd, char* base, DeltaArgs* a) {
   };
   a->square = 4096 * value;
   a->rows = int64_t(a->columns) * 64 * value;
-  const int kept = width == 64 && p.dtype != LINREC_DTYPE_F32 ? 6 : value;  // (kept_planes)
-  a->rows_n = int64_t(a->columns) * 64 * kept;
+  const int three = p.dtype != LINREC_DTYPE_F32 ? 6 : value, kept = width == 64 ? three : value;  // (chain_planes, kept_planes)
+  a->rows_n = int64_t(a->columns) * 64 * three;
   a->state = int64_t(a->columns) * width * kept;
   a->m = part(a->square);
   a->c = part(a->square);

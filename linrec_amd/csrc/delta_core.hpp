@@ -20,9 +20,9 @@
 // Precision.  States, sums and accumulators are fp32.  An operand of a matrix instruction that is not an input is split into
 // bf16 (or, beside fp16 inputs, fp16) numbers, its rounding, the rounding of the rest and so on: two bf16 carry 16 to 17 bits, three 24, two
 // fp16 22.  In the chain of products that makes a state from the one before, what meets an input is three bf16 or two fp16, and what meets M
-// three bf16; M, C and what is kept for the gradients are two, S, dS' and N up to 64 key channels three (kept_planes).  So a state is
-// 1e-6 off, the gradient of beta 4e-6 and that of log_decay 3e-6 up to 64 key channels, 5e-6 from there on (with two bf16 in the chain and
-// without the products of rests 1e-5 to 1.6e-5, with one bf16 2e-3).  fp32 inputs take the fp32 instructions.
+// three bf16; M, C and dB are two, N three, S and dS' as kept for the gradients three up to 64 key channels and two from there on (kept_planes).  So a state is
+// 1e-6 off, the gradient of beta 4e-6 and that of log_decay 3e-6 up to 64 key channels, 4e-6 from there on (with two of N 5e-6, and 1.1e-5 where
+// its sum cancels; with two bf16 in the chain and without the products of rests 1e-5 to 1.6e-5, with one bf16 2e-3).  fp32 inputs take the fp32 instructions.
 #pragma once
 #include <hip/hip_runtime.h>
 #include <stdint.h>
@@ -149,7 +149,7 @@ template <typename U>
 constexpr int chain_planes() {
   return std::is_same_v<U, __bf16> ? 3 : planes_of<U>();
 }
-// Planes of N, S and dS' as they are kept for the gradients.  With up to 64 key channels the gradients of the gates are sums of so few
+// Planes of S and dS' as they are kept for the gradients.  With up to 64 key channels the gradients of the gates are sums of so few
 // terms that the rounding of two shows: 1e-5 of them for 16 to 32 key channels, 3e-6 with three, which LDS has room for there.
 template <typename U, int DK>
 constexpr int kept_planes() {
@@ -448,7 +448,7 @@ struct DeltaArgs {
   double* sums;  // [64]: G
   char* s;       // [kept_planes][columns][DK] in pieces of 16 columns (store_rows), the state before the chunk
   char* d_s;     // the same of dS' behind it
-  char* n;       // [kept_planes][columns][64] in such pieces
+  char* n;       // [chain_planes][columns][64] in such pieces
   char* d_b;
   float* dots;   // [192], sums of the gates' gradients where key_dim comes in turns
   // for every (part, head), where sequences are cut (delta_segments.hpp)

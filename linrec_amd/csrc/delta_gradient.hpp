@@ -11,7 +11,7 @@
 // channels come 32 at a time through LDS, the next ones on their way in registers meanwhile.  Its waves have two parts, four waves
 // of 16 rows each: dQ and X, which multiply S, and Y, which multiplies dS'.  One wave for all three would hold more than its share of the
 // registers (what then goes through scratch costs more than the products: 2.4 ms for 8 x 4096 x 16 heads of 128 x 128 bf16), three
-// parts read S from LDS twice (0.79 ms); two 0.67 ms, for 2.1 GB of states, operands and results (0.42 at the rate of a
+// parts read S from LDS twice (0.79 ms); two 0.69 ms, for 2.3 GB of states, operands and results (0.45 at the rate of a
 // copy).  The 64 x 64 products F, F^T, E, E^T are computed as they are needed as operands: what a lane gets of a product is its part of an
 // operand over the product's rows.
 #pragma once
@@ -25,11 +25,11 @@ constexpr int GRADIENT_LANES = 512, GRADIENT_PART = 256;
 template <typename T, int DK>
 struct GradientShared {
   using U = Inner<T>;
-  static constexpr int P = planes_of<U>(), KEPT = kept_planes<U, DK>(), IN = input_planes<T>();
+  static constexpr int P = planes_of<U>(), KEPT = kept_planes<U, DK>(), CHAIN = chain_planes<U>(), IN = input_planes<T>();
   static constexpr int IN_V = 64 * 32 * int(sizeof(U)), BY_V = 32 * 64 * int(sizeof(U)), STATE = 32 * DK * int(sizeof(U)),
                        KEYS = Tile<U, DK>::BYTES;
   // one step's values, then both inputs of key channels
-  static constexpr int O = 0, V = O + IN * IN_V, B = V + IN * IN_V, N = B + P * BY_V, S = N + KEPT * BY_V, D = S + KEPT * STATE, STEP = D + KEPT * STATE;
+  static constexpr int O = 0, V = O + IN * IN_V, B = V + IN * IN_V, N = B + P * BY_V, S = N + CHAIN * BY_V, D = S + KEPT * STATE, STEP = D + KEPT * STATE;
   static constexpr int BUFFERS = 2 * STEP + 2 * IN * KEYS + 4096 <= 160 * 1024 ? 2 : 1;
   static constexpr int K = BUFFERS * STEP, Q = K + IN * KEYS, BYTES = Q + IN * KEYS;
   static_assert(64 * DK * 4 <= BUFFERS * STEP, "room to hand dK over");
@@ -86,7 +86,7 @@ __device__ __forceinline__ void gradient_part(const DeltaArgs& a, const Chunk& c
   using TI = Tile<U, 32>;  // dO, V
   using TB = Tile<U, 64>;  // dB, N: rows are channels
   using TK = Tile<U, DK>;  // K, Q; S, dS': rows are channels
-  constexpr int P = Sh::P, KEPT = Sh::KEPT, IN = Sh::IN, KT = DK / 16, LANES = GRADIENT_PART;
+  constexpr int P = Sh::P, KEPT = Sh::KEPT, CHAIN = Sh::CHAIN, IN = Sh::IN, KT = DK / 16, LANES = GRADIENT_PART;
   constexpr int64_t ROW = WIDE ? 2 * DK : DK;  // of the kept states
   const linrec_delta_t& p = a.p;
   const int lane = threadIdx.x & 63, r = lane & 15, q = lane >> 4, by0 = threadIdx.x & (LANES - 1);
@@ -98,14 +98,14 @@ __device__ __forceinline__ void gradient_part(const DeltaArgs& a, const Chunk& c
 
   // what a step needs on its way: the rows of dO and V with dB and N, or S and dS'
   InputStager<T, 32, LANES> so, sv;
-  Stager<U, 64, LANES, 32> sb[P], sn[KEPT];
+  Stager<U, 64, LANES, 32> sb[P], sn[CHAIN];
   Stager<U, DK, LANES, 32> ss[KEPT], sd[KEPT];
   // one wave has what belongs to the positions, a lane for each
   const bool keeper = BEHIND && wave == 0;
   double sum = 0.0;
   float gamma = 0.0f, rest = 0.0f, beta = 0.0f;
   // (loads are issued one part after the other between products: all at once they wait for each other, 2600 of a step's 8000 cycles)
-  constexpr int PARTS = BEHIND ? 2 * KEPT : 2 + P + KEPT;
+  constexpr int PARTS = BEHIND ? 2 * KEPT : 2 + P + CHAIN;
   auto fetch_gates = [&](int head) __attribute__((always_inline)) {
     if (keeper) {
       const int64_t block = slot * p.heads + head;
@@ -143,7 +143,7 @@ __device__ __forceinline__ void gradient_part(const DeltaArgs& a, const Chunk& c
       sv.put(to + Sh::V, by);
     }
 #pragma unroll
-    for (int k = 0; k < KEPT; ++k) {
+    for (int k = 0; k < (BEHIND ? KEPT : CHAIN); ++k) {
       if constexpr (!BEHIND) {
         if (k < P) sb[k].put_pieces(to + Sh::B + k * Sh::BY_V, by);
         sn[k].put_pieces(to + Sh::N + k * Sh::BY_V, by);
@@ -211,8 +211,10 @@ __device__ __forceinline__ void gradient_part(const DeltaArgs& a, const Chunk& c
         };
         const int rows_w = anew(rows_w0), rows_m = anew(rows_m0), cols_w = anew(cols_w0), cols_m = anew(cols_m0), cols_k = anew(cols_k0),
                   rows_v = anew(rows_v0);
+        // (dB.N is a sum of large terms of both signs where key channels are few: the products of rests count there)
+        constexpr int REST = KEPT == 3 ? 2 : 1;
         constexpr std::integral_constant<int, P> two{};
-        constexpr std::integral_constant<int, KEPT> kept{};
+        constexpr std::integral_constant<int, CHAIN> three{};
         auto rows_in = [&](int part, int view, int row) __attribute__((always_inline)) {
           Planes<U, IN> out;
 #pragma unroll
@@ -245,9 +247,9 @@ __device__ __forceinline__ void gradient_part(const DeltaArgs& a, const Chunk& c
 #pragma unroll
           for (int t = 0; t < 4; ++t)
             if (t / 2 <= wave / 2) {  // rows j of F^T and E^T up to this wave's columns i
-              const Planes<U, KEPT> n_t = by_v_mapped(Sh::N, t, kept);
+              const Planes<U, CHAIN> n_t = by_v_mapped(Sh::N, t, three);
               f[t] = mma_up_to<2>(n_t, do_w, f[t]);
-              ee[t] = mma_up_to<2>(n_t, db_w, ee[t]);
+              ee[t] = mma_up_to<REST>(n_t, db_w, ee[t]);
             }
           fetch_beside(std::integral_constant<int, 1>{}, all[0]);
           const Planes<U, KEPT> do_s = scaled<U, KEPT>(do_w, p.scale * sh.gamma[own]);
@@ -272,16 +274,16 @@ __device__ __forceinline__ void gradient_part(const DeltaArgs& a, const Chunk& c
               inner = mma_up_to<2>(s_v, d_v, inner);
             }
         } else {
-          const Planes<U, KEPT> n_w = by_v(Sh::N, kept);
+          const Planes<U, CHAIN> n_w = by_v(Sh::N, three);
 #pragma unroll
           for (int t = 0; t < 4; ++t)
             if (t / 2 >= wave / 2) {
               f[t] = mma_up_to<2>(rows_in(Sh::O, rows_m, TI::mapped_row(t)), n_w, f[t]);
-              ee[t] = mma_up_to<2>(by_v_mapped(Sh::B, t, two), n_w, ee[t]);
+              ee[t] = mma_up_to<REST>(by_v_mapped(Sh::B, t, two), n_w, ee[t]);
             }
           fetch_beside(std::integral_constant<int, 1>{}, all[0]);
           // (what goes into the gradient of log_decay through Z is a small sum of large terms: all that two numbers hold counts)
-          const Planes<U, chain_planes<U>()> n_s = scaled<U, chain_planes<U>()>(n_w, sh.rest[own]);
+          const Planes<U, CHAIN> n_s = scaled<U, CHAIN>(n_w, sh.rest[own]);
           static_for<KT>([&](auto u) __attribute__((always_inline)) {
             all[u] = mma(n_s, state(Sh::D, u), all[u]);
             fetch_beside(std::integral_constant<int, 2 + u()>{}, all[u]);
@@ -291,7 +293,8 @@ __device__ __forceinline__ void gradient_part(const DeltaArgs& a, const Chunk& c
       int cols_k = anew(cols_k0), points = anew(points0);
       const int r1 = anew(r), row1 = 16 * wave + 4 * anew(q);
       // the masks and decays; rows of results to operands
-      Planes<U, KEPT> fp[2], ep[2];
+      Planes<U, CHAIN> fp[2];
+      Planes<U, KEPT> ep[2];
       {
         // (all reads ahead of what they are compared for: a read that waits in a branch of its own costs its latency, 16 times over)
         typedef double v4d __attribute__((ext_vector_type(4)));
@@ -313,7 +316,7 @@ __device__ __forceinline__ void gradient_part(const DeltaArgs& a, const Chunk& c
         }
 #pragma unroll
         for (int b = 0; b < 2; ++b) {
-          fp[b] = split<U, KEPT>(f[2 * b], f[2 * b + 1]);
+          fp[b] = split<U, CHAIN>(f[2 * b], f[2 * b + 1]);
           ep[b] = split<U, KEPT>(ee[2 * b], ee[2 * b + 1]);
         }
       }

@@ -4,7 +4,7 @@
 // other half loads what the next chunk needs into LDS meanwhile (a state's chunks follow one another, so nothing else hides those loads: 290 us
 // with them, 604 without; where two chunks do not fit into LDS all waves load first and compute then).
 //
-// 8 x 4096, 16 heads of 128 x 128 bf16: 295 us with O, 290 with the states, for 0.67 and 1.14 GB (131 and 223 us at the rate of a copy).  A chunk
+// 8 x 4096, 16 heads of 128 x 128 bf16: 295 us with O and as many with the states, for 0.67 and 1.28 GB (131 and 250 us at the rate of a copy).  A chunk
 // is six products that wait for each other, by one wave of a SIMD, whose matrix instructions fill a third of the time.
 #pragma once
 #include "delta_core.hpp"
@@ -212,11 +212,10 @@ __global__ __launch_bounds__((ScanShared<T, DK, WAVES, MODE>::LANES)) void delta
     for (int b = 0; b < 2; ++b) np[b] = split<U>(nn[2 * b], nn[2 * b + 1]);
     if constexpr (MODE == SCAN_CARRY) {
     } else if constexpr (MODE == SCAN_STATES) {
-      constexpr int KEPT = kept_planes<U, DK>();
       U* to = reinterpret_cast<U*>(a.n + block * a.rows_n) + (col - r) * 64;
 #pragma unroll
       for (int b = 0; b < 2; ++b)
-        if (kept_column) store_rows(to, int64_t(a.columns) * 64, b, lane, split<U, KEPT>(nn[2 * b], nn[2 * b + 1]));
+        if (kept_column) store_rows(to, int64_t(a.columns) * 64, b, lane, split<U, CHAIN>(nn[2 * b], nn[2 * b + 1]));
     } else {
       T* o = static_cast<T*>(p.o) + ((span.batch * p.time + first) * p.heads + head) * int64_t(p.value_dim) + col;
       v4f y[4];

@@ -235,3 +235,36 @@ def test_one_tensor_as_two_arguments():
     assert torch.equal(o, o_many) and torch.equal(y, y2)
     for got, parts in ((d_k, (grads[0], grads[3])), (d_v, (grads[1],)), (d_gate, (grads[2], grads[4]))):
         ref.assert_near(got, sum(p.double() for p in parts).cpu(), 2.0 ** -22, "gradient")
+
+
+def test_offsets_beyond_32_bits():
+    """Rows a megabyte apart, over 2^31 elements in all, and a cache of more: the same bits as from dense tensors."""
+    apart, time = 1 << 20, 2100
+    room = torch.empty(time * apart, dtype=torch.bfloat16, device=DEV)
+
+    def far(at, *shape):  # (time, ...) in the rows of `room`
+        t = room.as_strided((time, *shape), (apart, *torch.empty(shape, device="meta").stride()), at)
+        return t.copy_(torch.randn((time, *shape), device=DEV))
+    q, k, v = far(0, 1, 16) / 4, far(64, 1, 16) / 4, far(128, 2, 24)
+    q, k = (far(at, 1, 16).copy_(t) for at, t in ((0, q), (64, k)))
+    d_o = far(256, 2, 24)
+    log_decay, beta = -torch.rand((time, 2), device=DEV), torch.rand((time, 2), device=DEV)
+    results = []
+    for form in (lambda t: t, lambda t: t.contiguous()):
+        leaves = [form(t).detach()[None].requires_grad_() for t in (q, k, v)]
+        o = linrec_amd.gated_delta(*leaves, log_decay[None], beta[None])
+        y, total = linrec_amd.rms_norm(leaves[2], residual=form(d_o)[None])
+        results.append([o, y, total, *torch.autograd.grad((o, y), leaves, (form(d_o)[None], form(d_o)[None]))])
+    assert q.stride(0) == apart and all(torch.equal(a, b) for a, b in zip(*results))
+    del room, q, k, v, d_o, results, leaves, o, y, total
+    rows, dims = 8200, (16, 128, 128)  # 2^31 + 2^21 values
+    cache = torch.empty((rows, *dims), device=DEV)
+    slots = torch.tensor([rows - 1, 0], dtype=torch.int32, device=DEV)
+    start = torch.randn((2, *dims), device=DEV)
+    cache[slots.long()] = start
+    q, k, v = (torch.randn((2, 16, 128), device=DEV) / 11 for _ in range(3))
+    gates = torch.rand((2, 16), device=DEV)
+    with torch.no_grad():
+        a = linrec_amd.gated_delta_step(q, k, v, -gates, gates, cache, slots=slots)
+        b = linrec_amd.gated_delta_step(q, k, v, -gates, gates, start)
+    assert torch.equal(a, b) and torch.equal(cache[slots.long()], start)

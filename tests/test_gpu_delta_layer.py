@@ -268,3 +268,24 @@ def test_offsets_beyond_32_bits():
         a = linrec_amd.gated_delta_step(q, k, v, -gates, gates, cache, slots=slots)
         b = linrec_amd.gated_delta_step(q, k, v, -gates, gates, start)
     assert torch.equal(a, b) and torch.equal(cache[slots.long()], start)
+
+
+@pytest.mark.parametrize("which", range(6))
+def test_gradients_against_differences(which):
+    """Along a random direction of one input, in fp32 with a step h of 2^-5.  f = <o, w> + <state, w'> is off by 8 * 2^-20 * sqrt(3) of its terms
+    (2e-5), over h by 6e-4; the third derivative adds h^2 / 6 = 2e-4, and nine times that for a log decay, whose steps add up over the ten
+    or so positions that a state remembers.  In all 2e-3 of what such a difference is large, |gradient|; 1e-2 allows for terms larger than that."""
+    g = torch.Generator(device=DEV).manual_seed(which)
+    q, k, v, log_decay, beta, h0 = (t.detach() for t in inputs(3, False))
+    leaves = [t.requires_grad_() for t in (q, k, v, -0.1 - 0.1 * log_decay.abs(), beta, h0)]
+    weights = [torch.randn(t.shape, device=DEV, generator=g) for t in (v, h0)]
+
+    def f(args):
+        o, state = linrec_amd.gated_delta(*args[:5], h0=args[5], return_state=True)
+        return [o, state]
+    grad = torch.autograd.grad(f(leaves), leaves[which], weights)[0].double()
+    step = torch.randn(grad.shape, device=DEV, generator=g) * 2.0 ** -5
+    with torch.no_grad():
+        up, down = ([t + s * step if n == which else t for n, t in enumerate(leaves)] for s in (1.0, -1.0))
+        change = sum(((a.double() - b.double()) * w.double()).sum() for a, b, w in zip(f(up), f(down), weights)) / 2
+    assert abs(float(change - (grad * step).sum())) <= 1e-2 * 2.0 ** -5 * float(grad.norm())

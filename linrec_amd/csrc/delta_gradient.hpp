@@ -5,14 +5,17 @@
 //   X  = E K - e^G dB S^T,  Z = e^{G_63 - G} N dS'^T,  Y = Z + F^T Q + E^T (beta K);      dK = beta X + Y
 //   dbeta = dB.V + K.X,  dG = Q.dQ + beta K.X - K.Y (row by row),  dG_63 += sum K.Z + e^{G_63} <S, dS'>
 //
-// and the gradient of log_decay is the sum of dG from a position to the chunk's end.
+// and the gradient of log_decay is the sum of dG from a position to the chunk's end.  The dots are those of one value head; the gradients of
+// q and k are the sums of dQ and dK over the heads that share them.
 //
 // A workgroup has a (chunk, key head) and walks over the value heads that share it, so that nothing is added by atomics.  Value
 // channels come 32 at a time through LDS, the next ones on their way in registers meanwhile.  Its waves have two parts, four waves
 // of 16 rows each: dQ and X, which multiply S, and Y, which multiplies dS'.  One wave for all three would hold more than its share of the
 // registers (what then goes through scratch costs more than the products: 2.4 ms for 8 x 4096 x 16 heads of 128 x 128 bf16), three
 // parts read S from LDS twice (0.79 ms); two 0.69 ms, for 2.3 GB of states, operands and results (0.45 at the rate of a
-// copy).  The 64 x 64 products F, F^T, E, E^T are computed as they are needed as operands: what a lane gets of a product is its part of an
+// copy).  beta X goes from the one part to the other through LDS, head by head, and is added to Y there, so each part keeps one sum over
+// the heads and what its head alone has (with differences of running sums for the latter, which took as long, 695 us, a small head lost its
+// digits).  The 64 x 64 products F, F^T, E, E^T are computed as they are needed as operands: what a lane gets of a product is its part of an
 // operand over the product's rows.
 #pragma once
 #include "delta_prepare.hpp"
@@ -32,7 +35,7 @@ struct GradientShared {
   static constexpr int O = 0, V = O + IN * IN_V, B = V + IN * IN_V, N = B + P * BY_V, S = N + CHAIN * BY_V, D = S + KEPT * STATE, STEP = D + KEPT * STATE;
   static constexpr int BUFFERS = 2 * STEP + 2 * IN * KEYS + 4096 <= 160 * 1024 ? 2 : 1;
   static constexpr int K = BUFFERS * STEP, Q = K + IN * KEYS, BYTES = Q + IN * KEYS;
-  static_assert(64 * DK * 4 <= BUFFERS * STEP, "room to hand dK over");
+  static_assert(64 * DK * 4 <= STEP, "room to hand beta X over");
 };
 
 // COLS columns of 64 rows of an input on their way to IN tiles of the inner type.
@@ -155,14 +158,9 @@ __device__ __forceinline__ void gradient_part(const DeltaArgs& a, const Chunk& c
   };
 
   for (int d0 = 0; d0 < (WIDE ? p.key_dim : 1); d0 += DK) {
-    // dQ, or Y, over the value heads (their rows are scaled on their way, so that products add to the sums themselves), and beta X
-    v4f all[KT], all_x[BEHIND ? 1 : KT];
-    v4f before = v4f{0, 0, 0, 0};  // Q dQ, or K Y, before this head, row by row
+    v4f all[KT];  // dQ, or dK, over the value heads
 #pragma unroll
     for (int u = 0; u < KT; ++u) all[u] = v4f{0, 0, 0, 0};
-    if constexpr (!BEHIND)
-#pragma unroll
-      for (int u = 0; u < KT; ++u) all_x[u] = v4f{0, 0, 0, 0};
     {
       InputStager<T, DK, LANES> keys;
       const T* from = BEHIND ? head_rows<T>(p.q, p.q_stride, ch.batch, ch.first, key_head) : head_rows<T>(p.k, p.k_stride, ch.batch, ch.first, key_head);
@@ -184,14 +182,20 @@ __device__ __forceinline__ void gradient_part(const DeltaArgs& a, const Chunk& c
         sh.rest[own] = rest;
         sh.beta[own] = beta;
       }
+      // dQ, or Y, of this head alone (rows are scaled on their way, so that products add to it), which the gates' gradients are dots of: a
+      // difference of sums over heads would lose the digits of a small head beside a large one, and all of them beside one that is not finite
+      v4f z[KT];
       v4f f[4], ee[4], x[BEHIND ? 1 : KT], bv = v4f{0, 0, 0, 0}, inner = v4f{0, 0, 0, 0};
+#pragma unroll
+      for (int u = 0; u < KT; ++u) z[u] = v4f{0, 0, 0, 0};
 #pragma unroll
       for (int t = 0; t < 4; ++t) f[t] = ee[t] = v4f{0, 0, 0, 0};
       if constexpr (!BEHIND)
 #pragma unroll
         for (int u = 0; u < KT; ++u) x[u] = v4f{0, 0, 0, 0};
+      char* at = smem;
       for (int v0 = 0; v0 < p.value_dim; v0 += 32) {
-        char* at = smem + (Sh::BUFFERS == 2 ? turn * Sh::STEP : 0);
+        at = smem + (Sh::BUFFERS == 2 ? turn * Sh::STEP : 0);
         if constexpr (Sh::BUFFERS == 1) __syncthreads();
         put(at);
         __syncthreads();
@@ -240,7 +244,7 @@ __device__ __forceinline__ void gradient_part(const DeltaArgs& a, const Chunk& c
           return out;
         };
         const int own = 16 * wave + anew(r);
-        fetch_beside(std::integral_constant<int, 0>{}, all[0]);
+        fetch_beside(std::integral_constant<int, 0>{}, z[0]);
         if constexpr (!BEHIND) {
           const Planes<U> db_w = by_v(Sh::B, two);
           const Planes<U, IN> do_w = rows_in(Sh::O, rows_w, 0);
@@ -251,14 +255,14 @@ __device__ __forceinline__ void gradient_part(const DeltaArgs& a, const Chunk& c
               f[t] = mma_up_to<2>(n_t, do_w, f[t]);
               ee[t] = mma_up_to<REST>(n_t, db_w, ee[t]);
             }
-          fetch_beside(std::integral_constant<int, 1>{}, all[0]);
+          fetch_beside(std::integral_constant<int, 1>{}, z[0]);
           const Planes<U, KEPT> do_s = scaled<U, KEPT>(do_w, p.scale * sh.gamma[own]);
           static_for<KT>([&](auto u) __attribute__((always_inline)) {
             const Planes<U, KEPT> s_u = state(Sh::S, u);
             // (the products of two rests too: without them the gradient of log_decay is a sixth further off, for 46 of 774 us)
-            all[u] = mma_up_to<2>(do_s, s_u, all[u]);
+            z[u] = mma_up_to<2>(do_s, s_u, z[u]);
             x[u] = mma_up_to<2>(db_w, s_u, x[u]);
-            fetch_beside(std::integral_constant<int, 2 + u()>{}, all[u]);
+            fetch_beside(std::integral_constant<int, 2 + u()>{}, z[u]);
           });
           bv = mma_up_to<2>(db_w, rows_in(Sh::V, rows_w, 0), bv);
           // <S, dS'> on the diagonal of S^T dS', 16 channels at a time
@@ -281,12 +285,12 @@ __device__ __forceinline__ void gradient_part(const DeltaArgs& a, const Chunk& c
               f[t] = mma_up_to<2>(rows_in(Sh::O, rows_m, TI::mapped_row(t)), n_w, f[t]);
               ee[t] = mma_up_to<REST>(by_v_mapped(Sh::B, t, two), n_w, ee[t]);
             }
-          fetch_beside(std::integral_constant<int, 1>{}, all[0]);
+          fetch_beside(std::integral_constant<int, 1>{}, z[0]);
           // (what goes into the gradient of log_decay through Z is a small sum of large terms: all that two numbers hold counts)
           const Planes<U, CHAIN> n_s = scaled<U, CHAIN>(n_w, sh.rest[own]);
           static_for<KT>([&](auto u) __attribute__((always_inline)) {
-            all[u] = mma(n_s, state(Sh::D, u), all[u]);
-            fetch_beside(std::integral_constant<int, 2 + u()>{}, all[u]);
+            z[u] = mma(n_s, state(Sh::D, u), z[u]);
+            fetch_beside(std::integral_constant<int, 2 + u()>{}, z[u]);
           });
         }
       }
@@ -339,7 +343,6 @@ __device__ __forceinline__ void gradient_part(const DeltaArgs& a, const Chunk& c
 #pragma unroll
       for (int u = 0; u < KT; ++u) {
         const v4f kv = values(Sh::K, u);
-        v4f z = all[u];
         if constexpr (!BEHIND) {
           const v4f qv = values(Sh::Q, u);
           v4f xu = down * x[u];
@@ -347,33 +350,29 @@ __device__ __forceinline__ void gradient_part(const DeltaArgs& a, const Chunk& c
           for (int b = 0; b < 2; ++b)
             if (b <= wave / 2) {
               const Planes<U, IN> k_b = keys(Sh::K, b, u);
-              z = mma_up_to<2>(fp[b], k_b, z);
+              z[u] = mma_up_to<2>(fp[b], k_b, z[u]);
               xu = mma_up_to<2>(ep[b], k_b, xu);
             }
-          dot += qv * z;
+          dot += qv * z[u];
           dot_x += kv * xu;
-          all_x[u] += beta_of * xu;
+          x[u] = beta_of * xu;
         } else {
-          ends += kv * z;
+          ends += kv * z[u];
 #pragma unroll
           for (int b = 0; b < 2; ++b)
             if (b >= wave / 2) {
-              z = mma_up_to<2>(fp[b], keys(Sh::Q, b, u), z);
-              z = mma_up_to<2>(ep[b], keys(Sh::K, b, u), z);
+              z[u] = mma_up_to<2>(fp[b], keys(Sh::Q, b, u), z[u]);
+              z[u] = mma_up_to<2>(ep[b], keys(Sh::K, b, u), z[u]);
             }
-          dot += kv * z;
+          dot += kv * z[u];
         }
         // (reads of the next columns, all ahead of their products, would push other values out of the registers)
         if constexpr (!BEHIND) {
           points = anew_after(points, dot);
-          cols_k = anew_after(cols_k, z);
+          cols_k = anew_after(cols_k, z[u]);
         }
-        all[u] = z;
+        all[u] += z[u];
       }
-      const v4f now = dot;
-      dot -= before;
-      ends -= before;
-      before = now;
       float* to = BEHIND ? sh.y : sh.q;
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
@@ -401,6 +400,16 @@ __device__ __forceinline__ void gradient_part(const DeltaArgs& a, const Chunk& c
       whole += __shfl_xor(whole, 32);
       if (lane == 0) sh.sum[BEHIND ? 4 + wave : wave] = whole;
       __syncthreads();
+      // beta X for the other part's dK, to the wave and lane that have the same rows and columns, through what was this step's place (nobody
+      // reads it any more, and it is written next behind a barrier more)
+      v4f* hand = reinterpret_cast<v4f*>(at) + wave * 64 + anew(lane);
+      if constexpr (!BEHIND)
+#pragma unroll
+        for (int u = 0; u < KT; ++u) hand[u * 256] = x[u];
+      __syncthreads();
+      if constexpr (BEHIND)
+#pragma unroll
+        for (int u = 0; u < KT; ++u) all[u] += hand[u * 256];
       if (keeper) {
         const int own = anew(lane);
         float* dots = a.dots + block * 192;  // (every place is written and read by one lane)
@@ -428,28 +437,16 @@ __device__ __forceinline__ void gradient_part(const DeltaArgs& a, const Chunk& c
         }
       }
     }
-    // the two shares of dK together
-    __syncthreads();
-    float* sh_k = reinterpret_cast<float*>(smem);
     const int r2 = anew(r), row2 = 16 * wave + 4 * anew(q);
-    if constexpr (BEHIND)
+    T* to = static_cast<T*>(BEHIND ? p.d_k : p.d_q);
 #pragma unroll
-      for (int u = 0; u < KT; ++u)
+    for (int e = 0; e < 4; ++e)
+      if (row2 + e < ch.length) {
+        const int64_t at = ((ch.batch * p.time + ch.first + row2 + e) * p.key_heads + key_head) * int64_t(p.key_dim) + d0;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) sh_k[(row2 + e) * DK + 16 * u + r2] = all[u][e];
-    __syncthreads();
-    if constexpr (!BEHIND)
-#pragma unroll
-      for (int e = 0; e < 4; ++e)
-        if (row2 + e < ch.length) {
-          const int64_t at = ((ch.batch * p.time + ch.first + row2 + e) * p.key_heads + key_head) * int64_t(p.key_dim) + d0;
-#pragma unroll
-          for (int u = 0; u < KT; ++u)
-            if (d0 + 16 * u + r2 < p.key_dim) {
-              static_cast<T*>(p.d_q)[at + 16 * u + r2] = T(all[u][e]);
-              static_cast<T*>(p.d_k)[at + 16 * u + r2] = T(all_x[u][e] + sh_k[(row2 + e) * DK + 16 * u + r2]);
-            }
-        }
+        for (int u = 0; u < KT; ++u)
+          if (d0 + 16 * u + r2 < p.key_dim) to[at + 16 * u + r2] = T(all[u][e]);
+      }
   }
 }
 

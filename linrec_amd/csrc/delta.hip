@@ -23,8 +23,8 @@ size_t aligned(size_t n) { return (n + 255) & ~size_t(255); }
 // two, the first with the columns of the unit matrix as well, and what goes from segment to segment: about half a chunk's time for
 // each, and two chunks' for two launches more.  What counts is n at which a pass's rounds are about to grow, and the most that leaves four
 // chunks to a segment (shorter ones gain nothing: 1 x 2048 with 8 heads of 64 x 64, forward and backward, 172 us with 4, 199 with 2, 214 with 8).
-// 1 x 8192 with 128 x 128 bf16, forward and backward, cut and not: 16 heads (8 segments) 906 and 1696 us, 32 heads (4) 1460 and 1988, 48 heads (2) 2441
-// and 2276, which is not cut.
+// 1 x 8192 with 128 x 128 bf16, forward and backward, cut and not: 16 heads (8 segments) 896 and 1723 us, 32 heads (4) 1528 and 1987; 48 heads,
+// where two segments took longer (2441 and 2276), are not cut.
 int segment_of(const DeltaArgs& a, int width) {
   constexpr int64_t CUS = 256, LEAST = 4;
   const linrec_delta_t& p = a.p;
@@ -57,29 +57,26 @@ size_t lay_out(const linrec_delta_t& p, bool bwd, char* base, DeltaArgs* a) {
   a->parts = !a->segment ? p.sequences : p.cu_seqlens ? a->slots / a->segment + p.sequences : p.batch * cdiv(cdiv(p.time, DELTA_CHUNK), a->segment);
   a->pairs = a->parts * p.heads;
   const size_t blocks = size_t(a->slots) * size_t(p.heads);
-  constexpr size_t value = 4;  // bytes of a value of inner type in all its planes
   size_t at = 0;
   auto part = [&](size_t bytes_of_block) {
     char* to = base + at;
     at += aligned(blocks * bytes_of_block);
     return to;
   };
-  a->square = 4096 * value;
-  a->rows = int64_t(a->columns) * 64 * value;
-  const int three = p.dtype != LINREC_DTYPE_F32 ? 6 : value, kept = width == 64 ? three : value;  // (chain_planes, kept_planes)
-  a->rows_n = int64_t(a->columns) * 64 * three;
-  a->state = int64_t(a->columns) * width * kept;
-  a->m = part(a->square);
-  a->c = part(a->square);
-  a->gates = reinterpret_cast<float*>(part(192 * 4));
+  a->rows = int64_t(a->columns) * 64;
+  a->state = int64_t(a->columns) * width;
+  auto floats = [&](size_t of_block) { return reinterpret_cast<float*>(part(of_block * 4)); };
+  a->m = floats(4096);
+  a->c = floats(4096);
+  a->gates = floats(192);
   if (bwd) {
     a->sums = reinterpret_cast<double*>(part(64 * 8));
-    a->m_t = part(a->square);
-    a->s = part(a->state);
-    a->d_s = part(a->state);
-    a->n = part(a->rows_n);
-    a->d_b = part(a->rows);
-    a->dots = reinterpret_cast<float*>(part(192 * 4));
+    a->m_t = floats(4096);
+    a->s = floats(a->state);
+    a->d_s = floats(a->state);
+    a->n = floats(a->rows);
+    a->d_b = floats(a->rows);
+    a->dots = floats(192);
   }
   if (a->segment) {
     a->carry = reinterpret_cast<float*>(base + at);

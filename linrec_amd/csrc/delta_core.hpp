@@ -17,12 +17,12 @@
 // of the time axis and keeps its key_dim x 16 part of S in accumulators; what it multiplies them with is the same for all waves and
 // comes through LDS.
 //
-// Precision.  States, sums and accumulators are fp32.  An operand of a matrix instruction that is not an input is split into
-// bf16 (or, beside fp16 inputs, fp16) numbers, its rounding, the rounding of the rest and so on: two bf16 carry 16 to 17 bits, three 24, two
-// fp16 22.  In the chain of products that makes a state from the one before, what meets an input is three bf16 or two fp16, and what meets M
-// three bf16; M, C and dB are two, N three, S and dS' as kept for the gradients three up to 64 key channels and two from there on (kept_planes).  So a state is
-// 1e-6 off, the gradient of beta 4e-6 and that of log_decay 3e-6 up to 64 key channels, 4e-6 from there on (with two of N 5e-6, and 1.1e-5 where
-// its sum cancels; with two bf16 in the chain and without the products of rests 1e-5 to 1.6e-5, with one bf16 2e-3).  fp32 inputs take the fp32 instructions.
+// Precision.  States, sums and accumulators are fp32, and so is all that one kernel leaves to another.  An operand of a matrix instruction
+// that is not an input is split into bf16 (or, beside fp16 inputs, fp16) numbers, its rounding, the rounding of the rest and so on: three bf16
+// carry 24 bits, two fp16 22, two bf16 16 to 17.  Whatever goes into a result in fp32 (states and the gradients of the gates and of h0) is three bf16
+// or two fp16: these are as near as sums in fp32 are, 2e-7 to 7e-7 (with M, C, dB and, above 64 key channels, the kept S and dS' in two: states
+// 2e-6, the gradient of beta 4e-6, that of log_decay 5e-6).  C N in the forward, which O alone sees, is the product of two and two, 2^-16
+// beside the 2^-9 of O's own rounding.  fp32 inputs take the fp32 instructions.
 #pragma once
 #include <hip/hip_runtime.h>
 #include <stdint.h>
@@ -37,7 +37,7 @@ namespace linrec {
 constexpr int DELTA_CHUNK = 64;
 constexpr float DELTA_LEAST_LOG = -1e4f;  // e^-10000 is zero, and sums of 64 of them keep their digits in fp64
 
-// Storage of what is computed inside: T for fp32, two bf16 for 16-bit inputs.
+// Type of operands that are computed: T for fp32, bf16 numbers for 16-bit inputs.
 template <typename T>
 using Inner = std::conditional_t<sizeof(T) == 4, float, __bf16>;
 template <typename U>
@@ -148,12 +148,6 @@ __device__ __forceinline__ Planes<U, N> split(const v4f& lo, const v4f& hi) {
 template <typename U>
 constexpr int chain_planes() {
   return std::is_same_v<U, __bf16> ? 3 : planes_of<U>();
-}
-// Planes of S and dS' as they are kept for the gradients.  With up to 64 key channels the gradients of the gates are sums of so few
-// terms that the rounding of two shows: 1e-5 of them for 16 to 32 key channels, 3e-6 with three, which LDS has room for there.
-template <typename U, int DK>
-constexpr int kept_planes() {
-  return DK == 64 ? chain_planes<U>() : planes_of<U>();
 }
 // The third of them, where two are there.
 __device__ __forceinline__ Planes<__bf16, 1> third_plane(const v4f& lo, const v4f& hi, const Planes<__bf16>& f) {
@@ -363,42 +357,6 @@ struct Stager {
 #pragma unroll
     for (int n = 0; n < N; ++n) v[n] = zero();
   }
-  // dense rows of scratch
-  __device__ __forceinline__ void fetch_dense(const T* from, int lane) {
-#pragma unroll
-    for (int n = 0; n < N; ++n)
-      if (ROWS % STEP == 0 || n * STEP + lane / L::UNITS < ROWS) v[n] = reinterpret_cast<const V*>(from)[n * LANES + lane];
-  }
-  // pieces of store_rows: PIECES of a group of 16 rows from FROM_PIECE on, of EVERY that it has
-  template <int EVERY = L::UNITS / 4>
-  __device__ __forceinline__ void fetch_pieces(const T* from, int from_piece, int lane) {
-    constexpr int GROUP = L::UNITS / 4 * 64;  // units of a group here
-    static_assert(LANES % 64 == 0 && ROWS % 16 == 0, "");
-#pragma unroll
-    for (int n = 0; n < N; ++n) {
-      const int i = n * LANES + lane, g = i / GROUP;
-      if (ROWS % STEP == 0 || i < ROWS * L::UNITS) v[n] = reinterpret_cast<const V*>(from)[(g * EVERY + from_piece) * 64 + i - g * GROUP];
-    }
-  }
-  __device__ __forceinline__ void put_pieces(char* tile, int lane) const {
-    constexpr int GROUP = L::UNITS / 4 * 64;
-#pragma unroll
-    for (int n = 0; n < N; ++n) {
-      const int i = n * LANES + lane, g = i / GROUP, k = (i - g * GROUP) >> 6, r = i & 15, q = (i >> 4) & 3;
-      if (ROWS % STEP == 0 || i < ROWS * L::UNITS)
-        *reinterpret_cast<V*>(tile + L::at(16 * g + r, L::HALF ? 4 * k + q : 8 * (k >> 1) + 2 * q + (k & 1))) = v[n];
-    }
-  }
-  // a triangle, without its empty quarter
-  template <bool UPPER>
-  __device__ __forceinline__ void put_triangle(char* tile, int lane) const {
-    const int row0 = lane / L::UNITS, unit = lane % L::UNITS;
-#pragma unroll
-    for (int n = 0; n < N; ++n) {
-      const int row = n * STEP + row0;
-      if (UPPER ? row < ROWS / 2 || unit >= L::UNITS / 2 : row >= ROWS / 2 || unit < L::UNITS / 2) *reinterpret_cast<V*>(tile + L::at(row, unit)) = v[n];
-    }
-  }
   __device__ __forceinline__ void put(char* tile, int lane) const {
 #pragma unroll
     for (int n = 0; n < N; ++n)
@@ -407,24 +365,98 @@ struct Stager {
   }
 };
 
-// Operands of 16 rows, a lane's as it has them: pieces of 1 KB that a wave stores and loads whole (rows of their own would be stored 64
-// bytes at a time).  `to`: of plane k at to + k * plane; b: which 32 columns.
-template <typename U, int N>
-__device__ __forceinline__ void store_rows(U* to, int64_t plane, int b, int lane, const Planes<U, N>& f) {
-#pragma unroll
-  for (int k = 0; k < N; ++k) {
+// Values of scratch, in fp32, on their way to a tile of ROWS rows of COLS columns in PLANES planes of U, eight of a row to a lane at a time.
+template <typename U, int COLS, int LANES, int ROWS, int PLANES = chain_planes<U>()>
+struct SplitStager {
+  using L = Tile<U, COLS>;
+  static constexpr int EIGHTS = COLS / 8, ALL = ROWS * EIGHTS, N = (ALL + LANES - 1) / LANES, BYTES = ROWS * L::ROW;  // (of a plane)
+  v4f v[N][2];
+
+  static __device__ __forceinline__ bool has(int n, int lane) { return (n + 1) * LANES <= ALL || n * LANES + lane < ALL; }
+  __device__ __forceinline__ void put_at(char* tile, int n, int row, int eighth) const {
     if constexpr (sizeof(U) == 2) {
-      *reinterpret_cast<Frag<U>*>(to + k * plane + b * 512 + lane * 8) = f.p[k];
+      const Planes<U, PLANES> f = split<U, PLANES>(v[n][0], v[n][1]);
+#pragma unroll
+      for (int k = 0; k < PLANES; ++k) *reinterpret_cast<Frag<U>*>(tile + k * BYTES + L::at(row, eighth)) = f.p[k];
     } else {
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        v4f x;
-#pragma unroll
-        for (int e = 0; e < 4; ++e) x[e] = f.p[k][4 * h + e];
-        *reinterpret_cast<v4f*>(to + k * plane + (2 * b + h) * 256 + lane * 4) = x;
-      }
+      for (int h = 0; h < 2; ++h) *reinterpret_cast<v4f*>(tile + L::at(row, 2 * eighth + h)) = v[n][h];
     }
   }
+
+  // pieces of store_rows: those of a group of 16 rows from `from_piece` on, of EVERY that it has; load n of N
+  template <int EVERY>
+  __device__ __forceinline__ void fetch_pieces(int n, const float* from, int from_piece, int lane) {
+    const int i = n * LANES + lane, g = i / (16 * EIGHTS), k = (i - g * (16 * EIGHTS)) >> 6;
+    if (has(n, lane))
+#pragma unroll
+      for (int h = 0; h < 2; ++h) v[n][h] = reinterpret_cast<const v4f*>(from)[(g * EVERY + from_piece + 2 * k + h) * 64 + (i & 63)];
+  }
+  __device__ __forceinline__ void put_pieces(char* tile, int lane) const {
+#pragma unroll
+    for (int n = 0; n < N; ++n) {
+      const int i = n * LANES + lane, g = i / (16 * EIGHTS), k = (i - g * (16 * EIGHTS)) >> 6;
+      if (has(n, lane)) put_at(tile, n, 16 * g + (i & 15), 4 * k + ((i >> 4) & 3));
+    }
+  }
+};
+
+// A triangle of a dense 64 x 64 square in LDS without its empty quarter: 64 rows of the 32 columns that are all full, the first ones of a lower and the
+// last ones of an upper triangle, and behind them the other 32 columns' rows.
+constexpr int TRIANGLE_ROWS = 96;
+template <typename U, bool UPPER, int LANES, int PLANES>
+struct TriangleStager : SplitStager<U, 32, LANES, TRIANGLE_ROWS, PLANES> {
+  using S = SplitStager<U, 32, LANES, TRIANGLE_ROWS, PLANES>;
+  static_assert(LANES == 256 || LANES == 128, "a load is of one part");
+  __device__ __forceinline__ void fetch(const float* from, int lane) {
+#pragma unroll
+    for (int n = 0; n < S::N; ++n) {
+      const int row = n * LANES / 4;  // (of the first lane)
+      const float* at = from + (row < 64 ? row * 64 + (UPPER ? 32 : 0) : (UPPER ? row - 64 : row - 32) * 64 + (UPPER ? 0 : 32)) + lane * 8 + (lane >> 2) * 32;
+      if (S::has(n, lane))
+#pragma unroll
+        for (int h = 0; h < 2; ++h) this->v[n][h] = *reinterpret_cast<const v4f*>(at + 4 * h);
+    }
+  }
+  __device__ __forceinline__ void put(char* tile, int lane) const {
+#pragma unroll
+    for (int n = 0; n < S::N; ++n)
+      if (S::has(n, lane)) S::put_at(tile, n, n * LANES / 4 + (lane >> 2), lane & 3);
+  }
+};
+template <typename U, int PLANES>
+constexpr int triangle_bytes() {
+  return TRIANGLE_ROWS * 32 * int(sizeof(U)) * PLANES;
+}
+// to += triangle . by, four tiles of 16 rows (row_of_tile); products of planes whose numbers add up to more than MOST are left out.
+template <bool UPPER, int MOST, int PLANES, typename U, int NB>
+__device__ __forceinline__ void mma_triangle(const char* tile, int view, const Planes<U, NB> (&by)[2], v4f (&to)[4]) {
+  using L = Tile<U, 32>;
+#pragma unroll
+  for (int b = 0; b < 2; ++b) {
+    const bool whole = b == (UPPER ? 1 : 0);  // these 32 columns have all rows
+#pragma unroll
+    for (int k = PLANES - 1; k >= 0; --k) {
+      Frag<U> f[4];
+#pragma unroll
+      for (int t = 0; t < 4; ++t)
+        if (whole || (UPPER ? t < 2 : t >= 2))
+          f[t] = L::frag(tile + k * (TRIANGLE_ROWS * L::ROW), view, L::mapped_row(t) + (whole ? 0 : UPPER ? 64 : 32), 0);
+#pragma unroll
+      for (int j = NB - 1; j >= 0; --j)
+        if (k + j <= MOST)
+#pragma unroll
+          for (int t = 0; t < 4; ++t)
+            if (whole || (UPPER ? t < 2 : t >= 2)) to[t] = mma(f[t], by[b].p[j], to[t]);
+    }
+  }
+}
+
+// Results that a wave has of 16 columns and 32 rows (columns of scratch), a lane's as it has them: pieces of 1 KB that a wave stores and loads whole (rows of
+// their own would be stored 64 bytes at a time).  b: which 32.
+__device__ __forceinline__ void store_rows(float* to, int b, int lane, const v4f& lo, const v4f& hi) {
+  *reinterpret_cast<v4f*>(to + b * 512 + lane * 4) = lo;
+  *reinterpret_cast<v4f*>(to + b * 512 + 256 + lane * 4) = hi;
 }
 
 // ---- chunks and scratch ----------------------------------------------------------------------------------------------------------
@@ -439,17 +471,17 @@ struct DeltaArgs {
   int64_t pairs; // parts x heads
   int64_t parts; // sequences, or segments of them
   int segment;   // chunks of a segment, 0: sequences are not cut
-  // scratch, for every (slot, head): m[planes][64][64] and so on.  Bytes from one to the next:
-  int64_t square, state, rows, rows_n;
-  char* m;
-  char* m_t;
-  char* c;       // C scale, transposed in the backward
+  // scratch, for every (slot, head); values from one to the next of d_b and n, and of s and d_s:
+  int64_t rows, state;
+  float* m;      // [64][64] as m_t and c, whose empty quarters are not written
+  float* m_t;    // transposed
+  float* c;      // C scale, transposed in the backward
   float* gates;  // [3][64]: e^G, e^{G_63 - G}, beta
   double* sums;  // [64]: G
-  char* s;       // [kept_planes][columns][DK] in pieces of 16 columns (store_rows), the state before the chunk
-  char* d_s;     // the same of dS' behind it
-  char* n;       // [chain_planes][columns][64] in such pieces
-  char* d_b;
+  float* s;      // [columns][DK] in pieces of 16 columns (store_rows), the state before the chunk
+  float* d_s;    // the same of dS' behind it
+  float* n;      // [columns][64] in such pieces
+  float* d_b;
   float* dots;   // [192], sums of the gates' gradients where key_dim comes in turns
   // for every (part, head), where sequences are cut (delta_segments.hpp)
   float* carry;  // [columns + DK][DK]: what a segment makes of nothing, and of the unit matrix

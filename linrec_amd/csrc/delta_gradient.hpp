@@ -11,10 +11,11 @@
 // A workgroup has a (chunk, key head) and walks over the value heads that share it, so that nothing is added by atomics.  Value
 // channels come 32 at a time through LDS, the next ones on their way in registers meanwhile.  Its waves have two parts, four waves
 // of 16 rows each: dQ and X, which multiply S, and Y, which multiplies dS'.  One wave for all three would hold more than its share of the
-// registers (what then goes through scratch costs more than the products: 2.4 ms for 8 x 4096 x 16 heads of 128 x 128 bf16), three
-// parts read S from LDS twice (0.79 ms); two 0.69 ms, for 2.3 GB of states, operands and results (0.45 at the rate of a
+// registers (with two numbers an operand 2.4 ms for 8 x 4096, 16 heads of 128 x 128 bf16, what went through scratch cost more than the products), three
+// parts read S from LDS twice (0.79 ms); two 0.70 ms.  Now all that is not an input is three numbers (delta_core.hpp), with which two steps
+// no longer fit into LDS above 64 key channels: 0.83 to 0.89 ms, for 2.1 GB of states, operands and results (0.42 at the rate of a
 // copy).  beta X goes from the one part to the other through LDS, head by head, and is added to Y there, so each part keeps one sum over
-// the heads and what its head alone has (with differences of running sums for the latter, which took as long, 695 us, a small head lost its
+// the heads and what its head alone has (with differences of running sums for the latter, which took as long, a small head lost its
 // digits).  The 64 x 64 products F, F^T, E, E^T are computed as they are needed as operands: what a lane gets of a product is its part of an
 // operand over the product's rows.
 #pragma once
@@ -28,11 +29,11 @@ constexpr int GRADIENT_LANES = 512, GRADIENT_PART = 256;
 template <typename T, int DK>
 struct GradientShared {
   using U = Inner<T>;
-  static constexpr int P = planes_of<U>(), KEPT = kept_planes<U, DK>(), CHAIN = chain_planes<U>(), IN = input_planes<T>();
+  static constexpr int CHAIN = chain_planes<U>(), IN = input_planes<T>();
   static constexpr int IN_V = 64 * 32 * int(sizeof(U)), BY_V = 32 * 64 * int(sizeof(U)), STATE = 32 * DK * int(sizeof(U)),
                        KEYS = Tile<U, DK>::BYTES;
   // one step's values, then both inputs of key channels
-  static constexpr int O = 0, V = O + IN * IN_V, B = V + IN * IN_V, N = B + P * BY_V, S = N + CHAIN * BY_V, D = S + KEPT * STATE, STEP = D + KEPT * STATE;
+  static constexpr int O = 0, V = O + IN * IN_V, B = V + IN * IN_V, N = B + CHAIN * BY_V, S = N + CHAIN * BY_V, D = S + CHAIN * STATE, STEP = D + CHAIN * STATE;
   static constexpr int BUFFERS = 2 * STEP + 2 * IN * KEYS + 4096 <= 160 * 1024 ? 2 : 1;
   static constexpr int K = BUFFERS * STEP, Q = K + IN * KEYS, BYTES = Q + IN * KEYS;
   static_assert(64 * DK * 4 <= STEP, "room to hand beta X over");
@@ -89,7 +90,7 @@ __device__ __forceinline__ void gradient_part(const DeltaArgs& a, const Chunk& c
   using TI = Tile<U, 32>;  // dO, V
   using TB = Tile<U, 64>;  // dB, N: rows are channels
   using TK = Tile<U, DK>;  // K, Q; S, dS': rows are channels
-  constexpr int P = Sh::P, KEPT = Sh::KEPT, CHAIN = Sh::CHAIN, IN = Sh::IN, KT = DK / 16, LANES = GRADIENT_PART;
+  constexpr int CHAIN = Sh::CHAIN, IN = Sh::IN, KT = DK / 16, LANES = GRADIENT_PART;
   constexpr int64_t ROW = WIDE ? 2 * DK : DK;  // of the kept states
   const linrec_delta_t& p = a.p;
   const int lane = threadIdx.x & 63, r = lane & 15, q = lane >> 4, by0 = threadIdx.x & (LANES - 1);
@@ -101,14 +102,15 @@ __device__ __forceinline__ void gradient_part(const DeltaArgs& a, const Chunk& c
 
   // what a step needs on its way: the rows of dO and V with dB and N, or S and dS'
   InputStager<T, 32, LANES> so, sv;
-  Stager<U, 64, LANES, 32> sb[P], sn[CHAIN];
-  Stager<U, DK, LANES, 32> ss[KEPT], sd[KEPT];
+  SplitStager<U, 64, LANES, 32> sb, sn;
+  SplitStager<U, DK, LANES, 32> ss, sd;
   // one wave has what belongs to the positions, a lane for each
   const bool keeper = BEHIND && wave == 0;
   double sum = 0.0;
   float gamma = 0.0f, rest = 0.0f, beta = 0.0f;
-  // (loads are issued one part after the other between products: all at once they wait for each other, 2600 of a step's 8000 cycles)
-  constexpr int PARTS = BEHIND ? 2 * KEPT : 2 + P + CHAIN;
+  // (loads are issued one part after the other between products; all at once at the step's start 879 us instead of 870)
+  constexpr int LOADS = decltype(ss)::N, PARTS = BEHIND ? 2 * LOADS : 4;
+  static_assert(decltype(sb)::N == 1, "");
   auto fetch_gates = [&](int head) __attribute__((always_inline)) {
     if (keeper) {
       const int64_t block = slot * p.heads + head;
@@ -126,17 +128,14 @@ __device__ __forceinline__ void gradient_part(const DeltaArgs& a, const Chunk& c
         so.fetch(head_rows<T>(p.d_o, p.d_o_stride, ch.batch, ch.first, head) + v0, p.d_o_stride[1], ch.length, p.value_dim - v0, by);
       } else if constexpr (part() == 1) {
         sv.fetch(head_rows<T>(p.v, p.v_stride, ch.batch, ch.first, head) + v0, p.v_stride[1], ch.length, p.value_dim - v0, by);
-      } else if constexpr (part() < 2 + P) {
-        constexpr int k = part() - 2;
-        sb[k].fetch_pieces(reinterpret_cast<const U*>(a.d_b + block * a.rows) + (int64_t(k) * a.columns + v0) * 64, 0, by);
+      } else if constexpr (part() == 2) {
+        sb.template fetch_pieces<4>(0, a.d_b + block * a.rows + v0 * 64, 0, by);
       } else {
-        constexpr int k = part() - 2 - P;
-        sn[k].fetch_pieces(reinterpret_cast<const U*>(a.n + block * a.rows_n) + (int64_t(k) * a.columns + v0) * 64, 0, by);
+        sn.template fetch_pieces<4>(0, a.n + block * a.rows + v0 * 64, 0, by);
       }
     } else {
-      constexpr int k = part() % KEPT, EVERY = int(ROW * int64_t(sizeof(U)) / 64);
-      const U* from = reinterpret_cast<const U*>((part() < KEPT ? a.s : a.d_s) + block * a.state) + (int64_t(k) * a.columns + v0) * ROW;
-      (part() < KEPT ? ss : sd)[k].template fetch_pieces<EVERY>(from, WIDE ? d0 * int(sizeof(U)) / 64 : 0, by);
+      const float* from = (part() < LOADS ? a.s : a.d_s) + block * a.state + v0 * ROW;
+      (part() < LOADS ? ss : sd).template fetch_pieces<int(ROW / 16)>(part() % LOADS, from, WIDE ? d0 / 16 : 0, by);
     }
   };
   auto put = [&](char* to) __attribute__((always_inline)) {
@@ -144,16 +143,11 @@ __device__ __forceinline__ void gradient_part(const DeltaArgs& a, const Chunk& c
     if constexpr (!BEHIND) {
       so.put(to + Sh::O, by);
       sv.put(to + Sh::V, by);
-    }
-#pragma unroll
-    for (int k = 0; k < (BEHIND ? KEPT : CHAIN); ++k) {
-      if constexpr (!BEHIND) {
-        if (k < P) sb[k].put_pieces(to + Sh::B + k * Sh::BY_V, by);
-        sn[k].put_pieces(to + Sh::N + k * Sh::BY_V, by);
-      } else {
-        ss[k].put_pieces(to + Sh::S + k * Sh::STATE, by);
-        sd[k].put_pieces(to + Sh::D + k * Sh::STATE, by);
-      }
+      sb.put_pieces(to + Sh::B, by);
+      sn.put_pieces(to + Sh::N, by);
+    } else {
+      ss.put_pieces(to + Sh::S, by);
+      sd.put_pieces(to + Sh::D, by);
     }
   };
 
@@ -205,7 +199,6 @@ __device__ __forceinline__ void gradient_part(const DeltaArgs& a, const Chunk& c
         if (!same && h + 1 < a.shared) fetch_gates(next);
         const bool more = same || h + 1 < a.shared;
         // the parts of a sixth of the step, not before a product is there: at its start, behind F and E, and with the first four column tiles
-        // (with all eight tiles, and none before, 684 us instead of 666)
         auto fetch_beside = [&](auto sixth, v4f& after) __attribute__((always_inline)) {
           if (more) {
             static_for<PARTS>([&](auto part) __attribute__((always_inline)) {
@@ -215,51 +208,47 @@ __device__ __forceinline__ void gradient_part(const DeltaArgs& a, const Chunk& c
         };
         const int rows_w = anew(rows_w0), rows_m = anew(rows_m0), cols_w = anew(cols_w0), cols_m = anew(cols_m0), cols_k = anew(cols_k0),
                   rows_v = anew(rows_v0);
-        // (dB.N is a sum of large terms of both signs where key channels are few: the products of rests count there)
-        constexpr int REST = KEPT == 3 ? 2 : 1;
-        constexpr std::integral_constant<int, P> two{};
-        constexpr std::integral_constant<int, CHAIN> three{};
         auto rows_in = [&](int part, int view, int row) __attribute__((always_inline)) {
           Planes<U, IN> out;
 #pragma unroll
           for (int k = 0; k < IN; ++k) out.p[k] = TI::frag(at + part + k * Sh::IN_V, view, row, 0);
           return out;
         };
-        auto by_v = [&](int part, auto planes) __attribute__((always_inline)) {  // this wave's rows
-          Planes<U, planes()> out;
+        auto by_v = [&](int part) __attribute__((always_inline)) {  // this wave's rows
+          Planes<U, CHAIN> out;
 #pragma unroll
-          for (int k = 0; k < planes(); ++k) out.p[k] = TB::template column_frag<false>(at + part + k * Sh::BY_V, cols_w, 0, 0);
+          for (int k = 0; k < CHAIN; ++k) out.p[k] = TB::template column_frag<false>(at + part + k * Sh::BY_V, cols_w, 0, 0);
           return out;
         };
-        auto by_v_mapped = [&](int part, int t, auto planes) __attribute__((always_inline)) {
-          Planes<U, planes()> out;
+        auto by_v_mapped = [&](int part, int t) __attribute__((always_inline)) {
+          Planes<U, CHAIN> out;
 #pragma unroll
-          for (int k = 0; k < planes(); ++k) out.p[k] = TB::template column_frag<true>(at + part + k * Sh::BY_V, cols_m, 0, t);
+          for (int k = 0; k < CHAIN; ++k) out.p[k] = TB::template column_frag<true>(at + part + k * Sh::BY_V, cols_m, 0, t);
           return out;
         };
         auto state = [&](int part, int u) __attribute__((always_inline)) {
-          Planes<U, KEPT> out;
+          Planes<U, CHAIN> out;
 #pragma unroll
-          for (int k = 0; k < KEPT; ++k) out.p[k] = TK::template column_frag<false>(at + part + k * Sh::STATE, cols_k, 0, u);
+          for (int k = 0; k < CHAIN; ++k) out.p[k] = TK::template column_frag<false>(at + part + k * Sh::STATE, cols_k, 0, u);
           return out;
         };
         const int own = 16 * wave + anew(r);
         fetch_beside(std::integral_constant<int, 0>{}, z[0]);
         if constexpr (!BEHIND) {
-          const Planes<U> db_w = by_v(Sh::B, two);
+          const Planes<U, CHAIN> db_w = by_v(Sh::B);
           const Planes<U, IN> do_w = rows_in(Sh::O, rows_w, 0);
 #pragma unroll
           for (int t = 0; t < 4; ++t)
             if (t / 2 <= wave / 2) {  // rows j of F^T and E^T up to this wave's columns i
-              const Planes<U, CHAIN> n_t = by_v_mapped(Sh::N, t, three);
+              const Planes<U, CHAIN> n_t = by_v_mapped(Sh::N, t);
               f[t] = mma_up_to<2>(n_t, do_w, f[t]);
-              ee[t] = mma_up_to<REST>(n_t, db_w, ee[t]);
+              ee[t] = mma_up_to<2>(n_t, db_w, ee[t]);
             }
           fetch_beside(std::integral_constant<int, 1>{}, z[0]);
-          const Planes<U, KEPT> do_s = scaled<U, KEPT>(do_w, p.scale * sh.gamma[own]);
+          const Planes<U, CHAIN> do_s = scaled<U, CHAIN>(do_w, p.scale * sh.gamma[own]);
           static_for<KT>([&](auto u) __attribute__((always_inline)) {
-            const Planes<U, KEPT> s_u = state(Sh::S, u);
-            // (the products of two rests too: without them the gradient of log_decay is a sixth further off, for 46 of 774 us)
+            const Planes<U, CHAIN> s_u = state(Sh::S, u);
+            // (the products of two rests too: without them the gradients of the gates are 1.2e-6 to 4e-6 off instead of 2e-7 to 7e-7, for 50 of 870 us)
             z[u] = mma_up_to<2>(do_s, s_u, z[u]);
             x[u] = mma_up_to<2>(db_w, s_u, x[u]);
             fetch_beside(std::integral_constant<int, 2 + u()>{}, z[u]);
@@ -269,24 +258,23 @@ __device__ __forceinline__ void gradient_part(const DeltaArgs& a, const Chunk& c
 #pragma unroll
           for (int b = 0; b < DK / 32; ++b)
             if ((b & 1) == wave >> 1) {
-              Planes<U, KEPT> s_v, d_v;
+              Planes<U, CHAIN> s_v, d_v;
 #pragma unroll
-              for (int k = 0; k < KEPT; ++k) {
+              for (int k = 0; k < CHAIN; ++k) {
                 s_v.p[k] = TK::frag(at + Sh::S + k * Sh::STATE, rows_v, 0, b);
                 d_v.p[k] = TK::frag(at + Sh::D + k * Sh::STATE, rows_v, 0, b);
               }
               inner = mma_up_to<2>(s_v, d_v, inner);
             }
         } else {
-          const Planes<U, CHAIN> n_w = by_v(Sh::N, three);
+          const Planes<U, CHAIN> n_w = by_v(Sh::N);
 #pragma unroll
           for (int t = 0; t < 4; ++t)
             if (t / 2 >= wave / 2) {
               f[t] = mma_up_to<2>(rows_in(Sh::O, rows_m, TI::mapped_row(t)), n_w, f[t]);
-              ee[t] = mma_up_to<REST>(by_v_mapped(Sh::B, t, two), n_w, ee[t]);
+              ee[t] = mma_up_to<2>(by_v_mapped(Sh::B, t), n_w, ee[t]);
             }
           fetch_beside(std::integral_constant<int, 1>{}, z[0]);
-          // (what goes into the gradient of log_decay through Z is a small sum of large terms: all that two numbers hold counts)
           const Planes<U, CHAIN> n_s = scaled<U, CHAIN>(n_w, sh.rest[own]);
           static_for<KT>([&](auto u) __attribute__((always_inline)) {
             z[u] = mma(n_s, state(Sh::D, u), z[u]);
@@ -298,7 +286,7 @@ __device__ __forceinline__ void gradient_part(const DeltaArgs& a, const Chunk& c
       const int r1 = anew(r), row1 = 16 * wave + 4 * anew(q);
       // the masks and decays; rows of results to operands
       Planes<U, CHAIN> fp[2];
-      Planes<U, KEPT> ep[2];
+      Planes<U, CHAIN> ep[2];
       {
         // (all reads ahead of what they are compared for: a read that waits in a branch of its own costs its latency, 16 times over)
         typedef double v4d __attribute__((ext_vector_type(4)));
@@ -321,7 +309,7 @@ __device__ __forceinline__ void gradient_part(const DeltaArgs& a, const Chunk& c
 #pragma unroll
         for (int b = 0; b < 2; ++b) {
           fp[b] = split<U, CHAIN>(f[2 * b], f[2 * b + 1]);
-          ep[b] = split<U, KEPT>(ee[2 * b], ee[2 * b + 1]);
+          ep[b] = split<U, CHAIN>(ee[2 * b], ee[2 * b + 1]);
         }
       }
       auto keys = [&](int part, int b, int u) __attribute__((always_inline)) {

@@ -5,7 +5,7 @@
 // then of 32 and of 64 by M21 = -M22 A21 M11 with the fp32 matrix instruction.  (Substitution over all 64 rows would be 64 dependent
 // steps; powers of A, whose binomials cancel, lose all digits where keys are alike.)
 //
-// 8 x 4096, 16 heads of 128 x 128 bf16: 140 us forward and 160 backward for 0.40 and 0.54 GB (79 and 105 us at the rate of a copy); ten meetings
+// 8 x 4096, 16 heads of 128 x 128 bf16: 130 us forward and 145 backward for 0.34 and 0.44 GB (66 and 86 us at the rate of a copy); ten meetings
 // of a workgroup, three of which fit into a CU.
 #pragma once
 #include "delta_core.hpp"
@@ -14,19 +14,18 @@ namespace linrec {
 
 constexpr int PREPARE_STRIDE = 68;  // floats of a row in LDS
 
-// Rows of 64 values in LDS to planes of a [64][64] block; TRANSPOSED: columns.
-template <typename U, bool TRANSPOSED>
-__device__ __forceinline__ void store_square(char* to, const float* from) {
+// Rows of 64 values in LDS to a [64][64] block, without the quarter above the diagonal; TRANSPOSED: columns, without that below.
+template <bool TRANSPOSED>
+__device__ __forceinline__ void store_triangle(float* to, const float* from) {
   constexpr int S = PREPARE_STRIDE;
 #pragma unroll
-  for (int n = 0; n < 2; ++n) {
-    const int i = n * 256 + int(threadIdx.x), row = i >> 3, c = (i & 7) * 8;
-    v4f x[2];
+  for (int n = 0; n < 4; ++n) {
+    const int i = n * 256 + int(threadIdx.x), row = i >> 4, c = (i & 15) * 4;
+    if (TRANSPOSED ? row >= 32 && c < 32 : row < 32 && c >= 32) continue;
+    v4f x;
 #pragma unroll
-    for (int e = 0; e < 8; ++e) x[e >> 2][e & 3] = TRANSPOSED ? from[(c + e) * S + row] : from[row * S + c + e];
-    const Planes<U> f = split<U>(x[0], x[1]);
-#pragma unroll
-    for (int k = 0; k < planes_of<U>(); ++k) *reinterpret_cast<Frag<U>*>(to + ((k * 64 + row) * 64 + c) * int(sizeof(U))) = f.p[k];
+    for (int e = 0; e < 4; ++e) x[e] = TRANSPOSED ? from[(c + e) * S + row] : from[row * S + c + e];
+    *reinterpret_cast<v4f*>(to + row * 64 + c) = x;
   }
 }
 
@@ -45,7 +44,6 @@ __device__ __forceinline__ double chunk_sum(float g, int lane) {
 
 template <typename T, int DK, bool BWD>
 __global__ __launch_bounds__(256) void delta_prepare_kernel(DeltaArgs a) {
-  using U = Inner<T>;
   using TK = Tile<T, DK>;
   constexpr int S = PREPARE_STRIDE, SQUARES = 2 * 64 * S * 4;
   __shared__ __align__(16) float sh_a[64 * S];
@@ -161,9 +159,9 @@ __global__ __launch_bounds__(256) void delta_prepare_kernel(DeltaArgs a) {
     for (int e = 0; e < 4; ++e) sh_m[(32 + 16 * rt + 4 * q + e) * S + 16 * ct + r] = -y[e];
   }
   __syncthreads();
-  store_square<U, false>(a.m + block * a.square, sh_m);
-  if constexpr (BWD) store_square<U, true>(a.m_t + block * a.square, sh_m);
-  store_square<U, BWD>(a.c + block * a.square, sh_c);
+  store_triangle<false>(a.m + block * 4096, sh_m);
+  if constexpr (BWD) store_triangle<true>(a.m_t + block * 4096, sh_m);
+  store_triangle<BWD>(a.c + block * 4096, sh_c);
 }
 
 }  // namespace linrec

@@ -2,7 +2,7 @@
 //
 // As the forward's: a workgroup has a (sequence, head), a wave of its first half 16 columns of dS, and the other half loads.
 //
-// 8 x 4096, 16 heads of 128 x 128 bf16: 445 us for 1.47 GB (289 us at the rate of a copy); without waves that load 794.
+// 8 x 4096, 16 heads of 128 x 128 bf16: 430 us for 1.41 GB (276 us at the rate of a copy); without waves that load 560.
 #pragma once
 #include "delta_scan.hpp"
 
@@ -11,12 +11,9 @@ namespace linrec {
 template <typename T, int DK, int WAVES>
 struct ReverseShared {
   using U = Inner<T>;
-  static constexpr int KEYS = Tile<T, DK>::BYTES, VALUES = Tile<T, 16 * WAVES>::BYTES;
-  static constexpr bool QUERIES = 2 * KEYS + VALUES + 2 * square_bytes<U>() + 1024 <= 160 * 1024;
-  static constexpr int K = 0, Q = K + KEYS, O = Q + (QUERIES ? KEYS : 0), M = O + VALUES, C = M + square_bytes<U>(),
-                       TILES = C + square_bytes<U>();
-  static constexpr GatePlace<U, true> GATES{TILES, C, true};
-  static constexpr int BYTES = GATES.bytes;
+  static constexpr int KEYS = Tile<T, DK>::BYTES, VALUES = Tile<T, 16 * WAVES>::BYTES, SQUARE = triangle_bytes<U, chain_planes<U>()>(), GATE_BYTES = 3 * 64 * 4;
+  static constexpr bool QUERIES = 2 * KEYS + VALUES + 2 * SQUARE + GATE_BYTES <= 160 * 1024;
+  static constexpr int K = 0, Q = K + KEYS, O = Q + (QUERIES ? KEYS : 0), M = O + VALUES, C = M + SQUARE, GATES = C + SQUARE, BYTES = GATES + GATE_BYTES;
   static constexpr bool LOADERS = 2 * BYTES <= 160 * 1024;
   static constexpr int LANES = 64 * WAVES * (LOADERS ? 2 : 1);
 };
@@ -28,8 +25,7 @@ __global__ __launch_bounds__((ReverseShared<T, DK, WAVES>::LANES)) void delta_re
   using Sh = ReverseShared<T, DK, WAVES>;
   using TK = Tile<T, DK>;
   using TV = Tile<T, 16 * WAVES>;
-  using TS = Tile<U, 64>;
-  constexpr int P = planes_of<U>(), STAGING = 64 * WAVES, IN = input_planes<T>();
+  constexpr int CHAIN = chain_planes<U>(), STAGING = 64 * WAVES, IN = input_planes<T>();
   __shared__ __align__(16) char room[Sh::BYTES * (Sh::LOADERS ? 2 : 1)];
   const linrec_delta_t& p = a.p;
   int64_t pair;
@@ -51,31 +47,24 @@ __global__ __launch_bounds__((ReverseShared<T, DK, WAVES>::LANES)) void delta_re
     const int length = int(span.end - first < DELTA_CHUNK ? span.end - first : DELTA_CHUNK), by = wave * 64 + lane;
     Stager<T, DK, STAGING> k, qq;
     Stager<T, 16 * WAVES, STAGING> o;
-    Stager<U, 64, STAGING> m[P], cc[P];
+    TriangleStager<U, true, STAGING, CHAIN> m, cc;
     float gate[(192 + STAGING - 1) / STAGING];
     k.fetch(head_rows<T>(p.k, p.k_stride, span.batch, first, key_head), p.k_stride[1], length, p.key_dim, by);
     if constexpr (Sh::QUERIES) qq.fetch(head_rows<T>(p.q, p.q_stride, span.batch, first, key_head), p.q_stride[1], length, p.key_dim, by);
     o.fetch(head_rows<T>(p.d_o, p.d_o_stride, span.batch, first, head) + c0, p.d_o_stride[1], length, p.value_dim - c0, by);
-#pragma unroll
-    for (int k2 = 0; k2 < P; ++k2) {
-      m[k2].fetch_dense(reinterpret_cast<const U*>(a.m_t + block * a.square) + k2 * 4096, by);
-      cc[k2].fetch_dense(reinterpret_cast<const U*>(a.c + block * a.square) + k2 * 4096, by);
-    }
+    m.fetch(a.m_t + block * 4096, by);
+    cc.fetch(a.c + block * 4096, by);
 #pragma unroll
     for (int i = 0; i < (192 + STAGING - 1) / STAGING; ++i)
       if (i * STAGING + by < 192) gate[i] = a.gates[block * 192 + i * STAGING + by];
     k.put(smem + Sh::K, by);
     if constexpr (Sh::QUERIES) qq.put(smem + Sh::Q, by);
     o.put(smem + Sh::O, by);
-#pragma unroll
-    for (int k2 = 0; k2 < P; ++k2) {
-      m[k2].put(smem + Sh::M + k2 * TS::BYTES, by);
-      if constexpr (Sh::GATES.inside) cc[k2].template put_triangle<true>(smem + Sh::C + k2 * TS::BYTES, by);
-      else cc[k2].put(smem + Sh::C + k2 * TS::BYTES, by);
-    }
+    m.put(smem + Sh::M, by);
+    cc.put(smem + Sh::C, by);
 #pragma unroll
     for (int i = 0; i < (192 + STAGING - 1) / STAGING; ++i)
-      if (i * STAGING + by < 192) reinterpret_cast<float*>(smem + Sh::GATES.at)[Sh::GATES.place(i * STAGING + by)] = gate[i];
+      if (i * STAGING + by < 192) reinterpret_cast<float*>(smem + Sh::GATES)[i * STAGING + by] = gate[i];
   };
 
   v4f s[DK / 16];  // dS'
@@ -95,38 +84,23 @@ __global__ __launch_bounds__((ReverseShared<T, DK, WAVES>::LANES)) void delta_re
       }
   }
 
-  const int rows_k = TK::mapped_rows(r, q), rows_s = TS::mapped_rows(r, q), cols_k = TK::template columns<true>(r, q),
+  const int rows_k = TK::mapped_rows(r, q), rows_s = Tile<U, 32>::mapped_rows(r, q), cols_k = TK::template columns<true>(r, q),
             cols_v = TV::template column_tile<false>(TV::template columns<false>(r, q), wave);
   auto compute = [&](int64_t c, const char* smem) __attribute__((always_inline)) {
     const int64_t first = span.first + c * DELTA_CHUNK, block = (span.slot + c) * p.heads + head;
     const int length = int(span.end - first < DELTA_CHUNK ? span.end - first : DELTA_CHUNK);
-    const float* gates = reinterpret_cast<const float*>(smem + Sh::GATES.at);
+    const float* gates = reinterpret_cast<const float*>(smem + Sh::GATES);
+    auto four = [&](int kind, int t) __attribute__((always_inline)) { return *reinterpret_cast<const v4f*>(gates + kind * 64 + row_of_result(t, q)); };
     const T* qq = head_rows<T>(p.q, p.q_stride, span.batch, first, key_head);
     Planes<T> sp[DK / 32];
     float un_s;
     split_scaled(s, sp, &un_s);
     if constexpr (!CARRY) {
-      U* to = reinterpret_cast<U*>(a.d_s + block * a.state) + int64_t(col - r) * DK;
+      float* to = a.d_s + block * a.state + int64_t(col - r) * DK;
 #pragma unroll
-      for (int b = 0; b < DK / 32; ++b) {
-        if (!kept_column) break;
-        // (of bf16 inputs the first two are sp[b], which the compiler sees)
-        store_rows(to, int64_t(a.columns) * DK, b, lane, split<U, kept_planes<U, DK>()>(s[2 * b], s[2 * b + 1]));
-      }
+      for (int b = 0; b < DK / 32; ++b)
+        if (kept_column) store_rows(to, b, lane, s[2 * b], s[2 * b + 1]);
     }
-    // upper triangular: the first 32 positions have no part in rows from 32 on
-    auto upper = [&](int at, const auto(&by)[2], v4f* to) __attribute__((always_inline)) {
-      Planes<U> f[4];
-#pragma unroll
-      for (int b = 0; b < 2; ++b) {
-#pragma unroll
-        for (int t = 0; t < 2 + 2 * b; ++t)
-#pragma unroll
-          for (int k2 = 0; k2 < P; ++k2) f[t].p[k2] = TS::frag(smem + at + k2 * TS::BYTES, rows_s, TS::mapped_row(t), b);
-        if (b == 0) mma_tiles<0, 2, 2>(f, by[b], to);
-        else mma_tiles<0, 4, 2>(f, by[b], to);
-      }
-    };
     // dO of this wave's columns, a result's layout; fp16 as two bf16
     v4f d_o[4];
     Planes<U, IN> dop[2];
@@ -153,27 +127,26 @@ __global__ __launch_bounds__((ReverseShared<T, DK, WAVES>::LANES)) void delta_re
       mma_tiles<0, 4>(f, sp[b], x);
     }
 #pragma unroll
-    for (int t = 0; t < 4; ++t) x[t] *= Sh::GATES.four(gates + 64, 64, row_of_result(t, q)) * un_s;
-    upper(Sh::C, dop, x);
-    constexpr int CHAIN = chain_planes<U>();
+    for (int t = 0; t < 4; ++t) x[t] *= four(1, t) * un_s;
+    mma_triangle<true, CHAIN - 1, CHAIN>(smem + Sh::C, rows_s, dop, x);
     Planes<U, CHAIN> xp[2];
 #pragma unroll
     for (int b = 0; b < 2; ++b) xp[b] = split<U, CHAIN>(x[2 * b], x[2 * b + 1]);
     v4f db[4];
 #pragma unroll
     for (int t = 0; t < 4; ++t) db[t] = v4f{0, 0, 0, 0};
-    upper(Sh::M, xp, db);
+    mma_triangle<true, CHAIN - 1, CHAIN>(smem + Sh::M, rows_s, xp, db);
     if (!CARRY && kept_column) {
-      U* to = reinterpret_cast<U*>(a.d_b + block * a.rows) + (col - r) * 64;
+      float* to = a.d_b + block * a.rows + (col - r) * 64;
 #pragma unroll
-      for (int b = 0; b < 2; ++b) store_rows(to, int64_t(a.columns) * 64, b, lane, split<U>(db[2 * b], db[2 * b + 1]));
+      for (int b = 0; b < 2; ++b) store_rows(to, b, lane, db[2 * b], db[2 * b + 1]);
     }
     const int apart = p.heads * p.value_dim;
     T* d_v = static_cast<T*>(p.d_v) + ((span.batch * p.time + first) * p.heads + head) * int64_t(p.value_dim) + col;
 #pragma unroll
     for (int t = 0; t < 4; ++t) {
       const int row = row_of_result(t, q);
-      const v4f gamma = Sh::GATES.four(gates, 0, row), beta = Sh::GATES.four(gates + 128, 128, row);
+      const v4f gamma = four(0, t), beta = four(2, t);
       T* to = d_v + row * int64_t(apart);
 #pragma unroll
       for (int e = 0; e < 4; ++e) db[t][e] *= beta[e];
@@ -197,7 +170,7 @@ __global__ __launch_bounds__((ReverseShared<T, DK, WAVES>::LANES)) void delta_re
     float un_v, un_o;
     split_scaled(db, vp, &un_v);
     split_scaled(d_o, op, &un_o);
-    const float keep = gates[Sh::GATES.place(63)];
+    const float keep = gates[63];
 #pragma unroll
     for (int t = 0; t < DK / 16; ++t) {
       auto with_keys = [&](v4f to) __attribute__((always_inline)) {

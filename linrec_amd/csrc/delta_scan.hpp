@@ -1,38 +1,15 @@
 // Gated delta rule, the pass along the sequence: N, O and the state, chunk by chunk (delta_core.hpp).
 //
 // A workgroup has a (sequence, head), or a segment of one (delta_segments.hpp), and 16 columns of the state for each of half of its waves; the
-// other half loads what the next chunk needs into LDS meanwhile (a state's chunks follow one another, so nothing else hides those loads: 290 us
-// with them, 604 without; where two chunks do not fit into LDS all waves load first and compute then).
+// other half loads what the next chunk needs into LDS meanwhile (a state's chunks follow one another, so nothing else hides those loads: 310 us
+// with them, 420 without; where two chunks do not fit into LDS all waves load first and compute then).
 //
-// 8 x 4096, 16 heads of 128 x 128 bf16: 295 us with O and as many with the states, for 0.67 and 1.28 GB (131 and 250 us at the rate of a copy).  A chunk
-// is six products that wait for each other, by one wave of a SIMD, whose matrix instructions fill a third of the time.
+// 8 x 4096, 16 heads of 128 x 128 bf16: 310 us with O and 255 with the states, for 0.60 and 1.11 GB (118 and 217 us at the rate of a copy).  A chunk
+// is six products that wait for each other, by one wave of a SIMD: 182 matrix instructions of 16 cycles in 11600 cycles.
 #pragma once
 #include "delta_core.hpp"
 
 namespace linrec {
-
-template <typename U>
-constexpr int square_bytes() {
-  return 64 * 64 * int(sizeof(U)) * planes_of<U>();
-}
-
-// Where a chunk's gates lie: behind its tiles, or in the empty quarter of the triangle C, the last of them, where two chunks fit into LDS only so
-// (fp32 of 64 channels, 160 KB to the byte: 8 x 4096 with 16 heads of 64 x 64 575 us forward and 2042 with the backward, 710 and 2303 with one chunk).
-// In bytes; place() in floats.
-template <typename U, bool UPPER>
-struct GatePlace {
-  static constexpr int ALONE = 3 * 64 * 4;
-  bool inside;
-  int at, bytes;
-  constexpr GatePlace(int tiles, int c, bool has_c)
-      : inside(has_c && sizeof(U) == 4 && 2 * (tiles + ALONE) > 160 * 1024 && 2 * tiles <= 160 * 1024),
-        at(!inside ? tiles : c + (UPPER ? 32 * 64 : 32) * 4), bytes(inside ? tiles : tiles + ALONE) {}
-  constexpr __device__ __forceinline__ int place(int gate) const { return inside ? (gate >> 5) * 64 + (gate & 31) : gate; }
-  // four gates of a kind (from the first of them on) of rows from `row` on
-  __device__ __forceinline__ v4f four(const float* kind, int first, int row) const {
-    return *reinterpret_cast<const v4f*>(inside ? kind + (place(first + row) - first) : kind + row);
-  }
-};
 
 enum ScanMode {
   SCAN_OUT,     // the forward: O and the last state
@@ -44,13 +21,11 @@ template <typename T, int DK, int WAVES, ScanMode MODE>
 struct ScanShared {
   static constexpr bool STATES = MODE != SCAN_OUT;
   using U = Inner<T>;
-  static constexpr int KEYS = Tile<T, DK>::BYTES, VALUES = Tile<T, 16 * WAVES>::BYTES;
+  static constexpr int KEYS = Tile<T, DK>::BYTES, VALUES = Tile<T, 16 * WAVES>::BYTES, M_BYTES = triangle_bytes<U, chain_planes<U>()>(),
+                       C_BYTES = STATES ? 0 : triangle_bytes<U, planes_of<U>()>(), GATE_BYTES = 3 * 64 * 4;
   // (fp32 of 256 channels: queries are read from memory where they are used)
-  static constexpr bool QUERIES = !STATES && 2 * KEYS + VALUES + 2 * square_bytes<U>() + 1024 <= 160 * 1024;
-  static constexpr int K = 0, Q = K + KEYS, V = Q + (QUERIES ? KEYS : 0), M = V + VALUES, C = M + square_bytes<U>(),
-                       TILES = C + (STATES ? 0 : square_bytes<U>());
-  static constexpr GatePlace<U, false> GATES{TILES, C, !STATES};
-  static constexpr int BYTES = GATES.bytes;
+  static constexpr bool QUERIES = !STATES && 2 * KEYS + VALUES + M_BYTES + C_BYTES + GATE_BYTES <= 160 * 1024;
+  static constexpr int K = 0, Q = K + KEYS, V = Q + (QUERIES ? KEYS : 0), M = V + VALUES, C = M + M_BYTES, GATES = C + C_BYTES, BYTES = GATES + GATE_BYTES;
   static constexpr bool LOADERS = 2 * BYTES <= 160 * 1024;
   static constexpr int LANES = 64 * WAVES * (LOADERS ? 2 : 1);
 };
@@ -73,8 +48,7 @@ __global__ __launch_bounds__((ScanShared<T, DK, WAVES, MODE>::LANES)) void delta
   using Sh = ScanShared<T, DK, WAVES, MODE>;
   using TK = Tile<T, DK>;
   using TV = Tile<T, 16 * WAVES>;
-  using TS = Tile<U, 64>;
-  constexpr int P = planes_of<U>(), STAGING = 64 * WAVES;
+  constexpr int P = planes_of<U>(), CHAIN = chain_planes<U>(), STAGING = 64 * WAVES;
   __shared__ __align__(16) char room[Sh::BYTES * (Sh::LOADERS ? 2 : 1)];
   const linrec_delta_t& p = a.p;
   int64_t pair;
@@ -97,32 +71,26 @@ __global__ __launch_bounds__((ScanShared<T, DK, WAVES, MODE>::LANES)) void delta
     const int length = int(span.end - first < DELTA_CHUNK ? span.end - first : DELTA_CHUNK), by = wave * 64 + lane;
     Stager<T, DK, STAGING> k, qq;
     Stager<T, 16 * WAVES, STAGING> v;
-    Stager<U, 64, STAGING> m[P], cc[P];
+    TriangleStager<U, false, STAGING, CHAIN> m;
+    TriangleStager<U, false, STAGING, P> cc;
     float gate[(192 + STAGING - 1) / STAGING];
     k.fetch(head_rows<T>(p.k, p.k_stride, span.batch, first, key_head), p.k_stride[1], length, p.key_dim, by);
     if constexpr (Sh::QUERIES) qq.fetch(head_rows<T>(p.q, p.q_stride, span.batch, first, key_head), p.q_stride[1], length, p.key_dim, by);
     if (!unit) v.fetch(head_rows<T>(p.v, p.v_stride, span.batch, first, head) + c0, p.v_stride[1], length, p.value_dim - c0, by);
     else v.clear();
-#pragma unroll
-    for (int k2 = 0; k2 < P; ++k2) {
-      m[k2].fetch_dense(reinterpret_cast<const U*>(a.m + block * a.square) + k2 * 4096, by);
-      if constexpr (MODE == SCAN_OUT) cc[k2].fetch_dense(reinterpret_cast<const U*>(a.c + block * a.square) + k2 * 4096, by);
-    }
+    m.fetch(a.m + block * 4096, by);
+    if constexpr (MODE == SCAN_OUT) cc.fetch(a.c + block * 4096, by);
 #pragma unroll
     for (int i = 0; i < (192 + STAGING - 1) / STAGING; ++i)
       if (i * STAGING + by < 192) gate[i] = a.gates[block * 192 + i * STAGING + by];
     k.put(smem + Sh::K, by);
     if constexpr (Sh::QUERIES) qq.put(smem + Sh::Q, by);
     v.put(smem + Sh::V, by);
-#pragma unroll
-    for (int k2 = 0; k2 < P; ++k2) {
-      m[k2].put(smem + Sh::M + k2 * TS::BYTES, by);
-      if constexpr (Sh::GATES.inside) cc[k2].template put_triangle<false>(smem + Sh::C + k2 * TS::BYTES, by);
-      else if constexpr (MODE == SCAN_OUT) cc[k2].put(smem + Sh::C + k2 * TS::BYTES, by);
-    }
+    m.put(smem + Sh::M, by);
+    if constexpr (MODE == SCAN_OUT) cc.put(smem + Sh::C, by);
 #pragma unroll
     for (int i = 0; i < (192 + STAGING - 1) / STAGING; ++i)
-      if (i * STAGING + by < 192) reinterpret_cast<float*>(smem + Sh::GATES.at)[Sh::GATES.place(i * STAGING + by)] = gate[i];
+      if (i * STAGING + by < 192) reinterpret_cast<float*>(smem + Sh::GATES)[i * STAGING + by] = gate[i];
   };
 
   v4f s[DK / 16];
@@ -148,24 +116,22 @@ __global__ __launch_bounds__((ScanShared<T, DK, WAVES, MODE>::LANES)) void delta
       }
   }
 
-  const int rows_k = TK::mapped_rows(r, q), rows_s = TS::mapped_rows(r, q), cols_k = TK::template columns<true>(r, q),
+  const int rows_k = TK::mapped_rows(r, q), rows_s = Tile<U, 32>::mapped_rows(r, q), cols_k = TK::template columns<true>(r, q),
             cols_v = TV::template column_tile<false>(TV::template columns<false>(r, q), wave);
   auto compute = [&](int64_t c, const char* smem) __attribute__((always_inline)) {
     const int64_t first = span.first + c * DELTA_CHUNK, block = (span.slot + c) * p.heads + head;
     const int length = int(span.end - first < DELTA_CHUNK ? span.end - first : DELTA_CHUNK);
-    const float* gates = reinterpret_cast<const float*>(smem + Sh::GATES.at);
+    const float* gates = reinterpret_cast<const float*>(smem + Sh::GATES);
+    auto four = [&](int kind, int t) __attribute__((always_inline)) { return *reinterpret_cast<const v4f*>(gates + kind * 64 + row_of_result(t, q)); };
     const T* qq = head_rows<T>(p.q, p.q_stride, span.batch, first, key_head);
     Planes<T> sp[DK / 32];
     float un_s;
     split_scaled(s, sp, &un_s);
     if constexpr (MODE == SCAN_STATES) {
-      U* to = reinterpret_cast<U*>(a.s + block * a.state) + int64_t(col - r) * DK;
+      float* to = a.s + block * a.state + int64_t(col - r) * DK;
 #pragma unroll
-      for (int b = 0; b < DK / 32; ++b) {
-        if (!kept_column) break;
-        // (of bf16 inputs the first two are sp[b], which the compiler sees)
-        store_rows(to, int64_t(a.columns) * DK, b, lane, split<U, kept_planes<U, DK>()>(s[2 * b], s[2 * b + 1]));
-      }
+      for (int b = 0; b < DK / 32; ++b)
+        if (kept_column) store_rows(to, b, lane, s[2 * b], s[2 * b + 1]);
     }
     v4f x[4];  // K S, then beta (V - e^G K S)
 #pragma unroll
@@ -178,44 +144,26 @@ __global__ __launch_bounds__((ScanShared<T, DK, WAVES, MODE>::LANES)) void delta
       if constexpr (std::is_same_v<T, __bf16>) mma_tiles<0, 4>(f, third_plane(s[2 * b], s[2 * b + 1], sp[b]), x);
       mma_tiles<0, 4>(f, sp[b], x);
     }
-    // lower triangular: positions from 32 on have no part in the first 32 rows
-    auto lower = [&](int at, const auto(&by)[2], v4f* to) __attribute__((always_inline)) {
-      Planes<U> f[4];
-#pragma unroll
-      for (int b = 0; b < 2; ++b) {
-#pragma unroll
-        for (int t = 2 * b; t < 4; ++t)
-#pragma unroll
-          for (int k2 = 0; k2 < P; ++k2) f[t].p[k2] = TS::frag(smem + at + k2 * TS::BYTES, rows_s, TS::mapped_row(t), b);
-        if (b == 0) mma_tiles<0, 4>(f, by[b], to);
-        else mma_tiles<2, 2>(f, by[b], to);
-      }
-    };
 #pragma unroll
     for (int t = 0; t < 4; ++t) {
-      const int row = row_of_result(t, q);
       const auto v = TV::template column4<false>(smem + Sh::V, cols_v, TK::mapped_row(t), 0);
-      const v4f gamma = Sh::GATES.four(gates, 0, row), beta = Sh::GATES.four(gates + 128, 128, row);
+      const v4f gamma = four(0, t), beta = four(2, t);
 #pragma unroll
       for (int e = 0; e < 4; ++e) x[t][e] = beta[e] * fmaf(-gamma[e] * un_s, x[t][e], float(v[e]));
     }
-    constexpr int CHAIN = chain_planes<U>();
     Planes<U, CHAIN> xp[2];
 #pragma unroll
     for (int b = 0; b < 2; ++b) xp[b] = split<U, CHAIN>(x[2 * b], x[2 * b + 1]);
     v4f nn[4];
 #pragma unroll
     for (int t = 0; t < 4; ++t) nn[t] = v4f{0, 0, 0, 0};
-    lower(Sh::M, xp, nn);
-    Planes<U> np[2];
-#pragma unroll
-    for (int b = 0; b < 2; ++b) np[b] = split<U>(nn[2 * b], nn[2 * b + 1]);
+    mma_triangle<false, CHAIN - 1, CHAIN>(smem + Sh::M, rows_s, xp, nn);
     if constexpr (MODE == SCAN_CARRY) {
     } else if constexpr (MODE == SCAN_STATES) {
-      U* to = reinterpret_cast<U*>(a.n + block * a.rows_n) + (col - r) * 64;
+      float* to = a.n + block * a.rows + (col - r) * 64;
 #pragma unroll
       for (int b = 0; b < 2; ++b)
-        if (kept_column) store_rows(to, int64_t(a.columns) * 64, b, lane, split<U, CHAIN>(nn[2 * b], nn[2 * b + 1]));
+        if (kept_column) store_rows(to, b, lane, nn[2 * b], nn[2 * b + 1]);
     } else {
       T* o = static_cast<T*>(p.o) + ((span.batch * p.time + first) * p.heads + head) * int64_t(p.value_dim) + col;
       v4f y[4];
@@ -237,8 +185,11 @@ __global__ __launch_bounds__((ScanShared<T, DK, WAVES, MODE>::LANES)) void delta
         mma_tiles<0, 4>(f, sp[b], y);
       }
 #pragma unroll
-      for (int t = 0; t < 4; ++t) y[t] *= Sh::GATES.four(gates, 0, row_of_result(t, q)) * (un_s * p.scale);
-      lower(Sh::C, np, y);
+      for (int t = 0; t < 4; ++t) y[t] *= four(0, t) * (un_s * p.scale);
+      Planes<U> np[2];
+#pragma unroll
+      for (int b = 0; b < 2; ++b) np[b] = split<U>(nn[2 * b], nn[2 * b + 1]);
+      mma_triangle<false, P - 1, P>(smem + Sh::C, rows_s, np, y);
 #pragma unroll
       for (int t = 0; t < 4; ++t) {
         const int row = row_of_result(t, q);
@@ -255,11 +206,11 @@ __global__ __launch_bounds__((ScanShared<T, DK, WAVES, MODE>::LANES)) void delta
       }
     }
 #pragma unroll
-    for (int t = 0; t < 4; ++t) nn[t] *= Sh::GATES.four(gates + 64, 64, row_of_result(t, q));
+    for (int t = 0; t < 4; ++t) nn[t] *= four(1, t);
     Planes<T, chain_planes<T>()> nt[2];
     float un_n;
     split_scaled(nn, nt, &un_n);
-    const float keep = gates[Sh::GATES.place(63)];
+    const float keep = gates[63];
 #pragma unroll
     for (int t0 = 0; t0 < DK / 16; t0 += 4) {
       v4f to[4];

@@ -19,10 +19,9 @@
 //
 // Precision.  States, sums and accumulators are fp32, and so is all that one kernel leaves to another.  An operand of a matrix instruction
 // that is not an input is split into bf16 (or, beside fp16 inputs, fp16) numbers, its rounding, the rounding of the rest and so on: three bf16
-// carry 24 bits, two fp16 22, two bf16 16 to 17.  Whatever goes into a result in fp32 (states and the gradients of the gates and of h0) is three bf16
-// or two fp16: these are as near as sums in fp32 are, 2e-7 to 7e-7 (with M, C, dB and, above 64 key channels, the kept S and dS' in two: states
-// 2e-6, the gradient of beta 4e-6, that of log_decay 5e-6).  C N in the forward, which O alone sees, is the product of two and two, 2^-16
-// beside the 2^-9 of O's own rounding.  fp32 inputs take the fp32 instructions.
+// carry 24 bits, two fp16 22.  So results in fp32 are as near as sums in fp32 are, 1e-7 to 7e-7, and those in 16 bits are their roundings.  (With M, C, dB and,
+// above 64 key channels, the kept S and dS' in two bf16, 16 to 17 bits, states were 2e-6 off, the gradient of beta 4e-6 and that of log_decay 5e-6; with N and S in two where
+// O is concerned O was 4e-6 off before its rounding, for 5 of 325 us of 8 x 4096, 16 heads of 128 x 128.)  fp32 inputs take the fp32 instructions.
 #pragma once
 #include <hip/hip_runtime.h>
 #include <stdint.h>
@@ -365,11 +364,11 @@ struct Stager {
   }
 };
 
-// Values of scratch, in fp32, on their way to a tile of ROWS rows of COLS columns in PLANES planes of U, eight of a row to a lane at a time.
-template <typename U, int COLS, int LANES, int ROWS, int PLANES = chain_planes<U>()>
+// Values of scratch, in fp32, on their way to the planes of a tile of ROWS rows of COLS columns, eight of a row to a lane at a time.
+template <typename U, int COLS, int LANES, int ROWS>
 struct SplitStager {
   using L = Tile<U, COLS>;
-  static constexpr int EIGHTS = COLS / 8, ALL = ROWS * EIGHTS, N = (ALL + LANES - 1) / LANES, BYTES = ROWS * L::ROW;  // (of a plane)
+  static constexpr int PLANES = chain_planes<U>(), EIGHTS = COLS / 8, ALL = ROWS * EIGHTS, N = (ALL + LANES - 1) / LANES, BYTES = ROWS * L::ROW;  // (of a plane)
   v4f v[N][2];
 
   static __device__ __forceinline__ bool has(int n, int lane) { return (n + 1) * LANES <= ALL || n * LANES + lane < ALL; }
@@ -404,9 +403,9 @@ struct SplitStager {
 // A triangle of a dense 64 x 64 square in LDS without its empty quarter: 64 rows of the 32 columns that are all full, the first ones of a lower and the
 // last ones of an upper triangle, and behind them the other 32 columns' rows.
 constexpr int TRIANGLE_ROWS = 96;
-template <typename U, bool UPPER, int LANES, int PLANES>
-struct TriangleStager : SplitStager<U, 32, LANES, TRIANGLE_ROWS, PLANES> {
-  using S = SplitStager<U, 32, LANES, TRIANGLE_ROWS, PLANES>;
+template <typename U, bool UPPER, int LANES>
+struct TriangleStager : SplitStager<U, 32, LANES, TRIANGLE_ROWS> {
+  using S = SplitStager<U, 32, LANES, TRIANGLE_ROWS>;
   static_assert(LANES == 256 || LANES == 128, "a load is of one part");
   __device__ __forceinline__ void fetch(const float* from, int lane) {
 #pragma unroll
@@ -424,14 +423,15 @@ struct TriangleStager : SplitStager<U, 32, LANES, TRIANGLE_ROWS, PLANES> {
       if (S::has(n, lane)) S::put_at(tile, n, n * LANES / 4 + (lane >> 2), lane & 3);
   }
 };
-template <typename U, int PLANES>
+template <typename U>
 constexpr int triangle_bytes() {
-  return TRIANGLE_ROWS * 32 * int(sizeof(U)) * PLANES;
+  return TRIANGLE_ROWS * 32 * int(sizeof(U)) * chain_planes<U>();
 }
-// to += triangle . by, four tiles of 16 rows (row_of_tile); products of planes whose numbers add up to more than MOST are left out.
-template <bool UPPER, int MOST, int PLANES, typename U, int NB>
+// to += triangle . by, four tiles of 16 rows (row_of_tile).
+template <bool UPPER, typename U, int NB>
 __device__ __forceinline__ void mma_triangle(const char* tile, int view, const Planes<U, NB> (&by)[2], v4f (&to)[4]) {
   using L = Tile<U, 32>;
+  constexpr int PLANES = chain_planes<U>();
 #pragma unroll
   for (int b = 0; b < 2; ++b) {
     const bool whole = b == (UPPER ? 1 : 0);  // these 32 columns have all rows
@@ -444,7 +444,7 @@ __device__ __forceinline__ void mma_triangle(const char* tile, int view, const P
           f[t] = L::frag(tile + k * (TRIANGLE_ROWS * L::ROW), view, L::mapped_row(t) + (whole ? 0 : UPPER ? 64 : 32), 0);
 #pragma unroll
       for (int j = NB - 1; j >= 0; --j)
-        if (k + j <= MOST)
+        if (k + j < PLANES)
 #pragma unroll
           for (int t = 0; t < 4; ++t)
             if (whole || (UPPER ? t < 2 : t >= 2)) to[t] = mma(f[t], by[b].p[j], to[t]);

@@ -11,7 +11,7 @@ namespace linrec {
 template <typename T, int DK, int WAVES>
 struct ReverseShared {
   using U = Inner<T>;
-  static constexpr int KEYS = Tile<T, DK>::BYTES, VALUES = Tile<T, 16 * WAVES>::BYTES, SQUARE = triangle_bytes<U, chain_planes<U>()>(), GATE_BYTES = 3 * 64 * 4;
+  static constexpr int KEYS = Tile<T, DK>::BYTES, VALUES = Tile<T, 16 * WAVES>::BYTES, SQUARE = triangle_bytes<U>(), GATE_BYTES = 3 * 64 * 4;
   static constexpr bool QUERIES = 2 * KEYS + VALUES + 2 * SQUARE + GATE_BYTES <= 160 * 1024;
   static constexpr int K = 0, Q = K + KEYS, O = Q + (QUERIES ? KEYS : 0), M = O + VALUES, C = M + SQUARE, GATES = C + SQUARE, BYTES = GATES + GATE_BYTES;
   static constexpr bool LOADERS = 2 * BYTES <= 160 * 1024;
@@ -47,7 +47,7 @@ __global__ __launch_bounds__((ReverseShared<T, DK, WAVES>::LANES)) void delta_re
     const int length = int(span.end - first < DELTA_CHUNK ? span.end - first : DELTA_CHUNK), by = wave * 64 + lane;
     Stager<T, DK, STAGING> k, qq;
     Stager<T, 16 * WAVES, STAGING> o;
-    TriangleStager<U, true, STAGING, CHAIN> m, cc;
+    TriangleStager<U, true, STAGING> m, cc;
     float gate[(192 + STAGING - 1) / STAGING];
     k.fetch(head_rows<T>(p.k, p.k_stride, span.batch, first, key_head), p.k_stride[1], length, p.key_dim, by);
     if constexpr (Sh::QUERIES) qq.fetch(head_rows<T>(p.q, p.q_stride, span.batch, first, key_head), p.q_stride[1], length, p.key_dim, by);
@@ -128,14 +128,14 @@ __global__ __launch_bounds__((ReverseShared<T, DK, WAVES>::LANES)) void delta_re
     }
 #pragma unroll
     for (int t = 0; t < 4; ++t) x[t] *= four(1, t) * un_s;
-    mma_triangle<true, CHAIN - 1, CHAIN>(smem + Sh::C, rows_s, dop, x);
+    mma_triangle<true>(smem + Sh::C, rows_s, dop, x);
     Planes<U, CHAIN> xp[2];
 #pragma unroll
     for (int b = 0; b < 2; ++b) xp[b] = split<U, CHAIN>(x[2 * b], x[2 * b + 1]);
     v4f db[4];
 #pragma unroll
     for (int t = 0; t < 4; ++t) db[t] = v4f{0, 0, 0, 0};
-    mma_triangle<true, CHAIN - 1, CHAIN>(smem + Sh::M, rows_s, xp, db);
+    mma_triangle<true>(smem + Sh::M, rows_s, xp, db);
     if (!CARRY && kept_column) {
       float* to = a.d_b + block * a.rows + (col - r) * 64;
 #pragma unroll

@@ -2,10 +2,10 @@
 //
 // A workgroup has a (sequence, head), or a segment of one (delta_segments.hpp), and 16 columns of the state for each of half of its waves; the
 // other half loads what the next chunk needs into LDS meanwhile (a state's chunks follow one another, so nothing else hides those loads: 310 us
-// with them, 420 without; where two chunks do not fit into LDS all waves load first and compute then).
+// with them, 420 without, when Q S was not taken beside K S; where two chunks do not fit into LDS all waves load first and compute then).
 //
-// 8 x 4096, 16 heads of 128 x 128 bf16: 310 us with O and 255 with the states, for 0.60 and 1.11 GB (118 and 217 us at the rate of a copy).  A chunk
-// is six products that wait for each other, by one wave of a SIMD: 182 matrix instructions of 16 cycles in 11600 cycles.
+// 8 x 4096, 16 heads of 128 x 128 bf16: 325 us with O and 255 with the states, for 0.60 and 1.11 GB (118 and 217 us at the rate of a copy).  A chunk
+// is a chain of products by one wave of a SIMD: 216 matrix instructions of 16 cycles in 12200 cycles.
 #pragma once
 #include "delta_core.hpp"
 
@@ -21,11 +21,10 @@ template <typename T, int DK, int WAVES, ScanMode MODE>
 struct ScanShared {
   static constexpr bool STATES = MODE != SCAN_OUT;
   using U = Inner<T>;
-  static constexpr int KEYS = Tile<T, DK>::BYTES, VALUES = Tile<T, 16 * WAVES>::BYTES, M_BYTES = triangle_bytes<U, chain_planes<U>()>(),
-                       C_BYTES = STATES ? 0 : triangle_bytes<U, planes_of<U>()>(), GATE_BYTES = 3 * 64 * 4;
+  static constexpr int KEYS = Tile<T, DK>::BYTES, VALUES = Tile<T, 16 * WAVES>::BYTES, SQUARE = triangle_bytes<U>(), GATE_BYTES = 3 * 64 * 4;
   // (fp32 of 256 channels: queries are read from memory where they are used)
-  static constexpr bool QUERIES = !STATES && 2 * KEYS + VALUES + M_BYTES + C_BYTES + GATE_BYTES <= 160 * 1024;
-  static constexpr int K = 0, Q = K + KEYS, V = Q + (QUERIES ? KEYS : 0), M = V + VALUES, C = M + M_BYTES, GATES = C + C_BYTES, BYTES = GATES + GATE_BYTES;
+  static constexpr bool QUERIES = !STATES && 2 * KEYS + VALUES + 2 * SQUARE + GATE_BYTES <= 160 * 1024;
+  static constexpr int K = 0, Q = K + KEYS, V = Q + (QUERIES ? KEYS : 0), M = V + VALUES, C = M + SQUARE, GATES = C + (STATES ? 0 : SQUARE), BYTES = GATES + GATE_BYTES;
   static constexpr bool LOADERS = 2 * BYTES <= 160 * 1024;
   static constexpr int LANES = 64 * WAVES * (LOADERS ? 2 : 1);
 };
@@ -48,7 +47,7 @@ __global__ __launch_bounds__((ScanShared<T, DK, WAVES, MODE>::LANES)) void delta
   using Sh = ScanShared<T, DK, WAVES, MODE>;
   using TK = Tile<T, DK>;
   using TV = Tile<T, 16 * WAVES>;
-  constexpr int P = planes_of<U>(), CHAIN = chain_planes<U>(), STAGING = 64 * WAVES;
+  constexpr int CHAIN = chain_planes<U>(), STAGING = 64 * WAVES;
   __shared__ __align__(16) char room[Sh::BYTES * (Sh::LOADERS ? 2 : 1)];
   const linrec_delta_t& p = a.p;
   int64_t pair;
@@ -71,8 +70,7 @@ __global__ __launch_bounds__((ScanShared<T, DK, WAVES, MODE>::LANES)) void delta
     const int length = int(span.end - first < DELTA_CHUNK ? span.end - first : DELTA_CHUNK), by = wave * 64 + lane;
     Stager<T, DK, STAGING> k, qq;
     Stager<T, 16 * WAVES, STAGING> v;
-    TriangleStager<U, false, STAGING, CHAIN> m;
-    TriangleStager<U, false, STAGING, P> cc;
+    TriangleStager<U, false, STAGING> m, cc;
     float gate[(192 + STAGING - 1) / STAGING];
     k.fetch(head_rows<T>(p.k, p.k_stride, span.batch, first, key_head), p.k_stride[1], length, p.key_dim, by);
     if constexpr (Sh::QUERIES) qq.fetch(head_rows<T>(p.q, p.q_stride, span.batch, first, key_head), p.q_stride[1], length, p.key_dim, by);
@@ -133,16 +131,30 @@ __global__ __launch_bounds__((ScanShared<T, DK, WAVES, MODE>::LANES)) void delta
       for (int b = 0; b < DK / 32; ++b)
         if (kept_column) store_rows(to, b, lane, s[2 * b], s[2 * b + 1]);
     }
-    v4f x[4];  // K S, then beta (V - e^G K S)
+    v4f x[4], y[4];  // K S, then beta (V - e^G K S); Q S, then O
 #pragma unroll
-    for (int t = 0; t < 4; ++t) x[t] = v4f{0, 0, 0, 0};
+    for (int t = 0; t < 4; ++t) x[t] = y[t] = v4f{0, 0, 0, 0};
 #pragma unroll
     for (int b = 0; b < DK / 32; ++b) {
-      Frag<T> f[4];
+      Frag<T> f[4], g[4];
 #pragma unroll
-      for (int t = 0; t < 4; ++t) f[t] = TK::frag(smem + Sh::K, rows_k, TK::mapped_row(t), b);
-      if constexpr (std::is_same_v<T, __bf16>) mma_tiles<0, 4>(f, third_plane(s[2 * b], s[2 * b + 1], sp[b]), x);
-      mma_tiles<0, 4>(f, sp[b], x);
+      for (int t = 0; t < 4; ++t) {
+        f[t] = TK::frag(smem + Sh::K, rows_k, TK::mapped_row(t), b);
+        if constexpr (MODE != SCAN_OUT) {
+        } else if constexpr (Sh::QUERIES) {
+          g[t] = TK::frag(smem + Sh::Q, rows_k, TK::mapped_row(t), b);
+        } else {
+          const int from = row_of_tile(t, r);
+#pragma unroll
+          for (int e = 0; e < 8; ++e) g[t][e] = from < length && 32 * b + 8 * q + e < p.key_dim ? qq[from * p.q_stride[1] + 32 * b + 8 * q + e] : T(0.0f);
+        }
+      }
+      auto with = [&](const auto& planes) __attribute__((always_inline)) {
+        mma_tiles<0, 4>(f, planes, x);
+        if constexpr (MODE == SCAN_OUT) mma_tiles<0, 4>(g, planes, y);
+      };
+      if constexpr (std::is_same_v<T, __bf16>) with(third_plane(s[2 * b], s[2 * b + 1], sp[b]));
+      with(sp[b]);
     }
 #pragma unroll
     for (int t = 0; t < 4; ++t) {
@@ -157,7 +169,7 @@ __global__ __launch_bounds__((ScanShared<T, DK, WAVES, MODE>::LANES)) void delta
     v4f nn[4];
 #pragma unroll
     for (int t = 0; t < 4; ++t) nn[t] = v4f{0, 0, 0, 0};
-    mma_triangle<false, CHAIN - 1, CHAIN>(smem + Sh::M, rows_s, xp, nn);
+    mma_triangle<false>(smem + Sh::M, rows_s, xp, nn);
     if constexpr (MODE == SCAN_CARRY) {
     } else if constexpr (MODE == SCAN_STATES) {
       float* to = a.n + block * a.rows + (col - r) * 64;
@@ -166,30 +178,12 @@ __global__ __launch_bounds__((ScanShared<T, DK, WAVES, MODE>::LANES)) void delta
         if (kept_column) store_rows(to, b, lane, nn[2 * b], nn[2 * b + 1]);
     } else {
       T* o = static_cast<T*>(p.o) + ((span.batch * p.time + first) * p.heads + head) * int64_t(p.value_dim) + col;
-      v4f y[4];
-#pragma unroll
-      for (int t = 0; t < 4; ++t) y[t] = v4f{0, 0, 0, 0};
-#pragma unroll
-      for (int b = 0; b < DK / 32; ++b) {
-        Frag<T> f[4];
-#pragma unroll
-        for (int t = 0; t < 4; ++t) {
-          if constexpr (Sh::QUERIES) {
-            f[t] = TK::frag(smem + Sh::Q, rows_k, TK::mapped_row(t), b);
-          } else {
-            const int from = row_of_tile(t, r);
-#pragma unroll
-            for (int e = 0; e < 8; ++e) f[t][e] = from < length && 32 * b + 8 * q + e < p.key_dim ? qq[from * p.q_stride[1] + 32 * b + 8 * q + e] : T(0.0f);
-          }
-        }
-        mma_tiles<0, 4>(f, sp[b], y);
-      }
 #pragma unroll
       for (int t = 0; t < 4; ++t) y[t] *= four(0, t) * (un_s * p.scale);
-      Planes<U> np[2];
+      Planes<U, CHAIN> np[2];
 #pragma unroll
-      for (int b = 0; b < 2; ++b) np[b] = split<U>(nn[2 * b], nn[2 * b + 1]);
-      mma_triangle<false, P - 1, P>(smem + Sh::C, rows_s, np, y);
+      for (int b = 0; b < 2; ++b) np[b] = split<U, CHAIN>(nn[2 * b], nn[2 * b + 1]);
+      mma_triangle<false>(smem + Sh::C, rows_s, np, y);
 #pragma unroll
       for (int t = 0; t < 4; ++t) {
         const int row = row_of_result(t, q);

@@ -31,3 +31,17 @@ def test_results_in_float32_have_its_accuracy(lead, heads, dims, dtype):
     ref.assert_near(got_state, state, share, "state")
     for name, value, true in list(zip(NAMES, got, want))[3:]:
         ref.assert_near(value, true, 2 * share, name, (dims[0] * dims[1]) ** 0.5 if name == "d_log_decay" else 1.0)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("lead,heads,dims", [((16, 128), (2, 2), (128, 128)), ((16, 128), (1, 4), (48, 64)), ((8, 100), (1, 2), (200, 160))])
+def test_results_in_16_bits_are_roundings_of_such_results(lead, heads, dims, dtype):
+    """Beside the true result's rounding: a value is rounded to the other side with the probability |error| / step, and is a step off then.  The squares of
+    these add up to sum |error| step, at most |error| |step| in norm, with a step of 2^-7 (2^-10 in fp16) of a value at most."""
+    q, k, v, log_decay, beta, h0, *_ = make(lead, heads, dims, dtype, seed=12)
+    want, _ = ref.gated_delta(q, k, v, log_decay, beta, h0)
+    got = linrec_amd.gated_delta(*(t.to(DEV) for t in (q, k, v, log_decay, beta)), h0=h0.to(DEV))
+    rounded = want.to(dtype).double()
+    share = 8 * 2.0 ** -24 * (2 + lead[1] / 64) ** 0.5
+    off = float((got.double().cpu() - rounded).norm() / rounded.norm())
+    assert off <= (share * 2 * ref.HALF_STEP[dtype]) ** 0.5, off

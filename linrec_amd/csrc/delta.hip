@@ -19,12 +19,16 @@ size_t aligned(size_t n) { return (n + 255) & ~size_t(255); }
 
 // Chunks of a segment, 0 where sequences are not cut.
 //
-// A workgroup of a pass fills a CU, so `w` of them take ceil(w / 256) rounds, each as long as its chunks are many.  Cut into n segments a pass becomes
+// A workgroup of a pass is taken to fill a CU (the passes that keep states or carry segments leave room for a second one up to 64 key channels, in 16 bits, and
+// are counted as more rounds than they are), so `w` of them take ceil(w / 256) rounds, each as long as its chunks are many.  Cut into n segments a pass becomes
 // two, the first with the columns of the unit matrix as well, and what goes from segment to segment: about half a chunk's time for
 // each, and two chunks' for two launches more.  What counts is n at which a pass's rounds are about to grow, and the most that leaves four
-// chunks to a segment (shorter ones gain nothing: 1 x 2048 with 8 heads of 64 x 64, forward and backward, 172 us with 4, 199 with 2, 214 with 8).
-// 1 x 8192 with 128 x 128 bf16, forward and backward, cut and not: 16 heads (8 segments) 896 and 1723 us, 32 heads (4) 1528 and 1987; 48 heads,
-// where two segments took longer (2441 and 2276), are not cut.
+// chunks to a segment (1 x 2048 with 8 heads of 64 x 64, forward and backward: 198 us with 4, 231 with 8, 332 not cut; with 2, which is not taken, 179).
+// 1 x 8192 with 128 x 128 bf16, forward and backward, cut and not: 16 heads (8 segments) 892 and 1741 us, 32 heads (4) 1554 and 2004; 48 heads,
+// where two segments take longer (2544 and 2304), are not cut.
+//
+// Packed sequences are taken for as many of the mean length, since their bounds are not on the host: a long one among many short ones is not cut (one of 16384
+// positions with 4 heads of 128 x 128 bf16 beside 7 of 64: 191 us forward, beside 15: 928).
 int segment_of(const DeltaArgs& a, int width) {
   constexpr int64_t CUS = 256, LEAST = 4;
   const linrec_delta_t& p = a.p;

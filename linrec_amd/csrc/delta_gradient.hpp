@@ -13,7 +13,7 @@
 // of 16 rows each: dQ and X, which multiply S, and Y, which multiplies dS'.  One wave for all three would hold more than its share of the
 // registers (with two numbers an operand 2.4 ms for 8 x 4096, 16 heads of 128 x 128 bf16, what went through scratch cost more than the products), three
 // parts read S from LDS twice (0.79 ms); two 0.70 ms.  Now all that is not an input is three numbers (delta_core.hpp), with which two steps
-// no longer fit into LDS above 64 key channels: 0.83 to 0.89 ms, for 2.1 GB of states, operands and results (0.42 at the rate of a
+// no longer fit into LDS above 64 key channels: 0.87 to 0.94 ms, for 2.1 GB of states, operands and results (0.42 at the rate of a
 // copy).  beta X goes from the one part to the other through LDS, head by head, and is added to Y there, so each part keeps one sum over
 // the heads and what its head alone has (with differences of running sums for the latter, which took as long, a small head lost its
 // digits).  The 64 x 64 products F, F^T, E, E^T are computed as they are needed as operands: what a lane gets of a product is its part of an
